@@ -45,6 +45,8 @@ _sig("arcz_spare_bytes", _z)
 _sig("arcz_give_back", _z, _z)
 _sig("arcz_alloc", _p, _z)
 _sig("arcz_view", _p, _p, _z, _z)
+_sig("arcz_wrap", _p, _p, _z)
+_sig("arcz_stream", _p)
 _sig("arcz_free", _i, _p)
 _sig("arcz_mem_size", _z, _p)
 _sig("arcz_mem_ptr", _p, _p)
@@ -120,6 +122,15 @@ _sig("arcz_moe_layer_free", _i, _p, _p)
 _sig("arcz_engine_moe_sgate", _p, _p)
 _sig("arcz_engine_moe_buffer", _p, _p, _i)
 _sig("arcz_engine_moe_slots", _i, _p)
+_sig("arcz_rope_create", _p, _p, _i, _p, _p, _i, _i, C.c_float)
+_sig("arcz_rope_free", _i, _p, _p)
+_sig("arcz_engine_rope", _i, _p, _p, _p, _i, _i, _p, _i, _i, _i, _i, _i, _p, _i)
+_sig("arcz_kv_create", _p, _p, _i, _i, _i, _i, _i, _p, _p, _p, _p)
+_sig("arcz_kv_free", _i, _p, _p)
+_sig("arcz_kv_buffer", _p, _p, _i)
+_sig("arcz_engine_kv_write", _i, _p, _p, _p, _p, _i, _i, _p, _i, _i)
+_sig("arcz_engine_kv_read", _i, _p, _p, _p, _p, _i, _i, _p, _i, _i)
+_sig("arcz_engine_attention", _i, _p, _p, _p, _p, _i, _i, _i, _p, _i, _i, _p)
 _sig("arcz_engine_self_check", _i)
 _sig("arcz_engine_profile", None, _p, _i)
 _sig("arcz_engine_profile_collect", _i, _p)
@@ -140,11 +151,14 @@ _sig("arcz_gen_weights", _i, _u32, _u64, _z, _i, C.c_float, _p)
 # converted faster), or through ctypes where it was not built for this interpreter.
 _quantize, _rmsnorm_quant, _swiglu_quant = lib.arcz_engine_quantize, lib.arcz_engine_rmsnorm_quant, lib.arcz_engine_swiglu_quant
 _matmul, _gemv_gu, _layer_moe = lib.arcz_engine_matmul, lib.arcz_engine_gemv_gu, lib.arcz_engine_layer_moe
+_rope, _kv_write, _kv_read, _attention = lib.arcz_engine_rope, lib.arcz_engine_kv_write, lib.arcz_engine_kv_read, lib.arcz_engine_attention
 try:
     from . import _pycall
     _pycall.bind(_quantize, _rmsnorm_quant, _swiglu_quant, _matmul, _gemv_gu, _layer_moe)
+    _pycall.bind_attn(_rope, _kv_write, _kv_read, _attention)
     from ._pycall import gemv_gu as _gemv_gu, layer_moe as _layer_moe, matmul as _matmul, quantize as _quantize
     from ._pycall import rmsnorm_quant as _rmsnorm_quant, swiglu_quant as _swiglu_quant
+    from ._pycall import attention as _attention, kv_read as _kv_read, kv_write as _kv_write, rope as _rope
 except ImportError:
     pass
 
@@ -356,6 +370,19 @@ class Runtime:
         return Runtime.alloc(max(a.nbytes, 1)).write(a)
 
     @staticmethod
+    def wrap(ptr, nbytes):
+        """A handle onto device memory that is the caller's (a tensor's data_ptr()); free() forgets it."""
+        h = lib.arcz_wrap(ptr, nbytes)
+        if not h:
+            raise ArczError(-50, lib.arcz_last_error().decode())
+        return Buffer(h, owner=False)
+
+    @staticmethod
+    def stream():
+        """The library's stream, as an address (torch.cuda.ExternalStream takes it)."""
+        return lib.arcz_stream()
+
+    @staticmethod
     def sync():
         _check(lib.arcz_sync())
 
@@ -463,6 +490,54 @@ class MoeLayer:
         if self.h:
             lib.arcz_moe_layer_free(self.eng.h, self.h)
             self.h = None
+
+
+class Rope:
+    """A rotation by positions (Engine.make_rope)."""
+
+    def __init__(self, eng, h):
+        self.eng, self.h = eng, h
+
+    def free(self):
+        if self.h:
+            _check(lib.arcz_rope_free(self.eng.h, self.h), engine=True)
+            self.h = None
+
+
+class KvCache:
+    """A cache of keys and values in 8 bits (Engine.make_kv)."""
+
+    def __init__(self, eng, h, pages, page, block, heads, hd):
+        self.eng, self.h, self.pages, self.page, self.block, self.heads, self.hd = eng, h, pages, page, block, heads, hd
+
+    def buffer(self, which):
+        """0 keys, 1 values (int8), 2 and 3 their scales (f32)."""
+        return Buffer(lib.arcz_kv_buffer(self.h, which), owner=False)
+
+    def free(self):
+        if self.h:
+            _check(lib.arcz_kv_free(self.eng.h, self.h), engine=True)
+            self.h = None
+
+
+class KvBatch(C.Structure):
+    """The sequences of a call on a cache (arcz_kv_batch): buffers of rows [seqs + 1], len [seqs] and table [seqs][ld_table], all int32."""
+    _fields_ = [("rows", _p), ("len", _p), ("table", _p), ("seqs", _i), ("ld_table", _i), ("T", _i), ("max_rows", _i), ("max_len", _i)]
+
+    def __init__(self, rows, len, table, seqs, ld_table, T, max_rows, max_len=0):
+        super().__init__(rows.h, len.h, table.h, seqs, ld_table, T, max_rows, max_len)
+        self.held = (rows, len, table)
+        self.at = C.addressof(self)
+
+
+class Attention(C.Structure):
+    """The form of an attention (arcz_attn): slopes f32 [heads], prefix int32 [seqs], first int32 [T], each a buffer or None."""
+    _fields_ = [("scale", C.c_float), ("cap", C.c_float), ("window", _i), ("slopes", _p), ("prefix", _p), ("first", _p)]
+
+    def __init__(self, scale, cap=0.0, window=0, slopes=None, prefix=None, first=None):
+        super().__init__(scale, cap, window, *(b.h if b else None for b in (slopes, prefix, first)))
+        self.held = (slopes, prefix, first)
+        self.at = C.addressof(self)
 
 
 class Engine:
@@ -611,6 +686,48 @@ class Engine:
     @property
     def moe_slots(self):
         return lib.arcz_engine_moe_slots(self.h)
+
+    def make_rope(self, freq, axis=None, neighbours=False, mscale=1.0):
+        """A rotation of len(freq) pairs, freq radians a position step each, on the axes that axis names (None: one)."""
+        f = np.ascontiguousarray(freq, dtype=np.float64)
+        a = None if axis is None else np.ascontiguousarray(axis, dtype=np.uint8)
+        if a is not None and a.size != f.size:
+            raise ValueError("make_rope: an axis for each pair")
+        h = lib.arcz_rope_create(self.h, f.size, _np_ptr(f), None if a is None else _np_ptr(a), 1 if a is None else int(a.max()) + 1, 1 if neighbours else 0, mscale)
+        if not h:
+            raise ArczError(-100, lib.arcz_engine_error().decode())
+        return Rope(self, h)
+
+    def rope(self, rope, x, ldx, x_off, y, ldy, y_off, T, heads, hd, pos, ld_pos=None):
+        """T rows of `heads` heads of x, turned by their positions (int32 [axes][ld_pos], ld_pos: T) into y (x itself: in place)."""
+        r = _rope(self.h, rope.h, x.h, ldx, x_off, y.h, ldy, y_off, T, heads, hd, pos.h, T if ld_pos is None else ld_pos)
+        if r:
+            _check(r, engine=True)
+
+    def make_kv(self, pages, page, block, heads, hd, k=None, v=None, ks=None, vs=None):
+        """An 8-bit cache of `pages` pages of `page` tokens, a scale for each `block` tokens and head; on the caller's buffers, or its own."""
+        h = lib.arcz_kv_create(self.h, pages, page, block, heads, hd, *(b.h if b else None for b in (k, v, ks, vs)))
+        if not h:
+            raise ArczError(-100, lib.arcz_engine_error().decode())
+        return KvCache(self, h, pages, page, block, heads, hd)
+
+    def kv_write(self, kv, batch, k, ldk, k_off, v, ldv, v_off):
+        """The batch's rows of k and v into the cache, quantized."""
+        r = _kv_write(self.h, kv.h, batch.at, k.h, ldk, k_off, v.h, ldv, v_off)
+        if r:
+            _check(r, engine=True)
+
+    def kv_read(self, kv, batch, k, ldk, k_off, v, ldv, v_off):
+        """The values that the cache holds for the batch's rows, as f32."""
+        r = _kv_read(self.h, kv.h, batch.at, k.h, ldk, k_off, v.h, ldv, v_off)
+        if r:
+            _check(r, engine=True)
+
+    def attention(self, kv, batch, q, ldq, q_off, heads, out, ldo, o_off, form):
+        """out = softmax(scores) v of the batch's rows of q over the cache; form: an Attention."""
+        r = _attention(self.h, kv.h, batch.at, q.h, ldq, q_off, heads, out.h, ldo, o_off, form.at)
+        if r:
+            _check(r, engine=True)
 
     def profile(self, on=True):
         lib.arcz_engine_profile(self.h, 1 if on else 0)

@@ -10,6 +10,8 @@
 struct arcz_engine { Engine* e; };
 struct arcz_weight { GpuWeight w; };
 struct arcz_moe_layer { Engine::MoeLayer L; };
+struct arcz_rope { Engine::Rope r; };
+struct arcz_kv { Engine::Kv c; };
 
 namespace {
 std::string g_err;
@@ -244,6 +246,60 @@ arcz_mem* arcz_engine_moe_buffer(arcz_engine* e, int which) {
   return which >= 0 && which < 13 ? b[which] : nullptr;
 }
 int arcz_engine_moe_slots(arcz_engine* e) { return e->e->slots_; }
+
+arcz_rope* arcz_rope_create(arcz_engine* e, int pairs, const double* freq, const uint8_t* axis, int axes, int neighbours, float mscale) {
+  arcz_rope* r = new arcz_rope;
+  if (guarded([&] { r->r = e->e->make_rope(pairs, freq, axis, axes, neighbours != 0, mscale); }) != ARCZ_OK) {
+    delete r;
+    return nullptr;
+  }
+  return r;
+}
+int arcz_rope_free(arcz_engine* e, arcz_rope* r) {
+  if (!r) return ARCZ_OK;
+  const int k = guarded([&] { e->e->release(r->r.tab); });
+  if (k == ARCZ_OK) delete r;
+  return k;
+}
+int arcz_engine_rope(arcz_engine* e, arcz_rope* r, arcz_mem* x, int ldx, int x_off, arcz_mem* y, int ldy, int y_off, int T, int heads, int hd, arcz_mem* pos, int ld_pos) {
+  return guarded([&] {
+    if (!r) throw std::runtime_error("rope: no rotation");
+    e->e->rope(r->r, x, ldx, x_off, y, ldy, y_off, T, heads, hd, pos, ld_pos);
+  });
+}
+arcz_kv* arcz_kv_create(arcz_engine* e, int pages, int page, int block, int heads, int hd, arcz_mem* k, arcz_mem* v, arcz_mem* ks, arcz_mem* vs) {
+  arcz_kv* c = new arcz_kv;
+  arcz_mem* const given[4] = {k, v, ks, vs};
+  if (guarded([&] { c->c = e->e->make_kv(pages, page, block, heads, hd, given); }) != ARCZ_OK) {
+    delete c;
+    return nullptr;
+  }
+  return c;
+}
+int arcz_kv_free(arcz_engine* e, arcz_kv* c) {
+  if (!c) return ARCZ_OK;
+  const int r = guarded([&] { e->e->free_kv(c->c); });
+  if (r == ARCZ_OK) delete c;
+  return r;
+}
+arcz_mem* arcz_kv_buffer(arcz_kv* c, int which) { return c && which >= 0 && which < 4 ? c->c.b[which] : nullptr; }
+static Engine::Batch batch_of(const char* what, const arcz_kv* c, const arcz_kv_batch* b) {
+  if (!c || !b) throw std::runtime_error(std::string(what) + (c ? ": no batch" : ": no cache"));
+  return {b->rows, b->len, b->table, b->seqs, b->ld_table, b->T, b->max_rows, b->max_len};
+}
+int arcz_engine_kv_write(arcz_engine* e, arcz_kv* c, const arcz_kv_batch* b, arcz_mem* k, int ldk, int k_off, arcz_mem* v, int ldv, int v_off) {
+  return guarded([&] { e->e->kv_write(c ? c->c : Engine::Kv(), batch_of("kv_write", c, b), k, ldk, k_off, v, ldv, v_off); });
+}
+int arcz_engine_kv_read(arcz_engine* e, arcz_kv* c, const arcz_kv_batch* b, arcz_mem* k, int ldk, int k_off, arcz_mem* v, int ldv, int v_off) {
+  return guarded([&] { e->e->kv_read(c ? c->c : Engine::Kv(), batch_of("kv_read", c, b), k, ldk, k_off, v, ldv, v_off); });
+}
+int arcz_engine_attention(arcz_engine* e, arcz_kv* c, const arcz_kv_batch* b, arcz_mem* q, int ldq, int q_off, int heads, arcz_mem* out, int ldo, int o_off,
+                          const arcz_attn* a) {
+  return guarded([&] {
+    if (!a) throw std::runtime_error("attention: no form");
+    e->e->attention(c ? c->c : Engine::Kv(), batch_of("attention", c, b), q, ldq, q_off, heads, out, ldo, o_off, {a->scale, a->cap, a->window, a->slopes, a->prefix, a->first});
+  });
+}
 
 int arcz_engine_self_check(void) {
   return guarded([&] {

@@ -106,7 +106,7 @@ extern "C" {
 
 // the code objects, linked in by kernel_blobs.S
 extern const unsigned char arcz_blob_ops[], arcz_blob_decode[], arcz_blob_decode_q80[], arcz_blob_decode_q40[], arcz_blob_decode_q4k[],
-    arcz_blob_decode_q5k[], arcz_blob_decode_q6k[], arcz_blob_decode_iq4xs[], arcz_blob_decode_iq3s[], arcz_blob_decode_iq4nl[], arcz_blob_decode_mxfp4[], arcz_blob_decode_q3k[], arcz_blob_decode_iq3xxs[], arcz_blob_decode_mm[], arcz_blob_gemm[], arcz_blob_gemm_d[], arcz_blob_moe_d[], arcz_blob_moe[];
+    arcz_blob_decode_q5k[], arcz_blob_decode_q6k[], arcz_blob_decode_iq4xs[], arcz_blob_decode_iq3s[], arcz_blob_decode_iq4nl[], arcz_blob_decode_mxfp4[], arcz_blob_decode_q3k[], arcz_blob_decode_iq3xxs[], arcz_blob_decode_mm[], arcz_blob_gemm[], arcz_blob_gemm_d[], arcz_blob_moe_d[], arcz_blob_moe[], arcz_blob_rope[], arcz_blob_kv[], arcz_blob_attn_few[], arcz_blob_attn_many[];
 
 static std::vector<const unsigned char*> blobs_of(const std::string& which);
 
@@ -135,7 +135,7 @@ int arcz_init(int device) {
   }
   R.scratch = new arcz_mem{(char*)sp, sb, false};
   R.mems.insert(R.scratch);
-  for (const char* w : {"ops", "decode", "gemm", "moe"}) {
+  for (const char* w : {"ops", "decode", "gemm", "moe", "attn"}) {
     std::vector<hipModule_t> mods;
     for (const unsigned char* blob : blobs_of(w)) {
       hipModule_t mod;
@@ -290,6 +290,25 @@ arcz_mem* arcz_view(arcz_mem* parent, size_t offset, size_t bytes) {
   return m;
 }
 
+arcz_mem* arcz_wrap(void* p, size_t bytes) {
+  if (!R.up) { fail(ARCZ_E_DEVICE, "arcz_wrap before arcz_init"); return nullptr; }
+  // (device memory of this GPU, whole: what the runtime says of the address, asked without leaving its error behind)
+  hipPointerAttribute_t at;
+  memset(&at, 0, sizeof at);
+  hipDeviceptr_t base = nullptr;
+  size_t size = 0;
+  if (!p || !bytes || hipPointerGetAttributes(&at, p) != hipSuccess || at.type != hipMemoryTypeDevice || at.device != R.device ||
+      hipMemGetAddressRange(&base, &size, (hipDeviceptr_t)p) != hipSuccess || (char*)p < (char*)base || bytes > size - (size_t)((char*)p - (char*)base)) {
+    (void)hipGetLastError();
+    fail(ARCZ_E_ARG_VALUE, "arcz_wrap of %zu bytes at %p: not inside one allocation of device %d", bytes, p, R.device);
+    return nullptr;
+  }
+  arcz_mem* m = new arcz_mem{(char*)p, bytes, false};
+  R.mems.insert(m);
+  return m;
+}
+void* arcz_stream(void) { return R.up ? (void*)R.stream : nullptr; }
+
 int arcz_free(arcz_mem* m) {
   if (!m) return ARCZ_OK;
   if (m == R.scratch) return fail(ARCZ_E_ARG_VALUE, "arcz_free of the library's static scratch");
@@ -334,7 +353,7 @@ size_t arcz_device_mem_free(void) {
 }
 int arcz_mem_listed(const arcz_mem* m) {
   if (!m || !R.mems.count(const_cast<arcz_mem*>(m))) return 0;
-  arcz_mem* o = m->owner ? const_cast<arcz_mem*>(m) : m->parent;
+  arcz_mem* o = m->owner ? const_cast<arcz_mem*>(m) : m->parent;  // (none: memory of the caller's, arcz_wrap)
   for (const arcz_list* l : R.lists)
     if (l->owners.count(o)) return 1;
   return 0;
@@ -411,7 +430,7 @@ int arcz_fill(arcz_mem* dst, const void* pattern, size_t ps, size_t offset, size
     HIP_TRY(hipModuleLaunchKernel(k->fn, blocks, 1, 1, 256, 1, 1, 0, R.stream, params, nullptr));
     if (R.recording) {  // (recorded as the kernel it is; nothing to wait for)
       ++R.rec_launches;
-      R.rec_owners.insert(dst->owner ? dst : dst->parent);
+      if (dst->owner || dst->parent) R.rec_owners.insert(dst->owner ? dst : dst->parent);
       return ARCZ_OK;
     }
   } else {
@@ -430,6 +449,7 @@ static std::vector<const unsigned char*> blobs_of(const std::string& which) {
   if (which == "decode") return {arcz_blob_decode, arcz_blob_decode_q80, arcz_blob_decode_q40, arcz_blob_decode_q4k, arcz_blob_decode_q5k, arcz_blob_decode_q6k, arcz_blob_decode_iq4xs, arcz_blob_decode_iq3s, arcz_blob_decode_iq4nl, arcz_blob_decode_mxfp4, arcz_blob_decode_q3k, arcz_blob_decode_iq3xxs, arcz_blob_decode_mm};
   if (which == "gemm") return {arcz_blob_gemm, arcz_blob_gemm_d, arcz_blob_moe_d};
   if (which == "moe") return {arcz_blob_moe};
+  if (which == "attn") return {arcz_blob_rope, arcz_blob_kv, arcz_blob_attn_few, arcz_blob_attn_many};
   return {};
 }
 
@@ -570,7 +590,7 @@ int arcz_launch(arcz_kernel* k, unsigned dim, const size_t* global, const size_t
         if (!R.mems.count(m))
           return fail(ARCZ_E_ARG_VALUE, "%s: argument %u is not a live buffer", k->symbol.c_str(), i);
         memcpy(store[i], &m->ptr, 8);
-        if (R.recording) R.rec_owners.insert(m->owner ? m : m->parent);
+        if (R.recording && (m->owner || m->parent)) R.rec_owners.insert(m->owner ? m : m->parent);
       }
     }
     params[i] = store[i];

@@ -1,0 +1,261 @@
+// The attention block between the q|k|v product and the output projection: rotary positions, the 8-bit cache, attention over it.
+// A part of class Engine (included in it).
+
+  // ---- rotary positions.  freq: radians a position step, one for each pair; kept as 64-bit fractions of a turn (kernels/rope.hip).
+  struct Rope {
+    int pairs = 0, axes = 1;
+    bool neighbours = false;
+    float mscale = 1.0f;
+    cl_mem tab = nullptr;
+  };
+  Rope make_rope(int pairs, const double* freq, const uint8_t* axis, int axes, bool neighbours, float mscale) {
+    if (pairs < 1 || pairs > 512 || !freq || axes < 1 || axes > 255)
+      throw std::runtime_error("make_rope: 1 to 512 pairs on 1 to 255 axes");
+    std::vector<uint64_t> tab(pairs + (pairs + 1) / 2, 0);
+    for (int i = 0; i < pairs; ++i) {
+      if (!std::isfinite(freq[i])) throw std::runtime_error("make_rope: frequency " + std::to_string(i) + " is no number");
+      if (axis && axis[i] >= axes) throw std::runtime_error("make_rope: pair " + std::to_string(i) + " on axis " + std::to_string(axis[i]) + " of " + std::to_string(axes));
+      const long double turns = (long double)freq[i] / 6.283185307179586476925286766559L, part = turns - floorl(turns);
+      const long double f = floorl(part * 18446744073709551616.0L + 0.5L);
+      tab[i] = f >= 18446744073709551616.0L ? 0 : (uint64_t)f;   // (a whole turn)
+      ((int*)&tab[pairs])[i] = axis ? axis[i] : 0;
+    }
+    Rope r;
+    r.pairs = pairs;
+    r.axes = axes;
+    r.neighbours = neighbours;
+    r.mscale = mscale;
+    r.tab = buf(tab.size() * 8, tab.data());
+    return r;
+  }
+
+  // Rows of a buffer that a call of this part reads or writes: T rows of `width` values from column `off` on, a row every ld.
+  struct Rows {
+    cl_mem m;
+    int ld, off, width, T;
+    uintptr_t begin() const { return (uintptr_t)arcz_mem_ptr(m) + (size_t)off * 4; }
+    uintptr_t end() const { return begin() + ((size_t)(T - 1) * ld + width) * 4; }
+    bool vec() const { return begin() % 16 == 0 && ld % 4 == 0; }
+  };
+  static Rows rows_of(const char* what, cl_mem m, int ld, int off, int width, int T) {
+    if (off < 0 || width <= 0 || ld < 0 || (int64_t)off + width > ld)
+      throw std::runtime_error(std::string(what) + ": columns " + std::to_string(off) + " ... of " + std::to_string(width) + " in rows of " + std::to_string(ld));
+    if (!m || (uintptr_t)arcz_mem_ptr(m) % 4 || arcz_mem_size(m) < ((size_t)(T - 1) * ld + (size_t)off + width) * 4)
+      throw std::runtime_error(std::string(what) + ": the buffer is too small for " + std::to_string(T) + " rows of " + std::to_string(ld));
+    return {m, ld, off, width, T};
+  }
+  // Whether two such sets of rows have a value in common (or may have: rows of different strides in one place).
+  static bool overlap(const Rows& a, const Rows& b) {
+    if (a.end() <= b.begin() || b.end() <= a.begin()) return false;
+    if (a.ld != b.ld || (a.begin() > b.begin() ? a.begin() - b.begin() : b.begin() - a.begin()) % 4) return true;
+    const size_t ld = (size_t)a.ld;
+    const size_t d = a.begin() <= b.begin() ? (b.begin() - a.begin()) / 4 % ld : (ld - (a.begin() - b.begin()) / 4 % ld) % ld;
+    return d < (size_t)a.width || d + (size_t)b.width > ld;
+  }
+  static bool overlap(const Rows& a, cl_mem m) {
+    const uintptr_t b = (uintptr_t)arcz_mem_ptr(m), e = b + arcz_mem_size(m);
+    return !(a.end() <= b || e <= a.begin());
+  }
+  static cl_mem ints(const char* what, cl_mem m, size_t n) {
+    if (!m || (uintptr_t)arcz_mem_ptr(m) % 4 || arcz_mem_size(m) < n * 4) throw std::runtime_error(std::string(what) + " holds less than " + std::to_string(n) + " values");
+    return m;
+  }
+
+  void rope(const Rope& r, cl_mem x, int ldx, int x_off, cl_mem y, int ldy, int y_off, int T, int heads, int hd, cl_mem pos, int ld_pos) {
+    if (!r.tab) throw std::runtime_error("rope: no rotation");
+    if (T == 0) return;
+    if (T < 0 || heads < 1 || hd < 1 || (int64_t)heads * hd > 0x7FFFFFFF || 2 * r.pairs > hd)
+      throw std::runtime_error("rope: " + std::to_string(heads) + " heads of " + std::to_string(hd) + " values, " + std::to_string(r.pairs) + " pairs");
+    const Rows a = rows_of("rope: x", x, ldx, x_off, heads * hd, T), b = rows_of("rope: y", y, ldy, y_off, heads * hd, T);
+    if (!(a.begin() == b.begin() && ldx == ldy) && overlap(a, b)) throw std::runtime_error("rope: x and y overlap (in place: the same columns of the same rows)");
+    if (ld_pos < T) throw std::runtime_error("rope: positions of " + std::to_string(T) + " rows on axes " + std::to_string(ld_pos) + " apart");
+    ints("rope: pos", pos, (size_t)(r.axes - 1) * ld_pos + T);
+    int vec = a.vec() && b.vec() && hd % 4 == 0, nb = r.neighbours, ax = r.axes, pairs = r.pairs;
+    float ms = r.mscale;
+    // (few tokens: a token's heads over several work-groups)
+    int per = T >= 256 ? heads : std::min(heads, 8);
+    cl_kernel k = variant("attn", {}, "rope");
+    set_args(k, 0, x, ldx, x_off, y, ldy, y_off, pos, ld_pos, r.tab, pairs, ax, nb, ms, heads, hd, per, vec);
+    size_t g[2] = {(size_t)T * 256, (size_t)((heads + per - 1) / per)}, l[2] = {256, 1};
+    run("rope", k, 2, g, l);
+  }
+
+  // ---- the cache
+  struct Kv {
+    int pages = 0, page = 0, block = 0, heads = 0, hd = 0, ps = 0, bs = 0;
+    cl_mem b[4] = {nullptr, nullptr, nullptr, nullptr};   // keys, values (int8), their scales (f32)
+    bool mine[4] = {false, false, false, false};
+  };
+  static int log2_of(int v) {
+    int n = 0;
+    while ((1 << n) < v) ++n;
+    return n;
+  }
+  Kv make_kv(int pages, int page, int block, int heads, int hd, const cl_mem* given) {
+    if (pages < 1 || heads < 1 || heads > 32767 || (hd != 64 && hd != 128 && hd != 256) || page < 16 || page > 256 || (page & (page - 1)) || block < 1 || block > page || (block & (block - 1)))
+      throw std::runtime_error("make_kv: " + std::to_string(pages) + " pages of " + std::to_string(page) + " tokens in blocks of " + std::to_string(block) + ", " +
+                               std::to_string(heads) + " heads of " + std::to_string(hd) +
+                               " (pages of 16, 32, 64, 128 or 256 tokens, blocks of a power of two up to the page, heads of 64, 128 or 256)");
+    Kv c;
+    c.pages = pages; c.page = page; c.block = block; c.heads = heads; c.hd = hd;
+    c.ps = log2_of(page);
+    c.bs = log2_of(block);
+    const size_t rows = (size_t)pages * heads * page, size[4] = {rows * hd, rows * hd, rows / block * 4, rows / block * 4};
+    for (int i = 0; i < 4; ++i) {
+      cl_mem m = given ? given[i] : nullptr;
+      if (!m) continue;
+      if (arcz_mem_size(m) < size[i] || (uintptr_t)arcz_mem_ptr(m) % (i < 2 ? 16 : 4))
+        throw std::runtime_error("make_kv: buffer " + std::to_string(i) + " holds " + std::to_string(arcz_mem_size(m)) + " bytes, the cache takes " + std::to_string(size[i]) +
+                                 " (the values' at an address of 16)");
+      for (int j = 0; j < i; ++j)
+        if (c.b[j]) {
+          const uintptr_t a = (uintptr_t)arcz_mem_ptr(m), b = (uintptr_t)arcz_mem_ptr(c.b[j]);
+          if (!(a + size[i] <= b || b + size[j] <= a)) throw std::runtime_error("make_kv: two of the buffers overlap");
+        }
+      c.b[i] = m;
+    }
+    try {
+      for (int i = 0; i < 4; ++i)
+        if (!c.b[i]) {
+          c.b[i] = buf(size[i]);
+          c.mine[i] = true;
+        }
+    } catch (...) {
+      for (int i = 0; i < 4; ++i)
+        if (c.mine[i]) release(c.b[i]);
+      throw;
+    }
+    return c;
+  }
+  void free_kv(Kv& c) {
+    for (int i = 0; i < 4; ++i)
+      if (c.mine[i]) not_listed(c.b[i], "free_kv");
+    for (int i = 0; i < 4; ++i)
+      if (c.mine[i] && c.b[i]) {
+        release(c.b[i]);
+        c.b[i] = nullptr;
+      }
+  }
+
+  struct Batch {
+    cl_mem rows, len, table;
+    int seqs, ld_table, T, max_rows, max_len;
+  };
+  // false: nothing to do
+  bool check_batch(const char* what, const Kv& c, const Batch& b) {
+    if (!c.b[0]) throw std::runtime_error(std::string(what) + ": no cache");
+    if (b.seqs < 0 || b.T < 0 || b.max_rows < 0 || b.ld_table < 0 || b.seqs > 65535)
+      throw std::runtime_error(std::string(what) + ": a batch of " + std::to_string(b.seqs) + " sequences, " + std::to_string(b.T) + " rows");
+    if (b.seqs == 0 || b.T == 0 || b.max_rows == 0) return false;
+    if (b.ld_table < 1 || (int64_t)b.ld_table * c.page > 0x7FFFF000)
+      throw std::runtime_error(std::string(what) + ": " + std::to_string(b.ld_table) + " pages of " + std::to_string(c.page) + " a sequence");
+    ints((std::string(what) + ": rows").c_str(), b.rows, (size_t)b.seqs + 1);
+    ints((std::string(what) + ": len").c_str(), b.len, (size_t)b.seqs);
+    ints((std::string(what) + ": table").c_str(), b.table, (size_t)b.seqs * b.ld_table);
+    return true;
+  }
+  void kv_write(const Kv& c, const Batch& b, cl_mem k, int ldk, int k_off, cl_mem v, int ldv, int v_off) {
+    if (!check_batch("kv_write", c, b)) return;
+    const int w = c.heads * c.hd, most = std::min(b.max_rows, b.T);
+    const Rows rk = rows_of("kv_write: k", k, ldk, k_off, w, b.T), rv = rows_of("kv_write: v", v, ldv, v_off, w, b.T);
+    for (cl_mem m : c.b)
+      if (overlap(rk, m) || overlap(rv, m)) throw std::runtime_error("kv_write: the rows overlap the cache");
+    int vec = rk.vec() && rv.vec(), pages = c.pages, heads = c.heads, ps = c.ps, bs = c.bs, ldt = b.ld_table, T = b.T, mr = b.max_rows;
+    // a work-group's tokens: whole blocks, and rows enough for its threads
+    int tile = std::max(c.block, most == 1 ? 1 : std::min(64, 1 << log2_of(most)));
+    cl_kernel kn = variant("attn", {{"HD", c.hd}}, "kv_write");
+    set_args(kn, 0, k, ldk, k_off, v, ldv, v_off, c.b[0], c.b[1], c.b[2], c.b[3], pages, heads, ps, bs, b.rows, b.len, b.table, ldt, T, mr, tile, vec);
+    size_t g[3] = {((size_t)(most - 1) / tile + 2) * 256, (size_t)b.seqs, (size_t)heads * 2}, l[3] = {256, 1, 1};
+    if (most == 1) g[0] = 256;
+    run("kv_write", kn, 3, g, l);
+  }
+  void kv_read(const Kv& c, const Batch& b, cl_mem k, int ldk, int k_off, cl_mem v, int ldv, int v_off) {
+    if (!check_batch("kv_read", c, b)) return;
+    const int w = c.heads * c.hd, most = std::min(b.max_rows, b.T);
+    const Rows rk = rows_of("kv_read: k", k, ldk, k_off, w, b.T), rv = rows_of("kv_read: v", v, ldv, v_off, w, b.T);
+    if (overlap(rk, rv)) throw std::runtime_error("kv_read: k and v overlap");
+    for (cl_mem m : c.b)
+      if (overlap(rk, m) || overlap(rv, m)) throw std::runtime_error("kv_read: the rows overlap the cache");
+    int vec = rk.vec() && rv.vec(), pages = c.pages, heads = c.heads, hd = c.hd, ps = c.ps, bs = c.bs, ldt = b.ld_table, T = b.T, mr = b.max_rows;
+    int per = std::max(1, 4096 / w);   // (four values a thread, four times)
+    cl_kernel kn = variant("attn", {}, "kv_read");
+    set_args(kn, 0, k, ldk, k_off, v, ldv, v_off, c.b[0], c.b[1], c.b[2], c.b[3], pages, heads, hd, ps, bs, b.rows, b.len, b.table, ldt, T, mr, per, vec);
+    size_t g[3] = {(size_t)((most + per - 1) / per) * 256, (size_t)b.seqs, 2}, l[3] = {256, 1, 1};
+    run("kv_read", kn, 3, g, l);
+  }
+
+  // ---- attention
+  struct Attn {
+    float scale, cap;
+    int window;
+    cl_mem slopes, prefix, first;
+  };
+  // pieces that the keys of few rows are shared out in; grown, never shrunk (a list may name an older one, which stays)
+  cl_mem at_ws_ = nullptr;
+  size_t at_ws_bytes_ = 0;
+  cl_mem at_ws(size_t bytes) {
+    if (bytes > at_ws_bytes_) {
+      cl_mem m = buf(bytes);
+      if (at_ws_ && !arcz_mem_listed(at_ws_)) release(at_ws_);
+      at_ws_ = m;
+      at_ws_bytes_ = bytes;
+    }
+    return at_ws_;
+  }
+  void attention(const Kv& c, const Batch& b, cl_mem q, int ldq, int q_off, int heads, cl_mem out, int ldo, int o_off, const Attn& a) {
+    if (!check_batch("attention", c, b)) return;
+    if (heads < 1 || heads % c.heads || (int64_t)heads * c.hd > 0x7FFFFFFF) throw std::runtime_error("attention: " + std::to_string(heads) + " heads over " + std::to_string(c.heads) + " of the cache");
+    if (!std::isfinite(a.scale) || !(a.cap >= 0.0f) || !std::isfinite(a.cap) || a.window < 0 || b.max_len < 0)
+      throw std::runtime_error("attention: scale, cap, window or max_len");
+    const Rows rq = rows_of("attention: q", q, ldq, q_off, heads * c.hd, b.T), ro = rows_of("attention: out", out, ldo, o_off, heads * c.hd, b.T);
+    if (overlap(rq, ro)) throw std::runtime_error("attention: q and out overlap");
+    for (cl_mem m : c.b)
+      if (overlap(ro, m)) throw std::runtime_error("attention: out overlaps the cache");
+    if (a.slopes) ints("attention: slopes", a.slopes, (size_t)heads);
+    if (a.prefix) ints("attention: prefix", a.prefix, (size_t)b.seqs);
+    if (a.first) ints("attention: first", a.first, (size_t)b.T);
+    const int G = heads / c.heads, most = std::min(b.max_rows, b.T);
+    const int64_t M = (int64_t)most * G;
+    if (M > 0x7FFFFF00) throw std::runtime_error("attention: too many rows");
+    const size_t pairs = (size_t)b.seqs * c.heads;
+    int pages = c.pages, ps = c.ps, bs = c.bs, ldt = b.ld_table, T = b.T, mr = most, kvh = c.heads, window = std::min(a.window, 1 << 30), nsplit = 1;
+    float scale = a.scale, cap2 = a.cap * 1.4426950408889634f;
+    const int form = (a.cap > 0.0f ? 1 : 0) | (a.slopes ? 2 : 0);
+    const int keys = std::max(1, std::min(b.max_len > 0 ? b.max_len : ldt * c.page, window ? (int)std::min<int64_t>((int64_t)most + window, 0x7FFFF000) : 0x7FFFF000));
+    int vec = rq.vec() ? 1 : 0;
+    if (ro.vec()) vec |= 2;
+    const size_t most_x = 0xFFFFFFFFull / 256;
+    if (M <= 32) {
+      const int rt = M > 16 ? 2 : 1, pack = M <= 8 ? 1 : 0, rows = pack ? 8 : 16 * rt;
+      // two work-groups a compute unit, of at least 256 keys each
+      nsplit = (int)std::max<size_t>(1, std::min<size_t>(((size_t)2 * arcz_device_cus() + pairs - 1) / pairs, (size_t)(keys + 255) / 256));
+      cl_mem w = nsplit > 1 ? at_ws(pairs * nsplit * rows * (c.hd + 2) * 4) : nullptr;
+      if (pairs > most_x) throw std::runtime_error("attention: too many sequences");
+      vec &= 1;
+      cl_kernel k = variant("attn", {{"HD", c.hd}, {"RT", rt}, {"PACK", pack}, {"FORM", form}}, "attn_few");
+      set_args(k, 0, q, ldq, q_off, c.b[0], c.b[1], c.b[2], c.b[3], pages, ps, bs, b.rows, b.len, b.table, ldt, T, mr, heads, kvh, out, ldo, o_off, scale, cap2, window,
+               a.slopes, a.prefix, a.first, w, nsplit, vec);
+      size_t g[2] = {pairs * 256, (size_t)nsplit}, l[2] = {256, 1};
+      run("attention", k, 2, g, l);
+      if (nsplit > 1) join(c, b, w, nsplit, rows, 1, (int)M, mr, heads, out, ldo, o_off);
+      return;
+    }
+    int tiles = (int)((M + 127) / 128);
+    if (pairs * tiles > most_x) throw std::runtime_error("attention: too many rows");
+    // rows that fill less than the chip: their keys shared out, at least 512 to a piece
+    nsplit = (int)std::max<size_t>(1, std::min<size_t>((size_t)2 * arcz_device_cus() / (pairs * tiles), (size_t)(keys + 511) / 512));
+    cl_mem w = nsplit > 1 ? at_ws(pairs * tiles * nsplit * 128 * (c.hd + 2) * 4) : nullptr;
+    cl_kernel k = variant("attn", {{"HD", c.hd}, {"FORM", form}}, "attn_many");
+    set_args(k, 0, q, ldq, q_off, c.b[0], c.b[1], c.b[2], c.b[3], pages, ps, bs, b.rows, b.len, b.table, ldt, T, mr, heads, kvh, out, ldo, o_off, scale, cap2, window,
+             a.slopes, a.prefix, a.first, w, nsplit, tiles, vec);
+    size_t g[2] = {pairs * tiles * 256, (size_t)nsplit}, l[2] = {256, 1};
+    run("attention", k, 2, g, l);
+    if (nsplit > 1) join(c, b, w, nsplit, 128, tiles, 128, mr, heads, out, ldo, o_off);
+  }
+  void join(const Kv& c, const Batch& b, cl_mem w, int nsplit, int rows, int blocks, int used, int mr, int heads, cl_mem out, int ldo, int o_off) {
+    int hd = c.hd, most_len = b.ld_table * c.page, T = b.T, kvh = c.heads, per = 256 / c.hd;
+    cl_kernel k = variant("attn", {}, "attn_join");
+    set_args(k, 0, w, nsplit, rows, blocks, hd, b.rows, b.len, most_len, T, mr, heads, kvh, out, ldo, o_off);
+    size_t g[2] = {(size_t)b.seqs * c.heads * blocks * 256, (size_t)((used + per - 1) / per)}, l[2] = {256, 1};
+    run("attention_join", k, 2, g, l);
+  }

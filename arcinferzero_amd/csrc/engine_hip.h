@@ -488,6 +488,8 @@ class Engine {
     chunk_is(K, Mp, T, Mp, 1);
   }
 
+#include "engine_attn.h"
+
   // ---- matmul (zero/engine.h:1080-1112): C[:, c_off : c_off+N] (+)= act * W^T for the current chunk.  acc: 0 = store,
   // 1 = accumulate into C, 2 = C = silu(C) * result (GEMM path only).  With two-pass inputs the residual's half goes
   // through the same kernels a second time and accumulates; for 1-4 tokens the GEMV takes both halves in one launch

@@ -26,4 +26,8 @@
     BLOB arcz_blob_gemm_d, "gemm_d.hsaco"
     BLOB arcz_blob_moe_d, "moe_d.hsaco"
     BLOB arcz_blob_moe, "moe.hsaco"
+    BLOB arcz_blob_rope, "rope.hsaco"
+    BLOB arcz_blob_kv, "kv.hsaco"
+    BLOB arcz_blob_attn_few, "attn_few.hsaco"
+    BLOB arcz_blob_attn_many, "attn_many.hsaco"
     .section .note.GNU-stack,"",@progbits

@@ -124,5 +124,12 @@ static const KernelSpec kKernelTable[] = {
     {"moe", "moe_scatter", nullptr, "ppipppp", {nullptr}, {{"NU", 0, true}, {"NE", 0, true}, {"NPART", 0, true}, {nullptr, 0, false}}, 512},
     {"moe", "moe_quant", nullptr, "piipp", {nullptr}, {{"FV", 1 << 30, false}, {nullptr, 0, false}}, 256},
     {"moe", "moe_quant_sums", nullptr, "piippp", {nullptr}, {{"FV", 1 << 30, false}, {nullptr, 0, false}}, 256},
+    // ---- attn (-DHD: the head's length; -DFORM: bit 0 scores capped, bit 1 a bias by distance)
+    {"attn", "rope", nullptr, "piipiipipiiifiiii", {nullptr}, {{nullptr, 0, false}}, 256},
+    {"attn", "kv_write", nullptr, "piipiippppiiiipppiiiii", {"HD", nullptr}, {{nullptr, 0, false}}, 256},
+    {"attn", "kv_read", nullptr, "piipiippppiiiiipppiiiii", {nullptr}, {{nullptr, 0, false}}, 256},
+    {"attn", "attn_few", nullptr, "piippppiiipppiiiiipiiffippppii", {"HD", "RT", "PACK", "FORM", nullptr}, {{nullptr, 0, false}}, 256},
+    {"attn", "attn_many", nullptr, "piippppiiipppiiiiipiiffippppiii", {"HD", "FORM", nullptr}, {{nullptr, 0, false}}, 256},
+    {"attn", "attn_join", nullptr, "piiiippiiiiipii", {nullptr}, {{nullptr, 0, false}}, 256},
     {"moe", "moe_combine", nullptr, "pppppi", {nullptr}, {{"NU", 0, true}, {nullptr, 0, false}}, 256},
 };

@@ -1,0 +1,115 @@
+// What the attention block's kernels share: a batch's sequences, the cache in pages, eight-bit values as f16.
+//
+// Batch: rows [rows[s], rows[s + 1]) of the row buffers are the newest positions of sequence s, of which len[s] are in the
+// cache with them; row i of the sequence has position len - n + i.  table[s][p >> log2(page)] is the page of position p.
+// Cache: values int8 [pages][heads][page][hd], a scale f32 for each block of tokens and head [pages][heads][page / block];
+// value = int8 * scale.  (A page's rows of one head are contiguous: what a work-group reads or writes is whole runs of 128
+// bytes and more, and a token is appended without moving another.)
+//
+// Everything that comes from device memory -- rows, lengths, pages -- is held to the buffers before it addresses anything: rows
+// to [0, T], lengths to the table, and a page outside the cache holds no tokens.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+struct Seq {
+  int r0;    // its first row
+  int n;     // its rows that this launch takes (at most max_rows)
+  int p0;    // the position of its first row (below 0 where len says less than the rows)
+  int len;
+};
+__device__ inline Seq seq_of(const int* __restrict__ rows, const int* __restrict__ lens, int s, int T, int max_rows, int most_len) {
+  Seq q;
+  q.r0 = min(max(rows[s], 0), T);
+  const int all = min(max(rows[s + 1], q.r0), T) - q.r0;
+  q.n = min(all, max_rows);
+  q.len = min(max(lens[s], 0), most_len);
+  q.p0 = q.len - all;
+  return q;
+}
+__device__ inline int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
+__device__ inline float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ inline uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) { return __builtin_amdgcn_perm(hi, lo, sel); }
+// Eight-bit values as f16, exactly: with the sign bit turned over a byte is v + 128, behind 0x64 it is the f16 1024 + 128 + v.
+__device__ inline h2 biased(uint32_t u) {
+  h2 h;
+  __builtin_memcpy(&h, &u, 4);
+  return h - h2{(_Float16)1152.0f, (_Float16)1152.0f};
+}
+__device__ inline void cvt4(uint32_t w, h2& a, h2& b) {
+  w ^= 0x80808080u;
+  a = biased(perm(0x64646464u, w, 0x04010400u));
+  b = biased(perm(0x64646464u, w, 0x04030402u));
+}
+__device__ inline h8 cvt8(uint32_t w0, uint32_t w1) {
+  h2 a, b, c, d;
+  cvt4(w0, a, b);
+  cvt4(w1, c, d);
+  return h8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+// Four values of each of four tokens, token-major, to pairs of tokens for each value: p[v][0] = tokens 0 and 1, p[v][1] = 2 and 3.
+__device__ inline void cvt4x4(uint32_t t0, uint32_t t1, uint32_t t2, uint32_t t3, h2 (&p)[4][2]) {
+  t0 ^= 0x80808080u; t1 ^= 0x80808080u; t2 ^= 0x80808080u; t3 ^= 0x80808080u;
+  const uint32_t a01 = perm(t1, t0, 0x05010400u), a23 = perm(t1, t0, 0x07030602u);
+  const uint32_t b01 = perm(t3, t2, 0x05010400u), b23 = perm(t3, t2, 0x07030602u);
+  p[0][0] = biased(perm(0x64646464u, a01, 0x04010400u));
+  p[1][0] = biased(perm(0x64646464u, a01, 0x04030402u));
+  p[2][0] = biased(perm(0x64646464u, a23, 0x04010400u));
+  p[3][0] = biased(perm(0x64646464u, a23, 0x04030402u));
+  p[0][1] = biased(perm(0x64646464u, b01, 0x04010400u));
+  p[1][1] = biased(perm(0x64646464u, b01, 0x04030402u));
+  p[2][1] = biased(perm(0x64646464u, b23, 0x04010400u));
+  p[3][1] = biased(perm(0x64646464u, b23, 0x04030402u));
+}
+// An f32 pair as two f16 pairs whose sum has 22 bits of it: the first truncated, the second what it misses.
+__device__ inline void split2(float a, float b, h2& hi, h2& lo) {
+  auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
+  const float ra = a - (float)h[0], rb = b - (float)h[1];
+  auto l = __builtin_amdgcn_cvt_pkrtz(ra, rb);
+  __builtin_memcpy(&hi, &h, 4);
+  __builtin_memcpy(&lo, &l, 4);
+}
+
+// ---- a score's form
+struct Form {
+  float cap2;    // cap * log2(e), 0: not capped
+  int window;    // 0: none
+};
+// x = scale * q.k * log2(e), or with a cap 2 * scale * q.k / cap * log2(e):  tanh(y) = 1 - 2 / (1 + e^(2 y))
+template <bool CAP>
+__device__ inline float capped(float x, float cap2) {
+  if (!CAP) return x;
+  return fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(1.0f + exp2_f(x)), cap2);
+}
+// The positions [lo, hi) that a row at position p sees.
+__device__ inline void sees(int p, int len, int window, int prefix, int first, int& lo, int& hi) {
+  hi = min(len, max(p + 1, prefix));
+  lo = max(first, 0);
+  if (window) lo = max(lo, p - window + 1);
+}
+
+// The scales' part in a score.  A weight is carried as w = p * vs (p = e^(s - reference), vs the scale of the token's values), as
+// 2^(s log2(e) + log2(vs) - reference): the product with the scale costs no instruction of its own, the weights stay within a
+// fixed range whatever the scales are, and the softmax's sum is the sum of w / vs.  A block of zeros (a scale below 2^-120) takes the
+// scale of a block before it instead -- its values are zeros whatever it is -- so that its weights are near the others'; a
+// scale that is no number makes the score none, and its weight nothing where it is masked.
+__device__ inline void value_scale(float vs, float& carry, float& lv, float& iv) {
+  if (vs >= 0x1p-120f || vs != vs) {
+    lv = __builtin_amdgcn_logf(vs);
+    iv = vs != vs ? 1.0f : 1.0f / vs;
+    if (vs == vs) carry = lv;
+  } else {
+    lv = carry;
+    iv = exp2_f(-carry);
+  }
+}
+// The weights' reference is lowered so that they are at most 2^8 when it is set; it is set anew once one would pass 2^15 (f16
+// ends at 2^16).  With the second f16 of the split a weight keeps an absolute error of 2^-25, 2^-33 of the largest.
+constexpr float SETS = 8.0f, PASSES = 15.0f;
+constexpr float NOTHING = -1e30f;   // the reference before the first visible score

@@ -1,0 +1,146 @@
+// "attn" module: rows of keys and values into the 8-bit cache, and back.
+//
+// A block of `block` tokens of one head shares a scale.  Where new rows fall into it:
+//   top = max |x| over its new rows;  d = max(d_old, top / 127), d_old only if the block holds older tokens;  i = 1 / d (0 below
+//   2^-120: such a block is zeros);  q = rte(x * i), held to +-127;  where d > d_old the older tokens' values become
+//   rte(q * (d_old * i)).
+// Each step is one f32 operation, so the stored bytes are defined to the last bit.  A row with an infinity or a NaN makes the
+// block's scale NaN: everything read from the block is NaN until a row is written at the block's first position again.
+//
+// Mapping: a work-group has a tile of whole blocks (tile tokens, a power of two) of one head of one sequence, so no two
+// work-groups touch a block and the result does not depend on their order.  hd / 4 threads take a row, four values each.
+// Bound: 4 bytes of HBM read and one written a value; the second look at the rows comes from the L2.
+#include "attn.h"
+
+template <int HD>
+__device__ inline void kv_write_body(const float* __restrict__ x, int ld, int off, int8_t* __restrict__ q, float* __restrict__ d, int pages, int heads, int ps,
+                                     int bs, const int* __restrict__ table, int ldt, const Seq& sq, int tile, int vec) {
+  constexpr int TPR = HD / 4, RPP = 256 / TPR;   // threads a row, rows a pass
+  __shared__ uint32_t top[256];
+  __shared__ float inv[256], ratio[256];
+  const int h = blockIdx.z >> 1, lane = threadIdx.x % TPR, r0 = threadIdx.x / TPR;
+  // (rows whose positions lie below 0 have no place)
+  const int from = max(sq.p0, 0), to = sq.p0 + sq.n;
+  const int t0 = (from & -tile) + blockIdx.x * tile, block = 1 << bs, nb = tile >> bs;
+  if (t0 >= to) return;
+  for (int b = threadIdx.x; b < nb; b += 256) top[b] = 0;
+  __syncthreads();
+  auto load = [&](int p) {
+    const float* s = x + (size_t)(sq.r0 + p - sq.p0) * ld + off + h * HD + lane * 4;
+    return vec ? *(const float4*)s : make_float4(s[0], s[1], s[2], s[3]);
+  };
+  // (sign off, the order of the words is that of the magnitudes, with infinity and NaN on top)
+  for (int r = r0; r < tile; r += RPP) {
+    const int p = t0 + r;
+    if (p < from || p >= to) continue;
+    const float4 v = load(p);
+    uint32_t m = max(max(__float_as_uint(v.x) & 0x7FFFFFFFu, __float_as_uint(v.y) & 0x7FFFFFFFu),
+                     max(__float_as_uint(v.z) & 0x7FFFFFFFu, __float_as_uint(v.w) & 0x7FFFFFFFu));
+#pragma unroll
+    for (int o = 1; o < TPR; o *= 2) m = max(m, (uint32_t)__shfl_xor((int)m, o));
+    if (lane == 0) atomicMax(&top[r >> bs], m);
+  }
+  __syncthreads();
+  const int old0 = from & -block;   // the first block's beginning: [old0, from) are older tokens
+  auto place = [&](int p, size_t& row) {   // of a position: false where its page is none
+    const int pg = table[p >> ps];
+    row = (size_t)pg * heads + h;
+    return (uint32_t)pg < (uint32_t)pages;
+  };
+  for (int b = threadIdx.x; b < nb; b += 256) {
+    const int p = t0 + (b << bs);
+    inv[b] = ratio[b] = 0.0f;
+    if (p + block <= from || p >= to) continue;
+    size_t row;
+    if (!place(p, row)) continue;
+    float* at = d + (row << (ps - bs)) + ((p & ((1 << ps) - 1)) >> bs);
+    const float now = top[b] >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float(top[b]) / 127.0f;
+    const float was = p < from ? *at : 0.0f;
+    const float s = was != was || now != now ? __uint_as_float(0x7FC00000u) : fmaxf(was, now);
+    const float i = s >= 0x1p-120f ? 1.0f / s : 0.0f;
+    inv[b] = i;
+    if (s > was && p < from) ratio[b] = was * i;
+    else ratio[b] = -1.0f;   // (nothing to do)
+    *at = s;
+  }
+  __syncthreads();
+  auto byte = [](float v) { return (uint32_t)(int)fminf(fmaxf(__builtin_rintf(v), -127.0f), 127.0f) & 255u; };
+  for (int r = r0; r < tile; r += RPP) {
+    const int p = t0 + r, b = r >> bs;
+    if (p >= to) break;
+    if (p < from) {   // an older token of the first block
+      const float f = ratio[b];
+      if (p < old0 || !(f >= 0.0f)) continue;
+      size_t row;
+      if (!place(p, row)) continue;
+      uint32_t* at = (uint32_t*)(q + ((row << ps) + (p & ((1 << ps) - 1))) * HD) + lane;
+      const uint32_t w = *at;
+      uint32_t o = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o |= byte((float)(int8_t)(w >> 8 * k) * f) << 8 * k;
+      *at = o;
+      continue;
+    }
+    size_t row;
+    if (!place(p, row)) continue;
+    const float4 v = load(p);
+    const float i = inv[b];
+    // (times 0 is a value's sign and zero; a block whose scale is NaN gets zeros)
+    const uint32_t w = i > 0.0f ? byte(v.x * i) | byte(v.y * i) << 8 | byte(v.z * i) << 16 | byte(v.w * i) << 24 : 0u;
+    ((uint32_t*)(q + ((row << ps) + (p & ((1 << ps) - 1))) * HD))[lane] = w;
+  }
+}
+
+// grid (tiles of the most rows, sequences, 2 heads): even z the keys, odd the values.
+template <int HD>
+__device__ inline void kv_write_any(const float* k, int ldk, int k_off, const float* v, int ldv, int v_off, int8_t* kq, int8_t* vq, float* ks, float* vs, int pages,
+                                    int heads, int ps, int bs, const int* rows, const int* lens, const int* table, int ldt, int T, int max_rows, int tile,
+                                    int vec) {
+  const int s = blockIdx.y;
+  const Seq sq = seq_of(rows, lens, s, T, max_rows, ldt << ps);
+  const bool second = blockIdx.z & 1;
+  kv_write_body<HD>(second ? v : k, second ? ldv : ldk, second ? v_off : k_off, second ? vq : kq, second ? vs : ks, pages, heads, ps, bs, table + (size_t)s * ldt, ldt, sq,
+                    tile, vec);
+}
+#define KV_WRITE(HD)                                                                                                                                          \
+  extern "C" __global__ __launch_bounds__(256) void kv_write__HD##HD(const float* k, int ldk, int k_off, const float* v, int ldv, int v_off, int8_t* kq,      \
+                                                                     int8_t* vq, float* ks, float* vs, int pages, int heads, int ps, int bs, const int* rows, \
+                                                                     const int* lens, const int* table, int ldt, int T, int max_rows, int tile, int vec) {    \
+    kv_write_any<HD>(k, ldk, k_off, v, ldv, v_off, kq, vq, ks, vs, pages, heads, ps, bs, rows, lens, table, ldt, T, max_rows, tile, vec);                     \
+  }
+KV_WRITE(64)
+KV_WRITE(128)
+KV_WRITE(256)
+
+// Back to f32: rows of positions len - n + i.  A page that is none reads as zeros.  grid (ceil(max_rows / per), sequences, 2), a
+// work-group `per` rows, a thread four values at a time.
+extern "C" __global__ __launch_bounds__(256) void kv_read(float* k, int ldk, int k_off, float* v, int ldv, int v_off, const int8_t* __restrict__ kq,
+                                                          const int8_t* __restrict__ vq, const float* __restrict__ ks, const float* __restrict__ vs, int pages, int heads,
+                                                          int hd, int ps, int bs, const int* __restrict__ rows, const int* __restrict__ lens,
+                                                          const int* __restrict__ table, int ldt, int T, int max_rows, int per, int vec) {
+  const int s = blockIdx.y, second = blockIdx.z;
+  const Seq sq = seq_of(rows, lens, s, T, max_rows, ldt << ps);
+  const int8_t* q = second ? vq : kq;
+  const float* d = second ? vs : ks;
+  float* out = second ? v : k;
+  const int ld = second ? ldv : ldk, off = second ? v_off : k_off, w = heads * hd / 4, mask = (1 << ps) - 1;
+  const int i0 = blockIdx.x * per, n = min(per, sq.n - i0);
+  for (int u = threadIdx.x; u < n * w; u += 256) {
+    const int i = u / w, c = u - i * w, p = sq.p0 + i0 + i, h = 4 * c / hd;
+    if (p < 0) continue;
+    const int pg = table[(size_t)s * ldt + (p >> ps)];
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if ((uint32_t)pg < (uint32_t)pages) {
+      const size_t row = (size_t)pg * heads + h;
+      const uint32_t b = *(const uint32_t*)(q + ((row << ps) + (p & mask)) * hd + (4 * c - h * hd));
+      const float f = d[(row << (ps - bs)) + ((p & mask) >> bs)];
+      o = make_float4((float)(int8_t)b * f, (float)(int8_t)(b >> 8) * f, (float)(int8_t)(b >> 16) * f, (float)(int8_t)(b >> 24) * f);
+    }
+    float* to = out + (size_t)(sq.r0 + i0 + i) * ld + off + 4 * c;
+    if (vec) {
+      *(float4*)to = o;
+    } else {
+      to[0] = o.x; to[1] = o.y; to[2] = o.z; to[3] = o.w;
+    }
+  }
+}

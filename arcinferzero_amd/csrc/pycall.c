@@ -35,7 +35,7 @@ static int plain(const char* fmt, PyObject* const* a, Py_ssize_t n, union arg* o
 #define CALL(NAME, FMT, EXPR)                                                        \
   static PyObject* NAME##_ctypes;                                                    \
   static PyObject* NAME(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {  \
-    union arg v[12];                                                                 \
+    union arg v[16];                                                                 \
     int r;                                                                           \
     (void)self;                                                                      \
     if (!plain(FMT, args, nargs, v)) return otherwise(NAME##_ctypes, args, nargs);   \
@@ -55,25 +55,40 @@ CALL(swiglu_quant, "ppiiiiii", arcz_engine_swiglu_quant(E, v[1].p, v[2].i, v[3].
 CALL(matmul, "pspipiiii", arcz_engine_matmul(E, v[1].s, v[2].p, v[3].i, v[4].p, v[5].i, v[6].i, v[7].i, v[8].i))
 CALL(gemv_gu, "pppip", arcz_engine_gemv_gu(E, v[1].p, v[2].p, v[3].i, v[4].p))
 CALL(layer_moe, "pppipii", arcz_engine_layer_moe(E, v[1].p, v[2].p, v[3].i, v[4].p, v[5].i, v[6].i))
+CALL(rope, "pppiipiiiiipi",
+     arcz_engine_rope(E, v[1].p, v[2].p, v[3].i, v[4].i, v[5].p, v[6].i, v[7].i, v[8].i, v[9].i, v[10].i, v[11].p, v[12].i))
+CALL(kv_write, "ppppiipii", arcz_engine_kv_write(E, v[1].p, v[2].p, v[3].p, v[4].i, v[5].i, v[6].p, v[7].i, v[8].i))
+CALL(kv_read, "ppppiipii", arcz_engine_kv_read(E, v[1].p, v[2].p, v[3].p, v[4].i, v[5].i, v[6].p, v[7].i, v[8].i))
+CALL(attention, "ppppiiipiip", arcz_engine_attention(E, v[1].p, v[2].p, v[3].p, v[4].i, v[5].i, v[6].i, v[7].p, v[8].i, v[9].i, v[10].p))
 
-/* bind(quantize, rmsnorm_quant, swiglu_quant, matmul, gemv_gu, layer_moe): the ctypes functions */
-static PyObject* bind(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
-  PyObject** const to[6] = {&quantize_ctypes, &rmsnorm_quant_ctypes, &swiglu_quant_ctypes, &matmul_ctypes, &gemv_gu_ctypes, &layer_moe_ctypes};
-  (void)self;
-  if (nargs != 6) {
-    PyErr_SetString(PyExc_TypeError, "bind takes the six functions");
+/* bind(quantize, rmsnorm_quant, swiglu_quant, matmul, gemv_gu, layer_moe) and bind_attn(rope, kv_write, kv_read, attention): the ctypes
+ * functions */
+static PyObject* bind_to(PyObject** const* to, int n, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != n) {
+    PyErr_Format(PyExc_TypeError, "bind takes the %d functions", n);
     return NULL;
   }
-  for (int i = 0; i < 6; ++i) {
+  for (int i = 0; i < n; ++i) {
     Py_INCREF(args[i]);
     Py_XSETREF(*to[i], args[i]);
   }
   Py_RETURN_NONE;
 }
+static PyObject* bind(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  PyObject** const to[6] = {&quantize_ctypes, &rmsnorm_quant_ctypes, &swiglu_quant_ctypes, &matmul_ctypes, &gemv_gu_ctypes, &layer_moe_ctypes};
+  (void)self;
+  return bind_to(to, 6, args, nargs);
+}
+static PyObject* bind_attn(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  PyObject** const to[4] = {&rope_ctypes, &kv_write_ctypes, &kv_read_ctypes, &attention_ctypes};
+  (void)self;
+  return bind_to(to, 4, args, nargs);
+}
 
 #define METHOD(NAME) {#NAME, (PyCFunction)(void (*)(void))NAME, METH_FASTCALL, NULL}
 static PyMethodDef methods[] = {METHOD(quantize), METHOD(rmsnorm_quant), METHOD(swiglu_quant), METHOD(matmul),
-                                METHOD(gemv_gu), METHOD(layer_moe), METHOD(bind), {NULL, NULL, 0, NULL}};
+                                METHOD(gemv_gu), METHOD(layer_moe), METHOD(rope), METHOD(kv_write), METHOD(kv_read),
+                                METHOD(attention), METHOD(bind), METHOD(bind_attn), {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pycall", NULL, -1, methods, NULL, NULL, NULL, NULL};
 
 PyMODINIT_FUNC PyInit__pycall(void) { return PyModule_Create(&module); }

@@ -165,6 +165,70 @@ int arcz_engine_moe_route(arcz_engine* e, arcz_moe_layer* L, arcz_mem* logits, i
 arcz_mem* arcz_engine_moe_buffer(arcz_engine* e, int which);
 int arcz_engine_moe_slots(arcz_engine* e);
 
+/* ---- The attention block between the q|k|v product and the output projection (the reference's kernels of this place are
+ * zero/kernels/ops_attn.cl, ops_attn_g.cl, attn_x.cl; these operators are this library's own).  All rows are f32, as the
+ * products leave them: a call names a buffer, the values from one row to the next (ld) and the first column (off), so the
+ * columns of one q|k|v buffer are taken as they lie.  Nothing here waits or, once a sequence has run, allocates: a pass records
+ * into a launch list, and what changes from pass to pass -- positions, lengths, pages -- comes from device buffers. */
+
+/* Rotary positions.  Pair i of a head is turned by pos[axis[i]][row] * freq[i] radians: (a, b) -> (a cos - b sin, a sin + b cos) *
+ * mscale; the pair is values (i, pairs + i) of the head, or with `neighbours` (2 i, 2 i + 1); values behind the pairs are copied.
+ * freq [pairs] (finite; kept to 2^-64 of a turn, so that far positions lose nothing); axis [pairs] (NULL: all 0), each below
+ * `axes`: one axis for text, three (time, height, width) for images and video, dealt out over the pairs as the model has it.
+ * pairs <= 512.  A rotation back is one by negative positions. */
+typedef struct arcz_rope arcz_rope;
+arcz_rope* arcz_rope_create(arcz_engine* e, int pairs, const double* freq, const uint8_t* axis, int axes, int neighbours, float mscale);
+int arcz_rope_free(arcz_engine* e, arcz_rope* r);
+/* T rows of `heads` heads of hd values (2 pairs <= hd) of x, turned into y: the same columns of the same rows (in place), or
+ * columns that do not meet them.  pos int32 [axes][ld_pos], ld_pos >= T; any int32 is a position. */
+int arcz_engine_rope(arcz_engine* e, arcz_rope* r, arcz_mem* x, int ldx, int x_off, arcz_mem* y, int ldy, int y_off, int T, int heads, int hd, arcz_mem* pos, int ld_pos);
+
+/* A cache of keys and values in 8 bits: `pages` pages of `page` tokens (16, 32, 64, 128 or 256), `heads` heads of hd values (64, 128
+ * or 256), one f32 scale for each block of `block` tokens (a power of two, 1 to page) and head.  k, v: int8 [pages][heads][page][hd];
+ * ks, vs: f32 [pages][heads][page / block]; value = int8 * scale.  Each buffer is the caller's (kept until arcz_kv_free; k and v
+ * at addresses of 16 bytes) or, where NULL, the library's (arcz_kv_buffer).  A scale below
+ * 2^-120 (or below 0) belongs to a block whose values are all zero, as kv_write stores it. */
+typedef struct arcz_kv arcz_kv;
+arcz_kv* arcz_kv_create(arcz_engine* e, int pages, int page, int block, int heads, int hd, arcz_mem* k, arcz_mem* v, arcz_mem* ks, arcz_mem* vs);
+/* Frees the handle and the library's buffers; refused, with everything as it was, while a launch list names them. */
+int arcz_kv_free(arcz_engine* e, arcz_kv* c);
+arcz_mem* arcz_kv_buffer(arcz_kv* c, int which); /* 0 k, 1 v, 2 ks, 3 vs */
+/* The sequences of a call.  Rows [rows[s], rows[s + 1]) of the row buffers belong to sequence s (rows: int32 [seqs + 1], from 0 on,
+ * not falling); len[s] (int32) keys of it are in the cache, those of these rows with them, so its i-th row of n has position
+ * len - n + i (rows whose position is below 0 are left out).  table [seqs][ld_table] (int32): page of its positions page * i and
+ * on.  T: rows of the buffers; max_rows: the most rows of one sequence (those past it are left out); max_len: about the most
+ * keys of one, for sharing out the work (0: as many as the table holds).  rows, len and table are read when the launch runs and
+ * held to the buffers there: rows to [0, T], len to the table, and a page outside the cache is one without tokens -- nothing is
+ * written to it, its keys are not seen, it reads as zeros.  Rows of the buffers that belong to no sequence are left as they are. */
+typedef struct arcz_kv_batch {
+  arcz_mem *rows, *len, *table;
+  int seqs, ld_table, T, max_rows, max_len;
+} arcz_kv_batch;
+/* The batch's rows of k and v (T rows of heads * hd values each) into the cache, in one launch.  A block's scale is what its largest
+ * value needs, max |x| / 127; where older tokens share the block and the new ones are larger, the older values are brought to
+ * the new scale (rounded again), where they are smaller the scale stays.  Values are rounded to nearest even.  A row with an
+ * infinity or a NaN makes its blocks' scales NaN: they read as NaN until a row is written at their first position again.  No
+ * two sequences of a call may have a page that both write (a shared prefix ends on a page, or its last page is copied first). */
+int arcz_engine_kv_write(arcz_engine* e, arcz_kv* c, const arcz_kv_batch* b, arcz_mem* k, int ldk, int k_off, arcz_mem* v, int ldv, int v_off);
+/* ... and back: the values that the cache holds for the batch's rows. */
+int arcz_engine_kv_read(arcz_engine* e, arcz_kv* c, const arcz_kv_batch* b, arcz_mem* k, int ldk, int k_off, arcz_mem* v, int ldv, int v_off);
+
+/* A row at position p sees key j < len iff  j >= first[row],  j <= p or j < prefix[s],  and, with a window > 0, p - j < window.  Its score
+ * is scale * q.k, with cap > 0 cap * tanh(that / cap), then minus slopes[head] * |p - j|. */
+typedef struct arcz_attn {
+  float scale, cap;           /* cap 0: none */
+  int window;                 /* 0: none */
+  arcz_mem *slopes;           /* f32 [heads], NULL: no bias by distance */
+  arcz_mem *prefix;           /* int32 [seqs], NULL: causal */
+  arcz_mem *first;            /* int32 [T]: where the document of a row begins, NULL: 0 */
+} arcz_attn;
+/* out = softmax(scores) v for T rows of `heads` query heads (a multiple of the cache's; query head h takes the cache's head
+ * h / (heads / cache heads)): prompts, chunks behind a context, drafts and single tokens, mixed as they come.  A row that sees
+ * nothing gives zeros; what is masked has no effect, whatever the cache holds there.  out must not meet q or the cache.  Sums are
+ * those of f32 rows against the cache's values to about 2^-22; the same call gives the same bits. */
+int arcz_engine_attention(arcz_engine* e, arcz_kv* c, const arcz_kv_batch* b, arcz_mem* q, int ldq, int q_off, int heads, arcz_mem* out, int ldo, int o_off,
+                          const arcz_attn* a);
+
 /* The start-up check of the tuned GEMMs of 128 tokens and of the GEMM on digits against the simple one on the reference's
  * LCG data, both against integer sums counted on the host (the pattern of xmx_check, zero/engine_setup.h:424-520): the
  * weight types that make unit-scale blocks, the three accumulate modes, K in one piece and in several.  0, or ARCZ_E_ENGINE with the first

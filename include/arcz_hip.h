@@ -54,6 +54,14 @@ arcz_mem* arcz_alloc(size_t bytes);
 arcz_mem* arcz_alloc_if_free(size_t bytes);
 /* clCreateSubBuffer (clrt.h:752-762): a non-owning view; NULL if it would pass the parent's end. */
 arcz_mem* arcz_view(arcz_mem* parent, size_t offset, size_t bytes);
+/* A handle onto device memory that is the caller's -- another allocator's of the same process and GPU, a framework's tensor --
+ * [p, p + bytes) inside one allocation; NULL + error text otherwise (host memory, another GPU, past the allocation's end).  The
+ * memory stays the caller's: arcz_free forgets the handle, and the caller keeps it allocated for as long as the handle, a view
+ * of it or a recorded list that names it is used.  Calls on it run on the library's stream, like all others: it is ordered with
+ * the GPU's default (null) stream in both directions; work of other streams is ordered by their owner (arcz_stream). */
+arcz_mem* arcz_wrap(void* p, size_t bytes);
+/* The library's stream (a hipStream_t), for events that order another stream's work with it; NULL before arcz_init. */
+void* arcz_stream(void);
 /* clReleaseMemObject (clrt.h:763-769): waits for the stream, then frees (an owner) or forgets (a view).  The
  * caller frees views before their parents (zero/engine.h:251-252): an owner that still has live views is refused
  * (ARCZ_E_ARG_VALUE, nothing freed). */
@@ -89,7 +97,7 @@ void* arcz_host_alloc(size_t bytes);
 int arcz_host_free(void* p);
 
 /* Engine::kernel(which, defs, name) (zero/engine_setup.h:317-362) over ClRt::build + ClRt::kernel
- * (clrt.h:1189-1307): `which` names the module ("ops", "decode", "gemm", "moe"), `defs` is the reference's -D string
+ * (clrt.h:1189-1307): `which` names the module ("ops", "decode", "gemm", "moe", "attn"), `defs` is the reference's -D string
  * and `name` the kernel.  The reference compiles one program per -D string at run time; here every variant is
  * compiled ahead of time: the -D names a kernel is specialized on select the variant, the rest become trailing
  * integer arguments the launch appends, and options that are not -D are ignored.  NULL + error text if there is no
