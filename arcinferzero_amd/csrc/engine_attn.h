@@ -190,9 +190,11 @@
     int window;
     cl_mem slopes, prefix, first;
   };
-  // pieces that the keys of few rows are shared out in; grown, never shrunk (a list may name an older one, which stays)
-  cl_mem at_ws_ = nullptr;
-  size_t at_ws_bytes_ = 0;
+  // Room for the pieces that the keys of few rows are shared out in, and the counts of those that are written (zeros between
+  // launches); grown, never shrunk.  A launch list keeps the room that it was recorded with: all launches are in one stream's
+  // order, so lists and calls that use the same room do not meet there.
+  cl_mem at_ws_ = nullptr, at_counts_ = nullptr;
+  size_t at_ws_bytes_ = 0, at_counts_n_ = 0;
   cl_mem at_ws(size_t bytes) {
     if (bytes > at_ws_bytes_) {
       cl_mem m = buf(bytes);
@@ -201,6 +203,21 @@
       at_ws_bytes_ = bytes;
     }
     return at_ws_;
+  }
+  cl_mem at_counts(size_t n) {
+    if (n > at_counts_n_) {
+      n = std::max<size_t>(n, 1024);
+      cl_mem m = buf(n * 4);
+      const uint32_t zero = 0;
+      if (arcz_fill(m, &zero, 4, 0, n * 4) != 0) {
+        release(m);
+        throw std::runtime_error("attention: the counts are not cleared");
+      }
+      if (at_counts_ && !arcz_mem_listed(at_counts_)) release(at_counts_);
+      at_counts_ = m;
+      at_counts_n_ = n;
+    }
+    return at_counts_;
   }
   void attention(const Kv& c, const Batch& b, cl_mem q, int ldq, int q_off, int heads, cl_mem out, int ldo, int o_off, const Attn& a) {
     if (!check_batch("attention", c, b)) return;
@@ -225,19 +242,21 @@
     int vec = rq.vec() ? 1 : 0;
     if (ro.vec()) vec |= 2;
     const size_t most_x = 0xFFFFFFFFull / 256;
-    if (M <= 32) {
+    if (M <= (c.hd == 256 ? 16 : 32)) {
       const int rt = M > 16 ? 2 : 1, pack = M <= 8 ? 1 : 0, rows = pack ? 8 : 16 * rt;
-      // two work-groups a compute unit, of at least 256 keys each
-      nsplit = (int)std::max<size_t>(1, std::min<size_t>(((size_t)2 * arcz_device_cus() + pairs - 1) / pairs, (size_t)(keys + 255) / 256));
-      cl_mem w = nsplit > 1 ? at_ws(pairs * nsplit * rows * (c.hd + 2) * 4) : nullptr;
+      // Pieces of one length for all sequences, so that long ones are more work-groups, not longer ones: two work-groups a
+      // compute unit if every sequence has the most keys, of at least 256 keys each.
+      const size_t want = ((size_t)2 * arcz_device_cus() + pairs - 1) / pairs;
+      int least = (int)std::max<size_t>(8, ((size_t)(keys + 31) / 32 + want - 1) / want);
+      nsplit = (keys + 32 * least - 1) / (32 * least);
+      cl_mem w = nsplit > 1 ? at_ws(pairs * nsplit * rows * (c.hd + 2) * 4) : nullptr, counts = nsplit > 1 ? at_counts(pairs) : nullptr;
       if (pairs > most_x) throw std::runtime_error("attention: too many sequences");
       vec &= 1;
-      cl_kernel k = variant("attn", {{"HD", c.hd}, {"RT", rt}, {"PACK", pack}, {"FORM", form}}, "attn_few");
+      cl_kernel k = variant("attn", {{"HD", c.hd}, {"RT", rt}, {"PACK", pack}, {"FINE", c.block < 4 ? 1 : 0}, {"FORM", form}}, "attn_few");
       set_args(k, 0, q, ldq, q_off, c.b[0], c.b[1], c.b[2], c.b[3], pages, ps, bs, b.rows, b.len, b.table, ldt, T, mr, heads, kvh, out, ldo, o_off, scale, cap2, window,
-               a.slopes, a.prefix, a.first, w, nsplit, vec);
+               a.slopes, a.prefix, a.first, w, counts, nsplit, least, vec);
       size_t g[2] = {pairs * 256, (size_t)nsplit}, l[2] = {256, 1};
       run("attention", k, 2, g, l);
-      if (nsplit > 1) join(c, b, w, nsplit, rows, 1, (int)M, mr, heads, out, ldo, o_off);
       return;
     }
     int tiles = (int)((M + 127) / 128);
@@ -250,12 +269,12 @@
              a.slopes, a.prefix, a.first, w, nsplit, tiles, vec);
     size_t g[2] = {pairs * tiles * 256, (size_t)nsplit}, l[2] = {256, 1};
     run("attention", k, 2, g, l);
-    if (nsplit > 1) join(c, b, w, nsplit, 128, tiles, 128, mr, heads, out, ldo, o_off);
+    if (nsplit > 1) join(c, b, w, nsplit, 128, tiles, mr, heads, out, ldo, o_off);
   }
-  void join(const Kv& c, const Batch& b, cl_mem w, int nsplit, int rows, int blocks, int used, int mr, int heads, cl_mem out, int ldo, int o_off) {
-    int hd = c.hd, most_len = b.ld_table * c.page, T = b.T, kvh = c.heads, per = 256 / c.hd;
+  void join(const Kv& c, const Batch& b, cl_mem w, int nsplit, int rows, int blocks, int mr, int heads, cl_mem out, int ldo, int o_off) {
+    int hd = c.hd, most_len = b.ld_table * c.page, T = b.T, kvh = c.heads, per = 1024 / c.hd;
     cl_kernel k = variant("attn", {}, "attn_join");
     set_args(k, 0, w, nsplit, rows, blocks, hd, b.rows, b.len, most_len, T, mr, heads, kvh, out, ldo, o_off);
-    size_t g[2] = {(size_t)b.seqs * c.heads * blocks * 256, (size_t)((used + per - 1) / per)}, l[2] = {256, 1};
+    size_t g[2] = {(size_t)b.seqs * c.heads * blocks * 256, (size_t)((rows + per - 1) / per)}, l[2] = {256, 1};
     run("attention_join", k, 2, g, l);
   }

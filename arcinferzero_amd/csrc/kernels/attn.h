@@ -15,6 +15,8 @@
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 
 struct Seq {
@@ -76,6 +78,44 @@ __device__ inline void split2(float a, float b, h2& hi, h2& lo) {
   __builtin_memcpy(&lo, &l, 4);
 }
 
+// ---- pieces that work-groups on other XCDs, with L2s of their own, write and read within one launch: stores that go through to
+// memory (agent scope), waited for; a count of the work-groups that have come so far; loads past the
+// caches.  Nothing else of a work-group's stores is read by another, so the L2s need not be written back or emptied (fences of
+// agent scope, which do that, took 40 us of a launch of 512 work-groups that streams 270 MB).
+struct Shared {
+  __amdgpu_buffer_rsrc_t at;
+  __device__ explicit Shared(float* p) : at(__builtin_amdgcn_make_buffer_rsrc(p, 0, -1, 0x00027000)) {}
+  // (offsets in floats; 16: the agent's scope)
+  __device__ void put4(int i, float4 v) const {
+    u4 u;
+    __builtin_memcpy(&u, &v, 16);
+    __builtin_amdgcn_raw_buffer_store_b128(u, at, i * 4, 0, 16);
+  }
+  __device__ void put2(int i, float a, float b) const { __builtin_amdgcn_raw_buffer_store_b64(u2{__float_as_uint(a), __float_as_uint(b)}, at, i * 4, 0, 16); }
+  __device__ float4 get4(int i) const {
+    const u4 u = __builtin_amdgcn_raw_buffer_load_b128(at, i * 4, 0, 16);
+    return make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
+  }
+  __device__ float2 get2(int i) const {
+    const u2 u = __builtin_amdgcn_raw_buffer_load_b64(at, i * 4, 0, 16);
+    return make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+  }
+};
+// True in the work-group that is the last of n to come here; the count is 0 again behind it.
+__device__ inline bool last_of(unsigned* count, unsigned n) {
+  __shared__ unsigned seen;
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  __builtin_amdgcn_s_waitcnt(0);   // (this wave's stores have reached memory)
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    seen = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (seen == n - 1) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  return seen == n - 1;
+}
+
 // ---- a score's form
 struct Form {
   float cap2;    // cap * log2(e), 0: not capped
@@ -100,14 +140,11 @@ __device__ inline void sees(int p, int len, int window, int prefix, int first, i
 // scale of a block before it instead -- its values are zeros whatever it is -- so that its weights are near the others'; a
 // scale that is no number makes the score none, and its weight nothing where it is masked.
 __device__ inline void value_scale(float vs, float& carry, float& lv, float& iv) {
-  if (vs >= 0x1p-120f || vs != vs) {
-    lv = __builtin_amdgcn_logf(vs);
-    iv = vs != vs ? 1.0f : 1.0f / vs;
-    if (vs == vs) carry = lv;
-  } else {
-    lv = carry;
-    iv = exp2_f(-carry);
-  }
+  const bool number = vs == vs;
+  const float l = __builtin_amdgcn_logf(vs), r = __builtin_amdgcn_rcpf(vs);
+  carry = vs >= 0x1p-120f ? l : carry;
+  lv = number ? carry : vs;
+  iv = vs >= 0x1p-120f ? r : number ? exp2_f(-carry) : 1.0f;
 }
 // The weights' reference is lowered so that they are at most 2^8 when it is set; it is set anew once one would pass 2^15 (f16
 // ends at 2^16).  With the second f16 of the split a weight keeps an absolute error of 2^-25, 2^-33 of the largest.

@@ -281,8 +281,8 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
         *(float4*)at = make_float4(acc[d][4 * b], acc[d][4 * b + 1], acc[d][4 * b + 2], acc[d][4 * b + 3]);
       }
     if (hf == 0) {
-      to[BM * HD + row] = ref;
-      to[BM * HD + BM + row] = sum;
+      to[BM * HD + 2 * row] = ref;
+      to[BM * HD + 2 * row + 1] = sum;
     }
   }
 }
