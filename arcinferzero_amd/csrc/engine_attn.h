@@ -264,7 +264,7 @@
     // rows that fill less than the chip: their keys shared out, at least 512 to a piece
     nsplit = (int)std::max<size_t>(1, std::min<size_t>((size_t)2 * arcz_device_cus() / (pairs * tiles), (size_t)(keys + 511) / 512));
     cl_mem w = nsplit > 1 ? at_ws(pairs * tiles * nsplit * 128 * (c.hd + 2) * 4) : nullptr;
-    cl_kernel k = variant("attn", {{"HD", c.hd}, {"FORM", form}}, "attn_many");
+    cl_kernel k = variant("attn", {{"HD", c.hd}, {"FINE", c.block < 32 ? 1 : 0}, {"FORM", form}}, "attn_many");
     set_args(k, 0, q, ldq, q_off, c.b[0], c.b[1], c.b[2], c.b[3], pages, ps, bs, b.rows, b.len, b.table, ldt, T, mr, heads, kvh, out, ldo, o_off, scale, cap2, window,
              a.slopes, a.prefix, a.first, w, nsplit, tiles, vec);
     size_t g[2] = {pairs * tiles * 256, (size_t)nsplit}, l[2] = {256, 1};

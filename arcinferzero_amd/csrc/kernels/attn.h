@@ -69,10 +69,16 @@ __device__ inline void cvt4x4(uint32_t t0, uint32_t t1, uint32_t t2, uint32_t t3
   p[2][1] = biased(perm(0x64646464u, b23, 0x04010400u));
   p[3][1] = biased(perm(0x64646464u, b23, 0x04030402u));
 }
-// An f32 pair as two f16 pairs whose sum has 22 bits of it: the first truncated, the second what it misses.
-__device__ inline void split2(float a, float b, h2& hi, h2& lo) {
+// An f32 pair as two f16 pairs whose sum has 22 bits of it: the first truncated, the second what it misses.  `one` is 1.0 that the
+// compiler does not know (opaque_one): the difference is then one instruction that takes the f16 as it is, not two.
+__device__ inline float opaque_one() {
+  float one;
+  asm("v_mov_b32 %0, 1.0" : "=v"(one));
+  return one;
+}
+__device__ inline void split2(float a, float b, float one, h2& hi, h2& lo) {
   auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
-  const float ra = a - (float)h[0], rb = b - (float)h[1];
+  const float ra = fmaf(a, one, -(float)h[0]), rb = fmaf(b, one, -(float)h[1]);
   auto l = __builtin_amdgcn_cvt_pkrtz(ra, rb);
   __builtin_memcpy(&hi, &h, 4);
   __builtin_memcpy(&lo, &l, 4);

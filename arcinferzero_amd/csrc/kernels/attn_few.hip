@@ -118,6 +118,7 @@ __device__ inline void few_body(const float* __restrict__ q, int ldq, int q_off,
   }
 
   // ---- the rows in two f16 parts each, times 2^e (a row's largest value to 2^10 ... 2^11), while the first keys come
+  const float one = opaque_one();
   float slope[RT], kfac[RT];
   h8 qh[RT][KS], ql[RT][PACK ? 1 : KS];
 #pragma unroll
@@ -154,7 +155,7 @@ __device__ inline void few_body(const float* __restrict__ q, int ldq, int q_off,
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         h2 u, w;
-        split2(x[k][e] * up, x[k][e + 1] * up, u, w);
+        split2(x[k][e] * up, x[k][e + 1] * up, one, u, w);
         a[e] = u.x; a[e + 1] = u.y; b[e] = w.x; b[e + 1] = w.y;
       }
       if (PACK) {
@@ -249,7 +250,7 @@ __device__ inline void few_body(const float* __restrict__ q, int ldq, int q_off,
         sum[t] = fmaf(a, iv[e], sum[t]);
         sum[t] = fmaf(b, iv[e + 1], sum[t]);
         h2 u, w;
-        split2(a, b, u, w);
+        split2(a, b, one, u, w);
         if (PACK) {
           const h2 c = m < 8 ? u : w;
           ph[t][e] = c.x; ph[t][e + 1] = c.y;

@@ -14,7 +14,7 @@
 // the matrix pipe does twice the products of plain f16 rows; it is what bounds the kernel.
 #include "attn.h"
 
-template <int HD, int KT, bool CAP, bool BIAS>
+template <int HD, int KT, bool FINE, bool CAP, bool BIAS>
 __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off, const int8_t* __restrict__ kq, const int8_t* __restrict__ vq,
                                  const float* __restrict__ ks, const float* __restrict__ vs, int pages, int ps, int bs, const int* __restrict__ rows,
                                  const int* __restrict__ lens, const int* __restrict__ table, int ldt, int T, int max_rows, int heads, int kvh,
@@ -26,7 +26,9 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   constexpr int KLD = HD + 8, VLD = KT + 8;             // (rows 16 bytes longer: neighbouring rows four banks on)
   constexpr float LOG2E = 1.4426950408889634f;
   __shared__ _Float16 sk[2][KT * KLD], sv[2][HD * VLD];
-  __shared__ float skf[2][KT], slv[2][KT], siv[2][KT];
+  // scales: of each key, or of each 32 keys that share one (kf: the score's factor; lv, iv: value_scale)
+  constexpr int NS = FINE ? KT : NT;
+  __shared__ float skf[2][NS], slv[2][NS], siv[2][NS];
   __shared__ int red[4][3];
 
   const int sh = blockIdx.x / tiles, tile = tiles - 1 - (blockIdx.x - sh * tiles), s = sh / kvh, h = sh - s * kvh, G = heads / kvh;
@@ -89,13 +91,14 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   const int e2 = min(max(137 - (int)(big >> 23), -100), 100);   // (the largest of the work-group's rows to 2^10 ... 2^11)
   const float up = __uint_as_float((uint32_t)(127 + e2) << 23), down = __uint_as_float((uint32_t)(127 - e2) << 23);
   const float kfac = (CAP ? 2.0f * LOG2E * LOG2E / cap2 : LOG2E) * scale * down;   // (cap2 = cap log2 e)
+  const float one = opaque_one();
   h8 qh[KSTEPS], ql[KSTEPS];
 #pragma unroll
   for (int k = 0; k < KSTEPS; ++k)
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
       h2 a, b;
-      split2(x[k][e] * up, x[k][e + 1] * up, a, b);
+      split2(x[k][e] * up, x[k][e + 1] * up, one, a, b);
       qh[k][e] = a.x; qh[k][e + 1] = a.y; ql[k][e] = b.x; ql[k][e + 1] = b.y;
     }
 
@@ -103,12 +106,16 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   const int base = all_lo & -KT, steps = all_lo < all_hi ? (all_hi - base + KT - 1) / KT : 0;
   const int share = (steps + nsplit - 1) / nsplit, z0 = blockIdx.y * share, z1 = min(z0 + share, steps);
 
-  const int tk = threadIdx.x / TPK, kc = (threadIdx.x % TPK) * KB;         // this thread's key and bytes of it
-  const int tv = threadIdx.x / TPV * 4, vc = (threadIdx.x % TPV) * VB;     // ... and its four tokens, and bytes
+  // this thread's key and its bytes 16 kc, 16 (kc + TPK), ...; its four tokens and VB bytes of each.  (Threads side by side write
+  // side by side in LDS: a key's 16-byte pieces dealt out in turn, the tokens of one column.)
+  const int tk = threadIdx.x / TPK, kc = threadIdx.x % TPK * 16;
+  const int tv = threadIdx.x % (KT / 4) * 4, vc = threadIdx.x / (KT / 4) * VB;
   const int vpos = (tv & ~15) + ((tv >> 2 & 1) << 3) + ((tv >> 3 & 1) << 2);   // where they lie in LDS
+  const int ts = FINE ? threadIdx.x & (KT - 1) : (threadIdx.x & (NT - 1)) * 32;  // ... and the key whose scales it brings
   auto page_at = [&](int st, int t) {
     const int p = base + st * KT + t;
-    return st < z1 && p < sq.len ? table[p >> ps] : -1;
+    const int pg = table[min(p >> ps, ldt - 1)];
+    return st < z1 && p < sq.len ? pg : -1;
   };
   auto row_at = [&](int pg) { return (size_t)((uint32_t)pg < (uint32_t)pages ? pg : 0) * kvh + h; };
   uint4 kr[KB / 16];
@@ -118,7 +125,7 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
     const int t0 = base + st * KT;
     const int8_t* a = kq + ((row_at(pk) << ps) + ((t0 + tk) & pm)) * HD + kc;
 #pragma unroll
-    for (int b = 0; b < KB / 16; ++b) kr[b] = *(const uint4*)(a + 16 * b);
+    for (int b = 0; b < KB / 16; ++b) kr[b] = *(const uint4*)(a + 16 * TPK * b);
     const int8_t* v = vq + ((row_at(pv) << ps) + ((t0 + tv) & pm)) * HD + vc;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -126,8 +133,8 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
       if (VB == 8) { const uint2 u = *(const uint2*)(v + t * HD); vr[t][0] = u.x; vr[t][VB / 8] = u.y; }
       if (VB == 16) { const uint4 u = *(const uint4*)(v + t * HD); vr[t][0] = u.x; vr[t][VB / 16] = u.y; vr[t][VB / 8] = u.z; vr[t][VB / 4 - 1] = u.w; }
     }
-    if (threadIdx.x < KT) {
-      const size_t d = (row_at(pc) << (ps - bs)) + (((t0 + threadIdx.x) & pm) >> bs);
+    if (threadIdx.x < NS) {
+      const size_t d = (row_at(pc) << (ps - bs)) + (((t0 + ts) & pm) >> bs);
       rks = ks[d];
       rvs = vs[d];
     }
@@ -137,8 +144,8 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
     _Float16* a = &sk[buf][tk * KLD + kc];
 #pragma unroll
     for (int b = 0; b < KB / 16; ++b) {
-      *(h8*)(a + 16 * b) = cvt8(kr[b].x, kr[b].y);
-      *(h8*)(a + 16 * b + 8) = cvt8(kr[b].z, kr[b].w);
+      *(h8*)(a + 16 * TPK * b) = cvt8(kr[b].x, kr[b].y);
+      *(h8*)(a + 16 * TPK * b + 8) = cvt8(kr[b].z, kr[b].w);
     }
 #pragma unroll
     for (int w = 0; w < VB / 4; ++w) {
@@ -152,7 +159,7 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
         *(uint2*)&sv[buf][(vc + 4 * w + e) * VLD + vpos] = u;
       }
     }
-    if (threadIdx.x < KT) {   // (a token of no page: weight 0 whatever its score)
+    if (threadIdx.x < NS) {   // (a token of no page: weight 0 whatever its score)
       float lv, iv;
       value_scale(rvs, carry, lv, iv);
       const bool there = (uint32_t)pc < (uint32_t)pages;
@@ -167,21 +174,22 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[d][e] = 0.0f;
-  float ref = NOTHING, sum = 0.0f;
+  // (a row's weights are 2^(score - ref); before the first score that it sees ref is 0 and any score sets it)
+  float ref = 0.0f, limit = NOTHING, sum = 0.0f;
 
-  int pk = page_at(z0, tk), pv = page_at(z0, tv), pc = page_at(z0, threadIdx.x & (KT - 1));
+  int pk = page_at(z0, tk), pv = page_at(z0, tv), pc = page_at(z0, ts);
   if (z0 < z1) {
     load(z0, pk, pv, pc);
     store(0, pc);
   }
-  pk = page_at(z0 + 1, tk); pv = page_at(z0 + 1, tv); pc = page_at(z0 + 1, threadIdx.x & (KT - 1));
+  pk = page_at(z0 + 1, tk); pv = page_at(z0 + 1, tv); pc = page_at(z0 + 1, ts);
   __syncthreads();
   for (int st = z0; st < z1; ++st) {
     const int buf = (st - z0) & 1;
     const bool more = st + 1 < z1;
     const int pc1 = pc;
     if (more) load(st + 1, pk, pv, pc);
-    pk = page_at(st + 2, tk); pv = page_at(st + 2, tv); pc = page_at(st + 2, threadIdx.x & (KT - 1));
+    pk = page_at(st + 2, tk); pv = page_at(st + 2, tv); pc = page_at(st + 2, ts);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int j0 = base + st * KT + nt * 32;
@@ -197,45 +205,63 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
         sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[k], sc, 0, 0, 0);
       }
       // (register e of the product: key 8 (e / 4) + 4 hf + e % 4)
-      float top = NOTHING;
-      const bool mask = j0 < lo_max || j0 + 32 > hi_min;
+      float kf1 = 0.0f, lv1 = 0.0f, iv1 = 0.0f;
+      if (!FINE) { kf1 = skf[buf][nt]; lv1 = slv[buf][nt] - ref; iv1 = siv[buf][nt]; }
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const int j4 = nt * 32 + 8 * b + 4 * hf;
-        const f4 kf = *(const f4*)&skf[buf][j4], lv = *(const f4*)&slv[buf][j4];
+        f4 kf = {kf1, kf1, kf1, kf1}, lv = {lv1, lv1, lv1, lv1};
+        if (FINE) {
+          kf = *(const f4*)&skf[buf][j4];
+          lv = *(const f4*)&slv[buf][j4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) lv[e] -= ref;
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float v = sc[4 * b + e];
-          v = CAP ? capped<true>(v * kf[e], cap2) + lv[e] : fmaf(v, kf[e], lv[e]);
-          const int j = base + st * KT + j4 + e;
-          if (BIAS) v = fmaf(-slope, fabsf((float)(pos - j)), v);
-          if (mask) v = j >= lo && j < hi ? v : -INFINITY;
-          sc[4 * b + e] = v;
-          top = fmaxf(top, v);
+          const float v = sc[4 * b + e];
+          sc[4 * b + e] = CAP ? capped<true>(v * kf[e], cap2) + lv[e] : fmaf(v, kf[e], lv[e]);
+          if (BIAS) sc[4 * b + e] = fmaf(-slope, fabsf((float)(pos - (base + st * KT + j4 + e))), sc[4 * b + e]);
         }
       }
-      if (__any(top > ref + PASSES)) {
+      if (j0 < lo_max || j0 + 32 > hi_min) {
+        const int a = lo - (j0 + 4 * hf), z = hi - (j0 + 4 * hf);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int j = 8 * (e >> 2) + (e & 3);
+          sc[e] = j >= a && j < z ? sc[e] : -INFINITY;
+        }
+      }
+      float top = fmaxf(sc[0], sc[1]);
+#pragma unroll
+      for (int e = 2; e < 16; e += 2) top = fmaxf(fmaxf(top, sc[e]), sc[e + 1]);
+      if (__any(top > limit)) {
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float to = top > ref + PASSES ? top - SETS : ref;
-        const float f = exp2_f(ref - to);
-        ref = to;
+        const bool anew = top > limit;
+        const float by = anew ? top - SETS : 0.0f;
+        const float f = limit > NOTHING ? exp2_f(-by) : 1.0f;   // (nothing summed yet)
+        ref += by;
+        limit = anew ? PASSES : limit;
         sum *= f;
 #pragma unroll
         for (int d = 0; d < DT; ++d) acc[d] *= f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[e] -= by;
       }
 #pragma unroll
       for (int k = 0; k < 2; ++k) {   // 16 keys
         h8 ph, pl;
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          const f4 iv = *(const f4*)&siv[buf][nt * 32 + 16 * k + 8 * b + 4 * hf];
+          f4 iv = {iv1, iv1, iv1, iv1};
+          if (FINE) iv = *(const f4*)&siv[buf][nt * 32 + 16 * k + 8 * b + 4 * hf];
 #pragma unroll
           for (int e = 0; e < 4; e += 2) {
-            const float u = exp2_f(sc[8 * k + 4 * b + e] - ref), w = exp2_f(sc[8 * k + 4 * b + e + 1] - ref);
+            const float u = exp2_f(sc[8 * k + 4 * b + e]), w = exp2_f(sc[8 * k + 4 * b + e + 1]);
             sum = fmaf(u, iv[e], sum);
             sum = fmaf(w, iv[e + 1], sum);
             h2 a, l;
-            split2(u, w, a, l);
+            split2(u, w, one, a, l);
             ph[4 * b + e] = a.x; ph[4 * b + e + 1] = a.y; pl[4 * b + e] = l.x; pl[4 * b + e + 1] = l.y;
           }
         }
@@ -253,6 +279,7 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   }
 
   sum += __shfl_xor(sum, 32);
+  if (limit == NOTHING) ref = NOTHING;
   if (r >= M) return;
   if (nsplit == 1) {
     float* to = out + (size_t)(sq.r0 + i) * ldo + o_off + hq * HD;
@@ -288,15 +315,19 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
 }
 
 // grid (tiles of the most rows x sequences x kv heads, pieces), local 256; vec: bit 0 the rows, bit 1 the output in 16-byte pieces
-#define MANY(HD, KT, W, F)                                                                                                                                      \
-  extern "C" __global__ __launch_bounds__(256, W) void attn_many__HD##HD##_FORM##F(                                                                             \
+// -DFINE=1: blocks of less than 32 tokens
+#define MANY(HD, KT, W, FINE, F)                                                                                                                                \
+  extern "C" __global__ __launch_bounds__(256, W) void attn_many__HD##HD##_FINE##FINE##_FORM##F(                                                                \
       const float* q, int ldq, int q_off, const int8_t* kq, const int8_t* vq, const float* ks, const float* vs, int pages, int ps, int bs, const int* rows,     \
       const int* lens, const int* table, int ldt, int T, int max_rows, int heads, int kvh, float* out, int ldo, int o_off, float scale, float cap2, int window, \
       const float* slopes, const int* prefix, const int* first, float* ws, int nsplit, int tiles, int vec) {                                                    \
-    many_body<HD, KT, (F & 1) != 0, (F & 2) != 0>(q, ldq, q_off, kq, vq, ks, vs, pages, ps, bs, rows, lens, table, ldt, T, max_rows, heads, kvh, out, ldo,      \
-                                                  o_off, scale, cap2, window, slopes, prefix, first, ws, nsplit, tiles, vec);                                   \
+    many_body<HD, KT, FINE, (F & 1) != 0, (F & 2) != 0>(q, ldq, q_off, kq, vq, ks, vs, pages, ps, bs, rows, lens, table, ldt, T, max_rows, heads, kvh, out,     \
+                                                        ldo, o_off, scale, cap2, window, slopes, prefix, first, ws, nsplit, tiles, vec);                        \
   }
-#define MANYF(HD, KT, W) MANY(HD, KT, W, 0) MANY(HD, KT, W, 1) MANY(HD, KT, W, 2) MANY(HD, KT, W, 3)
-MANYF(64, 64, 2)
-MANYF(128, 64, 2)
-MANYF(256, 32, 1)
+#define MANYF(HD, KT, W, FINE) MANY(HD, KT, W, FINE, 0) MANY(HD, KT, W, FINE, 1) MANY(HD, KT, W, FINE, 2) MANY(HD, KT, W, FINE, 3)
+MANYF(64, 64, 2, 0)
+MANYF(64, 64, 2, 1)
+MANYF(128, 64, 2, 0)
+MANYF(128, 64, 2, 1)
+MANYF(256, 32, 1, 0)
+MANYF(256, 32, 1, 1)
