@@ -241,7 +241,6 @@
     const int keys = std::max(1, std::min(b.max_len > 0 ? b.max_len : ldt * c.page, window ? (int)std::min<int64_t>((int64_t)most + window, 0x7FFFF000) : 0x7FFFF000));
     int vec = rq.vec() ? 1 : 0;
     if (ro.vec()) vec |= 2;
-    const size_t most_x = 0xFFFFFFFFull / 256;
     if (M <= (c.hd == 256 ? 16 : 32)) {
       const int rt = M > 16 ? 2 : 1, pack = M <= 8 ? 1 : 0, rows = pack ? 8 : 16 * rt;
       // Pieces of one length for all sequences, so that long ones are more work-groups, not longer ones: two work-groups a
@@ -250,7 +249,7 @@
       int least = (int)std::max<size_t>(8, ((size_t)(keys + 31) / 32 + want - 1) / want);
       nsplit = (keys + 32 * least - 1) / (32 * least);
       cl_mem w = nsplit > 1 ? at_ws(pairs * nsplit * rows * (c.hd + 2) * 4) : nullptr, counts = nsplit > 1 ? at_counts(pairs) : nullptr;
-      if (pairs > most_x) throw std::runtime_error("attention: too many sequences");
+      if (pairs > 0xFFFFFFFFull / 256) throw std::runtime_error("attention: too many sequences");
       vec &= 1;
       cl_kernel k = variant("attn", {{"HD", c.hd}, {"RT", rt}, {"PACK", pack}, {"FINE", c.block < 4 ? 1 : 0}, {"FORM", form}}, "attn_few");
       set_args(k, 0, q, ldq, q_off, c.b[0], c.b[1], c.b[2], c.b[3], pages, ps, bs, b.rows, b.len, b.table, ldt, T, mr, heads, kvh, out, ldo, o_off, scale, cap2, window,
@@ -259,17 +258,18 @@
       run("attention", k, 2, g, l);
       return;
     }
-    int tiles = (int)((M + 127) / 128);
-    if (pairs * tiles > most_x) throw std::runtime_error("attention: too many rows");
+    const int waves = c.hd == 128 ? 8 : 4, bm = 32 * waves;
+    int tiles = (int)((M + bm - 1) / bm);
+    if (pairs * tiles > 0xFFFFFFFFull / (64 * waves)) throw std::runtime_error("attention: too many rows");
     // rows that fill less than the chip: their keys shared out, at least 512 to a piece
-    nsplit = (int)std::max<size_t>(1, std::min<size_t>((size_t)2 * arcz_device_cus() / (pairs * tiles), (size_t)(keys + 511) / 512));
-    cl_mem w = nsplit > 1 ? at_ws(pairs * tiles * nsplit * 128 * (c.hd + 2) * 4) : nullptr;
-    cl_kernel k = variant("attn", {{"HD", c.hd}, {"FINE", c.block < 32 ? 1 : 0}, {"FORM", form}}, "attn_many");
+    nsplit = (int)std::max<size_t>(1, std::min<size_t>((size_t)8 / waves * arcz_device_cus() / (pairs * tiles), (size_t)(keys + 511) / 512));
+    cl_mem w = nsplit > 1 ? at_ws(pairs * tiles * nsplit * bm * (c.hd + 2) * 4) : nullptr;
+    cl_kernel k = variant("attn", {{"HD", c.hd}, {"FINE", c.block < 32 ? 1 : 0}, {"FORM", form}, {waves == 8 ? "W8" : nullptr, 1}}, "attn_many");
     set_args(k, 0, q, ldq, q_off, c.b[0], c.b[1], c.b[2], c.b[3], pages, ps, bs, b.rows, b.len, b.table, ldt, T, mr, heads, kvh, out, ldo, o_off, scale, cap2, window,
              a.slopes, a.prefix, a.first, w, nsplit, tiles, vec);
-    size_t g[2] = {pairs * tiles * 256, (size_t)nsplit}, l[2] = {256, 1};
+    size_t g[2] = {pairs * tiles * 64 * waves, (size_t)nsplit}, l[2] = {(size_t)64 * waves, 1};
     run("attention", k, 2, g, l);
-    if (nsplit > 1) join(c, b, w, nsplit, 128, tiles, mr, heads, out, ldo, o_off);
+    if (nsplit > 1) join(c, b, w, nsplit, bm, tiles, mr, heads, out, ldo, o_off);
   }
   void join(const Kv& c, const Batch& b, cl_mem w, int nsplit, int rows, int blocks, int mr, int heads, cl_mem out, int ldo, int o_off) {
     int hd = c.hd, most_len = b.ld_table * c.page, T = b.T, kvh = c.heads, per = 1024 / c.hd;

@@ -129,6 +129,7 @@ static const KernelSpec kKernelTable[] = {
     {"attn", "kv_write", nullptr, "piipiippppiiiipppiiiii", {"HD", nullptr}, {{nullptr, 0, false}}, 256},
     {"attn", "kv_read", nullptr, "piipiippppiiiiipppiiiii", {nullptr}, {{nullptr, 0, false}}, 256},
     {"attn", "attn_few", nullptr, "piippppiiipppiiiiipiiffipppppiii", {"HD", "RT", "PACK", "FINE", "FORM", nullptr}, {{nullptr, 0, false}}, 256},
+    {"attn", "attn_many", "W8", "piippppiiipppiiiiipiiffippppiii", {"HD", "FINE", "FORM", "W8", nullptr}, {{nullptr, 0, false}}, 512},
     {"attn", "attn_many", nullptr, "piippppiiipppiiiiipiiffippppiii", {"HD", "FINE", "FORM", nullptr}, {{nullptr, 0, false}}, 256},
     {"attn", "attn_join", nullptr, "piiiippiiiiipii", {nullptr}, {{nullptr, 0, false}}, 256},
     {"moe", "moe_combine", nullptr, "pppppi", {nullptr}, {{"NU", 0, true}, {nullptr, 0, false}}, 256},

@@ -12,6 +12,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "attn_index.h"
+
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -19,20 +21,10 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 
-struct Seq {
-  int r0;    // its first row
-  int n;     // its rows that this launch takes (at most max_rows)
-  int p0;    // the position of its first row (below 0 where len says less than the rows)
-  int len;
-};
+using attn::Seq;
+using attn::sees;
 __device__ inline Seq seq_of(const int* __restrict__ rows, const int* __restrict__ lens, int s, int T, int max_rows, int most_len) {
-  Seq q;
-  q.r0 = min(max(rows[s], 0), T);
-  const int all = min(max(rows[s + 1], q.r0), T) - q.r0;
-  q.n = min(all, max_rows);
-  q.len = min(max(lens[s], 0), most_len);
-  q.p0 = q.len - all;
-  return q;
+  return attn::seq_at(rows[s], rows[s + 1], lens[s], T, max_rows, most_len);
 }
 __device__ inline int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
@@ -68,6 +60,14 @@ __device__ inline void cvt4x4(uint32_t t0, uint32_t t1, uint32_t t2, uint32_t t3
   p[1][1] = biased(perm(0x64646464u, b01, 0x04030402u));
   p[2][1] = biased(perm(0x64646464u, b23, 0x04010400u));
   p[3][1] = biased(perm(0x64646464u, b23, 0x04030402u));
+}
+// ... of values 2 e and 2 e + 1 alone: p[v][0] = tokens 0 and 1, p[v][1] = 2 and 3.
+__device__ inline void cvt4x2(uint32_t t0, uint32_t t1, uint32_t t2, uint32_t t3, int e, h2 (&p)[2][2]) {
+  const uint32_t a = perm(t1, t0, e ? 0x07030602u : 0x05010400u) ^ 0x80808080u, b = perm(t3, t2, e ? 0x07030602u : 0x05010400u) ^ 0x80808080u;
+  p[0][0] = biased(perm(0x64646464u, a, 0x04010400u));
+  p[1][0] = biased(perm(0x64646464u, a, 0x04030402u));
+  p[0][1] = biased(perm(0x64646464u, b, 0x04010400u));
+  p[1][1] = biased(perm(0x64646464u, b, 0x04030402u));
 }
 // An f32 pair as two f16 pairs whose sum has 22 bits of it: the first truncated, the second what it misses.  `one` is 1.0 that the
 // compiler does not know (opaque_one): the difference is then one instruction that takes the f16 as it is, not two.
@@ -123,23 +123,12 @@ __device__ inline bool last_of(unsigned* count, unsigned n) {
 }
 
 // ---- a score's form
-struct Form {
-  float cap2;    // cap * log2(e), 0: not capped
-  int window;    // 0: none
-};
 // x = scale * q.k * log2(e), or with a cap 2 * scale * q.k / cap * log2(e):  tanh(y) = 1 - 2 / (1 + e^(2 y))
 template <bool CAP>
 __device__ inline float capped(float x, float cap2) {
   if (!CAP) return x;
   return fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(1.0f + exp2_f(x)), cap2);
 }
-// The positions [lo, hi) that a row at position p sees.
-__device__ inline void sees(int p, int len, int window, int prefix, int first, int& lo, int& hi) {
-  hi = min(len, max(p + 1, prefix));
-  lo = max(first, 0);
-  if (window) lo = max(lo, p - window + 1);
-}
-
 // The scales' part in a score.  A weight is carried as w = p * vs (p = e^(s - reference), vs the scale of the token's values), as
 // 2^(s log2(e) + log2(vs) - reference): the product with the scale costs no instruction of its own, the weights stay within a
 // fixed range whatever the scales are, and the softmax's sum is the sum of w / vs.  A block of zeros (a scale below 2^-120) takes the

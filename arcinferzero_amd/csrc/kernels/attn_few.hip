@@ -68,14 +68,13 @@ __device__ inline void few_body(const float* __restrict__ q, int ldq, int q_off,
     all_lo = __builtin_amdgcn_readfirstlane(all_lo);
     all_hi = __builtin_amdgcn_readfirstlane(all_hi);
   }
-  const int base = all_lo & -32, steps = all_lo < all_hi ? (all_hi - base + 31) >> 5 : 0;
+  const attn::Span span = attn::span_of(all_lo, all_hi, 32);
+  const int base = span.base, steps = span.steps;
   const int share = max((steps + nsplit - 1) / nsplit, least), z0 = min((int)blockIdx.y * share, steps), z1 = min(z0 + share, steps);
 
-  auto page_of = [&](int st, int tile) {
-    const int p = base + st * 32 + tile * 16;
-    const int pg = table[min(p >> ps, ldt - 1)];   // (looked up in any case: no branch, so several lookups are on their way at once)
-    return st < z1 && p < sq.len ? pg : -1;
-  };
+  // (of keys behind the last: some entry of the table -- no row sees them.  Nothing is done with an entry here, so that a lookup is
+  //  not waited for before the bytes are asked for)
+  auto page_of = [&](int st, int tile) { return table[attn::entry_of(base + st * 32 + tile * 16, ps, ldt)]; };
   // A lane's part of 32 keys: keys in two tiles of 16, bytes 64 j + 16 g of key m; values, HD / 16 bytes of 8 tokens; a scale for
   // each of four keys or, in longer blocks, for all.  Keys are asked for again as soon as the scores are made of them, values once
   // they are in the sums: half a step's work and the other waves' hide the way, and the registers of one step suffice.
@@ -429,7 +428,7 @@ extern "C" __global__ __launch_bounds__(256) void attn_join(const float* __restr
 // W, WF: waves a SIMD that the registers are held to (WF: with a scale for each key)
 #define FEWF(HD, RT, PACK, W, WF) FEW4(HD, RT, PACK, 0, W) FEW4(HD, RT, PACK, 1, WF)
 FEWF(64, 1, 1, 4, 4)
-FEWF(64, 1, 0, 4, 4)
+FEWF(64, 1, 0, 4, 3)
 FEWF(64, 2, 0, 3, 2)
 FEWF(128, 1, 1, 3, 3)
 FEWF(128, 1, 0, 3, 2)

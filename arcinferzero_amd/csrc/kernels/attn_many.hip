@@ -14,24 +14,33 @@
 // the matrix pipe does twice the products of plain f16 rows; it is what bounds the kernel.
 #include "attn.h"
 
-template <int HD, int KT, bool FINE, bool CAP, bool BIAS>
+// Nothing is moved across by the compiler.
+__device__ inline void turn() { __builtin_amdgcn_sched_barrier(0); }
+// Worked out here, not where it is used.
+__device__ inline void stay(h8 (&a)[2], h8 (&b)[2]) { asm volatile("" : "+v"(a[0]), "+v"(a[1]), "+v"(b[0]), "+v"(b[1])); }
+
+template <int HD, int KT, int NW, bool FINE, bool CAP, bool BIAS>
 __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off, const int8_t* __restrict__ kq, const int8_t* __restrict__ vq,
                                  const float* __restrict__ ks, const float* __restrict__ vs, int pages, int ps, int bs, const int* __restrict__ rows,
                                  const int* __restrict__ lens, const int* __restrict__ table, int ldt, int T, int max_rows, int heads, int kvh,
                                  float* __restrict__ out, int ldo, int o_off, float scale, float cap2, int window, const float* __restrict__ slopes,
                                  const int* __restrict__ prefix, const int* __restrict__ first, float* __restrict__ ws, int nsplit, int tiles, int vec) {
-  constexpr int BM = 128, KSTEPS = HD / 16, DT = HD / 32, NT = KT / 32;
-  constexpr int TPK = 256 / KT, KB = HD / TPK;          // threads a key's row, bytes each
-  constexpr int TPV = 1024 / KT, VB = HD / TPV;         // threads four tokens' values, bytes each and token
+  constexpr int BM = 32 * NW, THREADS = 64 * NW, KSTEPS = HD / 16, DT = HD / 32, NT = KT / 32;
+  constexpr int TPK = THREADS / KT, KB = HD / TPK;      // threads a key's row, bytes each
+  constexpr int TPV = 4 * THREADS / KT, VB = HD / TPV;  // threads four tokens' values, bytes each and token
+  // 128 values: what the rows' first f16 miss stays in LDS (32 registers; with them there the loop's would not fit two waves a SIMD)
+  constexpr bool QLDS = HD == 128;
   constexpr int KLD = HD + 8, VLD = KT + 8;             // (rows 16 bytes longer: neighbouring rows four banks on)
   constexpr float LOG2E = 1.4426950408889634f;
   __shared__ _Float16 sk[2][KT * KLD], sv[2][HD * VLD];
   // scales: of each key, or of each 32 keys that share one (kf: the score's factor; lv, iv: value_scale)
   constexpr int NS = FINE ? KT : NT;
   __shared__ float skf[2][NS], slv[2][NS], siv[2][NS];
-  __shared__ int red[4][3];
+  __shared__ int red[NW][3];
+  __shared__ _Float16 sq_lo[QLDS ? NW * 32 * KLD : 1];
 
-  const int sh = blockIdx.x / tiles, tile = tiles - 1 - (blockIdx.x - sh * tiles), s = sh / kvh, h = sh - s * kvh, G = heads / kvh;
+  // (the rows that see the most keys first, of all heads; the heads in turn, so that with 8 of them each XCD's L2 holds one's cache)
+  const int pairs = gridDim.x / tiles, sh = blockIdx.x % pairs, tile = tiles - 1 - blockIdx.x / pairs, s = sh / kvh, h = sh - s * kvh, G = heads / kvh;
   const Seq sq = seq_of(rows, lens, s, T, max_rows, ldt << ps);
   const int M = sq.n * G;   // (the host holds max_rows * heads below 2^31)
   if (tile * BM >= M) return;
@@ -85,25 +94,37 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
     red[wave][0] = (int)big; red[wave][1] = lo_min; red[wave][2] = hi_max;
   }
   __syncthreads();
-  big = max(max((uint32_t)red[0][0], (uint32_t)red[1][0]), max((uint32_t)red[2][0], (uint32_t)red[3][0]));
-  const int all_lo = __builtin_amdgcn_readfirstlane(min(min(red[0][1], red[1][1]), min(red[2][1], red[3][1])));
-  const int all_hi = __builtin_amdgcn_readfirstlane(max(max(red[0][2], red[1][2]), max(red[2][2], red[3][2])));
+  int all_lo = red[0][1], all_hi = red[0][2];
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    big = max(big, (uint32_t)red[w][0]);
+    all_lo = min(all_lo, red[w][1]);
+    all_hi = max(all_hi, red[w][2]);
+  }
+  all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+  all_hi = __builtin_amdgcn_readfirstlane(all_hi);
   const int e2 = min(max(137 - (int)(big >> 23), -100), 100);   // (the largest of the work-group's rows to 2^10 ... 2^11)
   const float up = __uint_as_float((uint32_t)(127 + e2) << 23), down = __uint_as_float((uint32_t)(127 - e2) << 23);
   const float kfac = (CAP ? 2.0f * LOG2E * LOG2E / cap2 : LOG2E) * scale * down;   // (cap2 = cap log2 e)
   const float one = opaque_one();
-  h8 qh[KSTEPS], ql[KSTEPS];
+  h8 qh[KSTEPS], ql[QLDS ? 1 : KSTEPS];
+  _Float16* const mine = &sq_lo[QLDS ? (wave * 32 + c) * KLD + hf * 8 : 0];
 #pragma unroll
-  for (int k = 0; k < KSTEPS; ++k)
+  for (int k = 0; k < KSTEPS; ++k) {
+    h8 lo8;
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
       h2 a, b;
       split2(x[k][e] * up, x[k][e + 1] * up, one, a, b);
-      qh[k][e] = a.x; qh[k][e + 1] = a.y; ql[k][e] = b.x; ql[k][e + 1] = b.y;
+      qh[k][e] = a.x; qh[k][e + 1] = a.y; lo8[e] = b.x; lo8[e + 1] = b.y;
     }
+    if (QLDS) *(h8*)(mine + k * 16) = lo8;
+    else ql[QLDS ? 0 : k] = lo8;
+  }
 
   // ---- this work-group's tiles of keys
-  const int base = all_lo & -KT, steps = all_lo < all_hi ? (all_hi - base + KT - 1) / KT : 0;
+  const attn::Span span = attn::span_of(all_lo, all_hi, KT);
+  const int base = span.base, steps = span.steps;
   const int share = (steps + nsplit - 1) / nsplit, z0 = blockIdx.y * share, z1 = min(z0 + share, steps);
 
   // this thread's key and its bytes 16 kc, 16 (kc + TPK), ...; its four tokens and VB bytes of each.  (Threads side by side write
@@ -112,53 +133,71 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   const int tv = threadIdx.x % (KT / 4) * 4, vc = threadIdx.x / (KT / 4) * VB;
   const int vpos = (tv & ~15) + ((tv >> 2 & 1) << 3) + ((tv >> 3 & 1) << 2);   // where they lie in LDS
   const int ts = FINE ? threadIdx.x & (KT - 1) : (threadIdx.x & (NT - 1)) * 32;  // ... and the key whose scales it brings
-  auto page_at = [&](int st, int t) {
-    const int p = base + st * KT + t;
-    const int pg = table[min(p >> ps, ldt - 1)];
-    return st < z1 && p < sq.len ? pg : -1;
-  };
-  auto row_at = [&](int pg) { return (size_t)((uint32_t)pg < (uint32_t)pages ? pg : 0) * kvh + h; };
+  // Where a tile's bytes are: page * (bytes of a page of all heads) + this head's + the tile's place in the page (0 where pages are
+  // smaller than a tile) + the thread's own.  With pages of a tile and more the first three are the work-group's, in scalars.
+  const bool whole = (1 << ps) >= KT;
+  const uint32_t page_bytes = (uint32_t)(kvh << ps) * HD, page_scales = (uint32_t)(kvh << (ps - bs)) * 4;
+  const char* const kh = (const char*)kq + ((size_t)h << ps) * HD;
+  const char* const vh = (const char*)vq + ((size_t)h << ps) * HD;
+  const size_t sh0 = ((size_t)h << (ps - bs)) * 4;
+  const uint32_t ko = (uint32_t)((tk & pm) * HD + kc), vo = (uint32_t)((tv & pm) * HD + vc), so = (uint32_t)((ts & pm) >> bs) * 4;
+  // (of a key behind the last: some entry of the table -- no row sees it.  Nothing is done with the entry here: a lookup is not
+  //  waited for until the next tile's bytes are asked for)
+  auto page_at = [&](int st, int t) { return table[attn::entry_of(base + st * KT + t, ps, ldt)]; };
+  auto valid = [&](int pg) { return (uint32_t)pg < (uint32_t)pages ? (uint32_t)pg : 0u; };
   uint4 kr[KB / 16];
   uint32_t vr[4][VB / 4];
   float rks = 0.0f, rvs = 0.0f;
-  auto load = [&](int st, int pk, int pv, int pc) {
-    const int t0 = base + st * KT;
-    const int8_t* a = kq + ((row_at(pk) << ps) + ((t0 + tk) & pm)) * HD + kc;
+  auto take = [&](const char* ka, uint32_t k0, const char* va, uint32_t v0, const char* ksa, const char* vsa, uint32_t s0) {
 #pragma unroll
-    for (int b = 0; b < KB / 16; ++b) kr[b] = *(const uint4*)(a + 16 * TPK * b);
-    const int8_t* v = vq + ((row_at(pv) << ps) + ((t0 + tv) & pm)) * HD + vc;
+    for (int b = 0; b < KB / 16; ++b) kr[b] = *(const uint4*)(ka + (k0 + 16 * TPK * b));
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      if (VB == 4) vr[t][0] = *(const uint32_t*)(v + t * HD);
-      if (VB == 8) { const uint2 u = *(const uint2*)(v + t * HD); vr[t][0] = u.x; vr[t][VB / 8] = u.y; }
-      if (VB == 16) { const uint4 u = *(const uint4*)(v + t * HD); vr[t][0] = u.x; vr[t][VB / 16] = u.y; vr[t][VB / 8] = u.z; vr[t][VB / 4 - 1] = u.w; }
+      const char* v = va + (v0 + t * HD);
+      if (VB == 4) vr[t][0] = *(const uint32_t*)v;
+      if (VB == 8) { const uint2 u = *(const uint2*)v; vr[t][0] = u.x; vr[t][VB / 8] = u.y; }
+      if (VB == 16) { const uint4 u = *(const uint4*)v; vr[t][0] = u.x; vr[t][VB / 16] = u.y; vr[t][VB / 8] = u.z; vr[t][VB / 4 - 1] = u.w; }
     }
     if (threadIdx.x < NS) {
-      const size_t d = (row_at(pc) << (ps - bs)) + (((t0 + ts) & pm) >> bs);
-      rks = ks[d];
-      rvs = vs[d];
+      rks = *(const float*)(ksa + s0);
+      rvs = *(const float*)(vsa + s0);
+    }
+  };
+  struct Pages { int k, v, c; };
+  auto load = [&](int st, const Pages& pg3) {
+    const int in = (base + st * KT) & pm;
+    if (whole) {
+      const uint32_t pg = __builtin_amdgcn_readfirstlane(valid(pg3.k));
+      const size_t at = (size_t)pg * page_bytes + (size_t)in * HD, sat = (size_t)pg * page_scales + sh0 + (size_t)(in >> bs) * 4;
+      take(kh + at, ko, vh + at, vo, (const char*)ks + sat, (const char*)vs + sat, so);
+    } else {
+      const size_t ps0 = (size_t)valid(pg3.c) * page_scales + sh0;
+      take(kh + (size_t)valid(pg3.k) * page_bytes, ko, vh + (size_t)valid(pg3.v) * page_bytes, vo, (const char*)ks + ps0, (const char*)vs + ps0, so);
     }
   };
   float carry = -60.0f;
-  auto store = [&](int buf, int pc) {
-    _Float16* a = &sk[buf][tk * KLD + kc];
-#pragma unroll
-    for (int b = 0; b < KB / 16; ++b) {
-      *(h8*)(a + 16 * TPK * b) = cvt8(kr[b].x, kr[b].y);
-      *(h8*)(a + 16 * TPK * b + 8) = cvt8(kr[b].z, kr[b].w);
+  // ... to LDS in UNITS parts: half a key's 16 bytes each, then two columns of the four tokens each
+  constexpr int KU = KB / 8, UNITS = KU + VB / 2;
+  auto store = [&](int buf, int u) {
+    if (u < KU) {
+      // (eight threads side by side on a key's row: four write their second half while the others write their first)
+      const uint4 r = kr[u / 2];
+      const bool second = (u & 1) != (TPK > 4 && (threadIdx.x & 4));
+      *(h8*)&sk[buf][tk * KLD + kc + 16 * TPK * (u / 2) + (second ? 8 : 0)] = cvt8(second ? r.z : r.x, second ? r.w : r.y);
+      return;
     }
+    const int w = (u - KU) / 2, e = (u - KU) & 1;
+    h2 p[2][2];
+    cvt4x2(vr[0][w], vr[1][w], vr[2][w], vr[3][w], e, p);
 #pragma unroll
-    for (int w = 0; w < VB / 4; ++w) {
-      h2 p[4][2];
-      cvt4x4(vr[0][w], vr[1][w], vr[2][w], vr[3][w], p);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint2 u;
-        __builtin_memcpy(&u.x, &p[e][0], 4);
-        __builtin_memcpy(&u.y, &p[e][1], 4);
-        *(uint2*)&sv[buf][(vc + 4 * w + e) * VLD + vpos] = u;
-      }
+    for (int x = 0; x < 2; ++x) {
+      uint2 o;
+      __builtin_memcpy(&o.x, &p[x][0], 4);
+      __builtin_memcpy(&o.y, &p[x][1], 4);
+      *(uint2*)&sv[buf][(vc + 4 * w + 2 * e + x) * VLD + vpos] = o;
     }
+  };
+  auto store_scales = [&](int buf, int pc) {
     if (threadIdx.x < NS) {   // (a token of no page: weight 0 whatever its score)
       float lv, iv;
       value_scale(rvs, carry, lv, iv);
@@ -177,36 +216,62 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   // (a row's weights are 2^(score - ref); before the first score that it sees ref is 0 and any score sets it)
   float ref = 0.0f, limit = NOTHING, sum = 0.0f;
 
-  int pk = page_at(z0, tk), pv = page_at(z0, tv), pc = page_at(z0, ts);
+  // (looked up through vector memory, also where all threads have the same page: a wait for a scalar load among the LDS reads
+  //  would be a wait for all of them)
+  int zero;
+  asm("v_mov_b32 %0, 0" : "=v"(zero));
+  auto look = [&](int st) {
+    if (whole) {
+      const int pg = page_at(st, zero);
+      return Pages{pg, pg, pg};
+    }
+    return Pages{page_at(st, tk), page_at(st, tv), page_at(st, ts)};
+  };
+  Pages at = look(z0);
   if (z0 < z1) {
-    load(z0, pk, pv, pc);
-    store(0, pc);
+    load(z0, at);
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) store(0, u);
+    store_scales(0, at.c);
   }
-  pk = page_at(z0 + 1, tk); pv = page_at(z0 + 1, tv); pc = page_at(z0 + 1, ts);
+  at = look(z0 + 1);
   __syncthreads();
   for (int st = z0; st < z1; ++st) {
     const int buf = (st - z0) & 1;
     const bool more = st + 1 < z1;
-    const int pc1 = pc;
-    if (more) load(st + 1, pk, pv, pc);
-    pk = page_at(st + 2, tk); pv = page_at(st + 2, tv); pc = page_at(st + 2, ts);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int j0 = base + st * KT + nt * 32;
-      if (j0 >= hi_max || j0 + 32 <= lo_min) continue;   // (of no row of the wave)
-      f16v sc;
+    const int pc1 = at.c;
+    if (more) load(st + 1, at);
+    at = look(st + 2);
+    // The tile in parts of 32 keys.  The matrix pipe takes 32 cycles for a product, in which the wave can issue eight other
+    // instructions; so while one part's scores are made the weights of the part before are worked out, among its sums the next
+    // part's weights, among the last sums the next tile's way to LDS -- two products and their share of the other work at a time,
+    // in just this order (turn), the operand of a product read from LDS two turns ahead.
+    const int j0 = base + st * KT;
+    const bool work = j0 < hi_max && j0 + KT > lo_min;   // (else of no row of the wave)
+    auto scores = [&](int nt, f16v& sc, auto beside) {
+      const _Float16* kp = &sk[buf][(nt * 32 + c) * KLD + hf * 8];
+      h8 a[2] = {*(const h8*)kp, *(const h8*)(kp + 16)}, b[2];
+      if (QLDS) { b[0] = *(const h8*)mine; b[1] = *(const h8*)(mine + 16); }
 #pragma unroll
       for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
-      const _Float16* kp = &sk[buf][(nt * 32 + c) * KLD + hf * 8];
+      turn();
 #pragma unroll
       for (int k = 0; k < KSTEPS; ++k) {
-        const h8 a = *(const h8*)(kp + k * 16);
-        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[k], sc, 0, 0, 0);
-        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[k], sc, 0, 0, 0);
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[k % 2], qh[k], sc, 0, 0, 0);
+        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[k % 2], QLDS ? b[k % 2] : ql[QLDS ? 0 : k], sc, 0, 0, 0);
+        if (k + 2 < KSTEPS) {
+          a[k % 2] = *(const h8*)(kp + (k + 2) * 16);
+          if (QLDS) b[k % 2] = *(const h8*)(mine + (k + 2) * 16);
+        }
+        beside(k);
+        turn();
       }
-      // (register e of the product: key 8 (e / 4) + 4 hf + e % 4)
-      float kf1 = 0.0f, lv1 = 0.0f, iv1 = 0.0f;
-      if (!FINE) { kf1 = skf[buf][nt]; lv1 = slv[buf][nt] - ref; iv1 = siv[buf][nt]; }
+    };
+    // (register e of the product: key 8 (e / 4) + 4 hf + e % 4)
+    auto refer = [&](int nt, f16v& sc) {
+      const int jn = j0 + nt * 32;
+      float kf1 = 0.0f, lv1 = 0.0f;
+      if (!FINE) { kf1 = skf[buf][nt]; lv1 = slv[buf][nt] - ref; }
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const int j4 = nt * 32 + 8 * b + 4 * hf;
@@ -221,11 +286,11 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
         for (int e = 0; e < 4; ++e) {
           const float v = sc[4 * b + e];
           sc[4 * b + e] = CAP ? capped<true>(v * kf[e], cap2) + lv[e] : fmaf(v, kf[e], lv[e]);
-          if (BIAS) sc[4 * b + e] = fmaf(-slope, fabsf((float)(pos - (base + st * KT + j4 + e))), sc[4 * b + e]);
+          if (BIAS) sc[4 * b + e] = fmaf(-slope, fabsf((float)(pos - (j0 + j4 + e))), sc[4 * b + e]);
         }
       }
-      if (j0 < lo_max || j0 + 32 > hi_min) {
-        const int a = lo - (j0 + 4 * hf), z = hi - (j0 + 4 * hf);
+      if (jn < lo_max || jn + 32 > hi_min) {
+        const int a = lo - (jn + 4 * hf), z = hi - (jn + 4 * hf);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int j = 8 * (e >> 2) + (e & 3);
@@ -238,7 +303,7 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
       if (__any(top > limit)) {
         top = fmaxf(top, __shfl_xor(top, 32));
         const bool anew = top > limit;
-        const float by = anew ? top - SETS : 0.0f;
+        const float by = anew ? ceilf(top) - SETS : 0.0f;   // (whole octaves: weights already made are brought along exactly)
         const float f = limit > NOTHING ? exp2_f(-by) : 1.0f;   // (nothing summed yet)
         ref += by;
         limit = anew ? PASSES : limit;
@@ -247,34 +312,77 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
         for (int d = 0; d < DT; ++d) acc[d] *= f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) sc[e] -= by;
+        return f;
       }
+      return 1.0f;
+    };
+    // two weights of a part (of eight pairs)
+    auto weigh = [&](int nt, const f16v& sc, int p, float iv1, h8 (&ph)[2], h8 (&pl)[2]) {
+      float2 iv;
+      if (FINE) iv = *(const float2*)&siv[buf][nt * 32 + 8 * (p / 2) + 4 * hf + 2 * (p & 1)];
+      else iv.x = iv.y = iv1;
+      const float u = exp2_f(sc[2 * p]), w = exp2_f(sc[2 * p + 1]);
+      sum = fmaf(u, iv.x, sum);
+      sum = fmaf(w, iv.y, sum);
+      h2 a, l;
+      split2(u, w, one, a, l);
+      const int k = p / 4, e = p % 4 * 2;
+      ph[k][e] = a.x; ph[k][e + 1] = a.y; pl[k][e] = l.x; pl[k][e + 1] = l.y;
+    };
+    constexpr int SUMS = 2 * DT;
+    auto add = [&](int nt, const h8 (&ph)[2], const h8 (&pl)[2], auto beside) {
+      const _Float16* vp = &sv[buf][c * VLD + nt * 32 + hf * 8];
+      auto at = [&](int i) { return *(const h8*)(vp + 16 * (i / DT) + (i % DT) * 32 * VLD); };
+      h8 a[2] = {at(0), at(1)};
+      turn();
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {   // 16 keys
-        h8 ph, pl;
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          f4 iv = {iv1, iv1, iv1, iv1};
-          if (FINE) iv = *(const f4*)&siv[buf][nt * 32 + 16 * k + 8 * b + 4 * hf];
-#pragma unroll
-          for (int e = 0; e < 4; e += 2) {
-            const float u = exp2_f(sc[8 * k + 4 * b + e]), w = exp2_f(sc[8 * k + 4 * b + e + 1]);
-            sum = fmaf(u, iv[e], sum);
-            sum = fmaf(w, iv[e + 1], sum);
-            h2 a, l;
-            split2(u, w, one, a, l);
-            ph[4 * b + e] = a.x; ph[4 * b + e + 1] = a.y; pl[4 * b + e] = l.x; pl[4 * b + e + 1] = l.y;
-          }
-        }
-        const _Float16* vp = &sv[buf][c * VLD + nt * 32 + 16 * k + hf * 8];
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          const h8 a = *(const h8*)(vp + d * 32 * VLD);
-          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph, acc[d], 0, 0, 0);
-          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl, acc[d], 0, 0, 0);
-        }
+      for (int i = 0; i < SUMS; ++i) {
+        const int k = i / DT, d = i % DT;
+        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i % 2], ph[k], acc[d], 0, 0, 0);
+        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[i % 2], pl[k], acc[d], 0, 0, 0);
+        if (i + 2 < SUMS) a[i % 2] = at(i + 2);
+        beside(i);
+        turn();
       }
+    };
+    auto store_some = [&](int i) {   // (behind the last tile: bytes of the one before, which nobody reads)
+#pragma unroll
+      for (int u = i * UNITS / SUMS; u < (i + 1) * UNITS / SUMS; ++u) store(buf ^ 1, u);
+    };
+    if (work) {
+      f16v s0, s1;
+      h8 ph0[2], pl0[2], ph1[2], pl1[2];
+      const float iv0 = FINE ? 0.0f : siv[buf][0], iv1 = FINE ? 0.0f : siv[buf][NT - 1];
+      scores(0, s0, [](int) {});
+      refer(0, s0);
+      if (NT == 2) {
+        scores(1, s1, [&](int k) {
+#pragma unroll
+          for (int p = k * 8 / KSTEPS; p < (k + 1) * 8 / KSTEPS; ++p) weigh(0, s0, p, iv0, ph0, pl0);
+        });
+        stay(ph0, pl0);
+        // (a reference set anew here lowers the first part's weights too, which are not in the sums yet)
+        const float f = refer(1, s1);
+        if (__any(f != 1.0f)) {
+          const _Float16 f16 = (_Float16)f;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) { ph0[k] *= f16; pl0[k] *= f16; }
+        }
+        add(0, ph0, pl0, [&](int i) {
+#pragma unroll
+          for (int p = i * 8 / SUMS; p < (i + 1) * 8 / SUMS; ++p) weigh(1, s1, p, iv1, ph1, pl1);
+        });
+        add(1, ph1, pl1, store_some);
+      } else {
+#pragma unroll
+        for (int p = 0; p < 8; ++p) weigh(0, s0, p, iv0, ph0, pl0);
+        add(0, ph0, pl0, store_some);
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) store(buf ^ 1, u);
     }
-    if (more) store(buf ^ 1, pc1);
+    if (more) store_scales(buf ^ 1, pc1);
     __syncthreads();
   }
 
@@ -315,19 +423,24 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
 }
 
 // grid (tiles of the most rows x sequences x kv heads, pieces), local 256; vec: bit 0 the rows, bit 1 the output in 16-byte pieces
-// -DFINE=1: blocks of less than 32 tokens
-#define MANY(HD, KT, W, FINE, F)                                                                                                                                \
-  extern "C" __global__ __launch_bounds__(256, W) void attn_many__HD##HD##_FINE##FINE##_FORM##F(                                                                \
+// -DFINE=1: blocks of less than 32 tokens; -DW8: work-groups of eight waves, 256 rows, where the bytes of a tile are fewer for each
+// thread -- and what the rows take of LDS leaves room for one work-group a compute unit in any case
+#define MANY(NAME, HD, KT, NW, W, FINE, F)                                                                                                                      \
+  extern "C" __global__ __launch_bounds__(64 * NW, W) void NAME(                                                                                                \
       const float* q, int ldq, int q_off, const int8_t* kq, const int8_t* vq, const float* ks, const float* vs, int pages, int ps, int bs, const int* rows,     \
       const int* lens, const int* table, int ldt, int T, int max_rows, int heads, int kvh, float* out, int ldo, int o_off, float scale, float cap2, int window, \
       const float* slopes, const int* prefix, const int* first, float* ws, int nsplit, int tiles, int vec) {                                                    \
-    many_body<HD, KT, FINE, (F & 1) != 0, (F & 2) != 0>(q, ldq, q_off, kq, vq, ks, vs, pages, ps, bs, rows, lens, table, ldt, T, max_rows, heads, kvh, out,     \
-                                                        ldo, o_off, scale, cap2, window, slopes, prefix, first, ws, nsplit, tiles, vec);                        \
+    many_body<HD, KT, NW, FINE, (F & 1) != 0, (F & 2) != 0>(q, ldq, q_off, kq, vq, ks, vs, pages, ps, bs, rows, lens, table, ldt, T, max_rows, heads, kvh, out, \
+                                                            ldo, o_off, scale, cap2, window, slopes, prefix, first, ws, nsplit, tiles, vec);                    \
   }
-#define MANYF(HD, KT, W, FINE) MANY(HD, KT, W, FINE, 0) MANY(HD, KT, W, FINE, 1) MANY(HD, KT, W, FINE, 2) MANY(HD, KT, W, FINE, 3)
-MANYF(64, 64, 2, 0)
-MANYF(64, 64, 2, 1)
-MANYF(128, 64, 2, 0)
-MANYF(128, 64, 2, 1)
-MANYF(256, 32, 1, 0)
-MANYF(256, 32, 1, 1)
+#define MANY4(HD, KT, NW, W, FINE, S)                              \
+  MANY(attn_many__HD##HD##_FINE##FINE##_FORM0##S, HD, KT, NW, W, FINE, 0) \
+  MANY(attn_many__HD##HD##_FINE##FINE##_FORM1##S, HD, KT, NW, W, FINE, 1) \
+  MANY(attn_many__HD##HD##_FINE##FINE##_FORM2##S, HD, KT, NW, W, FINE, 2) \
+  MANY(attn_many__HD##HD##_FINE##FINE##_FORM3##S, HD, KT, NW, W, FINE, 3)
+MANY4(64, 64, 4, 2, 0, )
+MANY4(64, 64, 4, 2, 1, )
+MANY4(128, 64, 8, 2, 0, _W81)
+MANY4(128, 64, 8, 2, 1, _W81)
+MANY4(256, 32, 4, 1, 0, )
+MANY4(256, 32, 4, 1, 1, )
