@@ -175,6 +175,15 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
       take(kh + (size_t)valid(pg3.k) * page_bytes, ko, vh + (size_t)valid(pg3.v) * page_bytes, vo, (const char*)ks + ps0, (const char*)vs + ps0, so);
     }
   };
+  // (the bytes are waited for here: what is done with them in two branches is not brought in front of both)
+  auto arrive = [&] {
+#pragma unroll
+    for (int b = 0; b < KB / 16; ++b) asm volatile("" : "+v"(kr[b].x), "+v"(kr[b].y), "+v"(kr[b].z), "+v"(kr[b].w));
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int w = 0; w < VB / 4; ++w) asm volatile("" : "+v"(vr[t][w]));
+  };
   float carry = -60.0f;
   // ... to LDS in UNITS parts: half a key's 16 bytes each, then two columns of the four tokens each
   constexpr int KU = KB / 8, UNITS = KU + VB / 2;
@@ -220,28 +229,31 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   //  would be a wait for all of them)
   int zero;
   asm("v_mov_b32 %0, 0" : "=v"(zero));
-  auto look = [&](int st) {
-    if (whole) {
-      const int pg = page_at(st, zero);
-      return Pages{pg, pg, pg};
+  const int tl = whole ? zero : tk;
+  Pages at = {0, 0, 0};
+  auto look = [&](int st) {   // (with whole pages the other two are left alone: writing them would wait for all loads on the way)
+    at.k = page_at(st, tl);
+    if (!whole) {
+      at.v = page_at(st, tv);
+      at.c = page_at(st, ts);
     }
-    return Pages{page_at(st, tk), page_at(st, tv), page_at(st, ts)};
   };
-  Pages at = look(z0);
+  look(z0);
   if (z0 < z1) {
     load(z0, at);
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) store(0, u);
-    store_scales(0, at.c);
+    store_scales(0, whole ? at.k : at.c);
   }
-  at = look(z0 + 1);
+  look(z0 + 1);
   __syncthreads();
   for (int st = z0; st < z1; ++st) {
     const int buf = (st - z0) & 1;
     const bool more = st + 1 < z1;
-    const int pc1 = at.c;
+    int pc1 = whole ? at.k : at.c;
+    asm volatile("" : "+v"(pc1));   // (the lookups of the turn before, done with before anything else is on its way)
     if (more) load(st + 1, at);
-    at = look(st + 2);
+    look(st + 2);
     // The tile in parts of 32 keys.  The matrix pipe takes 32 cycles for a product, in which the wave can issue eight other
     // instructions; so while one part's scores are made the weights of the part before are worked out, among its sums the next
     // part's weights, among the last sums the next tile's way to LDS -- two products and their share of the other work at a time,
@@ -372,13 +384,16 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
 #pragma unroll
           for (int p = i * 8 / SUMS; p < (i + 1) * 8 / SUMS; ++p) weigh(1, s1, p, iv1, ph1, pl1);
         });
+        arrive();
         add(1, ph1, pl1, store_some);
       } else {
 #pragma unroll
         for (int p = 0; p < 8; ++p) weigh(0, s0, p, iv0, ph0, pl0);
+        arrive();
         add(0, ph0, pl0, store_some);
       }
     } else {
+      arrive();
 #pragma unroll
       for (int u = 0; u < UNITS; ++u) store(buf ^ 1, u);
     }
