@@ -133,46 +133,48 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   const int tv = threadIdx.x % (KT / 4) * 4, vc = threadIdx.x / (KT / 4) * VB;
   const int vpos = (tv & ~15) + ((tv >> 2 & 1) << 3) + ((tv >> 3 & 1) << 2);   // where they lie in LDS
   const int ts = FINE ? threadIdx.x & (KT - 1) : (threadIdx.x & (NT - 1)) * 32;  // ... and the key whose scales it brings
-  // Where a tile's bytes are: page * (bytes of a page of all heads) + this head's + the tile's place in the page (0 where pages are
-  // smaller than a tile) + the thread's own.  With pages of a tile and more the first three are the work-group's, in scalars.
+  // Where a tile's bytes are: page * (bytes of a page of all heads) + the tile's place in the page (0 where pages are smaller than a
+  // tile) + the thread's own.  With pages of a tile and more all threads have the same page (at.k).  Every address lies in the cache,
+  // also that of a tile behind the last, which is asked for and not used.
   const bool whole = (1 << ps) >= KT;
   const uint32_t page_bytes = (uint32_t)(kvh << ps) * HD, page_scales = (uint32_t)(kvh << (ps - bs)) * 4;
-  const char* const kh = (const char*)kq + ((size_t)h << ps) * HD;
-  const char* const vh = (const char*)vq + ((size_t)h << ps) * HD;
-  const size_t sh0 = ((size_t)h << (ps - bs)) * 4;
-  const uint32_t ko = (uint32_t)((tk & pm) * HD + kc), vo = (uint32_t)((tv & pm) * HD + vc), so = (uint32_t)((ts & pm) >> bs) * 4;
+  const char* const kmine = (const char*)kq + ((size_t)h << ps) * HD + ((tk & pm) * HD + kc);
+  const char* const vmine = (const char*)vq + ((size_t)h << ps) * HD + ((tv & pm) * HD + vc);
+  const size_t smine = (((size_t)h << (ps - bs)) + ((ts & pm) >> bs)) * 4;
   // (of a key behind the last: some entry of the table -- no row sees it.  Nothing is done with the entry here: a lookup is not
   //  waited for until the next tile's bytes are asked for)
   auto page_at = [&](int st, int t) { return table[attn::entry_of(base + st * KT + t, ps, ldt)]; };
   auto valid = [&](int pg) { return (uint32_t)pg < (uint32_t)pages ? (uint32_t)pg : 0u; };
+  struct Pages { int k, v, c; };
+  Pages at = {0, 0, 0};
   uint4 kr[KB / 16];
   uint32_t vr[4][VB / 4];
   float rks = 0.0f, rvs = 0.0f;
-  auto take = [&](const char* ka, uint32_t k0, const char* va, uint32_t v0, const char* ksa, const char* vsa, uint32_t s0) {
-#pragma unroll
-    for (int b = 0; b < KB / 16; ++b) kr[b] = *(const uint4*)(ka + (k0 + 16 * TPK * b));
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const char* v = va + (v0 + t * HD);
-      if (VB == 4) vr[t][0] = *(const uint32_t*)v;
-      if (VB == 8) { const uint2 u = *(const uint2*)v; vr[t][0] = u.x; vr[t][VB / 8] = u.y; }
-      if (VB == 16) { const uint4 u = *(const uint4*)v; vr[t][0] = u.x; vr[t][VB / 16] = u.y; vr[t][VB / 8] = u.z; vr[t][VB / 4 - 1] = u.w; }
-    }
-    if (threadIdx.x < NS) {
-      rks = *(const float*)(ksa + s0);
-      rvs = *(const float*)(vsa + s0);
-    }
+  const char *ka, *va;
+  size_t sa;
+  auto address = [&](int st) {
+    const uint32_t in = (uint32_t)((base + st * KT) & pm);
+    const int pv = whole ? at.k : at.v, pc = whole ? at.k : at.c;
+    ka = kmine + ((size_t)valid(at.k) * page_bytes + in * HD);
+    va = vmine + ((size_t)valid(pv) * page_bytes + in * HD);
+    sa = smine + ((size_t)valid(pc) * page_scales + (in >> bs) * 4);
+    return pc;
   };
-  struct Pages { int k, v, c; };
-  auto load = [&](int st, const Pages& pg3) {
-    const int in = (base + st * KT) & pm;
-    if (whole) {
-      const uint32_t pg = __builtin_amdgcn_readfirstlane(valid(pg3.k));
-      const size_t at = (size_t)pg * page_bytes + (size_t)in * HD, sat = (size_t)pg * page_scales + sh0 + (size_t)(in >> bs) * 4;
-      take(kh + at, ko, vh + at, vo, (const char*)ks + sat, (const char*)vs + sat, so);
+  auto load = [&](int part) {   // (four parts)
+    if (part == 0) {
+#pragma unroll
+      for (int b = 0; b < KB / 16; ++b) kr[b] = *(const uint4*)(ka + 16 * TPK * b);
+    } else if (part < 3) {
+#pragma unroll
+      for (int t = 2 * part - 2; t < 2 * part; ++t) {
+        const char* v = va + t * HD;
+        if (VB == 4) vr[t][0] = *(const uint32_t*)v;
+        if (VB == 8) { const uint2 u = *(const uint2*)v; vr[t][0] = u.x; vr[t][VB / 8] = u.y; }
+        if (VB == 16) { const uint4 u = *(const uint4*)v; vr[t][0] = u.x; vr[t][VB / 16] = u.y; vr[t][VB / 8] = u.z; vr[t][VB / 4 - 1] = u.w; }
+      }
     } else {
-      const size_t ps0 = (size_t)valid(pg3.c) * page_scales + sh0;
-      take(kh + (size_t)valid(pg3.k) * page_bytes, ko, vh + (size_t)valid(pg3.v) * page_bytes, vo, (const char*)ks + ps0, (const char*)vs + ps0, so);
+      rks = *(const float*)((const char*)ks + sa);
+      rvs = *(const float*)((const char*)vs + sa);
     }
   };
   // (the bytes are waited for here: what is done with them in two branches is not brought in front of both)
@@ -230,7 +232,6 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   int zero;
   asm("v_mov_b32 %0, 0" : "=v"(zero));
   const int tl = whole ? zero : tk;
-  Pages at = {0, 0, 0};
   auto look = [&](int st) {   // (with whole pages the other two are left alone: writing them would wait for all loads on the way)
     at.k = page_at(st, tl);
     if (!whole) {
@@ -240,20 +241,19 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   };
   look(z0);
   if (z0 < z1) {
-    load(z0, at);
+    const int pc = address(z0);
+#pragma unroll
+    for (int part = 0; part < 4; ++part) load(part);
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) store(0, u);
-    store_scales(0, whole ? at.k : at.c);
+    store_scales(0, pc);
   }
   look(z0 + 1);
   __syncthreads();
   for (int st = z0; st < z1; ++st) {
     const int buf = (st - z0) & 1;
-    const bool more = st + 1 < z1;
-    int pc1 = whole ? at.k : at.c;
-    asm volatile("" : "+v"(pc1));   // (the lookups of the turn before, done with before anything else is on its way)
-    if (more) load(st + 1, at);
-    look(st + 2);
+    int pc1 = address(st + 1);
+    asm volatile("" : "+v"(ka), "+v"(va), "+v"(sa), "+v"(pc1));   // (worked out from the lookups of the turn before: they are here now)
     // The tile in parts of 32 keys.  The matrix pipe takes 32 cycles for a product, in which the wave can issue eight other
     // instructions; so while one part's scores are made the weights of the part before are worked out, among its sums the next
     // part's weights, among the last sums the next tile's way to LDS -- two products and their share of the other work at a time,
@@ -365,7 +365,10 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
       f16v s0, s1;
       h8 ph0[2], pl0[2], ph1[2], pl1[2];
       const float iv0 = FINE ? 0.0f : siv[buf][0], iv1 = FINE ? 0.0f : siv[buf][NT - 1];
-      scores(0, s0, [](int) {});
+      scores(0, s0, [&](int k) {   // (the next tile's bytes, then the lookup for the one behind it)
+        if (k < 4) load(k);
+        if (k == 3) look(st + 2);
+      });
       refer(0, s0);
       if (NT == 2) {
         scores(1, s1, [&](int k) {
@@ -393,11 +396,14 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
         add(0, ph0, pl0, store_some);
       }
     } else {
+#pragma unroll
+      for (int part = 0; part < 4; ++part) load(part);
+      look(st + 2);
       arrive();
 #pragma unroll
       for (int u = 0; u < UNITS; ++u) store(buf ^ 1, u);
     }
-    if (more) store_scales(buf ^ 1, pc1);
+    store_scales(buf ^ 1, pc1);
     __syncthreads();
   }
 
