@@ -371,7 +371,8 @@ class Runtime:
 
     @staticmethod
     def wrap(ptr, nbytes):
-        """A handle onto device memory that is the caller's (a tensor's data_ptr()); free() forgets it."""
+        """A handle onto device memory that is the caller's (a tensor's data_ptr()); free() forgets it.  torch brings its own HIP runtime:
+        import it before this package, so that both use that one."""
         h = lib.arcz_wrap(ptr, nbytes)
         if not h:
             raise ArczError(-50, lib.arcz_last_error().decode())

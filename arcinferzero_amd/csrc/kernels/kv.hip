@@ -12,82 +12,102 @@
 // Bound: 4 bytes of HBM read and one written a value; the second look at the rows comes from the L2.
 #include "attn.h"
 
+// NP passes of a tile are held in registers, so that a tile of that size is read once and all its loads are on their way at once;
+// larger ones (long blocks) are read again from the L2.
 template <int HD>
 __device__ inline void kv_write_body(const float* __restrict__ x, int ld, int off, int8_t* __restrict__ q, float* __restrict__ d, int pages, int heads, int ps,
                                      int bs, const int* __restrict__ table, int ldt, const Seq& sq, int tile, int vec) {
-  constexpr int TPR = HD / 4, RPP = 256 / TPR;   // threads a row, rows a pass
+  constexpr int TPR = HD / 4, RPP = 256 / TPR, NP = 8, CHUNK = RPP * NP;   // threads a row, rows a pass
   __shared__ uint32_t top[256];
   __shared__ float inv[256], ratio[256];
-  const int h = blockIdx.z >> 1, lane = threadIdx.x % TPR, r0 = threadIdx.x / TPR;
+  __shared__ int page[256];   // a page for each 16 tokens at most
+  const int h = blockIdx.z >> 1, lane = threadIdx.x % TPR, r0 = threadIdx.x / TPR, pm = (1 << ps) - 1;
   // (rows whose positions lie below 0 have no place)
   const int from = max(sq.p0, 0), to = sq.p0 + sq.n;
-  const int t0 = (from & -tile) + blockIdx.x * tile, block = 1 << bs, nb = tile >> bs;
+  const int t0 = (from & -tile) + blockIdx.x * tile, block = 1 << bs, nb = (tile + block - 1) >> bs, end = min(t0 + tile, to);
   if (t0 >= to) return;
+  const int ntab = ((end - 1) >> ps) - (t0 >> ps) + 1;   // (at most tile / 16 + 1)
+  for (int b = threadIdx.x; b < ntab; b += 256) page[b] = table[(t0 >> ps) + b];
   for (int b = threadIdx.x; b < nb; b += 256) top[b] = 0;
-  __syncthreads();
-  auto load = [&](int p) {
-    const float* s = x + (size_t)(sq.r0 + p - sq.p0) * ld + off + h * HD + lane * 4;
-    return vec ? *(const float4*)s : make_float4(s[0], s[1], s[2], s[3]);
-  };
-  // (sign off, the order of the words is that of the magnitudes, with infinity and NaN on top)
-  for (int r = r0; r < tile; r += RPP) {
-    const int p = t0 + r;
-    if (p < from || p >= to) continue;
-    const float4 v = load(p);
-    uint32_t m = max(max(__float_as_uint(v.x) & 0x7FFFFFFFu, __float_as_uint(v.y) & 0x7FFFFFFFu),
-                     max(__float_as_uint(v.z) & 0x7FFFFFFFu, __float_as_uint(v.w) & 0x7FFFFFFFu));
+  float4 v[NP];
+  auto load = [&](int c) {   // the rows of pass NP c ... that are new
 #pragma unroll
-    for (int o = 1; o < TPR; o *= 2) m = max(m, (uint32_t)__shfl_xor((int)m, o));
-    if (lane == 0) atomicMax(&top[r >> bs], m);
+    for (int k = 0; k < NP; ++k) {
+      const int p = t0 + c * CHUNK + k * RPP + r0;
+      v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (p >= from && p < end) {
+        const float* s = x + (size_t)(sq.r0 + p - sq.p0) * ld + off + h * HD + lane * 4;
+        v[k] = vec ? *(const float4*)s : make_float4(s[0], s[1], s[2], s[3]);
+      }
+    }
+  };
+  const int chunks = (tile + CHUNK - 1) / CHUNK;
+  load(0);
+  __syncthreads();
+  for (int c = 0; c < chunks; ++c) {
+    if (c) load(c);
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      // (sign off, the order of the words is that of the magnitudes, with infinity and NaN on top)
+      uint32_t m = max(max(__float_as_uint(v[k].x) & 0x7FFFFFFFu, __float_as_uint(v[k].y) & 0x7FFFFFFFu),
+                       max(__float_as_uint(v[k].z) & 0x7FFFFFFFu, __float_as_uint(v[k].w) & 0x7FFFFFFFu));
+#pragma unroll
+      for (int o = 1; o < TPR; o *= 2) m = max(m, (uint32_t)__shfl_xor((int)m, o));
+      const int r = c * CHUNK + k * RPP + r0;
+      if (lane == 0 && t0 + r >= from && t0 + r < end) atomicMax(&top[r >> bs], m);
+    }
   }
   __syncthreads();
   const int old0 = from & -block;   // the first block's beginning: [old0, from) are older tokens
-  auto place = [&](int p, size_t& row) {   // of a position: false where its page is none
-    const int pg = table[p >> ps];
-    row = (size_t)pg * heads + h;
-    return (uint32_t)pg < (uint32_t)pages;
+  auto row_of = [&](int p) {        // of a position's page: below 0 where that is none
+    const int pg = page[(p >> ps) - (t0 >> ps)];
+    return (uint32_t)pg < (uint32_t)pages ? (long)pg * heads + h : -1L;
   };
   for (int b = threadIdx.x; b < nb; b += 256) {
     const int p = t0 + (b << bs);
-    inv[b] = ratio[b] = 0.0f;
-    if (p + block <= from || p >= to) continue;
-    size_t row;
-    if (!place(p, row)) continue;
-    float* at = d + (row << (ps - bs)) + ((p & ((1 << ps) - 1)) >> bs);
+    inv[b] = 0.0f;
+    ratio[b] = -1.0f;   // (nothing to do)
+    if (p + block <= from || p >= end) continue;
+    const long row = row_of(p);
+    if (row < 0) continue;
+    float* at = d + ((size_t)row << (ps - bs)) + ((p & pm) >> bs);
     const float now = top[b] >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __uint_as_float(top[b]) / 127.0f;
     const float was = p < from ? *at : 0.0f;
     const float s = was != was || now != now ? __uint_as_float(0x7FC00000u) : fmaxf(was, now);
     const float i = s >= 0x1p-120f ? 1.0f / s : 0.0f;
     inv[b] = i;
     if (s > was && p < from) ratio[b] = was * i;
-    else ratio[b] = -1.0f;   // (nothing to do)
     *at = s;
   }
   __syncthreads();
   auto byte = [](float v) { return (uint32_t)(int)fminf(fmaxf(__builtin_rintf(v), -127.0f), 127.0f) & 255u; };
-  for (int r = r0; r < tile; r += RPP) {
-    const int p = t0 + r, b = r >> bs;
-    if (p >= to) break;
-    if (p < from) {   // an older token of the first block
-      const float f = ratio[b];
-      if (p < old0 || !(f >= 0.0f)) continue;
-      size_t row;
-      if (!place(p, row)) continue;
-      uint32_t* at = (uint32_t*)(q + ((row << ps) + (p & ((1 << ps) - 1))) * HD) + lane;
-      const uint32_t w = *at;
-      uint32_t o = 0;
+  for (int c = 0; c < chunks; ++c) {
+    if (chunks > 1) load(c);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) o |= byte((float)(int8_t)(w >> 8 * k) * f) << 8 * k;
-      *at = o;
-      continue;
+    for (int k = 0; k < NP; ++k) {
+      const int r = c * CHUNK + k * RPP + r0, p = t0 + r;
+      if (p < from || p >= end) continue;
+      const long row = row_of(p);
+      const float i = inv[r >> bs];
+      // (times 0 is a value's sign and zero; a block whose scale is NaN gets zeros)
+      const uint32_t w = i > 0.0f ? byte(v[k].x * i) | byte(v[k].y * i) << 8 | byte(v[k].z * i) << 16 | byte(v[k].w * i) << 24 : 0u;
+      if (row >= 0) ((uint32_t*)(q + (((size_t)row << ps) + (p & pm)) * HD))[lane] = w;
     }
-    size_t row;
-    if (!place(p, row)) continue;
-    const float4 v = load(p);
-    const float i = inv[b];
-    // (times 0 is a value's sign and zero; a block whose scale is NaN gets zeros)
-    const uint32_t w = i > 0.0f ? byte(v.x * i) | byte(v.y * i) << 8 | byte(v.z * i) << 16 | byte(v.w * i) << 24 : 0u;
-    ((uint32_t*)(q + ((row << ps) + (p & ((1 << ps) - 1))) * HD))[lane] = w;
+  }
+  // the older tokens of the first block, where its scale has grown
+  const int b0 = max(old0, t0);
+  if (b0 < from) {
+    const float f = ratio[(b0 - t0) >> bs];
+    const long row = row_of(b0);
+    if (f >= 0.0f && row >= 0)
+      for (int p = b0 + r0; p < from; p += RPP) {
+        uint32_t* at = (uint32_t*)(q + (((size_t)row << ps) + (p & pm)) * HD) + lane;
+        const uint32_t w = *at;
+        uint32_t o = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o |= byte((float)(int8_t)(w >> 8 * k) * f) << 8 * k;
+        *at = o;
+      }
   }
 }
 
@@ -113,11 +133,12 @@ KV_WRITE(128)
 KV_WRITE(256)
 
 // Back to f32: rows of positions len - n + i.  A page that is none reads as zeros.  grid (ceil(max_rows / per), sequences, 2), a
-// work-group `per` rows, a thread four values at a time.
+// work-group `per` rows, a thread four values at a time, four times with all its loads on their way.
 extern "C" __global__ __launch_bounds__(256) void kv_read(float* k, int ldk, int k_off, float* v, int ldv, int v_off, const int8_t* __restrict__ kq,
                                                           const int8_t* __restrict__ vq, const float* __restrict__ ks, const float* __restrict__ vs, int pages, int heads,
                                                           int hd, int ps, int bs, const int* __restrict__ rows, const int* __restrict__ lens,
                                                           const int* __restrict__ table, int ldt, int T, int max_rows, int per, int vec) {
+  constexpr int N = 4;
   const int s = blockIdx.y, second = blockIdx.z;
   const Seq sq = seq_of(rows, lens, s, T, max_rows, ldt << ps);
   const int8_t* q = second ? vq : kq;
@@ -125,22 +146,37 @@ extern "C" __global__ __launch_bounds__(256) void kv_read(float* k, int ldk, int
   float* out = second ? v : k;
   const int ld = second ? ldv : ldk, off = second ? v_off : k_off, w = heads * hd / 4, mask = (1 << ps) - 1;
   const int i0 = blockIdx.x * per, n = min(per, sq.n - i0);
-  for (int u = threadIdx.x; u < n * w; u += 256) {
-    const int i = u / w, c = u - i * w, p = sq.p0 + i0 + i, h = 4 * c / hd;
-    if (p < 0) continue;
-    const int pg = table[(size_t)s * ldt + (p >> ps)];
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if ((uint32_t)pg < (uint32_t)pages) {
-      const size_t row = (size_t)pg * heads + h;
-      const uint32_t b = *(const uint32_t*)(q + ((row << ps) + (p & mask)) * hd + (4 * c - h * hd));
-      const float f = d[(row << (ps - bs)) + ((p & mask) >> bs)];
-      o = make_float4((float)(int8_t)b * f, (float)(int8_t)(b >> 8) * f, (float)(int8_t)(b >> 16) * f, (float)(int8_t)(b >> 24) * f);
+  table += (size_t)s * ldt;
+  for (int u0 = threadIdx.x; u0 < n * w; u0 += 256 * N) {
+    int i[N], c[N], pg[N];
+    uint32_t b[N];
+    float f[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int u = min(u0 + 256 * e, n * w - 1);
+      i[e] = u / w;
+      c[e] = u - i[e] * w;
+      pg[e] = table[max(sq.p0 + i0 + i[e], 0) >> ps];
     }
-    float* to = out + (size_t)(sq.r0 + i0 + i) * ld + off + 4 * c;
-    if (vec) {
-      *(float4*)to = o;
-    } else {
-      to[0] = o.x; to[1] = o.y; to[2] = o.z; to[3] = o.w;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int p = max(sq.p0 + i0 + i[e], 0), h = 4 * c[e] / hd;
+      const bool there = (uint32_t)pg[e] < (uint32_t)pages;
+      const size_t row = (size_t)(there ? pg[e] : 0) * heads + h;
+      b[e] = *(const uint32_t*)(q + ((row << ps) + (p & mask)) * hd + (4 * c[e] - h * hd));
+      f[e] = d[(row << (ps - bs)) + ((p & mask) >> bs)];
+      if (!there) { b[e] = 0; f[e] = 0.0f; }
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      if (u0 + 256 * e >= n * w || sq.p0 + i0 + i[e] < 0) continue;
+      const float4 o = make_float4((float)(int8_t)b[e] * f[e], (float)(int8_t)(b[e] >> 8) * f[e], (float)(int8_t)(b[e] >> 16) * f[e], (float)(int8_t)(b[e] >> 24) * f[e]);
+      float* to = out + (size_t)(sq.r0 + i0 + i[e]) * ld + off + 4 * c[e];
+      if (vec) {
+        *(float4*)to = o;
+      } else {
+        to[0] = o.x; to[1] = o.y; to[2] = o.z; to[3] = o.w;
+      }
     }
   }
 }

@@ -58,7 +58,8 @@ arcz_mem* arcz_view(arcz_mem* parent, size_t offset, size_t bytes);
  * [p, p + bytes) inside one allocation; NULL + error text otherwise (host memory, another GPU, past the allocation's end).  The
  * memory stays the caller's: arcz_free forgets the handle, and the caller keeps it allocated for as long as the handle, a view
  * of it or a recorded list that names it is used.  Calls on it run on the library's stream, like all others: it is ordered with
- * the GPU's default (null) stream in both directions; work of other streams is ordered by their owner (arcz_stream). */
+ * the GPU's default (null) stream in both directions; work of other streams is ordered by their owner (arcz_stream).  The process
+ * has to have one HIP runtime: a framework that brings its own is loaded before this library. */
 arcz_mem* arcz_wrap(void* p, size_t bytes);
 /* The library's stream (a hipStream_t), for events that order another stream's work with it; NULL before arcz_init. */
 void* arcz_stream(void);
