@@ -260,11 +260,16 @@
       run("attention", k, 2, g, l);
       return;
     }
-    const int waves = c.hd == 128 ? 8 : 4, bm = 32 * waves;
+    // Heads of 128 values: work-groups of eight waves and 256 rows, one a compute unit, where rows are many and see thousands of keys; else
+    // of four and 128 rows, two of them, which fill the chip sooner and read and write rows while the other computes.  (us, 32 heads
+    // over 8, eight waves / four: 8192 rows over 9000 keys 1200 / 1249, 4096 over 4096 280 / 297, 512 over 8192 142 / 149; 2048 over
+    // 2048 117 / 107, 512 over 512 48 / 36, 100 over 4000 50 / 42, ragged documents 102 / 85)
+    const int seen = std::max(0, (b.max_len > 0 ? b.max_len : ldt * c.page) - most / 2);
+    const int waves = c.hd == 128 && M >= 1024 && !a.first && (window ? std::min(window, seen) : seen) >= 2000 ? 8 : 4, bm = 32 * waves;
     int tiles = (int)((M + bm - 1) / bm);
     if (pairs * tiles > 0xFFFFFFFFull / (64 * waves)) throw std::runtime_error("attention: too many rows");
-    // rows that fill less than the chip: their keys shared out, at least 512 to a piece
-    nsplit = (int)std::max<size_t>(1, std::min<size_t>((size_t)8 / waves * arcz_device_cus() / (pairs * tiles), (size_t)(keys + 511) / 512));
+    // rows that fill less than the chip: their keys shared out, at least 256 to a piece
+    nsplit = (int)std::max<size_t>(1, std::min<size_t>((size_t)8 / waves * arcz_device_cus() / (pairs * tiles), (size_t)(keys + 255) / 256));
     cl_mem w = nsplit > 1 ? at_ws(pairs * tiles * nsplit * bm * (c.hd + 2) * 4) : nullptr;
     cl_kernel k = variant("attn", {{"HD", c.hd}, {"FINE", c.block < 32 ? 1 : 0}, {"FORM", form}, {waves == 8 ? "W8" : nullptr, 1}}, "attn_many");
     set_args(k, 0, q, ldq, q_off, c.b[0], c.b[1], c.b[2], c.b[3], pages, ps, bs, b.rows, b.len, b.table, ldt, T, mr, heads, kvh, out, ldo, o_off, scale, cap2, window,

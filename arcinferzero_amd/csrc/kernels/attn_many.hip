@@ -29,7 +29,7 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   constexpr int TPK = THREADS / KT, KB = HD / TPK;      // threads a key's row, bytes each
   constexpr int TPV = 4 * THREADS / KT, VB = HD / TPV;  // threads four tokens' values, bytes each and token
   // 128 values: what the rows' first f16 miss stays in LDS (32 registers; with them there the loop's would not fit two waves a SIMD)
-  constexpr bool QLDS = HD == 128;
+  constexpr bool QLDS = NW == 8;
   constexpr int KLD = HD + 8, VLD = KT + 8;             // (rows 16 bytes longer: neighbouring rows four banks on)
   constexpr float LOG2E = 1.4426950408889634f;
   __shared__ _Float16 sk[2][KT * KLD], sv[2][HD * VLD];
@@ -461,6 +461,8 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   MANY(attn_many__HD##HD##_FINE##FINE##_FORM3##S, HD, KT, NW, W, FINE, 3)
 MANY4(64, 64, 4, 2, 0, )
 MANY4(64, 64, 4, 2, 1, )
+MANY4(128, 32, 4, 2, 0, )
+MANY4(128, 32, 4, 2, 1, )
 MANY4(128, 64, 8, 2, 0, _W81)
 MANY4(128, 64, 8, 2, 1, _W81)
 MANY4(256, 32, 4, 1, 0, )

@@ -76,8 +76,8 @@ class Cache:
                 p = e
 
 
-def attention(cache, q, rows, lens, table, scale, cap=0.0, window=0, slopes=None, prefix=None, first=None, max_rows=1 << 30):
-    """q [T][heads][hd] -> (out f64 [T][heads][hd], bound on each value's error, rows that were computed).
+def attention(cache, q, rows, lens, table, scale, cap=0.0, window=0, slopes=None, prefix=None, first=None, max_rows=1 << 30, only=None):
+    """q [T][heads][hd] -> (out f64 [T][heads][hd], bound on each value's error, rows that were computed: all, or those of `only`).
 
     The bound counts the f32 steps behind the exact 8-bit values: a score's error is that of a sum of 2 hd products of f16 parts
     (22 bits of each row's value: 2^-22; the sum in f32: each of hd / 16 steps' result rounded, both parts, and inside a step
@@ -101,6 +101,8 @@ def attention(cache, q, rows, lens, table, scale, cap=0.0, window=0, slopes=None
         j = np.arange(l)
         for i in range(min(n, max_rows)):
             t, p = rows[s] + i, l - n + i
+            if only is not None and t not in only:
+                continue
             done[t] = True
             see = there & ((j <= p) | (j < (prefix[s] if prefix is not None else 0)))
             if window:
