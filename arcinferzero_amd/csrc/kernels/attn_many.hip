@@ -32,7 +32,13 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   constexpr bool QLDS = NW == 8;
   constexpr int KLD = HD + 8, VLD = KT + 8;             // (rows 16 bytes longer: neighbouring rows four banks on)
   constexpr float LOG2E = 1.4426950408889634f;
-  __shared__ _Float16 sk[2][KT * KLD], sv[2][HD * VLD];
+  // (the rows on their way in, and out, pass through the tiles' place: SLD floats a row of the wave's 32, 64 columns at a time)
+  constexpr int SLD = 68;
+  struct Tiles { _Float16 k[2][KT * KLD], v[2][HD * VLD]; };
+  static_assert(sizeof(Tiles) >= NW * 32 * SLD * 4, "the rows pass through the tiles' place");
+  __shared__ __attribute__((aligned(16))) Tiles tl2;
+  auto& sk = tl2.k;
+  auto& sv = tl2.v;
   // scales: of each key, or of each 32 keys that share one (kf: the score's factor; lv, iv: value_scale)
   constexpr int NS = FINE ? KT : NT;
   __shared__ float skf[2][NS], slv[2][NS], siv[2][NS];
@@ -53,26 +59,40 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   sees(pos, sq.len, window, prefix ? prefix[s] : 0, first ? first[sq.r0 + i] : 0, lo, hi);
   if (r >= M) hi = lo = 0;
   const float slope = BIAS ? slopes[hq] * LOG2E : 0.0f;
+  // The rows come, and go, 64 columns at a time through LDS: four rows' 256 bytes a load, where a lane's own 16 bytes of 32 rows
+  // would be 64 places.  A lane moves 16 bytes of rows 4 n + lane / 16.
+  float* const pass = (float*)&tl2 + wave * 32 * SLD;
+  const int quarter = lane >> 4, col = (lane & 15) * 4;
+  auto of_row = [&](long v, int n) { return (long)__shfl((long long)v, n * 4 + quarter); };
   uint32_t big = 0;
   float x[KSTEPS][8];
   {
-    const float* src = q + (size_t)(sq.r0 + i) * ldq + q_off + hq * HD + hf * 8;
+    const long from = (long)(sq.r0 + i) * ldq + q_off + hq * HD;
 #pragma unroll
-    for (int k = 0; k < KSTEPS; ++k) {
-      const float* a = src + k * 16;
-      if (vec) {
-        const float4 u = *(const float4*)a, w = *(const float4*)(a + 4);
-        x[k][0] = u.x; x[k][1] = u.y; x[k][2] = u.z; x[k][3] = u.w;
-        x[k][4] = w.x; x[k][5] = w.y; x[k][6] = w.z; x[k][7] = w.w;
-      } else {
+    for (int cc = 0; cc < HD / 64; ++cc) {
+      float4 u[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[k][e] = a[e];
+      for (int n = 0; n < 8; ++n) {
+        const float* a = q + of_row(from, n) + cc * 64 + col;
+        u[n] = vec & 1 ? *(const float4*)a : make_float4(a[0], a[1], a[2], a[3]);
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t b = __float_as_uint(x[k][e]) & 0x7FFFFFFFu;
-        if (b < 0x7F800000u) big = max(big, b);
+      for (int n = 0; n < 8; ++n) *(float4*)&pass[(n * 4 + quarter) * SLD + col] = u[n];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");   // (among the wave's lanes)
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float4 a = *(const float4*)&pass[c * SLD + k * 16 + hf * 8], b = *(const float4*)&pass[c * SLD + k * 16 + hf * 8 + 4];
+        float (&y)[8] = x[cc * 4 + k];
+        y[0] = a.x; y[1] = a.y; y[2] = a.z; y[3] = a.w; y[4] = b.x; y[5] = b.y; y[6] = b.z; y[7] = b.w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t b2 = __float_as_uint(y[e]) & 0x7FFFFFFFu;
+          if (b2 < 0x7F800000u) big = max(big, b2);
+        }
       }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+      __builtin_amdgcn_wave_barrier();
     }
   }
   // (rows that see nothing take no part in the wave's range)
@@ -409,41 +429,46 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
 
   sum += __shfl_xor(sum, 32);
   if (limit == NOTHING) ref = NOTHING;
-  if (r >= M) return;
-  if (nsplit == 1) {
-    float* to = out + (size_t)(sq.r0 + i) * ldo + o_off + hq * HD;
-    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+  // (pieces: the sums of each row, then its reference and its sum of weights)
+  float* const piece = nsplit == 1 ? nullptr : ws + ((size_t)(sh * tiles + tile) * nsplit + blockIdx.y) * BM * (HD + 2);
+  if (piece && r < M && hf == 0) {
+    piece[BM * HD + 2 * (wave * 32 + c)] = ref;
+    piece[BM * HD + 2 * (wave * 32 + c) + 1] = sum;
+  }
+  const float f = piece ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+  float* const to = piece ? piece : out;
+  const long place = r >= M ? -1 : piece ? (long)(wave * 32 + c) * HD : (long)(sq.r0 + i) * ldo + o_off + hq * HD;
+  const bool whole16 = piece || (vec & 2);
+  for (int cc = 0; cc < HD / 64; ++cc) {
 #pragma unroll
     for (int d = 0; d < DT; ++d)
+      if (d / 2 == cc) {
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        float* at = to + d * 32 + 8 * b + 4 * hf;
-        const float4 o = sum == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
-                                     : make_float4(acc[d][4 * b] * f, acc[d][4 * b + 1] * f, acc[d][4 * b + 2] * f, acc[d][4 * b + 3] * f);
-        if (vec & 2) {
-          *(float4*)at = o;
+        for (int b = 0; b < 4; ++b)
+          *(float4*)&pass[c * SLD + (d & 1) * 32 + 8 * b + 4 * hf] =
+              sum == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                          : make_float4(acc[d][4 * b] * f, acc[d][4 * b + 1] * f, acc[d][4 * b + 2] * f, acc[d][4 * b + 3] * f);
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const long o = of_row(place, n);
+      const float4 v = *(const float4*)&pass[(n * 4 + quarter) * SLD + col];
+      if (o >= 0) {
+        float* at = to + o + cc * 64 + col;
+        if (whole16) {
+          *(float4*)at = v;
         } else {
-          at[0] = o.x; at[1] = o.y; at[2] = o.z; at[3] = o.w;
+          at[0] = v.x; at[1] = v.y; at[2] = v.z; at[3] = v.w;
         }
       }
-  } else {   // (pieces: the sums of each row, then its reference and its sum of weights)
-    float* to = ws + ((size_t)(sh * tiles + tile) * nsplit + blockIdx.y) * BM * (HD + 2);
-    const int row = wave * 32 + c;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        float* at = to + row * HD + d * 32 + 8 * b + 4 * hf;
-        *(float4*)at = make_float4(acc[d][4 * b], acc[d][4 * b + 1], acc[d][4 * b + 2], acc[d][4 * b + 3]);
-      }
-    if (hf == 0) {
-      to[BM * HD + 2 * row] = ref;
-      to[BM * HD + 2 * row + 1] = sum;
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
-// grid (tiles of the most rows x sequences x kv heads, pieces), local 256; vec: bit 0 the rows, bit 1 the output in 16-byte pieces
 // -DFINE=1: blocks of less than 32 tokens; -DW8: work-groups of eight waves, 256 rows, where the bytes of a tile are fewer for each
 // thread -- and what the rows take of LDS leaves room for one work-group a compute unit in any case
 #define MANY(NAME, HD, KT, NW, W, FINE, F)                                                                                                                      \
