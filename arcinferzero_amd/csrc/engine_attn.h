@@ -260,12 +260,13 @@
       run("attention", k, 2, g, l);
       return;
     }
-    // Heads of 128 values: work-groups of eight waves and 256 rows, one a compute unit, where rows are many and see thousands of keys; else
-    // of four and 128 rows, two of them, which fill the chip sooner and read and write rows while the other computes.  (us, 32 heads
-    // over 8, eight waves / four: 8192 rows over 9000 keys 1200 / 1249, 4096 over 4096 280 / 297, 512 over 8192 142 / 149; 2048 over
-    // 2048 117 / 107, 512 over 512 48 / 36, 100 over 4000 50 / 42, ragged documents 102 / 85)
+    // Heads of 128 values, blocks of 32 tokens and more: work-groups of eight waves and 256 rows, one a compute unit, where rows are many
+    // and see thousands of keys; else of four and 128 rows, two of them, which fill the chip sooner and read and write rows while the
+    // other computes.  (us, 32 heads over 8, eight waves / four: 8192 rows over 9000 keys 1200 / 1249, 4096 over 4096 280 / 297, 512
+    // over 8192 142 / 149; 2048 over 2048 117 / 107, 512 over 512 48 / 36, 100 over 4000 50 / 42, ragged documents 102 / 85; blocks of
+    // 16, 2000 rows over 4000 1354 / 1348)
     const int seen = std::max(0, (b.max_len > 0 ? b.max_len : ldt * c.page) - most / 2);
-    const int waves = c.hd == 128 && M >= 1024 && !a.first && (window ? std::min(window, seen) : seen) >= 2000 ? 8 : 4, bm = 32 * waves;
+    const int waves = c.hd == 128 && c.block >= 32 && M >= 1024 && !a.first && (window ? std::min(window, seen) : seen) >= 2000 ? 8 : 4, bm = 32 * waves;
     int tiles = (int)((M + bm - 1) / bm);
     if (pairs * tiles > 0xFFFFFFFFull / (64 * waves)) throw std::runtime_error("attention: too many rows");
     // rows that fill less than the chip: their keys shared out, at least 256 to a piece

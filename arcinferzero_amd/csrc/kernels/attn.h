@@ -123,11 +123,28 @@ __device__ inline bool last_of(unsigned* count, unsigned n) {
 }
 
 // ---- a score's form
-// x = scale * q.k * log2(e), or with a cap 2 * scale * q.k / cap * log2(e):  tanh(y) = 1 - 2 / (1 + e^(2 y))
-template <bool CAP>
-__device__ inline float capped(float x, float cap2) {
-  if (!CAP) return x;
-  return fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(1.0f + exp2_f(x)), cap2);
+// N scores over their cap, y, to cap tanh(y) log2(e) (cap2 = cap log2(e)).  Up to 1 as y times a quotient of polynomials (the continued
+// fraction y / (1 + y^2 / (3 + y^2 / (5 + ...))) cut off behind its 9: 6e-8 of the value), so that a score's error is relative to the
+// score; beyond as 1 - 2 / (1 + e^(2 y)), whose error is one of the cap (there an eighth of 2^-22 of it).
+template <int N>
+__device__ inline void cap_scores(float (&v)[N], float cap2) {
+  auto near = [&](float y) {
+    const float z = y * y;
+    return (cap2 * y) * fmaf(z, z + 105.0f, 945.0f) * __builtin_amdgcn_rcpf(fmaf(z, fmaf(z, 15.0f, 420.0f), 945.0f));
+  };
+  float most = 0.0f;
+#pragma unroll
+  for (int e = 0; e < N; ++e) most = fmaxf(most, fabsf(v[e]));
+  if (!__any(most >= 1.0f)) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = near(v[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float far = fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(1.0f + exp2_f(v[e] * 2.8853900817779268f)), cap2);
+      v[e] = fabsf(v[e]) >= 1.0f ? far : near(v[e]);
+    }
+  }
 }
 // The scales' part in a score.  A weight is carried as w = p * vs (p = e^(s - reference), vs the scale of the token's values), as
 // 2^(s log2(e) + log2(vs) - reference): the product with the scale costs no instruction of its own, the weights stay within a

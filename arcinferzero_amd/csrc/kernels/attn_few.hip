@@ -147,7 +147,7 @@ __device__ inline void few_body(const float* __restrict__ q, int ldq, int q_off,
     big = fmaxf(big, __shfl_xor(big, 32));
     const int e2 = min(max(137 - (int)(__float_as_uint(big) >> 23), -100), 100);
     const float up = __uint_as_float((uint32_t)(127 + e2) << 23), down = __uint_as_float((uint32_t)(127 - e2) << 23);
-    kfac[t] = (CAP ? 2.0f * LOG2E * LOG2E / cap2 : LOG2E) * scale * down;   // (cap2 = cap log2 e)
+    kfac[t] = (CAP ? LOG2E / cap2 : LOG2E) * scale * down;   // (cap2 = cap log2 e)
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       h8 a, b;
@@ -207,15 +207,21 @@ __device__ inline void few_body(const float* __restrict__ q, int ldq, int q_off,
       }
       const int j0 = base + st * 32 + tile * 16;
 #pragma unroll
-      for (int t = 0; t < RT; ++t)
+      for (int t = 0; t < RT; ++t) {
+        float v[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float kf = kv[r] * kfac[t];
-          float v = PACK ? plus_8(sc[t][r]) : sc[t][r];
-          v = CAP ? capped<true>(v * kf, cap2) + lv[r] : fmaf(v, kf, lv[r]);
-          if (BIAS) v = fmaf(-slope[t], fabsf((float)(pos[t] - (j0 + g * 4 + r))), v);
-          t8[t][tile * 4 + r] = v;
+          v[r] = PACK ? plus_8(sc[t][r]) : sc[t][r];
+          v[r] = CAP ? v[r] * (kv[r] * kfac[t]) : fmaf(v[r], kv[r] * kfac[t], lv[r]);
         }
+        if (CAP) cap_scores(v, cap2);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (CAP) v[r] += lv[r];
+          if (BIAS) v[r] = fmaf(-slope[t], fabsf((float)(pos[t] - (j0 + g * 4 + r))), v[r]);
+          t8[t][tile * 4 + r] = v[r];
+        }
+      }
       const bool there = (uint32_t)pg[tile] < (uint32_t)pages;
       if (!there || j0 < lo_max || j0 + 16 > hi_min) {
 #pragma unroll

@@ -125,7 +125,7 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   all_hi = __builtin_amdgcn_readfirstlane(all_hi);
   const int e2 = min(max(137 - (int)(big >> 23), -100), 100);   // (the largest of the work-group's rows to 2^10 ... 2^11)
   const float up = __uint_as_float((uint32_t)(127 + e2) << 23), down = __uint_as_float((uint32_t)(127 - e2) << 23);
-  const float kfac = (CAP ? 2.0f * LOG2E * LOG2E / cap2 : LOG2E) * scale * down;   // (cap2 = cap log2 e)
+  const float kfac = (CAP ? LOG2E / cap2 : LOG2E) * scale * down;   // (cap2 = cap log2 e)
   const float one = opaque_one();
   h8 qh[KSTEPS], ql[QLDS ? 1 : KSTEPS];
   _Float16* const mine = &sq_lo[QLDS ? (wave * 32 + c) * KLD + hf * 8 : 0];
@@ -316,9 +316,21 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float v = sc[4 * b + e];
-          sc[4 * b + e] = CAP ? capped<true>(v * kf[e], cap2) + lv[e] : fmaf(v, kf[e], lv[e]);
+          sc[4 * b + e] = CAP ? sc[4 * b + e] * kf[e] : fmaf(sc[4 * b + e], kf[e], lv[e]);
+          if (CAP) continue;
           if (BIAS) sc[4 * b + e] = fmaf(-slope, fabsf((float)(pos - (j0 + j4 + e))), sc[4 * b + e]);
+        }
+      }
+      if (CAP) {
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = sc[e];
+        cap_scores(v, cap2);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int j4 = nt * 32 + 8 * (e >> 2) + 4 * hf;
+          sc[e] = v[e] + (FINE ? slv[buf][j4 + (e & 3)] - ref : lv1);
+          if (BIAS) sc[e] = fmaf(-slope, fabsf((float)(pos - (j0 + j4 + (e & 3)))), sc[e]);
         }
       }
       if (jn < lo_max || jn + 32 > hi_min) {
@@ -469,8 +481,8 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   }
 }
 
-// -DFINE=1: blocks of less than 32 tokens; -DW8: work-groups of eight waves, 256 rows, where the bytes of a tile are fewer for each
-// thread -- and what the rows take of LDS leaves room for one work-group a compute unit in any case
+// -DFINE=1: blocks of less than 32 tokens; -DW8: work-groups of eight waves, 256 rows, one a compute unit: a tile is staged once for
+// twice the rows (for blocks of 32 tokens and more: with a scale for each key its loop does not fit the registers)
 #define MANY(NAME, HD, KT, NW, W, FINE, F)                                                                                                                      \
   extern "C" __global__ __launch_bounds__(64 * NW, W) void NAME(                                                                                                \
       const float* q, int ldq, int q_off, const int8_t* kq, const int8_t* vq, const float* ks, const float* vs, int pages, int ps, int bs, const int* rows,     \
@@ -489,6 +501,5 @@ MANY4(64, 64, 4, 2, 1, )
 MANY4(128, 32, 4, 2, 0, )
 MANY4(128, 32, 4, 2, 1, )
 MANY4(128, 64, 8, 2, 0, _W81)
-MANY4(128, 64, 8, 2, 1, _W81)
 MANY4(256, 32, 4, 1, 0, )
 MANY4(256, 32, 4, 1, 1, )
