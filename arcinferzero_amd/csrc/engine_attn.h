@@ -224,7 +224,7 @@
   void attention(const Kv& c, const Batch& b, cl_mem q, int ldq, int q_off, int heads, cl_mem out, int ldo, int o_off, const Attn& a) {
     if (!check_batch("attention", c, b)) return;
     if (heads < 1 || heads % c.heads || (int64_t)heads * c.hd > 0x7FFFFFFF) throw std::runtime_error("attention: " + std::to_string(heads) + " heads over " + std::to_string(c.heads) + " of the cache");
-    if (!std::isfinite(a.scale) || !(a.cap >= 0.0f) || !std::isfinite(a.cap) || a.window < 0 || b.max_len < 0)
+    if (!std::isfinite(a.scale) || !(a.cap >= 0.0f) || a.cap > 0x1p100f || (a.cap > 0.0f && a.cap < 0x1p-100f) || a.window < 0 || b.max_len < 0)
       throw std::runtime_error("attention: scale, cap, window or max_len");
     const Rows rq = rows_of("attention: q", q, ldq, q_off, heads * c.hd, b.T), ro = rows_of("attention: out", out, ldo, o_off, heads * c.hd, b.T);
     if (overlap(rq, ro)) throw std::runtime_error("attention: q and out overlap");
@@ -262,9 +262,9 @@
     }
     // Heads of 128 values, blocks of 32 tokens and more: work-groups of eight waves and 256 rows, one a compute unit, where rows are many
     // and see thousands of keys; else of four and 128 rows, two of them, which fill the chip sooner and read and write rows while the
-    // other computes.  (us, 32 heads over 8, eight waves / four: 8192 rows over 9000 keys 1200 / 1249, 4096 over 4096 280 / 297, 512
-    // over 8192 142 / 149; 2048 over 2048 117 / 107, 512 over 512 48 / 36, 100 over 4000 50 / 42, ragged documents 102 / 85; blocks of
-    // 16, 2000 rows over 4000 1354 / 1348)
+    // other computes.  (us, 32 heads over 8, eight waves / four: 1024 rows over 9000
+    // keys 278 / 296, 4096 over 4096 271 / 287, 512 over 8192 144 / 150, 2048 over 16000 895 / 936; of fewer keys, before the rows
+    // passed through LDS: 2048 over 2048 117 / 107, 512 over 512 48 / 36, 100 over 4000 50 / 42, ragged documents 102 / 85.)
     const int seen = std::max(0, (b.max_len > 0 ? b.max_len : ldt * c.page) - most / 2);
     const int waves = c.hd == 128 && c.block >= 32 && M >= 1024 && !a.first && (window ? std::min(window, seen) : seen) >= 2000 ? 8 : 4, bm = 32 * waves;
     int tiles = (int)((M + bm - 1) / bm);

@@ -148,16 +148,19 @@ __device__ inline void cap_scores(float (&v)[N], float cap2) {
 }
 // The scales' part in a score.  A weight is carried as w = p * vs (p = e^(s - reference), vs the scale of the token's values), as
 // 2^(s log2(e) + log2(vs) - reference): the product with the scale costs no instruction of its own, the weights stay within a
-// fixed range whatever the scales are, and the softmax's sum is the sum of w / vs.  A block of zeros (a scale below 2^-120) takes the
-// scale of a block before it instead -- its values are zeros whatever it is -- so that its weights are near the others'; a
-// scale that is no number makes the score none, and its weight nothing where it is masked.
-__device__ inline void value_scale(float vs, float& carry, float& lv, float& iv) {
-  const bool number = vs == vs;
+// fixed range whatever the scales are, and the softmax's sum is the sum of w / vs.  (That sum, of at most 2^31 keys' w <= 2^15, stays in f32
+// for scales from 2^-82 on; the values of a cache that holds smaller ones alone may be read as zeros.)  A block of zeros (a scale below
+// 2^-120) takes the smallest scale that this thread has met, 2^-60 at most, instead -- its values are zeros whatever it is: with a scale
+// above the others' its weights could set the reference and leave the others' f16 nothing, with a smaller one they are small, and
+// count in the sum alone, in f32.  A scale that is no number makes the score none, and its weight nothing where it is masked.
+__device__ inline void value_scale(float vs, float& low, float& lv, float& iv) {
+  const bool number = vs == vs, holds = vs >= 0x1p-120f;
   const float l = __builtin_amdgcn_logf(vs), r = __builtin_amdgcn_rcpf(vs);
-  carry = vs >= 0x1p-120f ? l : carry;
-  lv = number ? carry : vs;
-  iv = vs >= 0x1p-120f ? r : number ? exp2_f(-carry) : 1.0f;
+  low = holds ? fminf(low, l) : low;
+  lv = holds ? l : number ? low : vs;
+  iv = holds ? r : number ? exp2_f(-low) : 1.0f;
 }
+constexpr float LOW = -60.0f;
 // The weights' reference is lowered so that they are at most 2^8 when it is set; it is set anew once one would pass 2^15 (f16
 // ends at 2^16).  With the second f16 of the split a weight keeps an absolute error of 2^-25, 2^-33 of the largest.
 constexpr float SETS = 8.0f, PASSES = 15.0f;

@@ -167,7 +167,7 @@ __device__ inline void few_body(const float* __restrict__ q, int ldq, int q_off,
   }
 
   f4 acc[RT][DT];
-  float ref[RT], sum[RT], carry = -60.0f;
+  float ref[RT], sum[RT], low = LOW;
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     ref[t] = NOTHING;
@@ -200,7 +200,7 @@ __device__ inline void few_body(const float* __restrict__ q, int ldq, int q_off,
       for (int r = 0; r < 4; ++r) {
         if (FINE || r == 0) {
           kv[r] = ksb[tile][FINE ? r : 0];
-          value_scale(vsb[tile][FINE ? r : 0], carry, lv[r], iv[tile * 4 + r]);
+          value_scale(vsb[tile][FINE ? r : 0], low, lv[r], iv[tile * 4 + r]);
         } else {
           kv[r] = kv[0]; lv[r] = lv[0]; iv[tile * 4 + r] = iv[tile * 4];
         }

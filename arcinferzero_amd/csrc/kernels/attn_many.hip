@@ -206,7 +206,7 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
 #pragma unroll
       for (int w = 0; w < VB / 4; ++w) asm volatile("" : "+v"(vr[t][w]));
   };
-  float carry = -60.0f;
+  float low = LOW;
   // ... to LDS in UNITS parts: half a key's 16 bytes each, then two columns of the four tokens each
   constexpr int KU = KB / 8, UNITS = KU + VB / 2;
   auto store = [&](int buf, int u) {
@@ -231,7 +231,7 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   auto store_scales = [&](int buf, int pc) {
     if (threadIdx.x < NS) {   // (a token of no page: weight 0 whatever its score)
       float lv, iv;
-      value_scale(rvs, carry, lv, iv);
+      value_scale(rvs, low, lv, iv);
       const bool there = (uint32_t)pc < (uint32_t)pages;
       skf[buf][threadIdx.x] = there ? rks * kfac : 0.0f;
       slv[buf][threadIdx.x] = there ? lv : -INFINITY;

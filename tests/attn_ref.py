@@ -89,7 +89,8 @@ def attention(cache, q, rows, lens, table, scale, cap=0.0, window=0, slopes=None
 
     A weight times its values' scale is held in two f16, whose last place ends at 2^-24; the row's largest is at least 2^8 there.  So
     every key adds its 8-bit value times up to 2^-32 of the row's largest weight times scale -- what is left of the error where the
-    keys that count hold a zero in some column."""
+    keys that count hold a zero in some column.  A block of zeros has a weight there too, its own times a scale of at most 2^-60:
+    where such blocks have all of a row's weight, the f16 of the other keys, whose parts are then less than 2^-60 of it, end at that."""
     T, H, hd = q.shape
     G = H // cache.heads
     out, tol, done = np.zeros((T, H, hd)), np.zeros((T, H, hd)), np.zeros(T, bool)
@@ -135,7 +136,7 @@ def attention(cache, q, rows, lens, table, scale, cap=0.0, window=0, slopes=None
                     tol[t, h] = (e * rel) @ np.abs(vv[:, g] - out[t, h]) + np.abs(out[t, h]) * 2.0 ** -20 + (e @ np.abs(vv[:, g])) * 2.0 ** -21
                     d = vs[see, g]
                     ints = np.abs(np.divide(vv[:, g], d[:, None], out=np.zeros_like(vv[:, g]), where=d[:, None] > 0))
-                    tol[t, h] += 2.0 ** -32 * np.max(e * d) * ints.sum(0)
+                    tol[t, h] += 2.0 ** -32 * np.max(e * np.where(d > 0, d, 2.0 ** -60)) * ints.sum(0)
     return out, tol, done
 
 

@@ -220,6 +220,46 @@ def test_scales_of_every_size(eng, seqs, kind):
     check(eng, seqs, 8, 2, 128, page, block, b=b, c=c)
 
 
+@pytest.mark.parametrize("seqs", [[(1, 400), (1, 330)], [(70, 400), (30, 330)]])
+@pytest.mark.parametrize("block", [1, 8, 32])
+def test_zero_blocks_behind_an_outlier(eng, seqs, block):
+    """Blocks of zeros behind keys of huge scales that hardly count or are not seen: the other keys' weights stay what they are."""
+    page = 32
+    b = ref.Batch(seqs, page, seed=2)
+    rng = np.random.default_rng(8)
+
+    def cache(scale):
+        c = ref.Cache(b.pages, page, block, 2, 128, seed=3)
+        c.d[1][rng.random(c.d[1].shape) < 0.4] = 0.0
+        for s in range(len(seqs)):
+            c.d[1][b.table[s, :4]] = scale
+        c.q[1].reshape(c.d[1].shape + (block, 128))[c.d[1] == 0.0] = 0
+        return c
+    # (the row's own distance: 2^60 e^-140 and less of the others' weights)
+    check(eng, seqs, 8, 2, 128, page, block, dict(slopes=np.ones(8)), b=b, c=cache(2.0 ** 60))
+    first = np.full(b.T, 4 * page + 3)
+    for huge in (2.0 ** 60, 3e38, np.inf):
+        c = cache(huge)
+        want = ref.Cache(b.pages, page, block, 2, 128, seed=3)
+        want.q, want.d = c.q.copy(), c.d.copy()
+        for s in range(len(seqs)):
+            want.d[1][b.table[s, :5]] = 0.0
+            c.d[1][b.table[s, 4]] = huge
+        for f in (dict(first=first + page - 3), dict(first=np.full(b.T, 5 * page - 1))):
+            if f["first"][0] == 5 * page - 1:     # (the last key of the spoiled page is seen: as zeros in both)
+                for x in (c, want):
+                    for s in range(len(seqs)):
+                        x.d[1][b.table[s, 4], :, -1] = 0.0
+                        x.q[1][b.table[s, 4], :, -block:] = 0
+            f = dict(f, scale=0.09)
+            q = np.random.default_rng(4).standard_normal((b.T, 1024)).astype(np.float32)
+            hold = []
+            a, _ = run(eng, want, b, q, 1024, 0, 8, f, hold)
+            g, _ = run(eng, c, b, q, 1024, 0, 8, f, hold)
+            assert np.array_equal(a, g)
+            ref.free(hold)
+
+
 @pytest.mark.parametrize("seqs", [[(1, 300), (2, 40)], [(70, 300), (30, 30)]])
 @pytest.mark.parametrize("q_std", [0.0, 1e-6, 40.0, 1e3, 1e-30, 1e30])
 def test_rows_of_every_size(eng, seqs, q_std):
@@ -303,6 +343,24 @@ def test_same_bits_again_and_in_another_batch(eng, seqs):
     three, _ = run(eng, x, b, q, 1024, 0, 8, dict(scale=0.09), hold)
     assert np.array_equal(one, three)
     ref.free(hold)
+
+
+def test_caps_that_are_refused(eng):
+    """A cap's part of a score is formed in f32."""
+    kv = eng.make_kv(2, 16, 16, 2, 64)
+    i = az.Runtime.from_numpy(np.zeros(8, np.int32))
+    x, y = az.Runtime.alloc(4 * 256), az.Runtime.alloc(4 * 256)
+    for cap in (1e-38, 1e-45, 2.0 ** 101, 3e38):
+        with pytest.raises(az.ArczError):
+            eng.attention(kv, az.KvBatch(i, i, i, 1, 2, 1, 1), x, 256, 0, 4, y, 256, 0, az.Attention(0.1, cap=cap))
+    for b in (kv, i, x, y):
+        b.free()
+
+
+@pytest.mark.parametrize("cap", [2.0 ** -100, 1e-6, 1e12, 2.0 ** 100])
+def test_smallest_and_largest_caps(eng, cap):
+    check(eng, [(1, 90), (40, 60)], 4, 2, 64, 16, 16, dict(cap=cap))
+    check(eng, [(1, 90), (2, 60)], 4, 2, 64, 16, 16, dict(cap=cap))
 
 
 def test_refusals(eng):
