@@ -9,6 +9,12 @@
 //   O^T += V^T P^T  A = 16 of the head's values, B = the weights just as the scores' product left them: a lane's eight keys of
 //                  two tiles are the eight of its k slot, so the weights go from one product into the other in registers
 //
+// Pieces of one length for all sequences, about two work-groups a compute unit where all are long; they are joined in this launch by the
+// last work-group of their rows to come (joined by a launch of its own: 41 us more behind 131072 keys).
+// Measured, heads of 128 values: one token behind 131072, 40 heads over 8, 56.6 us (4.75 TB/s, a large copy 4.9); 64
+// sequences of up to 8100 keys, 32 over 4, 76.5 us (3.8 TB/s); one behind 517, 9.0 us, and four sequences of eight tokens with heads of
+// 256 under a window 15.9 us: dependent loads -- rows, page, bytes -- and the joining, not bytes.
+//
 // The eight-bit values are exact in f16.  Rows and weights are split into two f16 each (22 bits), so the sums are those of f32
 // rows to about 2^-22.  Up to eight rows both parts go through one product: the first parts in columns 0-7, what they miss in
 // 8-15.
@@ -388,7 +394,7 @@ __device__ inline void few_body(const float* __restrict__ q, int ldq, int q_off,
     if (k * 256 + threadIdx.x < M * (HD / 4)) put(ur[k], ud[k], o[k], l[k]);
 }
 
-// The pieces of the rows of attn_many joined, a work-group 256 / (hd / 4) rows.  grid (row blocks x sequences x kv heads, row groups)
+// The pieces of the rows of attn_many joined, a work-group 256 / (hd / 4) rows: 4 hd bytes a row and piece, read once.  grid (row blocks x sequences x kv heads, row groups)
 //   ws: per (block of rows_of rows of a sequence and kv head) nsplit pieces.
 extern "C" __global__ __launch_bounds__(256) void attn_join(const float* __restrict__ ws, int nsplit, int rows_of, int blocks, int hd, const int* __restrict__ rows,
                                                             const int* __restrict__ lens, int most_len, int T, int max_rows, int heads, int kvh,
