@@ -1,6 +1,7 @@
 """The attention block's operators together, as a forward pass uses them: behind the q|k|v product, in front of the output projection; in
 launch lists; on buffers of another allocator."""
 import ctypes as C
+import importlib.util
 import os
 import subprocess
 import sys
@@ -206,7 +207,8 @@ def test_two_engines_and_profile(eng):
 
 def test_buffers_of_another_allocator(eng):
     """Tensors of torch as buffers (below, in a process of its own)."""
-    pytest.importorskip("torch")
+    if importlib.util.find_spec("torch") is None:   # (not imported here: a second HIP runtime under the first one's name)
+        pytest.skip("no torch")
     r = subprocess.run([sys.executable, os.path.abspath(__file__)], capture_output=True, text=True, timeout=110)
     assert r.returncode == 0 and "tensors as buffers: ok" in r.stdout, r.stdout[-2000:] + r.stderr[-4000:]
 
