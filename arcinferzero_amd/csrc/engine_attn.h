@@ -249,7 +249,7 @@
       // compute unit if every sequence has the most keys, of at least 256 keys each.
       const size_t want = ((size_t)2 * arcz_device_cus() + pairs - 1) / pairs;
       int least = (int)std::max<size_t>(8, ((size_t)(keys + 31) / 32 + want - 1) / want);
-      nsplit = (keys + 32 * least - 1) / (32 * least);
+      nsplit = (int)(((int64_t)keys + (int64_t)32 * least - 1) / ((int64_t)32 * least));
       cl_mem w = nsplit > 1 ? at_ws(pairs * nsplit * rows * (c.hd + 2) * 4) : nullptr, counts = nsplit > 1 ? at_counts(pairs) : nullptr;
       if (pairs > 0xFFFFFFFFull / 256) throw std::runtime_error("attention: too many sequences");
       vec &= 1;

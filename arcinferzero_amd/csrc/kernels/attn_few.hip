@@ -75,8 +75,8 @@ __device__ inline void few_body(const float* __restrict__ q, int ldq, int q_off,
     all_hi = __builtin_amdgcn_readfirstlane(all_hi);
   }
   const attn::Span span = attn::span_of(all_lo, all_hi, 32);
-  const int base = span.base, steps = span.steps;
-  const int share = max((steps + nsplit - 1) / nsplit, least), z0 = min((int)blockIdx.y * share, steps), z1 = min(z0 + share, steps);
+  const attn::Part part = attn::part_of(span.steps, nsplit, least, blockIdx.y);
+  const int base = span.base, z0 = part.z0, z1 = part.z1;
 
   // (of keys behind the last: some entry of the table -- no row sees them.  Nothing is done with an entry here, so that a lookup is
   //  not waited for before the bytes are asked for)

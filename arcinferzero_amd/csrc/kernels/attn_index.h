@@ -45,6 +45,17 @@ ATTN_FN Span span_of(int lo, int hi, int unit) {
   }
   return s;
 }
+// The steps [z0, z1) of piece z of `pieces`, at least `least` to a piece that has any (behind the last step: none, from there on).
+struct Part {
+  int z0, z1;
+};
+ATTN_FN Part part_of(int steps, int pieces, int least, int z) {
+  const int share = upper((steps + pieces - 1) / pieces, least);
+  Part p;
+  p.z0 = lower(z * share, steps);
+  p.z1 = lower(p.z0 + share, steps);
+  return p;
+}
 // Where the table has the page of a position: within its row of ldt entries also for a position behind the last key (up to 4096
 // behind it; most_len is at most 2^31 - 4096).
 ATTN_FN int entry_of(int p, int ps, int ldt) { return lower(p >> ps, ldt - 1); }

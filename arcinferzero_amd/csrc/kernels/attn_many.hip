@@ -150,8 +150,9 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
 
   // ---- this work-group's tiles of keys
   const attn::Span span = attn::span_of(all_lo, all_hi, KT);
-  const int base = span.base, steps = span.steps;
-  const int share = (steps + nsplit - 1) / nsplit, z0 = blockIdx.y * share, z1 = min(z0 + share, steps);
+  const int base = span.base;
+  const attn::Part part = attn::part_of(span.steps, nsplit, 1, blockIdx.y);
+  const int z0 = part.z0, z1 = part.z1;
 
   // this thread's key and its bytes 16 kc, 16 (kc + TPK), ...; its four tokens and VB bytes of each.  (Threads side by side write
   // side by side in LDS: a key's 16-byte pieces dealt out in turn, the tokens of one column.)

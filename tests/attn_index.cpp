@@ -52,6 +52,15 @@ int main() {
       // the last work-group's steps and what it looks up ahead of them: up to 12 steps of 32 (three waves on, two rounds ahead), or
       // two tiles of 64
       const int last = s.steps, ahead = unit == 32 ? 12 : 2;
+      // (pieces: one behind the other, the last to the end; what a piece without steps looks up is no further than that)
+      const int pieces = 1 + (int)(rng() % 1024), least = rng() % 2 ? 1 : 1 + (int)(rng() % 64);
+      int behind = 0;
+      for (int z = 0; z < pieces; ++z) {
+        const attn::Part p = attn::part_of(s.steps, pieces, least, z);
+        NEED(p.z0 == behind && p.z0 <= p.z1 && p.z1 <= s.steps);
+        behind = p.z1;
+      }
+      NEED(behind == s.steps);
       for (int st : {0, 1, last / 2, last - 1, last, last + ahead}) {
         if (st < 0) continue;
         for (int t = 0; t < unit; t += 4) {

@@ -326,6 +326,27 @@ def test_far_pages(eng):
         ref.free(hold)
 
 
+@pytest.mark.parametrize("rows", [1, 2, 40])
+@pytest.mark.parametrize("form", ["first", "window"])
+def test_the_last_positions_there_are(eng, rows, form):
+    """The end of the longest sequence that a table can name: what a row sees there is what it would see at the end of a short one."""
+    page, seen, long = 256, 300, 0x7FFFF000
+    b = ref.Batch([(rows, 3 * page)], page, seed=1, ld_extra=0)
+    c = ref.Cache(b.pages, page, 32, 2, 128, seed=3)
+    q = np.random.default_rng(4).standard_normal((rows, 1024)).astype(np.float32)
+    f = dict(scale=0.09, window=seen) if form == "window" else dict(scale=0.09, first=np.full(rows, 3 * page - seen))
+    want, tol, _ = ref.attention(c, q.reshape(rows, 8, 128), b.rows, b.lens, b.table, **f)
+    tail, b.table = b.table, np.full((1, long // page), -1, np.int32)
+    b.table[0, -3:] = tail
+    b.ldt, b.lens, b.max_len = long // page, np.array([long], np.int32), long
+    if form == "first":
+        f["first"] = np.full(rows, long - seen)
+    hold = []
+    got, _ = run(eng, c, b, q, 1024, 0, 8, f, hold)
+    assert (np.abs(got - want) <= tol).all()
+    ref.free(hold)
+
+
 @pytest.mark.parametrize("seqs", [[(1, 900), (1, 33)], [(70, 300), (30, 30)]])
 def test_same_bits_again_and_in_another_batch(eng, seqs):
     """The same call gives the same bits; so does the first sequence's call with other pages in another order."""
