@@ -65,48 +65,11 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   sees(pos, sq.len, window, prefix ? prefix[s] : 0, first ? first[sq.r0 + i] : 0, lo, hi);
   if (r >= M) hi = lo = 0;
   const float slope = BIAS ? slopes[hq] * LOG2E : 0.0f;
-  // The rows come, and go, 64 columns at a time through LDS: four rows' 256 bytes a load, where a lane's own 16 bytes of 32 rows
-  // would be 64 places.  A lane moves 16 bytes of rows 4 n + lane / 16.
-  float* const pass = (float*)&tl2 + wave * 32 * SLD;
-  const int quarter = lane >> 4, col = (lane & 15) * 4;
-  auto of_row = [&](long v, int n) { return (long)__shfl((long long)v, n * 4 + quarter); };
-  uint32_t big = 0;
-  float x[KSTEPS][8];
-  {
-    const long from = (long)(sq.r0 + i) * ldq + q_off + hq * HD;
-#pragma unroll
-    for (int cc = 0; cc < HD / 64; ++cc) {
-      float4 u[8];
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        const float* a = q + of_row(from, n) + cc * 64 + col;
-        u[n] = vec & 1 ? *(const float4*)a : make_float4(a[0], a[1], a[2], a[3]);
-      }
-#pragma unroll
-      for (int n = 0; n < 8; ++n) *(float4*)&pass[(n * 4 + quarter) * SLD + col] = u[n];
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");   // (among the wave's lanes)
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float4 a = *(const float4*)&pass[c * SLD + k * 16 + hf * 8], b = *(const float4*)&pass[c * SLD + k * 16 + hf * 8 + 4];
-        float (&y)[8] = x[cc * 4 + k];
-        y[0] = a.x; y[1] = a.y; y[2] = a.z; y[3] = a.w; y[4] = b.x; y[5] = b.y; y[6] = b.z; y[7] = b.w;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t b2 = __float_as_uint(y[e]) & 0x7FFFFFFFu;
-          if (b2 < 0x7F800000u) big = max(big, b2);
-        }
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-      __builtin_amdgcn_wave_barrier();
-    }
-  }
   // (rows that see nothing take no part in the wave's range)
   int lo_min = lo < hi ? lo : 0x7FFFFFFF, lo_max = lo < hi ? lo : 0, hi_min = lo < hi ? hi : 0x7FFFFFFF, hi_max = lo < hi ? hi : 0;
   int blind = lo < hi ? 0 : 1;
 #pragma unroll
   for (int o = 1; o < 64; o *= 2) {
-    big = max(big, (uint32_t)__shfl_xor((int)big, o));
     lo_min = min(lo_min, __shfl_xor(lo_min, o));
     lo_max = max(lo_max, __shfl_xor(lo_max, o));
     hi_min = min(hi_min, __shfl_xor(hi_min, o));
@@ -117,36 +80,17 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   lo_min = __builtin_amdgcn_readfirstlane(lo_min); lo_max = __builtin_amdgcn_readfirstlane(lo_max);
   hi_min = __builtin_amdgcn_readfirstlane(hi_min); hi_max = __builtin_amdgcn_readfirstlane(hi_max);
   if (lane == 0) {
-    red[wave][0] = (int)big; red[wave][1] = lo_min; red[wave][2] = hi_max;
+    red[wave][0] = lo_min; red[wave][1] = hi_max;
   }
   __syncthreads();
-  int all_lo = red[0][1], all_hi = red[0][2];
+  int all_lo = red[0][0], all_hi = red[0][1];
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
-    big = max(big, (uint32_t)red[w][0]);
-    all_lo = min(all_lo, red[w][1]);
-    all_hi = max(all_hi, red[w][2]);
+    all_lo = min(all_lo, red[w][0]);
+    all_hi = max(all_hi, red[w][1]);
   }
   all_lo = __builtin_amdgcn_readfirstlane(all_lo);
   all_hi = __builtin_amdgcn_readfirstlane(all_hi);
-  const int e2 = min(max(137 - (int)(big >> 23), -100), 100);   // (the largest of the work-group's rows to 2^10 ... 2^11)
-  const float up = __uint_as_float((uint32_t)(127 + e2) << 23), down = __uint_as_float((uint32_t)(127 - e2) << 23);
-  const float kfac = (CAP ? LOG2E / cap2 : LOG2E) * scale * down;   // (cap2 = cap log2 e)
-  const float one = opaque_one();
-  h8 qh[KSTEPS], ql[QLDS ? 1 : KSTEPS];
-  _Float16* const mine = &sq_lo[QLDS ? (wave * 32 + c) * KLD + hf * 8 : 0];
-#pragma unroll
-  for (int k = 0; k < KSTEPS; ++k) {
-    h8 lo8;
-#pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      h2 a, b;
-      split2(x[k][e] * up, x[k][e + 1] * up, one, a, b);
-      qh[k][e] = a.x; qh[k][e + 1] = a.y; lo8[e] = b.x; lo8[e + 1] = b.y;
-    }
-    if (QLDS) *(h8*)(mine + k * 16) = lo8;
-    else ql[QLDS ? 0 : k] = lo8;
-  }
 
   // ---- this work-group's tiles of keys
   const attn::Span span = attn::span_of(all_lo, all_hi, KT);
@@ -204,6 +148,89 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
       rvs = *(const float*)((const char*)vs + sa);
     }
   };
+  // (looked up through vector memory, also where all threads have the same page: a wait for a scalar load among the LDS reads
+  //  would be a wait for all of them)
+  int zero;
+  asm("v_mov_b32 %0, 0" : "=v"(zero));
+  const int tl = whole ? zero : tk;
+  auto look = [&](int st) {   // (with whole pages the other two are left alone: writing them would wait for all loads on the way)
+    at.k = page_at(st, tl);
+    if (!whole) {
+      at.v = page_at(st, tv);
+      at.c = page_at(st, ts);
+    }
+  };
+  // (the first tile's way is begun before the rows': they come together)
+  look(z0);
+  int pc0 = 0;
+
+  // The rows come, and go, 64 columns at a time through LDS: four rows' 256 bytes a load, where a lane's own 16 bytes of 32 rows
+  // would be 64 places.  A lane moves 16 bytes of rows 4 n + lane / 16.
+  float* const pass = (float*)&tl2 + wave * 32 * SLD;
+  const int quarter = lane >> 4, col = (lane & 15) * 4;
+  auto of_row = [&](long v, int n) { return (long)__shfl((long long)v, n * 4 + quarter); };
+  uint32_t big = 0;
+  float x[KSTEPS][8];
+  {
+    const long from = (long)(sq.r0 + i) * ldq + q_off + hq * HD;
+#pragma unroll
+    for (int cc = 0; cc < HD / 64; ++cc) {
+      float4 u[8];
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const float* a = q + of_row(from, n) + cc * 64 + col;
+        u[n] = vec & 1 ? *(const float4*)a : make_float4(a[0], a[1], a[2], a[3]);
+      }
+      if (cc == 0 && z0 < z1) {
+        pc0 = address(z0);
+#pragma unroll
+        for (int part = 0; part < 4; ++part) load(part);
+        look(z0 + 1);
+      }
+#pragma unroll
+      for (int n = 0; n < 8; ++n) *(float4*)&pass[(n * 4 + quarter) * SLD + col] = u[n];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");   // (among the wave's lanes)
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float4 a = *(const float4*)&pass[c * SLD + k * 16 + hf * 8], b = *(const float4*)&pass[c * SLD + k * 16 + hf * 8 + 4];
+        float (&y)[8] = x[cc * 4 + k];
+        y[0] = a.x; y[1] = a.y; y[2] = a.z; y[3] = a.w; y[4] = b.x; y[5] = b.y; y[6] = b.z; y[7] = b.w;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t b2 = __float_as_uint(y[e]) & 0x7FFFFFFFu;
+          if (b2 < 0x7F800000u) big = max(big, b2);
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) big = max(big, (uint32_t)__shfl_xor((int)big, o));
+  if (lane == 0) red[wave][2] = (int)big;
+  __syncthreads();   // (and all rows have passed through the tiles' place)
+#pragma unroll
+  for (int w = 0; w < NW; ++w) big = max(big, (uint32_t)red[w][2]);
+  const int e2 = min(max(137 - (int)(big >> 23), -100), 100);   // (the largest of the work-group's rows to 2^10 ... 2^11)
+  const float up = __uint_as_float((uint32_t)(127 + e2) << 23), down = __uint_as_float((uint32_t)(127 - e2) << 23);
+  const float kfac = (CAP ? LOG2E / cap2 : LOG2E) * scale * down;   // (cap2 = cap log2 e)
+  const float one = opaque_one();
+  h8 qh[KSTEPS], ql[QLDS ? 1 : KSTEPS];
+  _Float16* const mine = &sq_lo[QLDS ? (wave * 32 + c) * KLD + hf * 8 : 0];
+#pragma unroll
+  for (int k = 0; k < KSTEPS; ++k) {
+    h8 lo8;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      h2 a, b;
+      split2(x[k][e] * up, x[k][e + 1] * up, one, a, b);
+      qh[k][e] = a.x; qh[k][e + 1] = a.y; lo8[e] = b.x; lo8[e + 1] = b.y;
+    }
+    if (QLDS) *(h8*)(mine + k * 16) = lo8;
+    else ql[QLDS ? 0 : k] = lo8;
+  }
+
   // (the bytes are waited for here: what is done with them in two branches is not brought in front of both)
   auto arrive = [&] {
 #pragma unroll
@@ -254,28 +281,11 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   // (a row's weights are 2^(score - ref); before the first score that it sees ref is 0 and any score sets it)
   float ref = 0.0f, limit = NOTHING, sum = 0.0f;
 
-  // (looked up through vector memory, also where all threads have the same page: a wait for a scalar load among the LDS reads
-  //  would be a wait for all of them)
-  int zero;
-  asm("v_mov_b32 %0, 0" : "=v"(zero));
-  const int tl = whole ? zero : tk;
-  auto look = [&](int st) {   // (with whole pages the other two are left alone: writing them would wait for all loads on the way)
-    at.k = page_at(st, tl);
-    if (!whole) {
-      at.v = page_at(st, tv);
-      at.c = page_at(st, ts);
-    }
-  };
-  look(z0);
   if (z0 < z1) {
-    const int pc = address(z0);
-#pragma unroll
-    for (int part = 0; part < 4; ++part) load(part);
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) store(0, u);
-    store_scales(0, pc);
+    store_scales(0, pc0);
   }
-  look(z0 + 1);
   __syncthreads();
   for (int st = z0; st < z1; ++st) {
     const int buf = (st - z0) & 1;
