@@ -56,6 +56,12 @@ ATTN_FN Part part_of(int steps, int pieces, int least, int z) {
   p.z1 = lower(p.z0 + share, steps);
   return p;
 }
+// Where the i-th tile of `tile` positions (a power of two) from a whole one on begins, for rows at [from, to); -1: there is none.  (Work-groups
+// are launched for the most rows of any sequence: i * tile alone may lead past 2^31.)
+ATTN_FN int tile_at(int from, int to, int tile, int i) {
+  const int t0 = from & -tile;
+  return from < to && i <= (to - 1 - t0) / tile ? t0 + i * tile : -1;
+}
 // Where the table has the page of a position: within its row of ldt entries also for a position behind the last key (up to 4096
 // behind it; most_len is at most 2^31 - 4096).
 ATTN_FN int entry_of(int p, int ps, int ldt) { return lower(p >> ps, ldt - 1); }

@@ -27,8 +27,8 @@ __device__ inline void kv_write_body(const float* __restrict__ x, int ld, int of
   const int h = blockIdx.z >> 1, lane = threadIdx.x % TPR, r0 = threadIdx.x / TPR, pm = (1 << ps) - 1;
   // (rows whose positions lie below 0 have no place)
   const int from = max(sq.p0, 0), to = sq.p0 + sq.n;
-  const int t0 = (from & -tile) + blockIdx.x * tile, block = 1 << bs, nb = (tile + block - 1) >> bs, end = min(t0 + tile, to);
-  if (t0 >= to) return;
+  const int t0 = attn::tile_at(from, to, tile, blockIdx.x), block = 1 << bs, nb = (tile + block - 1) >> bs, end = min(t0 + tile, to);
+  if (t0 < 0) return;
   const int ntab = ((end - 1) >> ps) - (t0 >> ps) + 1;   // (at most tile / 16 + 1)
   for (int b = threadIdx.x; b < ntab; b += 256) page[b] = table[(t0 >> ps) + b];
   for (int b = threadIdx.x; b < nb; b += 256) top[b] = 0;

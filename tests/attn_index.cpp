@@ -70,7 +70,18 @@ int main() {
         }
       }
     }
-    // kv_write and kv_read: positions of rows
+    // kv_write and kv_read: positions of rows, and tiles of them up to the last that is launched for 2^30 rows
+    const int from = attn::upper(q.p0, 0), to = q.p0 + q.n, tile = 1 << (rng() % 9);
+    int next = from & -tile;
+    for (int i = 0; i < 302; ++i) {
+      const int t0 = attn::tile_at(from, to, tile, i);
+      NEED(from < to && next < to ? t0 == next : t0 == -1);
+      if (t0 >= 0) {
+        NEED((t0 >> ps) >= 0 && (attn::lower(t0 + tile, to) - 1) >> ps < ldt);
+        next += tile;
+      }
+    }
+    for (int i : {1000, 1 << 20, (1 << 30) / tile + 1}) NEED(attn::tile_at(from, to, tile, i) == -1);
     for (int i = 0; i < q.n; ++i)
       if (q.p0 + i >= 0) NEED((q.p0 + i) >> ps < ldt);
   }

@@ -189,6 +189,35 @@ def test_far_pages(eng):
     ref.free(hold)
 
 
+@pytest.mark.parametrize("hd", [64, 256])
+def test_the_last_positions_there_are(eng, hd):
+    """Rows at the end of the longest sequence that a table can name, in a batch whose longest is told to be far longer."""
+    page, long, rows, w = 256, 0x7FFFF000, 5, 2 * hd
+    b = ref.Batch([(rows, 3 * page)], page, seed=1, ld_extra=0, T=rows + 20000, max_rows=rows + 20000)
+    c = ref.Cache(b.pages, page, 32, 2, hd, seed=2)
+    x = rows_of(b.T, 2 * w, seed=3)
+    hold = []
+    kv, xb = ref.device_cache(eng, c, hold), az.Runtime.from_numpy(x)
+    yb = az.Runtime.from_numpy(np.full(x.shape, 7.5, np.float32))
+    hold += [xb, yb]
+    for which in (0, 1):
+        c.write(which, b.table[0], 3 * page - rows, x[:rows, which * w:which * w + w].reshape(rows, 2, hd))
+    tail, b.table = b.table, np.full((1, long // page), -1, np.int32)
+    b.table[0, -3:] = tail
+    b.ldt, b.lens = long // page, np.array([long], np.int32)
+    batch = b.device(hold)
+    eng.kv_write(kv, batch, xb, 2 * w, 0, xb, 2 * w, w)
+    q, d = ref.read_cache(kv, c)
+    assert np.array_equal(d, c.d) and np.array_equal(q, c.q)
+    eng.kv_read(kv, batch, yb, 2 * w, 0, yb, 2 * w, w)
+    y = yb.read(np.float32, x.size).reshape(x.shape)
+    for which in (0, 1):
+        v = c.values(which, tail[0], 3 * page)[-rows:].reshape(rows, w)
+        assert np.array_equal(y[:rows, which * w:which * w + w], v.astype(np.float32))
+    assert (y[rows:] == 7.5).all()
+    ref.free(hold)
+
+
 def test_refusals(eng):
     for pages, page, block, heads, hd in [(0, 16, 1, 1, 64), (1, 8, 1, 1, 64), (1, 48, 16, 1, 64), (1, 512, 1, 1, 64), (1, 16, 32, 1, 64), (1, 16, 3, 1, 64),
                                           (1, 16, 0, 1, 64), (1, 16, 1, 0, 64), (1, 16, 1, 1, 80), (1, 16, 1, 40000, 64)]:
