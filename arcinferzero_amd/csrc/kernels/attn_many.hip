@@ -13,8 +13,8 @@
 // anew.  Rows and weights are split into two f16 (22 bits of the f32 value; the sums are those of f32 rows to about 2^-22), so
 // the matrix pipe does twice the products of plain f16 rows; it is what bounds the kernel.
 //
-// Measured, 32 query heads over 8 of 128 values: 8192 rows behind 808 keys, causal, 1118 - 1144 us = 575 - 587 TFLOP/s of attention,
-// 1150 - 1174 of products (a large f16 matrix product of the library: 1211); the matrix pipe is busy 61 % of the cycles at the clock
+// Measured, 32 query heads over 8 of 128 values: 8192 rows behind 808 keys, causal, 1118 - 1184 us = 556 - 587 TFLOP/s of attention,
+// 1112 - 1174 of products (a large f16 matrix product of the library: 1211); the matrix pipe is busy 61 % of the cycles at the clock
 // that it then holds.  On the way there: 2000 us with the tiles' rows 8 and 16 bytes apart in the same banks (conflicts in 64 % of the
 // LDS's cycles, now 0.3 %); 1303 with the rows that see the most keys first; 1141 with no wait for a page's number inside the loop.
 // Rows of several documents (1333 rows, 40 heads): 68.6 us, the matrix pipe busy 22 %: most tiles are one document's end.
