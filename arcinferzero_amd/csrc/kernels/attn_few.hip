@@ -255,11 +255,12 @@ __device__ inline void few_body(const float* __restrict__ q, int ldq, int q_off,
 #pragma unroll
         for (int i = 0; i < DT; ++i) acc[t][i] *= f;
       }
+      float part = 0.0f;   // (the row's sum is rounded once a step, like the sums of values, not once a key)
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         const float a = exp2_f(t8[t][e] - ref[t]), b = exp2_f(t8[t][e + 1] - ref[t]);
-        sum[t] = fmaf(a, iv[e], sum[t]);
-        sum[t] = fmaf(b, iv[e + 1], sum[t]);
+        part = fmaf(a, iv[e], part);
+        part = fmaf(b, iv[e + 1], part);
         h2 u, w;
         split2(a, b, one, u, w);
         if (PACK) {
@@ -270,6 +271,7 @@ __device__ inline void few_body(const float* __restrict__ q, int ldq, int q_off,
           pl[t][e] = w.x; pl[t][e + 1] = w.y;
         }
       }
+      sum[t] += part;
     }
     // values
 #pragma unroll

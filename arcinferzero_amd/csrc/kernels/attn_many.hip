@@ -377,14 +377,15 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
       }
       return 1.0f;
     };
-    // two weights of a part (of eight pairs)
-    auto weigh = [&](int nt, const f16v& sc, int p, float iv1, h8 (&ph)[2], h8 (&pl)[2]) {
+    // Two weights of a part (of eight pairs); their sum apart from the row's: that is rounded once a part, like the sums of values, not
+    // once a key, where it would lose what is 2^-25 of it however many keys there are.
+    auto weigh = [&](int nt, const f16v& sc, int p, float iv1, h8 (&ph)[2], h8 (&pl)[2], float& part) {
       float2 iv;
       if (FINE) iv = *(const float2*)&siv[buf][nt * 32 + 8 * (p / 2) + 4 * hf + 2 * (p & 1)];
       else iv.x = iv.y = iv1;
       const float u = exp2_f(sc[2 * p]), w = exp2_f(sc[2 * p + 1]);
-      sum = fmaf(u, iv.x, sum);
-      sum = fmaf(w, iv.y, sum);
+      part = p == 0 ? u * iv.x : fmaf(u, iv.x, part);
+      part = fmaf(w, iv.y, part);
       h2 a, l;
       split2(u, w, one, a, l);
       const int k = p / 4, e = p % 4 * 2;
@@ -414,6 +415,7 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
       f16v s0, s1;
       h8 ph0[2], pl0[2], ph1[2], pl1[2];
       const float iv0 = FINE ? 0.0f : siv[buf][0], iv1 = FINE ? 0.0f : siv[buf][NT - 1];
+      float sum0 = 0.0f, sum1 = 0.0f;
       scores(0, s0, [&](int k) {   // (the next tile's bytes, then the lookup for the one behind it)
         if (k < 4) load(k);
         if (k == 3) look(st + 2);
@@ -422,9 +424,10 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
       if (NT == 2) {
         scores(1, s1, [&](int k) {
 #pragma unroll
-          for (int p = k * 8 / KSTEPS; p < (k + 1) * 8 / KSTEPS; ++p) weigh(0, s0, p, iv0, ph0, pl0);
+          for (int p = k * 8 / KSTEPS; p < (k + 1) * 8 / KSTEPS; ++p) weigh(0, s0, p, iv0, ph0, pl0, sum0);
         });
         stay(ph0, pl0);
+        sum += sum0;
         // (a reference set anew here lowers the first part's weights too, which are not in the sums yet)
         const float f = refer(1, s1);
         if (__any(f != 1.0f)) {
@@ -434,13 +437,15 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
         }
         add(0, ph0, pl0, [&](int i) {
 #pragma unroll
-          for (int p = i * 8 / SUMS; p < (i + 1) * 8 / SUMS; ++p) weigh(1, s1, p, iv1, ph1, pl1);
+          for (int p = i * 8 / SUMS; p < (i + 1) * 8 / SUMS; ++p) weigh(1, s1, p, iv1, ph1, pl1, sum1);
         });
+        sum += sum1;
         arrive();
         add(1, ph1, pl1, store_some);
       } else {
 #pragma unroll
-        for (int p = 0; p < 8; ++p) weigh(0, s0, p, iv0, ph0, pl0);
+        for (int p = 0; p < 8; ++p) weigh(0, s0, p, iv0, ph0, pl0, sum0);
+        sum += sum0;
         arrive();
         add(0, ph0, pl0, store_some);
       }

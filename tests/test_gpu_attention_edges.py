@@ -1,0 +1,45 @@
+"""Attention over the 8-bit cache where its parts and its ranges end: against 64 bits, with attn_ref.attention's tolerance of each value."""
+import numpy as np
+import pytest
+
+import arcinferzero_amd as az
+import attn_ref as ref
+from test_gpu_attention import check
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def eng(rt):
+    e = az.Engine(16, 256)
+    yield e
+    e.close()
+
+
+STEP = 0.3   # octaves of a score to one of a key's first value (scored)
+
+
+def scored(b, page, block, kv, hd, steps):
+    """A cache of scale 1 whose position p of sequence 0 has the score steps.get(p, 0) * STEP octaves with every row of `lines`."""
+    c = ref.Cache(b.pages, page, block, kv, hd, seed=3)
+    c.d[:] = 1.0
+    c.q[0] = 0
+    for p, v in steps.items():
+        c.q[0, b.table[0, p // page], :, p % page, 0] = v
+    return c
+
+
+def lines(T, heads, hd):
+    q = np.zeros((T, heads, hd), np.float32)
+    q[:, :, 0] = STEP * np.log(2.0)
+    return q.reshape(T, heads * hd)
+
+
+@pytest.mark.parametrize("hd,page,block,heads,kv,seqs", [(64, 64, 64, 1, 1, [(40, 250)]), (64, 16, 4, 2, 1, [(100, 250)]), (128, 64, 16, 2, 2, [(40, 250)]), (128, 64, 64, 1, 1, [(40, 250)]),
+                                                         (256, 64, 64, 1, 1, [(40, 250)]), (128, 64, 64, 4, 1, [(300, 4100)]), (64, 64, 64, 8, 8, [(1, 4000)] + [(1, 1)] * 63),
+                                                         (128, 16, 1, 16, 8, [(1, 4000)] + [(1, 1)] * 63)])
+def test_many_keys_far_below_one(eng, hd, page, block, heads, kv, seqs):
+    """One key 24 octaves above all others: each of those is half a step of the sum's f32, all together many of its steps."""
+    b = ref.Batch(seqs, page, seed=1)
+    rows = seqs[0][0]
+    check(eng, seqs, heads, kv, hd, page, block, dict(scale=1.0), b=b, c=scored(b, page, block, kv, hd, {3: 80}), q=lines(b.T, heads, hd), only={0, 1, rows // 2, rows - 1})
