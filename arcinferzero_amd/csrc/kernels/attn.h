@@ -161,7 +161,8 @@ __device__ inline void value_scale(float vs, float& low, float& lv, float& iv) {
   iv = holds ? r : number ? exp2_f(-low) : 1.0f;
 }
 constexpr float LOW = -60.0f;
-// The weights' reference is lowered so that they are at most 2^8 when it is set; it is set anew once one would pass 2^15 (f16
-// ends at 2^16).  With the second f16 of the split a weight keeps an absolute error of 2^-25, 2^-33 of the largest.
+// The weights' reference is lowered so that the largest is at least 2^8 when it is set (2^8 for few rows, below 2^9 for many, whose
+// reference moves by whole octaves); it is set anew once one would pass 2^15 (f16 ends at 2^16).  With the second f16 of the split,
+// cut off at 2^-24, a weight keeps an absolute error of 2^-24, 2^-32 of the largest.
 constexpr float SETS = 8.0f, PASSES = 15.0f;
 constexpr float NOTHING = -1e30f;   // the reference before the first visible score

@@ -364,7 +364,7 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
       if (__any(top > limit)) {
         top = fmaxf(top, __shfl_xor(top, 32));
         const bool anew = top > limit;
-        const float by = anew ? ceilf(top) - SETS : 0.0f;   // (whole octaves: weights already made are brought along exactly)
+        const float by = anew ? floorf(top) - SETS : 0.0f;   // (whole octaves: weights already made are brought along exactly)
         const float f = limit > NOTHING ? exp2_f(-by) : 1.0f;   // (nothing summed yet)
         ref += by;
         limit = anew ? PASSES : limit;

@@ -43,3 +43,15 @@ def test_many_keys_far_below_one(eng, hd, page, block, heads, kv, seqs):
     b = ref.Batch(seqs, page, seed=1)
     rows = seqs[0][0]
     check(eng, seqs, heads, kv, hd, page, block, dict(scale=1.0), b=b, c=scored(b, page, block, kv, hd, {3: 80}), q=lines(b.T, heads, hd), only={0, 1, rows // 2, rows - 1})
+
+
+@pytest.mark.parametrize("hd,page,block,rows,heads", [(64, 64, 64, 40, 1), (64, 16, 4, 40, 2), (128, 64, 64, 40, 1), (128, 32, 8, 40, 1), (256, 64, 64, 40, 1), (128, 64, 64, 1, 1), (64, 16, 1, 2, 8)])
+@pytest.mark.parametrize("jump", [124, 125, 126, 127])
+def test_weights_at_the_last_place_of_their_f16(eng, hd, page, block, rows, heads, jump):
+    """32 keys 2^-30 to 2^-31 of the largest weight, which alone fill a column of the values: cut off at 2^-32 of it, not above."""
+    b = ref.Batch([(rows, 240)], page, seed=1)
+    c = scored(b, page, block, 1, hd, {**{64 + j: 23 for j in range(32)}, 3: jump})
+    c.q[1, :, :, :, 5] = 0
+    for j in range(32):
+        c.q[1, b.table[0, (64 + j) // page], :, (64 + j) % page, 5] = 127
+    check(eng, [(rows, 240)], heads, 1, hd, page, block, dict(scale=1.0), b=b, c=c, q=lines(b.T, heads, hd))
