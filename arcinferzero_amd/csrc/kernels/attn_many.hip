@@ -428,12 +428,18 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
         });
         stay(ph0, pl0);
         sum += sum0;
-        // (a reference set anew here lowers the first part's weights too, which are not in the sums yet)
+        // (A reference set anew here lowers the first part's weights too, which are not in the sums yet: as the f32 values that their two
+        //  f16 hold exactly, split again -- f itself may lie below the smallest f16, a weight of 2^15 times f does not.)
         const float f = refer(1, s1);
         if (__any(f != 1.0f)) {
-          const _Float16 f16 = (_Float16)f;
 #pragma unroll
-          for (int k = 0; k < 2; ++k) { ph0[k] *= f16; pl0[k] *= f16; }
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+              h2 a, l;
+              split2(((float)ph0[k][e] + (float)pl0[k][e]) * f, ((float)ph0[k][e + 1] + (float)pl0[k][e + 1]) * f, one, a, l);
+              ph0[k][e] = a.x; ph0[k][e + 1] = a.y; pl0[k][e] = l.x; pl0[k][e + 1] = l.y;
+            }
         }
         add(0, ph0, pl0, [&](int i) {
 #pragma unroll

@@ -55,3 +55,20 @@ def test_weights_at_the_last_place_of_their_f16(eng, hd, page, block, rows, head
     for j in range(32):
         c.q[1, b.table[0, (64 + j) // page], :, (64 + j) % page, 5] = 127
     check(eng, [(rows, 240)], heads, 1, hd, page, block, dict(scale=1.0), b=b, c=c, q=lines(b.T, heads, hd))
+
+
+# heads of 64 with and without a scale for each key, in one work-group and two; heads of 128 in work-groups of eight waves
+@pytest.mark.parametrize("hd,page,block,rows,keys,heads", [(64, 64, 64, 40, 240, 1), (64, 16, 4, 40, 240, 1), (64, 64, 32, 100, 400, 2), (128, 64, 64, 300, 4100, 4)])
+@pytest.mark.parametrize("jump", [57, 67, 80, 84, 100, 113, 127])
+def test_weights_that_a_later_key_of_the_tile_puts_far_behind(eng, hd, page, block, rows, keys, heads, jump):
+    """A tile of 64 keys that begins with 32 keys 6.9 octaves above all before it and goes on with one key 17 to 38 octaves above: the
+    32 keys' weights have to come along.  One column of the values is filled by them alone."""
+    b = ref.Batch([(rows, keys)], page, seed=1)
+    t = 33 * 64 if keys > 4000 else 64
+    c = scored(b, page, block, 1, hd, {**{t + j: 23 for j in range(32)}, t + 39: jump})
+    c.q[1, :, :, :, 5] = 0
+    for j in range(32):
+        c.q[1, b.table[0, (t + j) // page], :, (t + j) % page, 5] = 127
+    only = {0, 1, 31, 32, rows // 2, rows - 1}
+    got = check(eng, [(rows, keys)], heads, 1, hd, page, block, dict(scale=1.0), b=b, c=c, q=lines(b.T, heads, hd), only=only)
+    assert (got[sorted(only), :, 5] > 0).all()
