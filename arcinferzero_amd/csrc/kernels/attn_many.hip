@@ -45,10 +45,10 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   __shared__ __attribute__((aligned(16))) Tiles tl2;
   auto& sk = tl2.k;
   auto& sv = tl2.v;
-  // scales: of each key, or of each 32 keys that share one (kf: the score's factor; lv, iv: value_scale)
+  // scales: of each key, or of each 32 keys that share one (kf: the keys'; lv, iv: value_scale)
   constexpr int NS = FINE ? KT : NT;
   __shared__ float skf[2][NS], slv[2][NS], siv[2][NS];
-  __shared__ int red[NW][3];
+  __shared__ int red[NW][2];
   __shared__ _Float16 sq_lo[QLDS ? NW * 32 * KLD : 1];
 
   // (the rows that see the most keys first, of all heads; the heads in turn, so that with 8 of them each XCD's L2 holds one's cache)
@@ -169,7 +169,7 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   float* const pass = (float*)&tl2 + wave * 32 * SLD;
   const int quarter = lane >> 4, col = (lane & 15) * 4;
   auto of_row = [&](long v, int n) { return (long)__shfl((long long)v, n * 4 + quarter); };
-  uint32_t big = 0;
+  float big = 0.0f;
   float x[KSTEPS][8];
   {
     const long from = (long)(sq.r0 + i) * ldq + q_off + hq * HD;
@@ -197,22 +197,16 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
         float (&y)[8] = x[cc * 4 + k];
         y[0] = a.x; y[1] = a.y; y[2] = a.z; y[3] = a.w; y[4] = b.x; y[5] = b.y; y[6] = b.z; y[7] = b.w;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t b2 = __float_as_uint(y[e]) & 0x7FFFFFFFu;
-          if (b2 < 0x7F800000u) big = max(big, b2);
-        }
+        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(y[e]));
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
       __builtin_amdgcn_wave_barrier();
     }
   }
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) big = max(big, (uint32_t)__shfl_xor((int)big, o));
-  if (lane == 0) red[wave][2] = (int)big;
-  __syncthreads();   // (and all rows have passed through the tiles' place)
-#pragma unroll
-  for (int w = 0; w < NW; ++w) big = max(big, (uint32_t)red[w][2]);
-  const int e2 = min(max(137 - (int)(big >> 23), -100), 100);   // (the largest of the work-group's rows to 2^10 ... 2^11)
+  __syncthreads();   // (all rows have passed through the tiles' place)
+  // (the row's largest to 2^10 ... 2^11: the lane's own power of two, so that a row's bits do not hang on the rows beside it)
+  big = fmaxf(big, __shfl_xor(big, 32));
+  const int e2 = min(max(137 - (int)(__float_as_uint(big) >> 23), -100), 100);
   const float up = __uint_as_float((uint32_t)(127 + e2) << 23), down = __uint_as_float((uint32_t)(127 - e2) << 23);
   const float kfac = (CAP ? LOG2E / cap2 : LOG2E) * scale * down;   // (cap2 = cap log2 e)
   const float one = opaque_one();
@@ -267,7 +261,7 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
       float lv, iv;
       value_scale(rvs, low, lv, iv);
       const bool there = (uint32_t)pc < (uint32_t)pages;
-      skf[buf][threadIdx.x] = there ? rks * kfac : 0.0f;
+      skf[buf][threadIdx.x] = there ? rks : 0.0f;
       slv[buf][threadIdx.x] = there ? lv : -INFINITY;
       siv[buf][threadIdx.x] = there ? iv : 1.0f;
     }
@@ -320,13 +314,13 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
     auto refer = [&](int nt, f16v& sc) {
       const int jn = j0 + nt * 32;
       float kf1 = 0.0f, lv1 = 0.0f;
-      if (!FINE) { kf1 = skf[buf][nt]; lv1 = slv[buf][nt] - ref; }
+      if (!FINE) { kf1 = skf[buf][nt] * kfac; lv1 = slv[buf][nt] - ref; }
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const int j4 = nt * 32 + 8 * b + 4 * hf;
         f4 kf = {kf1, kf1, kf1, kf1}, lv = {lv1, lv1, lv1, lv1};
         if (FINE) {
-          kf = *(const f4*)&skf[buf][j4];
+          kf = *(const f4*)&skf[buf][j4] * kfac;
           lv = *(const f4*)&slv[buf][j4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) lv[e] -= ref;

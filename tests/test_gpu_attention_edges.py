@@ -72,3 +72,38 @@ def test_weights_that_a_later_key_of_the_tile_puts_far_behind(eng, hd, page, blo
     only = {0, 1, 31, 32, rows // 2, rows - 1}
     got = check(eng, [(rows, keys)], heads, 1, hd, page, block, dict(scale=1.0), b=b, c=c, q=lines(b.T, heads, hd), only=only)
     assert (got[sorted(only), :, 5] > 0).all()
+
+
+FORMS = [(64, 64, 16, 8, 2, [(64, 200)]), (128, 32, 8, 8, 2, [(64, 200)]), (128, 64, 64, 8, 2, [(64, 200), (9, 60)]), (256, 32, 16, 4, 2, [(50, 120)]),
+         (128, 64, 64, 8, 2, [(300, 4100)]), (128, 32, 8, 8, 2, [(2, 200)]), (64, 16, 16, 32, 1, [(1, 300)])]
+
+
+@pytest.mark.parametrize("hd,page,block,heads,kv,seqs", FORMS)
+@pytest.mark.parametrize("below", [18, 24, 40, 90])
+def test_rows_far_smaller_than_their_neighbours(eng, hd, page, block, heads, kv, seqs, below):
+    """A row's bits do not hang on the other rows of its work-group: every third one is 2^-below of the others, with a scale that gives
+    just those ordinary scores."""
+    T = sum(n for n, _ in seqs)
+    q = np.random.default_rng(4).standard_normal((T, heads, hd)).astype(np.float32)
+    small = np.arange(T) % 3 == 1 if T > 1 else np.array([True])
+    q[small] *= np.float32(2.0 ** -below)
+    if T == 1:
+        q[:, ::2] *= np.float32(2.0 ** below)
+    only = set(np.flatnonzero(small).tolist()[:: max(1, T // 60)])
+    if T == 1:      # (one row: heads of unlike sizes; the large ones' scores are one-hot)
+        only = None
+    check(eng, seqs, heads, kv, hd, page, block, dict(scale=0.09 * 2.0 ** below), q=q.reshape(T, -1), only=only)
+
+
+@pytest.mark.parametrize("hd,page,block,heads,kv", [(64, 64, 16, 8, 2), (128, 32, 8, 8, 2), (128, 64, 64, 8, 2), (256, 32, 16, 4, 2)])
+def test_rows_that_see_nothing_are_of_any_size(eng, hd, page, block, heads, kv):
+    """Stale rows -- at positions below 0, of a document that begins behind them -- of 1e30 beside rows of 1."""
+    rng = np.random.default_rng(4)
+    seqs = [(60, 40), (30, 200)]
+    q = rng.standard_normal((90, heads * hd)).astype(np.float32)
+    first = np.zeros(90, np.int64)
+    first[60:90:4] = 10000
+    q[:20] *= np.float32(1e30)
+    q[60:90:4] *= np.float32(1e30)
+    got = check(eng, seqs, heads, kv, hd, page, block, dict(first=first), q=q)
+    assert not got[:20].any() and not got[60:90:4].any()
