@@ -151,7 +151,7 @@ __device__ inline void few_body(const float* __restrict__ q, int ldq, int q_off,
       for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[k][e]));
     big = fmaxf(big, __shfl_xor(big, 16));
     big = fmaxf(big, __shfl_xor(big, 32));
-    const int e2 = min(max(137 - (int)(__float_as_uint(big) >> 23), -100), 100);
+    const int e2 = min(max(137 - (int)(__float_as_uint(big) >> 23), -118), 126);   // (2^e2 and 2^-e2 are normal numbers)
     const float up = __uint_as_float((uint32_t)(127 + e2) << 23), down = __uint_as_float((uint32_t)(127 - e2) << 23);
     kfac[t] = (CAP ? LOG2E / cap2 : LOG2E) * scale * down;   // (cap2 = cap log2 e)
 #pragma unroll

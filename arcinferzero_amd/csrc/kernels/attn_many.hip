@@ -206,7 +206,7 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   __syncthreads();   // (all rows have passed through the tiles' place)
   // (the row's largest to 2^10 ... 2^11: the lane's own power of two, so that a row's bits do not hang on the rows beside it)
   big = fmaxf(big, __shfl_xor(big, 32));
-  const int e2 = min(max(137 - (int)(__float_as_uint(big) >> 23), -100), 100);
+  const int e2 = min(max(137 - (int)(__float_as_uint(big) >> 23), -118), 126);   // (2^e2 and 2^-e2 are normal numbers)
   const float up = __uint_as_float((uint32_t)(127 + e2) << 23), down = __uint_as_float((uint32_t)(127 - e2) << 23);
   const float kfac = (CAP ? LOG2E / cap2 : LOG2E) * scale * down;   // (cap2 = cap log2 e)
   const float one = opaque_one();

@@ -107,3 +107,9 @@ def test_rows_that_see_nothing_are_of_any_size(eng, hd, page, block, heads, kv):
     q[60:90:4] *= np.float32(1e30)
     got = check(eng, seqs, heads, kv, hd, page, block, dict(first=first), q=q)
     assert not got[:20].any() and not got[60:90:4].any()
+
+
+@pytest.mark.parametrize("seqs", [[(1, 300), (2, 40)], [(70, 300), (30, 30)]])
+@pytest.mark.parametrize("q_std", [1e-37, 1e36])
+def test_rows_at_the_ends_of_f32(eng, seqs, q_std):
+    check(eng, seqs, 8, 2, 128, 32, 8, dict(scale=0.09 / q_std), q_std=q_std)
