@@ -165,4 +165,4 @@ constexpr float LOW = -60.0f;
 // reference moves by whole octaves); it is set anew once one would pass 2^15 (f16 ends at 2^16).  With the second f16 of the split,
 // cut off at 2^-24, a weight keeps an absolute error of 2^-24, 2^-32 of the largest.
 constexpr float SETS = 8.0f, PASSES = 15.0f;
-constexpr float NOTHING = -1e30f;   // the reference before the first visible score
+constexpr float NOTHING = -0x1.fffffep127f;   // the reference before the first visible score: below every finite one

@@ -113,3 +113,15 @@ def test_rows_that_see_nothing_are_of_any_size(eng, hd, page, block, heads, kv):
 @pytest.mark.parametrize("q_std", [1e-37, 1e36])
 def test_rows_at_the_ends_of_f32(eng, seqs, q_std):
     check(eng, seqs, 8, 2, 128, 32, 8, dict(scale=0.09 / q_std), q_std=q_std)
+
+
+@pytest.mark.parametrize("seqs", [[(1, 300), (2, 40)], [(70, 300), (30, 30)], [(1, 2000)]])
+@pytest.mark.parametrize("hd,block", [(64, 1), (128, 8), (128, 32)])
+def test_scores_far_below_zero(eng, seqs, hd, block):
+    """Every score of a row about -1e31 (they differ by more than f32's steps there): the largest has the weight, as anywhere."""
+    b = ref.Batch(seqs, 32, seed=2)
+    c = ref.Cache(b.pages, 32, block, 2, hd, seed=3)
+    c.q[0] = np.maximum(np.abs(c.q[0]), 1)
+    q = -np.abs(np.random.default_rng(5).standard_normal((b.T, 8 * hd))).astype(np.float32) * np.float32(2e30)
+    got = check(eng, seqs, 8, 2, hd, 32, block, dict(scale=0.5), b=b, c=c, q=q)
+    assert got.any(-1).all()
