@@ -148,14 +148,17 @@ __device__ inline void cap_scores(float (&v)[N], float cap2) {
 }
 // The scales' part in a score.  A weight is carried as w = p * vs (p = e^(s - reference), vs the scale of the token's values), as
 // 2^(s log2(e) + log2(vs) - reference): the product with the scale costs no instruction of its own, the weights stay within a
-// fixed range whatever the scales are, and the softmax's sum is the sum of w / vs.  (That sum, of at most 2^31 keys' w <= 2^15, stays in f32
-// for scales from 2^-82 on; the values of a cache that holds smaller ones alone may be read as zeros.)  A block of zeros (a scale below
+// fixed range whatever the scales are, and the softmax's sum is the sum of w / vs.  A block of zeros (a scale below
 // 2^-120) takes the smallest scale that this thread has met, 2^-60 at most, instead -- its values are zeros whatever it is: with a scale
 // above the others' its weights could set the reference and leave the others' f16 nothing, with a smaller one they are small, and
 // count in the sum alone, in f32.  A scale that is no number makes the score none, and its weight nothing where it is masked.
+// Range of the sum: w <= 2^15 and 1 / vs.  Scales below 2^-97 are taken as 2^-97 (the values, below 127 * 2^-97 then, miss by at most that):
+// 2^-97 leaves room for 2^15 keys of the largest weights, 2^21 of such as the reference is set for (with 2^-119 two of them overflow
+// it), and a key beside others of scale 1 counts down to 2^-37 of their weight (with 2^-119 to 2^-15).  At the other end, with scales
+// of 2^105 w / vs is a normal number down to 2^-29 of the largest weight.
 __device__ inline void value_scale(float vs, float& low, float& lv, float& iv) {
   const bool number = vs == vs, holds = vs >= 0x1p-120f;
-  const float l = __builtin_amdgcn_logf(vs), r = __builtin_amdgcn_rcpf(vs);
+  const float s = fmaxf(vs, 0x1p-97f), l = __builtin_amdgcn_logf(s), r = __builtin_amdgcn_rcpf(s);
   low = holds ? fminf(low, l) : low;
   lv = holds ? l : number ? low : vs;
   iv = holds ? r : number ? exp2_f(-low) : 1.0f;

@@ -187,8 +187,9 @@ int arcz_engine_rope(arcz_engine* e, arcz_rope* r, arcz_mem* x, int ldx, int x_o
  * or 256), one f32 scale for each block of `block` tokens (a power of two, 1 to page) and head.  k, v: int8 [pages][heads][page][hd];
  * ks, vs: f32 [pages][heads][page / block]; value = int8 * scale.  Each buffer is the caller's (kept until arcz_kv_free; k and v
  * at addresses of 16 bytes) or, where NULL, the library's (arcz_kv_buffer).  A scale below
- * 2^-120 (or below 0) belongs to a block whose values are all zero, as kv_write stores it.  A page in a sequence's table twice is
- * read twice; it must not be written so. */
+ * 2^-120 (or below 0) belongs to a block whose values are all zero, as kv_write stores it.  arcz_engine_attention is exact to its bound
+ * for scales of v from 2^-97 to 2^105; smaller ones it takes as 2^-97 (an error of at most 127 * 2^-97 of the value).  A page in a
+ * sequence's table twice is read twice; it must not be written so. */
 typedef struct arcz_kv arcz_kv;
 arcz_kv* arcz_kv_create(arcz_engine* e, int pages, int page, int block, int heads, int hd, arcz_mem* k, arcz_mem* v, arcz_mem* ks, arcz_mem* vs);
 /* Frees the handle and the library's buffers; refused, with everything as it was, while a launch list names them. */

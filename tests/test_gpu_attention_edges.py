@@ -125,3 +125,21 @@ def test_scores_far_below_zero(eng, seqs, hd, block):
     q = -np.abs(np.random.default_rng(5).standard_normal((b.T, 8 * hd))).astype(np.float32) * np.float32(2e30)
     got = check(eng, seqs, 8, 2, hd, 32, block, dict(scale=0.5), b=b, c=c, q=q)
     assert got.any(-1).all()
+
+
+@pytest.mark.parametrize("rows", [1, 9, 40])
+@pytest.mark.parametrize("block", [1, 8, 32])
+@pytest.mark.parametrize("kind", ["tiny", "tiny_and_zeros", "one_tiny_then_zeros"])
+def test_values_that_hardly_are_any(eng, rows, block, kind):
+    """Hundreds of keys whose values' scale is 2^-119, just what the cache holds as more than zeros, or blocks of zeros behind one
+    such: they count in the sum of weights as all keys do."""
+    b = ref.Batch([(rows, 1100)], 32, seed=2)
+    c = ref.Cache(b.pages, 32, block, 2, 128, seed=3)
+    for i in range(20):
+        c.d[1, b.table[0, i]] = 2.0 ** -119
+    if kind != "tiny":
+        keep = 1 if kind == "one_tiny_then_zeros" else 10
+        for i in range(keep, 20):
+            c.d[1, b.table[0, i]] = 0.0
+            c.q[1, b.table[0, i]] = 0
+    check(eng, [(rows, 1100)], 8, 2, 128, 32, block, b=b, c=c, q_std=0.3)
