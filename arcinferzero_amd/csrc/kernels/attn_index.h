@@ -26,9 +26,9 @@ ATTN_FN Seq seq_at(int row0, int row1, int length, int T, int max_rows, int most
   q.p0 = q.len - all;
   return q;
 }
-// The positions [lo, hi) that a row at position p sees (none: lo >= hi).
+// The positions [lo, hi) that a row at position p sees (none: lo >= hi; a row below position 0 sees none, whatever the prefix).
 ATTN_FN void sees(int p, int len, int window, int prefix, int first, int& lo, int& hi) {
-  hi = lower(len, upper(p + 1, prefix));
+  hi = p < 0 ? 0 : lower(len, upper(p + 1, prefix));
   lo = upper(first, 0);
   if (window) lo = upper(lo, p - window + 1);
 }

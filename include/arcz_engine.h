@@ -197,11 +197,12 @@ int arcz_kv_free(arcz_engine* e, arcz_kv* c);
 arcz_mem* arcz_kv_buffer(arcz_kv* c, int which); /* 0 k, 1 v, 2 ks, 3 vs */
 /* The sequences of a call.  Rows [rows[s], rows[s + 1]) of the row buffers belong to sequence s (rows: int32 [seqs + 1], from 0 on,
  * not falling); len[s] (int32) keys of it are in the cache, those of these rows with them, so its i-th row of n has position
- * len - n + i (rows whose position is below 0 are left out).  table [seqs][ld_table] (int32): page of its positions page * i and
- * on.  T: rows of the buffers; max_rows: the most rows of one sequence (those past it are left out); max_len: about the most
- * keys of one, for sharing out the work (0: as many as the table holds).  rows, len and table are read when the launch runs and
- * held to the buffers there: rows to [0, T], len to the table, and a page outside the cache is one without tokens -- nothing is
- * written to it, its keys are not seen, it reads as zeros.  Rows of the buffers that belong to no sequence are left as they are. */
+ * len - n + i (rows whose position is below 0 are left out; attention gives them zeros).  table [seqs][ld_table] (int32): page of its
+ * positions page * i and on.  T: rows of the buffers; max_rows: the most rows of one sequence (those past it are left out);
+ * max_len: about the most keys of one, for sharing out the work (0: as many as the table holds).  rows, len and table are read when
+ * the launch runs and held to the buffers there: rows to [0, T], len to the table, and a page outside the cache is one without
+ * tokens -- nothing is written to it, its keys are not seen, it reads as zeros.  Rows of the buffers that belong to no sequence are
+ * left as they are. */
 typedef struct arcz_kv_batch {
   arcz_mem *rows, *len, *table;
   int seqs, ld_table, T, max_rows, max_len;
@@ -215,7 +216,7 @@ int arcz_engine_kv_write(arcz_engine* e, arcz_kv* c, const arcz_kv_batch* b, arc
 /* ... and back: the values that the cache holds for the batch's rows. */
 int arcz_engine_kv_read(arcz_engine* e, arcz_kv* c, const arcz_kv_batch* b, arcz_mem* k, int ldk, int k_off, arcz_mem* v, int ldv, int v_off);
 
-/* A row at position p sees key j < len iff  j >= first[row],  j <= p or j < prefix[s],  and, with a window > 0, p - j < window.  Its score
+/* A row at position p >= 0 sees key j < len iff  j >= first[row],  j <= p or j < prefix[s],  and, with a window > 0, p - j < window.  Its score
  * is scale * q.k, with cap > 0 cap * tanh(that / cap), then minus slopes[head] * |p - j|. */
 typedef struct arcz_attn {
   float scale, cap;           /* cap 0: none, else 2^-100 to 2^100 */

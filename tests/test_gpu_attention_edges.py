@@ -143,3 +143,16 @@ def test_values_that_hardly_are_any(eng, rows, block, kind):
             c.d[1, b.table[0, i]] = 0.0
             c.q[1, b.table[0, i]] = 0
     check(eng, [(rows, 1100)], 8, 2, 128, 32, block, b=b, c=c, q_std=0.3)
+
+
+@pytest.mark.parametrize("seqs", [[(6, 3), (1, 50)], [(50, 30), (40, 70)]])
+@pytest.mark.parametrize("window", [0, 11])
+def test_rows_before_position_0_behind_a_prefix(eng, seqs, window):
+    """Rows whose position is below 0 are left out, zeros, whatever the prefix."""
+    T = sum(n for n, _ in seqs)
+    n, l = seqs[0]
+    out = n - l
+    got = check(eng, seqs, 8, 2, 128, 32, 32, dict(prefix=[2, 60], window=window), only=set(range(out, T)))
+    assert not got[:out].any()
+    got = check(eng, seqs, 8, 2, 128, 32, 32, dict(prefix=[2 ** 31 - 1, 60], window=window), only=set(range(out, T)))
+    assert not got[:out].any()
