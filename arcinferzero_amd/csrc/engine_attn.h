@@ -192,34 +192,24 @@
     int window;
     cl_mem slopes, prefix, first;
   };
-  // Room for the pieces that the keys of few rows are shared out in, and the counts of those that are written (zeros between
-  // launches); grown, never shrunk.  A launch list keeps the room that it was recorded with: all launches are in one stream's
-  // order, so lists and calls that use the same room do not meet there.
+  // Room for the pieces that keys are shared out in, and attn_few's counts of those that are written (zeros between launches).  Made by
+  // the first call that needs it, for the most that any call does, so that no longer sequence and no larger batch allocates or
+  // waits behind it: where keys are shared out, attn_many has at most 256 rows of pieces a compute unit, attn_few less than four
+  // pieces of at most 32 rows a compute unit, for less than two (sequence, head) pairs a compute unit (the rules in attention()); a
+  // piece has hd + 2 values a row (256 compute units: 68 MB).  Launch lists name it too: all launches are in one stream's order, so
+  // lists and calls that use it do not meet there.
   cl_mem at_ws_ = nullptr, at_counts_ = nullptr;
-  size_t at_ws_bytes_ = 0, at_counts_n_ = 0;
-  cl_mem at_ws(size_t bytes) {
-    if (bytes > at_ws_bytes_) {
-      cl_mem m = buf(bytes);
-      if (at_ws_ && !arcz_mem_listed(at_ws_)) release(at_ws_);
-      at_ws_ = m;
-      at_ws_bytes_ = bytes;
+  void at_room() {
+    const size_t cus = arcz_device_cus();
+    if (!at_ws_) at_ws_ = buf(256 * cus * (256 + 2) * 4);
+    if (at_counts_) return;
+    cl_mem m = buf(2 * cus * 4);
+    const uint32_t zero = 0;
+    if (arcz_fill(m, &zero, 4, 0, 2 * cus * 4) != 0) {
+      release(m);
+      throw std::runtime_error("attention: the counts are not cleared");
     }
-    return at_ws_;
-  }
-  cl_mem at_counts(size_t n) {
-    if (n > at_counts_n_) {
-      n = std::max<size_t>(n, 1024);
-      cl_mem m = buf(n * 4);
-      const uint32_t zero = 0;
-      if (arcz_fill(m, &zero, 4, 0, n * 4) != 0) {
-        release(m);
-        throw std::runtime_error("attention: the counts are not cleared");
-      }
-      if (at_counts_ && !arcz_mem_listed(at_counts_)) release(at_counts_);
-      at_counts_ = m;
-      at_counts_n_ = n;
-    }
-    return at_counts_;
+    at_counts_ = m;
   }
   void attention(const Kv& c, const Batch& b, cl_mem q, int ldq, int q_off, int heads, cl_mem out, int ldo, int o_off, const Attn& a) {
     if (!check_batch("attention", c, b)) return;
@@ -244,13 +234,14 @@
     int vec = rq.vec() ? 1 : 0;
     if (ro.vec()) vec |= 2;
     if (M <= (c.hd == 256 ? 16 : 32)) {
-      const int rt = M > 16 ? 2 : 1, pack = M <= 8 ? 1 : 0, rows = pack ? 8 : 16 * rt;
+      const int rt = M > 16 ? 2 : 1, pack = M <= 8 ? 1 : 0;
       // Pieces of one length for all sequences, so that long ones are more work-groups, not longer ones: two work-groups a
       // compute unit if every sequence has the most keys, of at least 256 keys each.
       const size_t want = ((size_t)2 * arcz_device_cus() + pairs - 1) / pairs;
       int least = (int)std::max<size_t>(8, ((size_t)(keys + 31) / 32 + want - 1) / want);
       nsplit = (int)(((int64_t)keys + (int64_t)32 * least - 1) / ((int64_t)32 * least));
-      cl_mem w = nsplit > 1 ? at_ws(pairs * nsplit * rows * (c.hd + 2) * 4) : nullptr, counts = nsplit > 1 ? at_counts(pairs) : nullptr;
+      if (nsplit > 1) at_room();
+      cl_mem w = nsplit > 1 ? at_ws_ : nullptr, counts = nsplit > 1 ? at_counts_ : nullptr;
       if (pairs > 0xFFFFFFFFull / 256) throw std::runtime_error("attention: too many sequences");
       vec &= 1;
       cl_kernel k = variant("attn", {{"HD", c.hd}, {"RT", rt}, {"PACK", pack}, {"FINE", c.block < 4 ? 1 : 0}, {"FORM", form}}, "attn_few");
@@ -271,7 +262,8 @@
     if (pairs * tiles > 0xFFFFFFFFull / (64 * waves)) throw std::runtime_error("attention: too many rows");
     // rows that fill less than the chip: their keys shared out, at least 256 to a piece
     nsplit = (int)std::max<size_t>(1, std::min<size_t>((size_t)8 / waves * arcz_device_cus() / (pairs * tiles), (size_t)(keys + 255) / 256));
-    cl_mem w = nsplit > 1 ? at_ws(pairs * tiles * nsplit * bm * (c.hd + 2) * 4) : nullptr;
+    if (nsplit > 1) at_room();
+    cl_mem w = nsplit > 1 ? at_ws_ : nullptr;
     cl_kernel k = variant("attn", {{"HD", c.hd}, {"FINE", c.block < 32 ? 1 : 0}, {"FORM", form}, {waves == 8 ? "W8" : nullptr, 1}}, "attn_many");
     set_args(k, 0, q, ldq, q_off, c.b[0], c.b[1], c.b[2], c.b[3], pages, ps, bs, b.rows, b.len, b.table, ldt, T, mr, heads, kvh, out, ldo, o_off, scale, cap2, window,
              a.slopes, a.prefix, a.first, w, nsplit, tiles, vec);

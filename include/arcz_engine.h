@@ -168,7 +168,8 @@ int arcz_engine_moe_slots(arcz_engine* e);
 /* ---- The attention block between the q|k|v product and the output projection (the reference's kernels of this place are
  * zero/kernels/ops_attn.cl, ops_attn_g.cl, attn_x.cl; these operators are this library's own).  All rows are f32, as the
  * products leave them: a call names a buffer, the values from one row to the next (ld) and the first column (off), so the
- * columns of one q|k|v buffer are taken as they lie.  Nothing here waits or, once a sequence has run, allocates: a pass records
+ * columns of one q|k|v buffer are taken as they lie.  Nothing here waits or allocates, but for an engine's first attention that
+ * shares a sequence's keys out over work-groups, which makes the room for that (68 MB, for any later call): behind it a pass records
  * into a launch list, and what changes from pass to pass -- positions, lengths, pages -- comes from device buffers. */
 
 /* Rotary positions.  Pair i of a head is turned by pos[axis[i]][row] * freq[i] radians: (a, b) -> (a cos - b sin, a sin + b cos) *
