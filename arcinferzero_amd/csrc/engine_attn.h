@@ -52,9 +52,14 @@
     const size_t d = a.begin() <= b.begin() ? (b.begin() - a.begin()) / 4 % ld : (ld - (a.begin() - b.begin()) / 4 % ld) % ld;
     return d < (size_t)a.width || d + (size_t)b.width > ld;
   }
-  static bool overlap(const Rows& a, cl_mem m) {
-    const uintptr_t b = (uintptr_t)arcz_mem_ptr(m), e = b + arcz_mem_size(m);
-    return !(a.end() <= b || e <= a.begin());
+  // ... and the first n bytes of a buffer, those that a call takes of it (rows of a stride: the columns between them too).
+  static bool overlap(const Rows& a, cl_mem m, size_t n) {
+    const uintptr_t b = (uintptr_t)arcz_mem_ptr(m);
+    return m && !(a.end() <= b || b + n <= a.begin());
+  }
+  static bool overlap(cl_mem a, size_t na, cl_mem b, size_t nb) {
+    const uintptr_t p = (uintptr_t)arcz_mem_ptr(a), q = (uintptr_t)arcz_mem_ptr(b);
+    return a && b && !(p + na <= q || q + nb <= p);
   }
   static cl_mem ints(const char* what, cl_mem m, size_t n) {
     if (!m || (uintptr_t)arcz_mem_ptr(m) % 4 || arcz_mem_size(m) < n * 4) throw std::runtime_error(std::string(what) + " holds less than " + std::to_string(n) + " values");
@@ -84,6 +89,7 @@
   struct Kv {
     int pages = 0, page = 0, block = 0, heads = 0, hd = 0, ps = 0, bs = 0;
     cl_mem b[4] = {nullptr, nullptr, nullptr, nullptr};   // keys, values (int8), their scales (f32)
+    size_t bytes[4] = {0, 0, 0, 0};                       // ... what the cache takes of each
     bool mine[4] = {false, false, false, false};
   };
   static int log2_of(int v) {
@@ -103,15 +109,13 @@
     const size_t rows = (size_t)pages * heads * page, size[4] = {rows * hd, rows * hd, rows / block * 4, rows / block * 4};
     for (int i = 0; i < 4; ++i) {
       cl_mem m = given ? given[i] : nullptr;
+      c.bytes[i] = size[i];
       if (!m) continue;
       if (arcz_mem_size(m) < size[i] || (uintptr_t)arcz_mem_ptr(m) % (i < 2 ? 16 : 4))
         throw std::runtime_error("make_kv: buffer " + std::to_string(i) + " holds " + std::to_string(arcz_mem_size(m)) + " bytes, the cache takes " + std::to_string(size[i]) +
                                  " (the values' at an address of 16)");
       for (int j = 0; j < i; ++j)
-        if (c.b[j]) {
-          const uintptr_t a = (uintptr_t)arcz_mem_ptr(m), b = (uintptr_t)arcz_mem_ptr(c.b[j]);
-          if (!(a + size[i] <= b || b + size[j] <= a)) throw std::runtime_error("make_kv: two of the buffers overlap");
-        }
+        if (overlap(m, size[i], c.b[j], size[j])) throw std::runtime_error("make_kv: two of the buffers overlap");
       c.b[i] = m;
     }
     try {
@@ -154,12 +158,16 @@
     ints((std::string(what) + ": table").c_str(), b.table, (size_t)b.seqs * b.ld_table);
     return true;
   }
+  static bool overlap(const Rows& a, const Kv& c) {
+    for (int i = 0; i < 4; ++i)
+      if (overlap(a, c.b[i], c.bytes[i])) return true;
+    return false;
+  }
   void kv_write(const Kv& c, const Batch& b, cl_mem k, int ldk, int k_off, cl_mem v, int ldv, int v_off) {
     if (!check_batch("kv_write", c, b)) return;
     const int w = c.heads * c.hd, most = std::min(b.max_rows, b.T);
     const Rows rk = rows_of("kv_write: k", k, ldk, k_off, w, b.T), rv = rows_of("kv_write: v", v, ldv, v_off, w, b.T);
-    for (cl_mem m : c.b)
-      if (overlap(rk, m) || overlap(rv, m)) throw std::runtime_error("kv_write: the rows overlap the cache");
+    if (overlap(rk, c) || overlap(rv, c)) throw std::runtime_error("kv_write: the rows overlap the cache");
     int vec = rk.vec() && rv.vec(), pages = c.pages, heads = c.heads, ps = c.ps, bs = c.bs, ldt = b.ld_table, T = b.T, mr = b.max_rows;
     // A work-group's tokens: whole blocks, and up to the eight rows a thread that it holds in registers (read once instead of twice:
     // 8192 rows x 8 heads x 128 values, blocks of 32 tokens, 25 -> 19.6 us; ragged prompts, 4 x 256, a scale a token, 26 -> 14.8).
@@ -176,8 +184,7 @@
     const int w = c.heads * c.hd, most = std::min(b.max_rows, b.T);
     const Rows rk = rows_of("kv_read: k", k, ldk, k_off, w, b.T), rv = rows_of("kv_read: v", v, ldv, v_off, w, b.T);
     if (overlap(rk, rv)) throw std::runtime_error("kv_read: k and v overlap");
-    for (cl_mem m : c.b)
-      if (overlap(rk, m) || overlap(rv, m)) throw std::runtime_error("kv_read: the rows overlap the cache");
+    if (overlap(rk, c) || overlap(rv, c)) throw std::runtime_error("kv_read: the rows overlap the cache");
     int vec = rk.vec() && rv.vec(), pages = c.pages, heads = c.heads, hd = c.hd, ps = c.ps, bs = c.bs, ldt = b.ld_table, T = b.T, mr = b.max_rows;
     int per = std::max(1, 4096 / w);   // (four values a thread, four times)
     cl_kernel kn = variant("attn", {}, "kv_read");
@@ -218,8 +225,7 @@
       throw std::runtime_error("attention: scale, cap, window or max_len");
     const Rows rq = rows_of("attention: q", q, ldq, q_off, heads * c.hd, b.T), ro = rows_of("attention: out", out, ldo, o_off, heads * c.hd, b.T);
     if (overlap(rq, ro)) throw std::runtime_error("attention: q and out overlap");
-    for (cl_mem m : c.b)
-      if (overlap(ro, m)) throw std::runtime_error("attention: out overlaps the cache");
+    if (overlap(ro, c)) throw std::runtime_error("attention: out overlaps the cache");
     if (a.slopes) ints("attention: slopes", a.slopes, (size_t)heads);
     if (a.prefix) ints("attention: prefix", a.prefix, (size_t)b.seqs);
     if (a.first) ints("attention: first", a.first, (size_t)b.T);

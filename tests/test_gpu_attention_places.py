@@ -1,0 +1,53 @@
+"""Which buffers of a call of the attention block may share memory: pieces of one allocation that do not meet."""
+import numpy as np
+import pytest
+
+import arcinferzero_amd as az
+import attn_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def eng(rt):
+    e = az.Engine(16, 256)
+    yield e
+    e.close()
+
+
+def test_pieces_of_one_allocation(eng):
+    """Cache, rows, outputs and the batch's arrays side by side in one allocation, the cache's handles as large as all of it: the results
+    are those of buffers of their own."""
+    page, block, kv, hd, heads = 16, 8, 2, 64, 4
+    seqs = [(5, 20), (3, 3)]
+    b = ref.Batch(seqs, page, seed=2)
+    c = ref.Cache(b.pages, page, block, kv, hd, seed=3)
+    rng = np.random.default_rng(4)
+    w = (heads + 2 * kv) * hd
+    x = rng.standard_normal((b.T, w)).astype(np.float32)
+    results = []
+    for one in (False, True):
+        hold = []
+        parts = [c.q[0], c.q[1], c.d[0], c.d[1], x, np.zeros((b.T, heads * hd), np.float32), np.zeros((b.T, 2 * kv * hd), np.float32), b.rows, b.lens, b.table]
+        if one:
+            at = np.cumsum([0] + [-(-p.nbytes // 64) * 64 for p in parts])
+            big = az.Runtime.alloc(int(at[-1]))
+            hold.append(big)
+            m = []
+            for o, p in zip(at[:-1], parts):
+                big.write(p, offset=int(o))
+                # (the cache's buffers: to the end of the allocation, more than it takes)
+                m.append(big.view(int(o), int(at[-1] - o) if len(m) < 4 else p.nbytes))
+        else:
+            m = [az.Runtime.from_numpy(p) for p in parts]
+        hold += m
+        k = eng.make_kv(c.pages, page, block, kv, hd, *m[:4])
+        hold.append(k)
+        batch = az.KvBatch(m[7], m[8], m[9], len(seqs), b.ldt, b.T, b.max_rows, b.max_len)
+        eng.kv_write(k, batch, m[4], w, heads * hd, m[4], w, (heads + kv) * hd)
+        eng.kv_read(k, batch, m[6], 2 * kv * hd, 0, m[6], 2 * kv * hd, kv * hd)
+        eng.attention(k, batch, m[4], w, 0, heads, m[5], heads * hd, 0, az.Attention(0.1))
+        results.append([p.read(np.uint8, q.nbytes) for p, q in zip(m, parts)])
+        ref.free(hold)
+    assert all(np.array_equal(p, q) for p, q in zip(*results))
+    assert results[0][5].any() and results[0][6].any()
