@@ -74,7 +74,9 @@
     const Rows a = rows_of("rope: x", x, ldx, x_off, heads * hd, T), b = rows_of("rope: y", y, ldy, y_off, heads * hd, T);
     if (!(a.begin() == b.begin() && ldx == ldy) && overlap(a, b)) throw std::runtime_error("rope: x and y overlap (in place: the same columns of the same rows)");
     if (ld_pos < T) throw std::runtime_error("rope: positions of " + std::to_string(T) + " rows on axes " + std::to_string(ld_pos) + " apart");
-    ints("rope: pos", pos, (size_t)(r.axes - 1) * ld_pos + T);
+    const size_t np = (size_t)(r.axes - 1) * ld_pos + T;
+    ints("rope: pos", pos, np);
+    if (overlap(b, pos, np * 4)) throw std::runtime_error("rope: y overlaps pos");
     int vec = a.vec() && b.vec() && hd % 4 == 0, nb = r.neighbours, ax = r.axes, pairs = r.pairs;
     float ms = r.mscale;
     // (few tokens: a token's heads over several work-groups)
@@ -158,6 +160,11 @@
     ints((std::string(what) + ": table").c_str(), b.table, (size_t)b.seqs * b.ld_table);
     return true;
   }
+  // What a launch reads of a batch is not what it writes: work-groups that begin later would see it changed.
+  static size_t table_bytes(const Batch& b) { return (size_t)b.seqs * b.ld_table * 4; }
+  static bool overlap(const Rows& a, const Batch& b) {
+    return overlap(a, b.rows, ((size_t)b.seqs + 1) * 4) || overlap(a, b.len, (size_t)b.seqs * 4) || overlap(a, b.table, table_bytes(b));
+  }
   static bool overlap(const Rows& a, const Kv& c) {
     for (int i = 0; i < 4; ++i)
       if (overlap(a, c.b[i], c.bytes[i])) return true;
@@ -168,6 +175,9 @@
     const int w = c.heads * c.hd, most = std::min(b.max_rows, b.T);
     const Rows rk = rows_of("kv_write: k", k, ldk, k_off, w, b.T), rv = rows_of("kv_write: v", v, ldv, v_off, w, b.T);
     if (overlap(rk, c) || overlap(rv, c)) throw std::runtime_error("kv_write: the rows overlap the cache");
+    for (int i = 0; i < 4; ++i)
+      if (overlap(c.b[i], c.bytes[i], b.rows, ((size_t)b.seqs + 1) * 4) || overlap(c.b[i], c.bytes[i], b.len, (size_t)b.seqs * 4) || overlap(c.b[i], c.bytes[i], b.table, table_bytes(b)))
+        throw std::runtime_error("kv_write: the cache overlaps the batch's rows, len or table");
     int vec = rk.vec() && rv.vec(), pages = c.pages, heads = c.heads, ps = c.ps, bs = c.bs, ldt = b.ld_table, T = b.T, mr = b.max_rows;
     // A work-group's tokens: whole blocks, and up to the eight rows a thread that it holds in registers (read once instead of twice:
     // 8192 rows x 8 heads x 128 values, blocks of 32 tokens, 25 -> 19.6 us; ragged prompts, 4 x 256, a scale a token, 26 -> 14.8).
@@ -185,6 +195,7 @@
     const Rows rk = rows_of("kv_read: k", k, ldk, k_off, w, b.T), rv = rows_of("kv_read: v", v, ldv, v_off, w, b.T);
     if (overlap(rk, rv)) throw std::runtime_error("kv_read: k and v overlap");
     if (overlap(rk, c) || overlap(rv, c)) throw std::runtime_error("kv_read: the rows overlap the cache");
+    if (overlap(rk, b) || overlap(rv, b)) throw std::runtime_error("kv_read: k or v overlaps the batch's rows, len or table");
     int vec = rk.vec() && rv.vec(), pages = c.pages, heads = c.heads, hd = c.hd, ps = c.ps, bs = c.bs, ldt = b.ld_table, T = b.T, mr = b.max_rows;
     int per = std::max(1, 4096 / w);   // (four values a thread, four times)
     cl_kernel kn = variant("attn", {}, "kv_read");
@@ -229,6 +240,8 @@
     if (a.slopes) ints("attention: slopes", a.slopes, (size_t)heads);
     if (a.prefix) ints("attention: prefix", a.prefix, (size_t)b.seqs);
     if (a.first) ints("attention: first", a.first, (size_t)b.T);
+    if (overlap(ro, b) || overlap(ro, a.slopes, (size_t)heads * 4) || overlap(ro, a.prefix, (size_t)b.seqs * 4) || overlap(ro, a.first, (size_t)b.T * 4))
+      throw std::runtime_error("attention: out overlaps rows, len, table, slopes, prefix or first");
     const int G = heads / c.heads, most = std::min(b.max_rows, b.T);
     const int64_t M = (int64_t)most * G;
     if (M > 0x7FFFFF00) throw std::runtime_error("attention: too many rows");

@@ -181,7 +181,7 @@ typedef struct arcz_rope arcz_rope;
 arcz_rope* arcz_rope_create(arcz_engine* e, int pairs, const double* freq, const uint8_t* axis, int axes, int neighbours, float mscale);
 int arcz_rope_free(arcz_engine* e, arcz_rope* r);
 /* T rows of `heads` heads of hd values (2 pairs <= hd) of x, turned into y: the same columns of the same rows (in place), or
- * columns that do not meet them.  pos int32 [axes][ld_pos], ld_pos >= T; any int32 is a position. */
+ * columns that do not meet them.  pos int32 [axes][ld_pos], ld_pos >= T; any int32 is a position.  y must not meet pos. */
 int arcz_engine_rope(arcz_engine* e, arcz_rope* r, arcz_mem* x, int ldx, int x_off, arcz_mem* y, int ldy, int y_off, int T, int heads, int hd, arcz_mem* pos, int ld_pos);
 
 /* A cache of keys and values in 8 bits: `pages` pages of `page` tokens (16, 32, 64, 128 or 256), `heads` heads of hd values (64, 128
@@ -203,7 +203,7 @@ arcz_mem* arcz_kv_buffer(arcz_kv* c, int which); /* 0 k, 1 v, 2 ks, 3 vs */
  * max_len: about the most keys of one, for sharing out the work (0: as many as the table holds).  rows, len and table are read when
  * the launch runs and held to the buffers there: rows to [0, T], len to the table, and a page outside the cache is one without
  * tokens -- nothing is written to it, its keys are not seen, it reads as zeros.  Rows of the buffers that belong to no sequence are
- * left as they are. */
+ * left as they are.  A call's outputs -- rows, or the cache -- must not meet rows, len or table. */
 typedef struct arcz_kv_batch {
   arcz_mem *rows, *len, *table;
   int seqs, ld_table, T, max_rows, max_len;
@@ -228,8 +228,8 @@ typedef struct arcz_attn {
 } arcz_attn;
 /* out = softmax(scores) v for T rows of `heads` query heads (a multiple of the cache's; query head h takes the cache's head
  * h / (heads / cache heads)): prompts, chunks behind a context, drafts and single tokens, mixed as they come.  A row that sees
- * nothing gives zeros; what is masked has no effect, whatever the cache holds there.  out must not meet q or the cache.  Sums are
- * those of f32 rows against the cache's values to about 2^-22; the same call gives the same bits. */
+ * nothing gives zeros; what is masked has no effect, whatever the cache holds there.  out must not meet q, the cache, slopes, prefix
+ * or first.  Sums are those of f32 rows against the cache's values to about 2^-22; the same call gives the same bits. */
 int arcz_engine_attention(arcz_engine* e, arcz_kv* c, const arcz_kv_batch* b, arcz_mem* q, int ldq, int q_off, int heads, arcz_mem* out, int ldo, int o_off,
                           const arcz_attn* a);
 

@@ -1,4 +1,5 @@
-"""Which buffers of a call of the attention block may share memory: pieces of one allocation that do not meet."""
+"""Which buffers of a call of the attention block may share memory: outputs and what a launch reads may not, pieces of one allocation that
+do not meet may."""
 import numpy as np
 import pytest
 
@@ -13,6 +14,51 @@ def eng(rt):
     e = az.Engine(16, 256)
     yield e
     e.close()
+
+
+def test_outputs_over_what_is_read_are_refused(eng):
+    """Every output against rows, len, table, pos, slopes, prefix and first: an error, and no launch."""
+    hold = []
+
+    def keep(b):
+        hold.append(b)
+        return b
+    # one allocation: [ints 256 | rows of q, k, v | cache]
+    big = keep(az.Runtime.alloc(1 << 20).fill(0))
+    w, kvw = 4 * 64, 2 * 64
+    ints = keep(big.view(0, 1024))
+    own = [keep(az.Runtime.from_numpy(np.array(a, np.int32))) for a in ([0, 4], [4], [0, 1])]
+    x = keep(az.Runtime.alloc(4 * 2 * w * 4).fill(0))
+    kv = keep(eng.make_kv(2, 16, 16, 2, 64))
+    rope = keep(eng.make_rope([1.0] * 32))
+    a = az.Attention(0.1)
+    n = az.lib.arcz_launch_count()
+
+    def batch(*parts):
+        return az.KvBatch(*parts, 1, 2, 4, 4)
+
+    def refused(f, *args):
+        with pytest.raises(az.ArczError):
+            f(*args)
+        assert az.lib.arcz_launch_count() == n
+    for i in range(3):
+        parts = list(own)
+        parts[i] = ints
+        refused(eng.attention, kv, batch(*parts), x, 2 * w, 0, 4, big, w, 0, a)
+        refused(eng.kv_read, kv, batch(*parts), big, kvw, 0, x, kvw, 0)
+        refused(eng.kv_read, kv, batch(*parts), x, kvw, 0, big, kvw, 0)
+        # (the cache on memory that the batch lies in)
+        c = eng.make_kv(2, 16, 16, 2, 64, k=big)
+        refused(eng.kv_write, c, batch(*parts), x, kvw, 0, x, kvw, 0)
+        c.free()
+        c = eng.make_kv(2, 16, 16, 2, 64, vs=big)
+        refused(eng.kv_write, c, batch(*parts), x, kvw, 0, x, kvw, 0)
+        c.free()
+    for part in ("slopes", "prefix", "first"):
+        refused(eng.attention, kv, batch(*own), x, 2 * w, 0, 4, big, w, 0, az.Attention(0.1, **{part: ints}))
+    refused(eng.rope, rope, x, w, 0, big, w, 0, 4, 4, 64, ints)
+    refused(eng.rope, rope, big, w, 0, big, w, 0, 4, 4, 64, ints)
+    ref.free(hold)
 
 
 def test_pieces_of_one_allocation(eng):
