@@ -150,6 +150,9 @@
   // false: nothing to do
   bool check_batch(const char* what, const Kv& c, const Batch& b) {
     if (!c.b[0]) throw std::runtime_error(std::string(what) + ": no cache");
+    for (int i = 0; i < 4; ++i)   // (a buffer that was freed under the cache, or another one in its handle's place)
+      if (arcz_mem_size(c.b[i]) < c.bytes[i] || (uintptr_t)arcz_mem_ptr(c.b[i]) % (i < 2 ? 16 : 4))
+        throw std::runtime_error(std::string(what) + ": a buffer of the cache is gone");
     if (b.seqs < 0 || b.T < 0 || b.max_rows < 0 || b.ld_table < 0 || b.seqs > 65535)
       throw std::runtime_error(std::string(what) + ": a batch of " + std::to_string(b.seqs) + " sequences, " + std::to_string(b.T) + " rows");
     if (b.seqs == 0 || b.T == 0 || b.max_rows == 0) return false;

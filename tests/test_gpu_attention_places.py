@@ -97,3 +97,22 @@ def test_pieces_of_one_allocation(eng):
         ref.free(hold)
     assert all(np.array_equal(p, q) for p, q in zip(*results))
     assert results[0][5].any() and results[0][6].any()
+
+
+@pytest.mark.parametrize("which", [0, 1, 2, 3])
+def test_a_buffer_freed_under_the_cache(eng, which):
+    """The caller's buffer freed before the cache, smaller ones made behind it (in its handle's place, as it happens): refused."""
+    size = (4 * 2 * 16 * 64, 4 * 2 * 16 * 64, 4 * 2 * 4, 4 * 2 * 4)
+    bufs = [az.Runtime.alloc(n).fill(0) for n in size]
+    kv = eng.make_kv(4, 16, 16, 2, 64, *bufs)
+    own = [az.Runtime.from_numpy(np.array(a, np.int32)) for a in ([0, 1], [1], [3, 3])]
+    batch, x, y = az.KvBatch(*own, 1, 2, 1, 1), az.Runtime.alloc(4 * 256).fill(0), az.Runtime.alloc(4 * 256).fill(0)
+    eng.kv_write(kv, batch, x, 128, 0, x, 128, 0)
+    bufs[which].free()
+    small = [az.Runtime.alloc(16) for _ in range(8)]
+    n = az.lib.arcz_launch_count()
+    for f, args in ((eng.kv_write, (x, 128, 0, x, 128, 0)), (eng.kv_read, (x, 128, 0, y, 128, 0)), (eng.attention, (x, 256, 0, 4, y, 256, 0, az.Attention(0.1)))):
+        with pytest.raises(az.ArczError):
+            f(kv, batch, *args)
+    assert az.lib.arcz_launch_count() == n
+    ref.free([b for i, b in enumerate(bufs) if i != which] + own + [x, y] + small + [kv])
