@@ -121,24 +121,23 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
   uint4 kr[KB / 16];
   uint32_t vr[4][VB / 4];
   float rks = 0.0f, rvs = 0.0f;
-  const char *ka, *va;
-  size_t sa;
+  size_t ka, va, sa;   // (from kmine, vmine, ks and vs on)
   auto address = [&](int st) {
     const uint32_t in = (uint32_t)((base + st * KT) & pm);
     const int pv = whole ? at.k : at.v, pc = whole ? at.k : at.c;
-    ka = kmine + ((size_t)valid(at.k) * page_bytes + in * HD);
-    va = vmine + ((size_t)valid(pv) * page_bytes + in * HD);
+    ka = (size_t)valid(at.k) * page_bytes + in * HD;
+    va = (size_t)valid(pv) * page_bytes + in * HD;
     sa = smine + ((size_t)valid(pc) * page_scales + (in >> bs) * 4);
     return pc;
   };
   auto load = [&](int part) {   // (four parts)
     if (part == 0) {
 #pragma unroll
-      for (int b = 0; b < KB / 16; ++b) kr[b] = *(const uint4*)(ka + 16 * TPK * b);
+      for (int b = 0; b < KB / 16; ++b) kr[b] = *(const uint4*)(kmine + ka + 16 * TPK * b);
     } else if (part < 3) {
 #pragma unroll
       for (int t = 2 * part - 2; t < 2 * part; ++t) {
-        const char* v = va + t * HD;
+        const char* v = vmine + va + t * HD;
         if (VB == 4) vr[t][0] = *(const uint32_t*)v;
         if (VB == 8) { const uint2 u = *(const uint2*)v; vr[t][0] = u.x; vr[t][VB / 8] = u.y; }
         if (VB == 16) { const uint4 u = *(const uint4*)v; vr[t][0] = u.x; vr[t][VB / 16] = u.y; vr[t][VB / 8] = u.z; vr[t][VB / 4 - 1] = u.w; }
