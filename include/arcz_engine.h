@@ -196,7 +196,7 @@ arcz_kv* arcz_kv_create(arcz_engine* e, int pages, int page, int block, int head
 /* Frees the handle and the library's buffers; refused, with everything as it was, while a launch list names them. */
 int arcz_kv_free(arcz_engine* e, arcz_kv* c);
 arcz_mem* arcz_kv_buffer(arcz_kv* c, int which); /* 0 k, 1 v, 2 ks, 3 vs */
-/* The sequences of a call.  Rows [rows[s], rows[s + 1]) of the row buffers belong to sequence s (rows: int32 [seqs + 1], from 0 on,
+/* The sequences of a call.  Rows [rows[s], rows[s + 1]) of the row buffers belong to sequence s (rows: int32 [seqs + 1], not below 0,
  * not falling); len[s] (int32) keys of it are in the cache, those of these rows with them, so its i-th row of n has position
  * len - n + i (rows whose position is below 0 are left out; attention gives them zeros).  table [seqs][ld_table] (int32): page of its
  * positions page * i and on.  T: rows of the buffers; max_rows: the most rows of one sequence (those past it are left out);
@@ -229,7 +229,10 @@ typedef struct arcz_attn {
 /* out = softmax(scores) v for T rows of `heads` query heads (a multiple of the cache's; query head h takes the cache's head
  * h / (heads / cache heads)): prompts, chunks behind a context, drafts and single tokens, mixed as they come.  A row that sees
  * nothing gives zeros; what is masked has no effect, whatever the cache holds there.  out must not meet q, the cache, slopes, prefix
- * or first.  Sums are those of f32 rows against the cache's values to about 2^-22; the same call gives the same bits. */
+ * or first.  Sums are those of f32 rows against the cache's values to about 2^-22; the same call gives the same bits.
+ * Speed: how a call is launched goes by max_rows.  Sequences of one or a few rows beside a prompt are right, but slow, one work-group
+ * to all keys of a sequence and head (a chunk of 2048 rows with 48 tokens behind 4000 keys 396 us, with one behind 131072 4978 us); as two
+ * calls, on views of rows, len and table from each kind's first sequence on, they take 184 and 160. */
 int arcz_engine_attention(arcz_engine* e, arcz_kv* c, const arcz_kv_batch* b, arcz_mem* q, int ldq, int q_off, int heads, arcz_mem* out, int ldo, int o_off,
                           const arcz_attn* a);
 
