@@ -29,41 +29,39 @@
     return r;
   }
 
-  // Rows of a buffer that a call of this part reads or writes: T rows of `width` values from column `off` on, a row every ld.
+  // The bytes of a buffer that a call takes (none: empty).  Each buffer's place is looked up once a call.
+  struct Place {
+    uintptr_t b = 0, e = 0;
+  };
+  static bool overlap(Place a, Place b) { return a.b < b.e && b.b < a.e; }
+  // Rows that a call of this part reads or writes: T rows of `width` values from column `off` on, a row every ld.
   struct Rows {
-    cl_mem m;
-    int ld, off, width, T;
-    uintptr_t begin() const { return (uintptr_t)arcz_mem_ptr(m) + (size_t)off * 4; }
-    uintptr_t end() const { return begin() + ((size_t)(T - 1) * ld + width) * 4; }
-    bool vec() const { return begin() % 16 == 0 && ld % 4 == 0; }
+    uintptr_t begin, end;
+    int ld, width;
+    bool vec() const { return begin % 16 == 0 && ld % 4 == 0; }
+    Place place() const { return {begin, end}; }   // (the columns between the rows too)
   };
   static Rows rows_of(const char* what, cl_mem m, int ld, int off, int width, int T) {
     if (off < 0 || width <= 0 || ld < 0 || (int64_t)off + width > ld)
       throw std::runtime_error(std::string(what) + ": columns " + std::to_string(off) + " ... of " + std::to_string(width) + " in rows of " + std::to_string(ld));
-    if (!m || (uintptr_t)arcz_mem_ptr(m) % 4 || arcz_mem_size(m) < ((size_t)(T - 1) * ld + (size_t)off + width) * 4)
+    const uintptr_t p = (uintptr_t)arcz_mem_ptr(m);
+    const size_t last = ((size_t)(T - 1) * ld + (size_t)off + width) * 4;
+    if (!m || p % 4 || arcz_mem_size(m) < last)
       throw std::runtime_error(std::string(what) + ": the buffer is too small for " + std::to_string(T) + " rows of " + std::to_string(ld));
-    return {m, ld, off, width, T};
+    return {p + (size_t)off * 4, p + last, ld, width};
   }
   // Whether two such sets of rows have a value in common (or may have: rows of different strides in one place).
   static bool overlap(const Rows& a, const Rows& b) {
-    if (a.end() <= b.begin() || b.end() <= a.begin()) return false;
-    if (a.ld != b.ld || (a.begin() > b.begin() ? a.begin() - b.begin() : b.begin() - a.begin()) % 4) return true;
+    if (!overlap(a.place(), b.place())) return false;
+    if (a.ld != b.ld || (a.begin > b.begin ? a.begin - b.begin : b.begin - a.begin) % 4) return true;
     const size_t ld = (size_t)a.ld;
-    const size_t d = a.begin() <= b.begin() ? (b.begin() - a.begin()) / 4 % ld : (ld - (a.begin() - b.begin()) / 4 % ld) % ld;
+    const size_t d = a.begin <= b.begin ? (b.begin - a.begin) / 4 % ld : (ld - (a.begin - b.begin) / 4 % ld) % ld;
     return d < (size_t)a.width || d + (size_t)b.width > ld;
   }
-  // ... and the first n bytes of a buffer, those that a call takes of it (rows of a stride: the columns between them too).
-  static bool overlap(const Rows& a, cl_mem m, size_t n) {
-    const uintptr_t b = (uintptr_t)arcz_mem_ptr(m);
-    return m && !(a.end() <= b || b + n <= a.begin());
-  }
-  static bool overlap(cl_mem a, size_t na, cl_mem b, size_t nb) {
-    const uintptr_t p = (uintptr_t)arcz_mem_ptr(a), q = (uintptr_t)arcz_mem_ptr(b);
-    return a && b && !(p + na <= q || q + nb <= p);
-  }
-  static cl_mem ints(const char* what, cl_mem m, size_t n) {
-    if (!m || (uintptr_t)arcz_mem_ptr(m) % 4 || arcz_mem_size(m) < n * 4) throw std::runtime_error(std::string(what) + " holds less than " + std::to_string(n) + " values");
-    return m;
+  static Place ints(const char* what, const char* part, cl_mem m, size_t n) {
+    const uintptr_t p = (uintptr_t)arcz_mem_ptr(m);
+    if (!m || p % 4 || arcz_mem_size(m) < n * 4) throw std::runtime_error(std::string(what) + ": " + part + " holds less than " + std::to_string(n) + " values");
+    return {p, p + n * 4};
   }
 
   void rope(const Rope& r, cl_mem x, int ldx, int x_off, cl_mem y, int ldy, int y_off, int T, int heads, int hd, cl_mem pos, int ld_pos) {
@@ -72,11 +70,9 @@
     if (T < 0 || heads < 1 || hd < 1 || (int64_t)heads * hd > 0x7FFFFFFF || 2 * r.pairs > hd)
       throw std::runtime_error("rope: " + std::to_string(heads) + " heads of " + std::to_string(hd) + " values, " + std::to_string(r.pairs) + " pairs");
     const Rows a = rows_of("rope: x", x, ldx, x_off, heads * hd, T), b = rows_of("rope: y", y, ldy, y_off, heads * hd, T);
-    if (!(a.begin() == b.begin() && ldx == ldy) && overlap(a, b)) throw std::runtime_error("rope: x and y overlap (in place: the same columns of the same rows)");
+    if (!(a.begin == b.begin && ldx == ldy) && overlap(a, b)) throw std::runtime_error("rope: x and y overlap (in place: the same columns of the same rows)");
     if (ld_pos < T) throw std::runtime_error("rope: positions of " + std::to_string(T) + " rows on axes " + std::to_string(ld_pos) + " apart");
-    const size_t np = (size_t)(r.axes - 1) * ld_pos + T;
-    ints("rope: pos", pos, np);
-    if (overlap(b, pos, np * 4)) throw std::runtime_error("rope: y overlaps pos");
+    if (overlap(b.place(), ints("rope", "pos", pos, (size_t)(r.axes - 1) * ld_pos + T))) throw std::runtime_error("rope: y overlaps pos");
     int vec = a.vec() && b.vec() && hd % 4 == 0, nb = r.neighbours, ax = r.axes, pairs = r.pairs;
     float ms = r.mscale;
     // (few tokens: a token's heads over several work-groups)
@@ -109,15 +105,18 @@
     c.ps = log2_of(page);
     c.bs = log2_of(block);
     const size_t rows = (size_t)pages * heads * page, size[4] = {rows * hd, rows * hd, rows / block * 4, rows / block * 4};
+    Place given_at[4];
     for (int i = 0; i < 4; ++i) {
       cl_mem m = given ? given[i] : nullptr;
       c.bytes[i] = size[i];
       if (!m) continue;
-      if (arcz_mem_size(m) < size[i] || (uintptr_t)arcz_mem_ptr(m) % (i < 2 ? 16 : 4))
+      const uintptr_t at = (uintptr_t)arcz_mem_ptr(m);
+      if (arcz_mem_size(m) < size[i] || at % (i < 2 ? 16 : 4))
         throw std::runtime_error("make_kv: buffer " + std::to_string(i) + " holds " + std::to_string(arcz_mem_size(m)) + " bytes, the cache takes " + std::to_string(size[i]) +
                                  " (the values' at an address of 16)");
+      given_at[i] = {at, at + size[i]};
       for (int j = 0; j < i; ++j)
-        if (overlap(m, size[i], c.b[j], size[j])) throw std::runtime_error("make_kv: two of the buffers overlap");
+        if (overlap(given_at[i], given_at[j])) throw std::runtime_error("make_kv: two of the buffers overlap");
       c.b[i] = m;
     }
     try {
@@ -147,40 +146,42 @@
     cl_mem rows, len, table;
     int seqs, ld_table, T, max_rows, max_len;
   };
+  // What a launch reads of a batch is not what it writes: work-groups that begin later would see it changed.
+  struct Places {
+    Place cache[4], rows, len, table;
+    bool in_cache(const Rows& r) const { return in_cache(r.place()); }
+    bool in_cache(Place p) const {
+      for (const Place& c : cache)
+        if (overlap(p, c)) return true;
+      return false;
+    }
+    bool in_batch(Place p) const { return overlap(p, rows) || overlap(p, len) || overlap(p, table); }
+  };
   // false: nothing to do
-  bool check_batch(const char* what, const Kv& c, const Batch& b) {
+  bool check_batch(const char* what, const Kv& c, const Batch& b, Places& at) {
     if (!c.b[0]) throw std::runtime_error(std::string(what) + ": no cache");
-    for (int i = 0; i < 4; ++i)   // (a buffer that was freed under the cache, or another one in its handle's place)
-      if (arcz_mem_size(c.b[i]) < c.bytes[i] || (uintptr_t)arcz_mem_ptr(c.b[i]) % (i < 2 ? 16 : 4))
-        throw std::runtime_error(std::string(what) + ": a buffer of the cache is gone");
+    for (int i = 0; i < 4; ++i) {   // (a buffer that was freed under the cache, or another one in its handle's place)
+      const uintptr_t p = (uintptr_t)arcz_mem_ptr(c.b[i]);
+      if (arcz_mem_size(c.b[i]) < c.bytes[i] || p % (i < 2 ? 16 : 4)) throw std::runtime_error(std::string(what) + ": a buffer of the cache is gone");
+      at.cache[i] = {p, p + c.bytes[i]};
+    }
     if (b.seqs < 0 || b.T < 0 || b.max_rows < 0 || b.ld_table < 0 || b.seqs > 65535)
       throw std::runtime_error(std::string(what) + ": a batch of " + std::to_string(b.seqs) + " sequences, " + std::to_string(b.T) + " rows");
     if (b.seqs == 0 || b.T == 0 || b.max_rows == 0) return false;
     if (b.ld_table < 1 || (int64_t)b.ld_table * c.page > 0x7FFFF000)
       throw std::runtime_error(std::string(what) + ": " + std::to_string(b.ld_table) + " pages of " + std::to_string(c.page) + " a sequence");
-    ints((std::string(what) + ": rows").c_str(), b.rows, (size_t)b.seqs + 1);
-    ints((std::string(what) + ": len").c_str(), b.len, (size_t)b.seqs);
-    ints((std::string(what) + ": table").c_str(), b.table, (size_t)b.seqs * b.ld_table);
+    at.rows = ints(what, "rows", b.rows, (size_t)b.seqs + 1);
+    at.len = ints(what, "len", b.len, (size_t)b.seqs);
+    at.table = ints(what, "table", b.table, (size_t)b.seqs * b.ld_table);
     return true;
   }
-  // What a launch reads of a batch is not what it writes: work-groups that begin later would see it changed.
-  static size_t table_bytes(const Batch& b) { return (size_t)b.seqs * b.ld_table * 4; }
-  static bool overlap(const Rows& a, const Batch& b) {
-    return overlap(a, b.rows, ((size_t)b.seqs + 1) * 4) || overlap(a, b.len, (size_t)b.seqs * 4) || overlap(a, b.table, table_bytes(b));
-  }
-  static bool overlap(const Rows& a, const Kv& c) {
-    for (int i = 0; i < 4; ++i)
-      if (overlap(a, c.b[i], c.bytes[i])) return true;
-    return false;
-  }
   void kv_write(const Kv& c, const Batch& b, cl_mem k, int ldk, int k_off, cl_mem v, int ldv, int v_off) {
-    if (!check_batch("kv_write", c, b)) return;
+    Places at;
+    if (!check_batch("kv_write", c, b, at)) return;
     const int w = c.heads * c.hd, most = std::min(b.max_rows, b.T);
     const Rows rk = rows_of("kv_write: k", k, ldk, k_off, w, b.T), rv = rows_of("kv_write: v", v, ldv, v_off, w, b.T);
-    if (overlap(rk, c) || overlap(rv, c)) throw std::runtime_error("kv_write: the rows overlap the cache");
-    for (int i = 0; i < 4; ++i)
-      if (overlap(c.b[i], c.bytes[i], b.rows, ((size_t)b.seqs + 1) * 4) || overlap(c.b[i], c.bytes[i], b.len, (size_t)b.seqs * 4) || overlap(c.b[i], c.bytes[i], b.table, table_bytes(b)))
-        throw std::runtime_error("kv_write: the cache overlaps the batch's rows, len or table");
+    if (at.in_cache(rk) || at.in_cache(rv)) throw std::runtime_error("kv_write: the rows overlap the cache");
+    if (at.in_cache(at.rows) || at.in_cache(at.len) || at.in_cache(at.table)) throw std::runtime_error("kv_write: the cache overlaps the batch's rows, len or table");
     int vec = rk.vec() && rv.vec(), pages = c.pages, heads = c.heads, ps = c.ps, bs = c.bs, ldt = b.ld_table, T = b.T, mr = b.max_rows;
     // A work-group's tokens: whole blocks, and up to the eight rows a thread that it holds in registers (read once instead of twice:
     // 8192 rows x 8 heads x 128 values, blocks of 32 tokens, 25 -> 19.6 us; ragged prompts, 4 x 256, a scale a token, 26 -> 14.8).
@@ -193,12 +194,13 @@
     run("kv_write", kn, 3, g, l);
   }
   void kv_read(const Kv& c, const Batch& b, cl_mem k, int ldk, int k_off, cl_mem v, int ldv, int v_off) {
-    if (!check_batch("kv_read", c, b)) return;
+    Places at;
+    if (!check_batch("kv_read", c, b, at)) return;
     const int w = c.heads * c.hd, most = std::min(b.max_rows, b.T);
     const Rows rk = rows_of("kv_read: k", k, ldk, k_off, w, b.T), rv = rows_of("kv_read: v", v, ldv, v_off, w, b.T);
     if (overlap(rk, rv)) throw std::runtime_error("kv_read: k and v overlap");
-    if (overlap(rk, c) || overlap(rv, c)) throw std::runtime_error("kv_read: the rows overlap the cache");
-    if (overlap(rk, b) || overlap(rv, b)) throw std::runtime_error("kv_read: k or v overlaps the batch's rows, len or table");
+    if (at.in_cache(rk) || at.in_cache(rv)) throw std::runtime_error("kv_read: the rows overlap the cache");
+    if (at.in_batch(rk.place()) || at.in_batch(rv.place())) throw std::runtime_error("kv_read: k or v overlaps the batch's rows, len or table");
     int vec = rk.vec() && rv.vec(), pages = c.pages, heads = c.heads, hd = c.hd, ps = c.ps, bs = c.bs, ldt = b.ld_table, T = b.T, mr = b.max_rows;
     int per = std::max(1, 4096 / w);   // (four values a thread, four times)
     cl_kernel kn = variant("attn", {}, "kv_read");
@@ -233,17 +235,19 @@
     at_counts_ = m;
   }
   void attention(const Kv& c, const Batch& b, cl_mem q, int ldq, int q_off, int heads, cl_mem out, int ldo, int o_off, const Attn& a) {
-    if (!check_batch("attention", c, b)) return;
+    Places at;
+    if (!check_batch("attention", c, b, at)) return;
     if (heads < 1 || heads % c.heads || (int64_t)heads * c.hd > 0x7FFFFFFF) throw std::runtime_error("attention: " + std::to_string(heads) + " heads over " + std::to_string(c.heads) + " of the cache");
     if (!std::isfinite(a.scale) || !(a.cap >= 0.0f) || a.cap > 0x1p100f || (a.cap > 0.0f && a.cap < 0x1p-100f) || a.window < 0 || b.max_len < 0)
       throw std::runtime_error("attention: scale, cap, window or max_len");
     const Rows rq = rows_of("attention: q", q, ldq, q_off, heads * c.hd, b.T), ro = rows_of("attention: out", out, ldo, o_off, heads * c.hd, b.T);
     if (overlap(rq, ro)) throw std::runtime_error("attention: q and out overlap");
-    if (overlap(ro, c)) throw std::runtime_error("attention: out overlaps the cache");
-    if (a.slopes) ints("attention: slopes", a.slopes, (size_t)heads);
-    if (a.prefix) ints("attention: prefix", a.prefix, (size_t)b.seqs);
-    if (a.first) ints("attention: first", a.first, (size_t)b.T);
-    if (overlap(ro, b) || overlap(ro, a.slopes, (size_t)heads * 4) || overlap(ro, a.prefix, (size_t)b.seqs * 4) || overlap(ro, a.first, (size_t)b.T * 4))
+    if (at.in_cache(ro)) throw std::runtime_error("attention: out overlaps the cache");
+    Place slopes, prefix, first;
+    if (a.slopes) slopes = ints("attention", "slopes", a.slopes, (size_t)heads);
+    if (a.prefix) prefix = ints("attention", "prefix", a.prefix, (size_t)b.seqs);
+    if (a.first) first = ints("attention", "first", a.first, (size_t)b.T);
+    if (at.in_batch(ro.place()) || overlap(ro.place(), slopes) || overlap(ro.place(), prefix) || overlap(ro.place(), first))
       throw std::runtime_error("attention: out overlaps rows, len, table, slopes, prefix or first");
     const int G = heads / c.heads, most = std::min(b.max_rows, b.T);
     const int64_t M = (int64_t)most * G;
