@@ -184,7 +184,8 @@
     if (at.in_cache(at.rows) || at.in_cache(at.len) || at.in_cache(at.table)) throw std::runtime_error("kv_write: the cache overlaps the batch's rows, len or table");
     int vec = rk.vec() && rv.vec(), pages = c.pages, heads = c.heads, ps = c.ps, bs = c.bs, ldt = b.ld_table, T = b.T, mr = b.max_rows;
     // A work-group's tokens: whole blocks, and up to the eight rows a thread that it holds in registers (read once instead of twice:
-    // 8192 rows x 8 heads x 128 values, blocks of 32 tokens, 25 -> 19.6 us; ragged prompts, 4 x 256, a scale a token, 26 -> 14.8).
+    // 8192 rows x 8 heads x 128 values, blocks of 32 tokens, 25 -> 19.6 us; ragged prompts, 4 x 256, a scale a token, 26 -> 14.8; the rows in
+    // the 256 MB behind the L2s).
     const int full = 8 * 1024 / c.hd;
     int tile = std::max(c.block, most == 1 ? 1 : std::min(full, 1 << log2_of(most)));
     cl_kernel kn = variant("attn", {{"HD", c.hd}}, "kv_write");
@@ -279,9 +280,10 @@
     }
     // Heads of 128 values, blocks of 32 tokens and more: work-groups of eight waves and 256 rows, one a compute unit, where rows are many
     // and see thousands of keys; else of four and 128 rows, two of them, which fill the chip sooner and read and write rows while the
-    // other computes.  (us, 32 heads over 8, eight waves / four: 1024 rows over 9000
-    // keys 278 / 296, 4096 over 4096 271 / 287, 512 over 8192 144 / 150, 2048 over 16000 895 / 936; of fewer keys, before the rows
-    // passed through LDS: 2048 over 2048 117 / 107, 512 over 512 48 / 36, 100 over 4000 50 / 42, ragged documents 102 / 85.)
+    // other computes.  (us, 32 heads over 8, eight waves / four: 1024 rows over 9000 keys 266 / 287, 4096 over 4096 257 / 279, 512 over
+    // 8192 139 / 145, 2048 over 16000 854 / 905, 8192 over 9000 1103 / 1158; 512 over 3000 71.2 / 70.8, 3000 over 3000 163 / 154, 2048 over
+    // 2048 107 / 99, 512 over 512 43 / 34, ragged documents 74.5 / 62.3.  Two that the rule misses: 1024 over 1024 54 / 55.5, 100 over 4000
+    // 44.7 / 46.2.)
     const int seen = std::max(0, (b.max_len > 0 ? b.max_len : ldt * c.page) - most / 2);
     const int waves = c.hd == 128 && c.block >= 32 && M >= 1024 && !a.first && (window ? std::min(window, seen) : seen) >= 2000 ? 8 : 4, bm = 32 * waves;
     int tiles = (int)((M + bm - 1) / bm);

@@ -11,9 +11,9 @@
 //
 // Pieces of one length for all sequences, about two work-groups a compute unit where all are long; they are joined in this launch by the
 // last work-group of their rows to come (joined by a launch of its own: 41 us more behind 131072 keys).
-// Measured, heads of 128 values: one token behind 131072, 40 heads over 8, 56.6 us (4.75 TB/s, a large copy 4.9); 64
-// sequences of up to 8100 keys, 32 over 4, 76.5 us (3.8 TB/s); one behind 517, 9.0 us, and four sequences of eight tokens with heads of
-// 256 under a window 15.9 us: dependent loads -- rows, page, bytes -- and the joining, not bytes.
+// Measured, heads of 128 values: one token behind 131072, 40 heads over 8, 56.7 us (4.75 TB/s, a large copy 4.9); 64
+// sequences of up to 8100 keys, 32 over 4, 75.7 us (3.8 TB/s); one behind 517, 9.0 us, and four sequences of eight tokens with heads of
+// 256 under a window 15.6 us: dependent loads -- rows, page, bytes --, two steps a wave one behind the other, and the joining, not bytes.
 //
 // The eight-bit values are exact in f16.  Rows and weights are split into two f16 each (22 bits), so the sums are those of f32
 // rows to about 2^-22.  Up to eight rows both parts go through one product: the first parts in columns 0-7, what they miss in

@@ -10,14 +10,19 @@
 //                  8 + 4 h + 0..3, so the values' tokens lie in that order in LDS): no weight goes through LDS
 //
 // A row's maximum and sum are its lane's own, but for the two halves of the wave, which meet only where the reference is set
-// anew.  Rows and weights are split into two f16 (22 bits of the f32 value; the sums are those of f32 rows to about 2^-22), so
-// the matrix pipe does twice the products of plain f16 rows; it is what bounds the kernel.
+// anew.  Rows and weights are split into two f16 (22 bits of the f32 value, a row on its own power of two; the sums are those of f32
+// rows to about 2^-22), so the matrix pipe does twice the products of plain f16 rows: most of the time of long prompts.
 //
-// Measured, 32 query heads over 8 of 128 values: 8192 rows behind 808 keys, causal, 1118 - 1184 us = 556 - 587 TFLOP/s of attention,
-// 1112 - 1174 of products (a large f16 matrix product of the library: 1211); the matrix pipe is busy 61 % of the cycles at the clock
-// that it then holds.  On the way there: 2000 us with the tiles' rows 8 and 16 bytes apart in the same banks (conflicts in 64 % of the
-// LDS's cycles, now 0.3 %); 1303 with the rows that see the most keys first; 1141 with no wait for a page's number inside the loop.
-// Rows of several documents (1333 rows, 40 heads): 68.6 us, the matrix pipe busy 22 %: most tiles are one document's end.
+// Measured, 32 query heads over 8 of 128 values: 8192 rows behind 808 keys, causal, 1109 - 1172 us by the card = 562 - 593 TFLOP/s of
+// attention, 1124 - 1186 of products (a large f16 matrix product of the library: 1211).  The matrix pipe is busy 62 % of 2.05 million
+// cycles, which makes about 1.85 GHz: like the library's product the launch runs below the card's highest clock, and the third of
+// the cycles in which no product is under way (a tile's meeting, weights that are not done when they are wanted) costs less time
+// than it would at that.  On the way there: 2000 us with the tiles' rows 8 and 16 bytes apart in the same banks (conflicts in 64 %
+// of the LDS's cycles, now 0.3 %); 1303 with the rows that see the most keys first; 1141 with no wait for a page's number inside the
+// loop; the last 7 to 10 with keys and values as global loads (through pointers of no known address space they counted among
+// the LDS reads, and every operand was waited for with them).
+// Rows of several documents (1333 rows, 40 heads): 67 us, the matrix pipe busy 22 %: most tiles are one document's end.
+// Heads of 256 with a scale for each few keys and a cap spill 4 and 8 registers, behind the loop.
 #include "attn.h"
 
 // Nothing is moved across by the compiler.

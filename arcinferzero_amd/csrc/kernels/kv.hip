@@ -11,8 +11,9 @@
 // work-groups touch a block and the result does not depend on their order.  hd / 4 threads take a row, four values each.
 // Bound: 4 bytes of HBM read and one written a value; the rows stay in registers between the largest value and the rounding where a
 // tile is at most eight rows a thread, else the second look at them comes from the L2.
-// Measured: 8192 tokens x 8 heads x 128 values written in 19.6 us (4.3 TB/s), read back in 16.5 us (5.1 TB/s); 48 tokens of as many
-// sequences, 32 heads, 5.7 and 7.9 us, of which a launch and the chain row count -> page -> value are most.
+// Measured: 8192 tokens x 8 heads x 128 values, columns of rows of 24 KB, written in 33.8 us from memory (2.5 TB/s), 19.6 us (4.3 TB/s) where
+// the rows are still in the 256 MB behind the L2s, as those of a product just made are; read back behind that in 16.8 us (5.0
+// TB/s); 48 tokens of as many sequences, 8 heads, 6.0 and 8.0 us, of which a launch and the chain row count -> page -> value are most.
 #include "attn.h"
 
 // NP passes of a tile are held in registers, so that a tile of that size is read once and all its loads are on their way at once;

@@ -9,8 +9,11 @@
 // most pi / 4 for the Taylor series of sine (to x^9, truncation 2e-9) and cosine (to x^10, 1e-10).
 //
 // Bound: 8 bytes of HBM a value; a work-group turns the heads of one token, whose sines and cosines it works out once into LDS (a head
-// to a work-group would work them out again for each; a work-group of several tokens would leave fewer than the chip takes).
-// Measured (launches back to back): 4096 tokens x 48 heads x 128 values on three axes 38.9 us, 5.2 TB/s (a large copy: 4.9); 777
+// to a work-group would work them out again for each).  A token of few heads does not fill its work-group: 8192 tokens of 5 heads of 64
+// values 8.4 us, 2.5 TB/s, of 10 of 128 15.2 us, 5.5 TB/s; several tokens a work-group were not tried.  Pairs that are no multiple of
+// four (of two, where neighbours) go value by value, a division each.
+// Measured (launches back to back): 4096 tokens x 48 heads x 128 values on three axes 38.9 us, 5.2 TB/s (a large copy: 4.9), 31
+// where the rows are still in the 256 MB behind the L2s; 777
 // tokens, half of each head turned, neighbours 6.5 us, 4.4 TB/s; one token 3.9 us, a launch's own time.
 #include "attn.h"
 
