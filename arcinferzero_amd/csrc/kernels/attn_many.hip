@@ -426,18 +426,20 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
         });
         stay(ph0, pl0);
         sum += sum0;
-        // (A reference set anew here lowers the first part's weights too, which are not in the sums yet: as the f32 values that their two
-        //  f16 hold exactly, split again -- f itself may lie below the smallest f16, a weight of 2^15 times f does not.)
+        // (A reference set anew here lowers the first part's weights too, which are not in the sums yet.  2^-25 and less is 0 in f16,
+        //  where a weight of 2^15 times it still is 2^-10: by 2^-24 first, then by the rest.  Both f16 are rounded by 2^-25 at most,
+        //  together what a split cuts off.  Split anew from their f32 values, rows with a distance, whose reference moves with every
+        //  tile, took 10 % longer.)
         const float f = refer(1, s1);
         if (__any(f != 1.0f)) {
+          const _Float16 f1 = (_Float16)fmaxf(f, 0x1p-24f);
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
+          for (int k = 0; k < 2; ++k) { ph0[k] *= f1; pl0[k] *= f1; }
+          if (__any(f < 0x1p-24f)) {
+            const _Float16 f2 = (_Float16)fminf(f * 0x1p24f, 1.0f);
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-              h2 a, l;
-              split2(((float)ph0[k][e] + (float)pl0[k][e]) * f, ((float)ph0[k][e + 1] + (float)pl0[k][e + 1]) * f, one, a, l);
-              ph0[k][e] = a.x; ph0[k][e + 1] = a.y; pl0[k][e] = l.x; pl0[k][e + 1] = l.y;
-            }
+            for (int k = 0; k < 2; ++k) { ph0[k] *= f2; pl0[k] *= f2; }
+          }
         }
         add(0, ph0, pl0, [&](int i) {
 #pragma unroll
