@@ -22,7 +22,8 @@
 // loop; the last 7 to 10 with keys and values as global loads (through pointers of no known address space they counted among
 // the LDS reads, and every operand was waited for with them).
 // Rows of several documents (1333 rows, 40 heads): 67 us, the matrix pipe busy 22 %: most tiles are one document's end.
-// Heads of 256 with a scale for each few keys and a cap spill 4 and 8 registers, behind the loop.
+// Spills, all before and behind the loop: 4 and 8 registers of heads of 256 with a scale for each few keys and a cap, 9 of eight waves with
+// a distance.
 #include "attn.h"
 
 // Nothing is moved across by the compiler.
@@ -315,7 +316,7 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
       }
     };
     // (register e of the product: key 8 (e / 4) + 4 hf + e % 4)
-    auto refer = [&](int nt, f16v& sc) {
+    auto against = [&](int nt, f16v& sc, int pos) {   // the scores against the reference; the largest
       const int jn = j0 + nt * 32;
       float kf1 = 0.0f, lv1 = 0.0f;
       if (!FINE) { kf1 = skf[buf][nt] * kfac; lv1 = slv[buf][nt] - ref; }
@@ -359,12 +360,40 @@ __device__ inline void many_body(const float* __restrict__ q, int ldq, int q_off
       float top = fmaxf(sc[0], sc[1]);
 #pragma unroll
       for (int e = 2; e < 16; e += 2) top = fmaxf(fmaxf(top, sc[e]), sc[e + 1]);
+      return top;
+    };
+    auto refer = [&](int nt, f16v& sc) {
+      float top = against(nt, sc, pos);
       if (__any(top > limit)) {
         top = fmaxf(top, __shfl_xor(top, 32));
+        const bool seen = limit > NOTHING;
+        const float old = ref;
+        // (Scores against a reference far below them are rounded to its distance, 2^-19 of an octave within 64 octaves of it.  Where a
+        //  row is further off its scores are made again, against 0 as the first ones are.  With a cap the distance is two of it at
+        //  most, and a score's error more than this.)
+        const bool far = !CAP && seen && top > 56.0f;
+        if (!CAP && __builtin_expect(__any(far), 0)) {
+          const _Float16* kp = &sk[buf][(nt * 32 + c) * KLD + hf * 8];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sc[e] = 0.0f;
+#pragma unroll
+          for (int k = 0; k < KSTEPS; ++k) {
+            const h8 a = *(const h8*)(kp + k * 16);
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[k], sc, 0, 0, 0);
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, QLDS ? *(const h8*)(mine + k * 16) : ql[QLDS ? 0 : k], sc, 0, 0, 0);
+            turn();
+          }
+          ref = far ? 0.0f : ref;
+          limit = far ? NOTHING : limit;
+          int p = pos;
+          asm volatile("" : "+v"(p));   // (the distances worked out again: they do not fit beside the scores)
+          top = against(nt, sc, p);
+          top = fmaxf(top, __shfl_xor(top, 32));
+        }
         const bool anew = top > limit;
         const float by = anew ? floorf(top) - SETS : 0.0f;   // (whole octaves: weights already made are brought along exactly)
-        const float f = limit > NOTHING ? exp2_f(-by) : 1.0f;   // (nothing summed yet)
         ref += by;
+        const float f = seen ? exp2_f(old - ref) : 1.0f;   // (else nothing summed yet)
         limit = anew ? PASSES : limit;
         sum *= f;
 #pragma unroll

@@ -156,3 +156,24 @@ def test_rows_before_position_0_behind_a_prefix(eng, seqs, window):
     assert not got[:out].any()
     got = check(eng, seqs, 8, 2, 128, 32, 32, dict(prefix=[2 ** 31 - 1, 60], window=window), only=set(range(out, T)))
     assert not got[:out].any()
+
+
+@pytest.mark.parametrize("hd,page,block,rows,keys,heads", [(64, 64, 64, 40, 240, 1), (64, 16, 4, 40, 240, 2), (64, 32, 32, 100, 250, 2), (128, 64, 16, 40, 240, 1), (128, 64, 64, 40, 240, 1),
+                                                           (256, 32, 32, 40, 240, 1), (256, 16, 16, 40, 240, 2), (128, 64, 64, 300, 4100, 4), (128, 64, 64, 2, 1000, 4)])
+@pytest.mark.parametrize("deep", [2.0, 8.0, 256.0])
+@pytest.mark.parametrize("form", ["plain", "cap", "distance"])
+def test_first_keys_far_below_the_others(eng, hd, page, block, rows, keys, heads, deep, form):
+    """The first 32 keys of a tile of 64 (of the one in front too, in work-groups of eight waves) have scores 76 to 9754 octaves below zero,
+    those behind them ordinary ones: no bits of those hang on the first reference."""
+    b = ref.Batch([(rows, keys)], page, seed=1)
+    rng = np.random.default_rng(2)
+    t = 32 * 64 if keys > 4000 else 0
+    n = 64 if keys > 4000 else 32
+    c = scored(b, page, block, 1, hd, {p: int(v) for p, v in enumerate(rng.integers(-20, 21, size=keys)) if not t <= p < t + n})
+    for p in range(t, t + n):
+        c.q[0, b.table[0, p // page], :, p % page, 0] = -127
+        if block <= 32 or n == 64:
+            c.d[0, b.table[0, p // page], :, p % page // block] = deep
+    q = lines(b.T, heads, hd)
+    f = dict(plain=dict(scale=1.0), cap=dict(scale=1.0, cap=8000.0), distance=dict(scale=1.0, slopes=np.full(heads, 2.0 ** -9)))[form]
+    check(eng, [(rows, keys)], heads, 1, hd, page, block, f, b=b, c=c, q=q, only={0, 1, rows // 2, rows - 1})
