@@ -125,6 +125,8 @@ _sig("arcz_engine_moe_slots", _i, _p)
 _sig("arcz_rope_create", _p, _p, _i, _p, _p, _i, _i, C.c_float)
 _sig("arcz_rope_free", _i, _p, _p)
 _sig("arcz_engine_rope", _i, _p, _p, _p, _i, _i, _p, _i, _i, _i, _i, _i, _p, _i)
+_sig("arcz_engine_norm_rope", _i, _p, _p, _p, _i, _i, _p, _i, _i, _i, _i, _i, _i, _p, _p, C.c_float, _p, _i)
+_sig("arcz_engine_kv_plan", _i, _p, _p, _p)
 _sig("arcz_kv_create", _p, _p, _i, _i, _i, _i, _i, _p, _p, _p, _p)
 _sig("arcz_kv_free", _i, _p, _p)
 _sig("arcz_kv_buffer", _p, _p, _i)
@@ -152,13 +154,16 @@ _sig("arcz_gen_weights", _i, _u32, _u64, _z, _i, C.c_float, _p)
 _quantize, _rmsnorm_quant, _swiglu_quant = lib.arcz_engine_quantize, lib.arcz_engine_rmsnorm_quant, lib.arcz_engine_swiglu_quant
 _matmul, _gemv_gu, _layer_moe = lib.arcz_engine_matmul, lib.arcz_engine_gemv_gu, lib.arcz_engine_layer_moe
 _rope, _kv_write, _kv_read, _attention = lib.arcz_engine_rope, lib.arcz_engine_kv_write, lib.arcz_engine_kv_read, lib.arcz_engine_attention
+_norm_rope, _kv_plan = lib.arcz_engine_norm_rope, lib.arcz_engine_kv_plan
 try:
     from . import _pycall
     _pycall.bind(_quantize, _rmsnorm_quant, _swiglu_quant, _matmul, _gemv_gu, _layer_moe)
     _pycall.bind_attn(_rope, _kv_write, _kv_read, _attention)
+    _pycall.bind_step(_norm_rope, _kv_plan)
     from ._pycall import gemv_gu as _gemv_gu, layer_moe as _layer_moe, matmul as _matmul, quantize as _quantize
     from ._pycall import rmsnorm_quant as _rmsnorm_quant, swiglu_quant as _swiglu_quant
     from ._pycall import attention as _attention, kv_read as _kv_read, kv_write as _kv_write, rope as _rope
+    from ._pycall import kv_plan as _kv_plan, norm_rope as _norm_rope
 except ImportError:
     pass
 
@@ -531,6 +536,17 @@ class KvBatch(C.Structure):
         self.at = C.addressof(self)
 
 
+class KvPlan(C.Structure):
+    """What Engine.kv_plan makes a batch of (arcz_kv_plan): buffers, all int32, of add and before [seqs], ring [pages], state and after [4], shared
+    [seqs], pos and slot [T], the last three or None."""
+    _fields_ = [(n, _p) for n in ("add", "before", "ring", "state", "after", "shared", "pos", "slot")] + [("pages", _i), ("page", _i)]
+
+    def __init__(self, pages, page, add, before, ring, state, after, pos=None, slot=None, shared=None):
+        self.held = (add, before, ring, state, after, shared, pos, slot)
+        super().__init__(*(b.h if b else None for b in self.held), pages, page)
+        self.at = C.addressof(self)
+
+
 class Attention(C.Structure):
     """The form of an attention (arcz_attn): slopes f32 [heads], prefix int32 [seqs], first int32 [T], each a buffer or None."""
     _fields_ = [("scale", C.c_float), ("cap", C.c_float), ("window", _i), ("slopes", _p), ("prefix", _p), ("first", _p)]
@@ -705,12 +721,26 @@ class Engine:
         if r:
             _check(r, engine=True)
 
+    def norm_rope(self, rope, x, ldx, x_off, y, ldy, y_off, T, heads, kv_heads, hd, wq, wk, eps, pos, ld_pos=None):
+        """T rows of `heads` heads of queries and kv_heads of keys behind them, each head brought to unit mean square, weighted (wq, wk: f32 [hd] or
+        None) and turned by the row's position."""
+        r = _norm_rope(self.h, rope.h, x.h, ldx, x_off, y.h, ldy, y_off, T, heads, kv_heads, hd, wq.h if wq else None, wk.h if wk else None, float(eps), pos.h,
+                       T if ld_pos is None else ld_pos)
+        if r:
+            _check(r, engine=True)
+
     def make_kv(self, pages, page, block, heads, hd, k=None, v=None, ks=None, vs=None):
         """An 8-bit cache of `pages` pages of `page` tokens, a scale for each `block` tokens and head; on the caller's buffers, or its own."""
         h = lib.arcz_kv_create(self.h, pages, page, block, heads, hd, *(b.h if b else None for b in (k, v, ks, vs)))
         if not h:
             raise ArczError(-100, lib.arcz_engine_error().decode())
         return KvCache(self, h, pages, page, block, heads, hd)
+
+    def kv_plan(self, batch, plan):
+        """The batch's rows, lengths and new pages (and its rows' positions and places) out of how many tokens each sequence gets."""
+        r = _kv_plan(self.h, batch.at, plan.at)
+        if r:
+            _check(r, engine=True)
 
     def kv_write(self, kv, batch, k, ldk, k_off, v, ldv, v_off):
         """The batch's rows of k and v into the cache, quantized."""

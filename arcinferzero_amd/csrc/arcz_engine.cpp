@@ -267,6 +267,13 @@ int arcz_engine_rope(arcz_engine* e, arcz_rope* r, arcz_mem* x, int ldx, int x_o
     e->e->rope(r->r, x, ldx, x_off, y, ldy, y_off, T, heads, hd, pos, ld_pos);
   });
 }
+int arcz_engine_norm_rope(arcz_engine* e, arcz_rope* r, arcz_mem* x, int ldx, int x_off, arcz_mem* y, int ldy, int y_off, int T, int heads, int kv_heads, int hd, arcz_mem* wq,
+                          arcz_mem* wk, float eps, arcz_mem* pos, int ld_pos) {
+  return guarded([&] {
+    if (!r) throw std::runtime_error("norm_rope: no rotation");
+    e->e->norm_rope(r->r, x, ldx, x_off, y, ldy, y_off, T, heads, kv_heads, hd, wq, wk, eps, pos, ld_pos);
+  });
+}
 arcz_kv* arcz_kv_create(arcz_engine* e, int pages, int page, int block, int heads, int hd, arcz_mem* k, arcz_mem* v, arcz_mem* ks, arcz_mem* vs) {
   arcz_kv* c = new arcz_kv;
   arcz_mem* const given[4] = {k, v, ks, vs};
@@ -286,6 +293,12 @@ arcz_mem* arcz_kv_buffer(arcz_kv* c, int which) { return c && which >= 0 && whic
 static Engine::Batch batch_of(const char* what, const arcz_kv* c, const arcz_kv_batch* b) {
   if (!c || !b) throw std::runtime_error(std::string(what) + (c ? ": no batch" : ": no cache"));
   return {b->rows, b->len, b->table, b->seqs, b->ld_table, b->T, b->max_rows, b->max_len};
+}
+int arcz_engine_kv_plan(arcz_engine* e, const arcz_kv_batch* b, const arcz_kv_plan* p) {
+  return guarded([&] {
+    if (!b || !p) throw std::runtime_error(b ? "kv_plan: no plan" : "kv_plan: no batch");
+    e->e->kv_plan({b->rows, b->len, b->table, b->seqs, b->ld_table, b->T, b->max_rows, b->max_len}, {p->add, p->before, p->ring, p->state, p->after, p->shared, p->pos, p->slot, p->pages, p->page});
+  });
 }
 int arcz_engine_kv_write(arcz_engine* e, arcz_kv* c, const arcz_kv_batch* b, arcz_mem* k, int ldk, int k_off, arcz_mem* v, int ldv, int v_off) {
   return guarded([&] { e->e->kv_write(c ? c->c : Engine::Kv(), batch_of("kv_write", c, b), k, ldk, k_off, v, ldv, v_off); });

@@ -83,6 +83,40 @@
     run("rope", k, 2, g, l);
   }
 
+  // Norm and rotation of `nq` heads of queries and nk of keys behind them (kernels/norm_rope.hip).
+  void norm_rope(const Rope& r, cl_mem x, int ldx, int x_off, cl_mem y, int ldy, int y_off, int T, int nq, int nk, int hd, cl_mem wq, cl_mem wk, float eps, cl_mem pos,
+                 int ld_pos) {
+    if (!r.tab) throw std::runtime_error("norm_rope: no rotation");
+    if (T < 0 || nq < 0 || nk < 0 || (int64_t)nq + nk < 1 || hd < 1 || ((int64_t)nq + nk) * hd > 0x7FFFFFFF || 2 * r.pairs > hd)
+      throw std::runtime_error("norm_rope: " + std::to_string(nq) + " and " + std::to_string(nk) + " heads of " + std::to_string(hd) + " values, " + std::to_string(r.pairs) + " pairs");
+    if (!std::isfinite(eps) || eps < 0.0f) throw std::runtime_error("norm_rope: eps");
+    if (T == 0) return;
+    int heads = nq + nk;
+    const Rows a = rows_of("norm_rope: x", x, ldx, x_off, heads * hd, T), b = rows_of("norm_rope: y", y, ldy, y_off, heads * hd, T);
+    if (!(a.begin == b.begin && ldx == ldy) && overlap(a, b)) throw std::runtime_error("norm_rope: x and y overlap (in place: the same columns of the same rows)");
+    if (ld_pos < T) throw std::runtime_error("norm_rope: positions of " + std::to_string(T) + " rows on axes " + std::to_string(ld_pos) + " apart");
+    Place weights[2];
+    if (wq) weights[0] = ints("norm_rope", "the queries' weight", wq, (size_t)hd);
+    if (wk) weights[1] = ints("norm_rope", "the keys' weight", wk, (size_t)hd);
+    if (overlap(b.place(), ints("norm_rope", "pos", pos, (size_t)(r.axes - 1) * ld_pos + T)) || overlap(b.place(), weights[0]) || overlap(b.place(), weights[1]))
+      throw std::runtime_error("norm_rope: y overlaps pos or a weight");
+    int nb = r.neighbours, ax = r.axes, pairs = r.pairs, rest = hd - 2 * pairs, L = 0;
+    float ms = r.mscale;
+    // lanes a head: eight values each, four behind the pairs
+    const int need = nb ? (hd + 7) / 8 : std::max(pairs, rest) / 4;
+    if (a.vec() && b.vec() && hd % 4 == 0 && pairs % (nb ? 2 : 4) == 0 && need <= 64) L = 1 << log2_of(need);
+    // Few tokens: a token's heads over several work-groups, as long as these are one round of the chip (40 heads of 128 values, us, one work-group a
+    // token / three: 64 tokens 4.8 / 3.6, 256 tokens 5.7 / 4.8; 777 11.2 / 12.5 (24 of 256), 2500 24.0 / 28.3, 8192 63 / 78).  Few heads: several tokens a
+    // work-group, as far as their sines fit.
+    const int lanes = L ? L : 64, round = 256 / lanes;
+    int per = (int64_t)T * ((heads + round - 1) / round) > 8 * arcz_device_cus() ? heads : std::min(heads, round), tpw = 1;
+    if (per == heads) tpw = std::max(1, std::min({T, round / heads, 512 / pairs}));
+    cl_kernel k = variant("attn", {{"FORM", L ? nb : 2}}, "norm_rope");
+    set_args(k, 0, x, ldx, x_off, y, ldy, y_off, wq, wk, eps, pos, ld_pos, r.tab, pairs, ax, nb, ms, T, nq, heads, hd, tpw, per, L);
+    size_t g[2] = {(size_t)((T + tpw - 1) / tpw) * 256, (size_t)((heads + per - 1) / per)}, l[2] = {256, 1};
+    run("norm_rope", k, 2, g, l);
+  }
+
   // ---- the cache
   struct Kv {
     int pages = 0, page = 0, block = 0, heads = 0, hd = 0, ps = 0, bs = 0;
@@ -175,6 +209,52 @@
     at.table = ints(what, "table", b.table, (size_t)b.seqs * b.ld_table);
     return true;
   }
+  // ---- a pass's batch made on the GPU (kernels/plan.hip)
+  struct Plan {
+    cl_mem add, before, ring, state, after, shared, pos, slot;
+    int pages, page;
+  };
+  void kv_plan(const Batch& b, const Plan& p) {
+    const std::string what = "kv_plan";
+    if (b.seqs < 0 || b.seqs > 65535 || b.T < 0 || b.max_rows < 0 || b.ld_table < 0)
+      throw std::runtime_error(what + ": a batch of " + std::to_string(b.seqs) + " sequences, " + std::to_string(b.T) + " rows");
+    if (p.pages < 1 || p.page < 16 || p.page > 256 || (p.page & (p.page - 1)))
+      throw std::runtime_error(what + ": " + std::to_string(p.pages) + " pages of " + std::to_string(p.page) + " tokens (16, 32, 64, 128 or 256)");
+    if (p.slot && (int64_t)p.pages * p.page > 0x7FFFFFFF) throw std::runtime_error(what + ": places of " + std::to_string(p.pages) + " pages of " + std::to_string(p.page) + " tokens do not fit 32 bits");
+    if (b.seqs == 0) return;
+    if (b.ld_table < 1 || (int64_t)b.ld_table * p.page > 0x7FFFF000) throw std::runtime_error(what + ": " + std::to_string(b.ld_table) + " pages of " + std::to_string(p.page) + " a sequence");
+    const size_t n = (size_t)b.seqs;
+    const char* const name = "kv_plan";
+    // what is written, then what is read
+    Place out[7] = {ints(name, "rows", b.rows, n + 1), ints(name, "len", b.len, n), ints(name, "table", b.table, n * b.ld_table), ints(name, "ring", p.ring, (size_t)p.pages),
+                    ints(name, "after", p.after, 4)};
+    if (p.pos) out[5] = ints(name, "pos", p.pos, (size_t)b.T);
+    if (p.slot) out[6] = ints(name, "slot", p.slot, (size_t)b.T);
+    Place in[4] = {ints(name, "add", p.add, n), ints(name, "before", p.before, n), ints(name, "state", p.state, 4)};
+    if (p.shared) in[3] = ints(name, "shared", p.shared, n);
+    for (int i = 0; i < 7; ++i) {
+      for (int j = 0; j < i; ++j)
+        if (overlap(out[i], out[j])) throw std::runtime_error(what + ": two of rows, len, table, ring, after, pos and slot overlap");
+      for (int j = 0; j < 4; ++j)   // (lengths and the ring's state may be brought on where they are)
+        if (overlap(out[i], in[j]) && !((i == 1 && j == 1) || (i == 4 && j == 2)) ) throw std::runtime_error(what + ": what is written overlaps add, before, state or shared");
+    }
+    if ((overlap(out[1], in[1]) && out[1].b != in[1].b) || (overlap(out[4], in[2]) && out[4].b != in[2].b))
+      throw std::runtime_error(what + ": before and len, or state and after, overlap (in place: the same values)");
+    // Up to PLAN_ROWS rows the work-group that makes the batch writes their places too; more are a second launch.
+    int seqs = b.seqs, ldt = b.ld_table, T = b.T, mr = b.max_rows, pages = p.pages, ps = log2_of(p.page);
+    const bool places = (p.pos || p.slot) && T > 0 && mr > 0;
+    int with = places && std::min<int64_t>(T, (int64_t)seqs * mr) <= PLAN_ROWS ? 1 : 0;
+    cl_kernel k = variant("attn", {}, "kv_plan");
+    set_args(k, 0, p.add, p.before, b.len, b.rows, b.table, ldt, p.ring, p.state, p.after, p.shared, p.pos, p.slot, seqs, T, mr, pages, ps, with);
+    size_t g1 = seqs <= 256 ? 256 : 1024, l1 = g1;
+    run("kv_plan", k, 1, &g1, &l1);
+    if (!places || with) return;
+    cl_kernel k2 = variant("attn", {}, "kv_places");
+    set_args(k2, 0, b.rows, b.len, b.table, ldt, p.pos, p.slot, T, mr, pages, ps);
+    size_t g[2] = {(size_t)((std::min(mr, T) - 1) / 1024 + 1) * 256, n}, l[2] = {256, 1};
+    run("kv_places", k2, 2, g, l);
+  }
+  static constexpr int PLAN_ROWS = 8192;
   void kv_write(const Kv& c, const Batch& b, cl_mem k, int ldk, int k_off, cl_mem v, int ldv, int v_off) {
     Places at;
     if (!check_batch("kv_write", c, b, at)) return;

@@ -27,6 +27,8 @@
     BLOB arcz_blob_moe_d, "moe_d.hsaco"
     BLOB arcz_blob_moe, "moe.hsaco"
     BLOB arcz_blob_rope, "rope.hsaco"
+    BLOB arcz_blob_norm_rope, "norm_rope.hsaco"
+    BLOB arcz_blob_plan, "plan.hsaco"
     BLOB arcz_blob_kv, "kv.hsaco"
     BLOB arcz_blob_attn_few, "attn_few.hsaco"
     BLOB arcz_blob_attn_many, "attn_many.hsaco"

@@ -126,6 +126,9 @@ static const KernelSpec kKernelTable[] = {
     {"moe", "moe_quant_sums", nullptr, "piippp", {nullptr}, {{"FV", 1 << 30, false}, {nullptr, 0, false}}, 256},
     // ---- attn (-DHD: the head's length; -DFORM: bit 0 scores capped, bit 1 a bias by distance)
     {"attn", "rope", nullptr, "piipiipipiiifiiii", {nullptr}, {{nullptr, 0, false}}, 256},
+    {"attn", "norm_rope", nullptr, "piipiippfpipiiifiiiiiii", {"FORM", nullptr}, {{nullptr, 0, false}}, 256},
+    {"attn", "kv_plan", nullptr, "pppppippppppiiiiii", {nullptr}, {{nullptr, 0, false}}, 0},
+    {"attn", "kv_places", nullptr, "pppippiiii", {nullptr}, {{nullptr, 0, false}}, 256},
     {"attn", "kv_write", nullptr, "piipiippppiiiipppiiiii", {"HD", nullptr}, {{nullptr, 0, false}}, 256},
     {"attn", "kv_read", nullptr, "piipiippppiiiiipppiiiii", {nullptr}, {{nullptr, 0, false}}, 256},
     {"attn", "attn_few", nullptr, "piippppiiipppiiiiipiiffipppppiii", {"HD", "RT", "PACK", "FINE", "FORM", nullptr}, {{nullptr, 0, false}}, 256},

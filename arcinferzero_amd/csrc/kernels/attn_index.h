@@ -65,4 +65,30 @@ ATTN_FN int tile_at(int from, int to, int tile, int i) {
 // Where the table has the page of a position: within its row of ldt entries also for a position behind the last key (up to 4096
 // behind it; most_len is at most 2^31 - 4096).
 ATTN_FN int entry_of(int p, int ps, int ldt) { return lower(p >> ps, ldt - 1); }
+// What a plan does to a sequence: `add` tokens behind the `before` that it has, or -add taken off, in pages of 2^ps tokens, `ldt` of them at most.  Its pages
+// are then the entries [0, has) of the table, [0, had) before; `take` of them new, or those from `has` on, `give` of them, given back -- never
+// those that lie whole in the first `shared` positions.  fits: no more than max_rows tokens, no more pages than the table has.
+struct Change {
+  int before, len, rows, had, has, take, give;
+  bool fits;
+};
+ATTN_FN Change change_of(int before, int add, int shared, int ps, int ldt, int max_rows) {
+  const int most = ldt << ps, mask = (1 << ps) - 1;   // (most: at most 2^31 - 4096)
+  Change c;
+  c.before = lower(upper(before, 0), most);
+  c.had = (c.before + mask) >> ps;
+  c.fits = add <= max_rows && add <= most - c.before;
+  c.rows = c.fits ? upper(add, 0) : 0;
+  c.len = add < 0 ? (c.before > -(add + 1) ? c.before + add : 0) : c.before + c.rows;
+  c.has = (c.len + mask) >> ps;
+  if (add < 0) c.has = lower(c.had, upper(c.has, lower(upper(shared, 0), most) >> ps));
+  c.take = upper(c.has - c.had, 0);
+  c.give = upper(c.had - c.has, 0);
+  return c;
+}
+// The i-th place behind `from` in a ring of n (from below n, i at most n).
+ATTN_FN unsigned ring_at(unsigned from, unsigned i, unsigned n) {
+  const unsigned k = from + i;   // (below 2^32: n is below 2^31)
+  return k >= n ? k - n : k;
+}
 }  // namespace attn

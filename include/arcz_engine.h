@@ -184,6 +184,13 @@ int arcz_rope_free(arcz_engine* e, arcz_rope* r);
  * columns that do not meet them.  pos int32 [axes][ld_pos], ld_pos >= T; any int32 is a position.  y must not meet pos. */
 int arcz_engine_rope(arcz_engine* e, arcz_rope* r, arcz_mem* x, int ldx, int x_off, arcz_mem* y, int ldy, int y_off, int T, int heads, int hd, arcz_mem* pos, int ld_pos);
 
+/* Norms of queries and keys, a head at a time, with the rotation in the same pass: the first `heads` heads of x are queries, kv_heads of keys
+ * lie behind them (either may be 0).  A head's values n = x / sqrt(mean(x^2) + eps) * w -- wq for queries, wk for keys, f32 [hd], NULL: no
+ * weight -- are then turned as arcz_engine_rope turns them; what lies behind the pairs is n as it is.  eps is finite and not below 0 (a head of
+ * zeros gives zeros).  No finite head overflows or vanishes on the way.  x, y, pos as there; y must not meet wq, wk or pos. */
+int arcz_engine_norm_rope(arcz_engine* e, arcz_rope* r, arcz_mem* x, int ldx, int x_off, arcz_mem* y, int ldy, int y_off, int T, int heads, int kv_heads, int hd, arcz_mem* wq,
+                          arcz_mem* wk, float eps, arcz_mem* pos, int ld_pos);
+
 /* A cache of keys and values in 8 bits: `pages` pages of `page` tokens (16, 32, 64, 128 or 256), `heads` heads of hd values (64, 128
  * or 256), one f32 scale for each block of `block` tokens (a power of two, 1 to page) and head.  k, v: int8 [pages][heads][page][hd];
  * ks, vs: f32 [pages][heads][page / block]; value = int8 * scale.  Each buffer is the caller's (kept until arcz_kv_free; k and v
@@ -208,6 +215,29 @@ typedef struct arcz_kv_batch {
   arcz_mem *rows, *len, *table;
   int seqs, ld_table, T, max_rows, max_len;
 } arcz_kv_batch;
+/* A pass's batch made on the GPU, out of how many tokens each sequence gets: rows, len and the new entries of table are outputs here, T,
+ * max_rows, seqs and ld_table what the buffers hold (max_len is not looked at).  All buffers are int32.
+ *   add [seqs]     > 0: so many tokens behind the sequence; < 0: so many of its last ones taken off (drafts that were refused, a sequence that
+ *                  is done: any number down to -2^31); at most max_rows
+ *   before [seqs]  the lengths so far; may be b->len itself
+ *   ring [pages]   the free pages: state[1] of them from place state[0] on, round the end.  New entries of the table are taken from its front,
+ *                  sequence by sequence; pages that a shorter sequence leaves go behind its end, to be taken by later plans
+ *   state [4]      in: the ring's first place and its count.  after [4], which may be state itself, out: both behind the plan; what was missing;
+ *                  the rows of the plan
+ *   shared [seqs]  (NULL: 0) the positions of a sequence's prefix whose whole pages are also others': they are not given back
+ *   pos [T]        (NULL: not wanted) the position of each row, as arcz_engine_rope takes them
+ *   slot [T]       (NULL: not wanted) page * (tokens a page) + position % (tokens a page), -1 where the table has no page of the cache
+ * `page` is the cache's tokens a page, `pages` its pages.  rows [seqs + 1] = the running sum of max(add, 0), len = max(0, before + add), row i
+ * of a sequence has position before + i.  All or nothing: where pages are missing (after[2] = how many), or an add is above max_rows, the rows
+ * above T, a length above what the table holds or the state none of such a ring (after[2] = -1), the lengths, the ring and the table stay as
+ * they are, rows is all 0 -- the pass's other calls then have nothing to do -- and pos and slot are left alone; else after[2] = 0.  Entries behind a sequence's pages are left as
+ * they are, and so are pos and slot behind the last row.  What is written must not meet what is read, nor each other, but for the two
+ * that may be brought on in place.  Pages of a table entry that is none of the cache are given back as they are found. */
+typedef struct arcz_kv_plan {
+  arcz_mem *add, *before, *ring, *state, *after, *shared, *pos, *slot;
+  int pages, page;
+} arcz_kv_plan;
+int arcz_engine_kv_plan(arcz_engine* e, const arcz_kv_batch* b, const arcz_kv_plan* p);
 /* The batch's rows of k and v (T rows of heads * hd values each) into the cache, in one launch.  A block's scale is what its largest
  * value needs, max |x| / 127; where older tokens share the block and the new ones are larger, the older values are brought to
  * the new scale (rounded again), where they are smaller the scale stays.  Values are rounded to nearest even.  A row with an
