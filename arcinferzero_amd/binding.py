@@ -133,6 +133,8 @@ _sig("arcz_kv_buffer", _p, _p, _i)
 _sig("arcz_engine_kv_write", _i, _p, _p, _p, _p, _i, _i, _p, _i, _i)
 _sig("arcz_engine_kv_read", _i, _p, _p, _p, _p, _i, _i, _p, _i, _i)
 _sig("arcz_engine_attention", _i, _p, _p, _p, _p, _i, _i, _i, _p, _i, _i, _p)
+_sig("arcz_engine_attention_shared_room", _z, _p, _p, _p, _p, _i, _p)
+_sig("arcz_engine_attention_shared", _i, _p, _p, _p, _p, _p, _i, _i, _i, _p, _i, _i, _p, _p)
 _sig("arcz_engine_self_check", _i)
 _sig("arcz_engine_profile", None, _p, _i)
 _sig("arcz_engine_profile_collect", _i, _p)
@@ -154,16 +156,16 @@ _sig("arcz_gen_weights", _i, _u32, _u64, _z, _i, C.c_float, _p)
 _quantize, _rmsnorm_quant, _swiglu_quant = lib.arcz_engine_quantize, lib.arcz_engine_rmsnorm_quant, lib.arcz_engine_swiglu_quant
 _matmul, _gemv_gu, _layer_moe = lib.arcz_engine_matmul, lib.arcz_engine_gemv_gu, lib.arcz_engine_layer_moe
 _rope, _kv_write, _kv_read, _attention = lib.arcz_engine_rope, lib.arcz_engine_kv_write, lib.arcz_engine_kv_read, lib.arcz_engine_attention
-_norm_rope, _kv_plan = lib.arcz_engine_norm_rope, lib.arcz_engine_kv_plan
+_norm_rope, _kv_plan, _attention_shared = lib.arcz_engine_norm_rope, lib.arcz_engine_kv_plan, lib.arcz_engine_attention_shared
 try:
     from . import _pycall
     _pycall.bind(_quantize, _rmsnorm_quant, _swiglu_quant, _matmul, _gemv_gu, _layer_moe)
     _pycall.bind_attn(_rope, _kv_write, _kv_read, _attention)
-    _pycall.bind_step(_norm_rope, _kv_plan)
+    _pycall.bind_step(_norm_rope, _kv_plan, _attention_shared)
     from ._pycall import gemv_gu as _gemv_gu, layer_moe as _layer_moe, matmul as _matmul, quantize as _quantize
     from ._pycall import rmsnorm_quant as _rmsnorm_quant, swiglu_quant as _swiglu_quant
     from ._pycall import attention as _attention, kv_read as _kv_read, kv_write as _kv_write, rope as _rope
-    from ._pycall import kv_plan as _kv_plan, norm_rope as _norm_rope
+    from ._pycall import attention_shared as _attention_shared, kv_plan as _kv_plan, norm_rope as _norm_rope
 except ImportError:
     pass
 
@@ -547,6 +549,16 @@ class KvPlan(C.Structure):
         self.at = C.addressof(self)
 
 
+class KvShared(C.Structure):
+    """Groups of a batch's sequences that share a prefix (arcz_kv_shared): buffers of groups [n + 1] and len [n], int32."""
+    _fields_ = [("groups", _p), ("len", _p), ("n", _i), ("max_rows", _i), ("max_len", _i)]
+
+    def __init__(self, groups, len, n, max_rows, max_len=0):
+        super().__init__(groups.h if groups else None, len.h if len else None, n, max_rows, max_len)
+        self.held = (groups, len)
+        self.at = C.addressof(self)
+
+
 class Attention(C.Structure):
     """The form of an attention (arcz_attn): slopes f32 [heads], prefix int32 [seqs], first int32 [T], each a buffer or None."""
     _fields_ = [("scale", C.c_float), ("cap", C.c_float), ("window", _i), ("slopes", _p), ("prefix", _p), ("first", _p)]
@@ -757,6 +769,19 @@ class Engine:
     def attention(self, kv, batch, q, ldq, q_off, heads, out, ldo, o_off, form):
         """out = softmax(scores) v of the batch's rows of q over the cache; form: an Attention."""
         r = _attention(self.h, kv.h, batch.at, q.h, ldq, q_off, heads, out.h, ldo, o_off, form.at)
+        if r:
+            _check(r, engine=True)
+
+    def attention_shared_room(self, kv, batch, shared, heads, form):
+        """The bytes of workspace that attention_shared takes for such a call."""
+        n = lib.arcz_engine_attention_shared_room(self.h, kv.h, batch.at, shared.at, heads, form.at)
+        if not n:
+            raise ArczError(-100, lib.arcz_engine_error().decode())
+        return n
+
+    def attention_shared(self, kv, batch, shared, q, ldq, q_off, heads, out, ldo, o_off, form, room):
+        """attention() for a batch whose sequences share prefixes in groups, each prefix read once; shared: a KvShared, room: a workspace."""
+        r = _attention_shared(self.h, kv.h, batch.at, shared.at, q.h, ldq, q_off, heads, out.h, ldo, o_off, form.at, room.h)
         if r:
             _check(r, engine=True)
 

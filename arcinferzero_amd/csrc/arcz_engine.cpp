@@ -314,6 +314,26 @@ int arcz_engine_attention(arcz_engine* e, arcz_kv* c, const arcz_kv_batch* b, ar
   });
 }
 
+static Engine::Shared shared_of(const arcz_kv_shared* g, const arcz_attn* a) {
+  if (!g || !a) throw std::runtime_error(g ? "attention_shared: no form" : "attention_shared: no groups");
+  return {g->groups, g->len, g->n, g->max_rows, g->max_len};
+}
+size_t arcz_engine_attention_shared_room(arcz_engine* e, arcz_kv* c, const arcz_kv_batch* b, const arcz_kv_shared* g, int heads, const arcz_attn* a) {
+  size_t bytes = 0;
+  guarded([&] {
+    const Engine::Shared sh = shared_of(g, a);
+    bytes = e->e->attention_shared_room(c ? c->c : Engine::Kv(), batch_of("attention_shared", c, b), sh, heads, {a->scale, a->cap, a->window, a->slopes, a->prefix, a->first});
+  });
+  return bytes;
+}
+int arcz_engine_attention_shared(arcz_engine* e, arcz_kv* c, const arcz_kv_batch* b, const arcz_kv_shared* g, arcz_mem* q, int ldq, int q_off, int heads, arcz_mem* out, int ldo,
+                                 int o_off, const arcz_attn* a, arcz_mem* room) {
+  return guarded([&] {
+    const Engine::Shared sh = shared_of(g, a);
+    e->e->attention_shared(c ? c->c : Engine::Kv(), batch_of("attention_shared", c, b), sh, q, ldq, q_off, heads, out, ldo, o_off, {a->scale, a->cap, a->window, a->slopes, a->prefix, a->first}, room);
+  });
+}
+
 int arcz_engine_self_check(void) {
   return guarded([&] {
     const std::string r = engine_self_check();

@@ -379,6 +379,120 @@
     run("attention", k, 2, g, l);
     if (nsplit > 1) join(c, b, w, nsplit, bm, tiles, mr, heads, out, ldo, o_off);
   }
+  // ---- attention for sequences that share a prefix (kernels/attn_shared.hip)
+  struct Shared {
+    cl_mem groups, len;
+    int n, max_rows, max_len;
+  };
+  // The launches of a call, by what the host knows of it, and where its workspace has what they leave.
+  struct SharedShape {
+    int G, form, M, M1, waves1, bm1, tiles1, n1, few, rt, pack, b2, tiles2, n2, least;
+    size_t info, ws1, ws2, bytes;
+  };
+  SharedShape shared_shape(const Kv& c, const Batch& b, const Shared& sh, int heads, const Attn& a) {
+    if (heads < 1 || heads % c.heads || (int64_t)heads * c.hd > 0x7FFFFFFF) throw std::runtime_error("attention_shared: " + std::to_string(heads) + " heads over " + std::to_string(c.heads) + " of the cache");
+    if (sh.n < 0 || sh.n > 65535 || sh.max_rows < 0 || sh.max_len < 0 || b.max_len < 0) throw std::runtime_error("attention_shared: " + std::to_string(sh.n) + " groups of " + std::to_string(sh.max_rows) + " rows");
+    SharedShape p = {};
+    p.G = heads / c.heads;
+    p.form = (a.cap > 0.0f ? 1 : 0) | (a.slopes ? 2 : 0);
+    const int64_t M = (int64_t)std::min(b.max_rows, b.T) * p.G, M1 = (int64_t)std::min(sh.max_rows, b.T) * p.G;
+    if (M > 0x7FFFFF00 || M1 > 0x7FFFFF00) throw std::runtime_error("attention_shared: too many rows");
+    p.M = (int)M;
+    p.M1 = (int)M1;
+    const size_t cus = (size_t)arcz_device_cus(), pairs = (size_t)b.seqs * c.heads, pairs1 = (size_t)sh.n * c.heads;
+    const int all = b.max_len > 0 ? b.max_len : b.ld_table * c.page, shared = sh.max_len > 0 ? std::min(sh.max_len, all) : all, own = std::max(1, sh.max_len > 0 ? all - shared : all);
+    // the group's keys: as many pieces as fill the chip, of at least 256 keys
+    p.waves1 = c.hd == 128 && c.block >= 32 && M1 > 128 ? 8 : 4;
+    p.bm1 = 32 * p.waves1;
+    p.tiles1 = (int)((M1 + p.bm1 - 1) / p.bm1);
+    p.n1 = p.tiles1 && pairs1 ? (int)std::max<size_t>(1, std::min<size_t>((size_t)8 / p.waves1 * cus / (pairs1 * p.tiles1), (size_t)(shared + 255) / 256)) : 0;
+    // its own: as attention() does
+    p.few = M <= (c.hd == 256 ? 16 : 32);
+    if (p.few) {
+      p.rt = M > 16 ? 2 : 1;
+      p.pack = M <= 8 ? 1 : 0;
+      p.b2 = p.pack ? 8 : 16 * p.rt;
+      p.tiles2 = 1;
+      const size_t want = (2 * cus + pairs - 1) / std::max<size_t>(1, pairs);
+      p.least = (int)std::max<size_t>(8, ((size_t)(own + 31) / 32 + want - 1) / std::max<size_t>(1, want));
+      p.n2 = (int)(((int64_t)own + (int64_t)32 * p.least - 1) / ((int64_t)32 * p.least));
+    } else {
+      p.b2 = 128;
+      p.tiles2 = (int)((M + 127) / 128);
+      p.n2 = (int)std::max<size_t>(1, std::min<size_t>(2 * cus / std::max<size_t>(1, pairs * p.tiles2), (size_t)(own + 255) / 256));
+    }
+    if (pairs * p.tiles2 > 0xFFFFFFFFull / 256 || pairs1 * p.tiles1 > 0xFFFFFFFFull / 512) throw std::runtime_error("attention_shared: too many rows");
+    auto place = [&](size_t bytes) {
+      const size_t at = p.bytes;
+      p.bytes += (bytes + 255) / 256 * 256;
+      return at;
+    };
+    place((size_t)b.T * 16);   // (spans)
+    p.info = place((size_t)b.seqs * 16);
+    p.ws1 = place(pairs1 * p.tiles1 * p.n1 * p.bm1 * (c.hd + 2) * 4);
+    p.ws2 = place(pairs * p.tiles2 * p.n2 * p.b2 * (c.hd + 2) * 4);
+    p.bytes = std::max<size_t>(p.bytes, 256);
+    return p;
+  }
+  size_t attention_shared_room(const Kv& c, const Batch& b, const Shared& sh, int heads, const Attn& a) {
+    Places at;
+    if (!check_batch("attention_shared", c, b, at)) return 256;
+    return shared_shape(c, b, sh, heads, a).bytes;
+  }
+  void attention_shared(const Kv& c, const Batch& b, const Shared& sh, cl_mem q, int ldq, int q_off, int heads, cl_mem out, int ldo, int o_off, const Attn& a, cl_mem room) {
+    Places at;
+    if (!check_batch("attention_shared", c, b, at)) return;
+    const SharedShape p = shared_shape(c, b, sh, heads, a);
+    if (!std::isfinite(a.scale) || !(a.cap >= 0.0f) || a.cap > 0x1p100f || (a.cap > 0.0f && a.cap < 0x1p-100f) || a.window < 0) throw std::runtime_error("attention_shared: scale, cap or window");
+    const Rows rq = rows_of("attention_shared: q", q, ldq, q_off, heads * c.hd, b.T), ro = rows_of("attention_shared: out", out, ldo, o_off, heads * c.hd, b.T);
+    const char* const name = "attention_shared";
+    Place in[5] = {};
+    if (a.slopes) in[0] = ints(name, "slopes", a.slopes, (size_t)heads);
+    if (a.prefix) in[1] = ints(name, "prefix", a.prefix, (size_t)b.seqs);
+    if (a.first) in[2] = ints(name, "first", a.first, (size_t)b.T);
+    if (sh.n) {
+      in[3] = ints(name, "groups", sh.groups, (size_t)sh.n + 1);
+      in[4] = ints(name, "the groups' len", sh.len, (size_t)sh.n);
+    }
+    const uintptr_t w = (uintptr_t)arcz_mem_ptr(room);
+    if (!room || w % 16 || arcz_mem_size(room) < p.bytes)
+      throw std::runtime_error("attention_shared: the room holds " + std::to_string(arcz_mem_size(room)) + " bytes, the call takes " + std::to_string(p.bytes) + " (at an address of 16)");
+    const Place work = {w, w + p.bytes};
+    if (overlap(rq, ro)) throw std::runtime_error("attention_shared: q and out overlap");
+    if (at.in_cache(ro) || at.in_batch(ro.place())) throw std::runtime_error("attention_shared: out overlaps the cache or the batch");
+    if (at.in_cache(work) || at.in_batch(work) || overlap(work, rq.place()) || overlap(work, ro.place())) throw std::runtime_error("attention_shared: the room overlaps the cache, the batch, q or out");
+    for (const Place& i : in)
+      if (overlap(ro.place(), i) || overlap(work, i)) throw std::runtime_error("attention_shared: out or the room overlaps slopes, prefix, first or the groups");
+    int pages = c.pages, ps = c.ps, bs = c.bs, ldt = b.ld_table, T = b.T, mr = std::min(b.max_rows, b.T), kvh = c.heads, window = std::min(a.window, 1 << 30), hd = c.hd, seqs = b.seqs, n = sh.n;
+    int most = ldt * c.page, mr1 = std::min(sh.max_rows, b.T), vec = rq.vec() ? 1 : 0, n1 = p.n1, n2 = p.n2, bm1 = p.bm1, b2 = p.b2, t1 = p.tiles1, t2 = p.tiles2, least = p.least;
+    float scale = a.scale, cap2 = a.cap * 1.4426950408889634f;
+    {
+      cl_kernel k = variant("attn", {}, "attn_spans");
+      set_args(k, 0, b.rows, b.len, most, T, mr, window, a.prefix, a.first, sh.groups, sh.len, n, seqs, room, p.info);
+      size_t g[2] = {(size_t)std::min((mr + 255) / 256, 64) * 256, (size_t)seqs}, l[2] = {256, 1};
+      run("attention_spans", k, 2, g, l);
+    }
+    auto part = [&](const char* name, cl_mem groups, size_t sets, int rows, int waves, int tiles, int nsplit, size_t ws) {
+      cl_kernel k = variant("attn", {{"HD", c.hd}, {"FINE", c.block < 32 ? 1 : 0}, {"FORM", p.form}, {waves == 8 ? "W8" : nullptr, 1}}, "attn_part");
+      set_args(k, 0, q, ldq, q_off, c.b[0], c.b[1], c.b[2], c.b[3], pages, ps, bs, b.rows, b.table, ldt, T, rows, heads, kvh, scale, cap2, a.slopes, groups, seqs, room, ws, nsplit, tiles, vec);
+      size_t g[2] = {sets * c.heads * tiles * 64 * waves, (size_t)nsplit}, l[2] = {(size_t)64 * waves, 1};
+      run(name, k, 2, g, l);
+    };
+    if (n1) part("attention_shared", sh.groups, (size_t)n, mr1, p.waves1, t1, n1, p.ws1);
+    if (p.few) {
+      cl_kernel k = variant("attn", {{"HD", c.hd}, {"RT", p.rt}, {"PACK", p.pack}, {"FINE", c.block < 4 ? 1 : 0}, {"FORM", p.form}}, "attn_part_few");
+      set_args(k, 0, q, ldq, q_off, c.b[0], c.b[1], c.b[2], c.b[3], pages, ps, bs, b.rows, b.len, b.table, ldt, T, mr, heads, kvh, scale, cap2, a.slopes, room, p.ws2, n2, least, vec);
+      size_t g[2] = {(size_t)seqs * c.heads * 256, (size_t)n2}, l[2] = {256, 1};
+      run("attention_own", k, 2, g, l);
+    } else {
+      part("attention_own", nullptr, (size_t)seqs, mr, 4, t2, n2, p.ws2);
+    }
+    cl_kernel k = variant("attn", {}, "attn_meet");
+    set_args(k, 0, room, p.info, p.ws1, n1, bm1, t1, mr1, p.ws2, n2, b2, t2, hd, b.rows, b.len, most, T, mr, heads, kvh, out, ldo, o_off);
+    const int per = 1024 / c.hd;
+    size_t g[2] = {(size_t)seqs * c.heads * 256, (size_t)((p.M + per - 1) / per)}, l[2] = {256, 1};
+    run("attention_meet", k, 2, g, l);
+  }
   void join(const Kv& c, const Batch& b, cl_mem w, int nsplit, int rows, int blocks, int mr, int heads, cl_mem out, int ldo, int o_off) {
     int hd = c.hd, most_len = b.ld_table * c.page, T = b.T, kvh = c.heads, per = 1024 / c.hd;
     cl_kernel k = variant("attn", {}, "attn_join");

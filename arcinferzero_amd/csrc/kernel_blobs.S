@@ -32,4 +32,6 @@
     BLOB arcz_blob_kv, "kv.hsaco"
     BLOB arcz_blob_attn_few, "attn_few.hsaco"
     BLOB arcz_blob_attn_many, "attn_many.hsaco"
+    BLOB arcz_blob_attn_shared, "attn_shared.hsaco"
+    BLOB arcz_blob_attn_shared_few, "attn_shared_few.hsaco"
     .section .note.GNU-stack,"",@progbits

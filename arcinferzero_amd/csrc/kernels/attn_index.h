@@ -65,6 +65,36 @@ ATTN_FN int tile_at(int from, int to, int tile, int i) {
 // Where the table has the page of a position: within its row of ldt entries also for a position behind the last key (up to 4096
 // behind it; most_len is at most 2^31 - 4096).
 ATTN_FN int entry_of(int p, int ps, int ldt) { return lower(p >> ps, ldt - 1); }
+// Sequences behind a shared prefix.  Group g has sequences [groups[g], groups[g + 1]), whose rows are one behind the other; without groups g is a
+// sequence.  Its rows, held to the buffers; len: its first sequence (0 where it has no rows).
+ATTN_FN Seq part_at(const int* groups, const int* rows, int g, int seqs, int T, int max_rows) {
+  int s0 = g, s1 = g + 1;
+  if (groups) {
+    s0 = lower(upper(groups[g], 0), seqs);
+    s1 = lower(upper(groups[g + 1], s0), seqs);
+  }
+  Seq q;
+  q.r0 = lower(upper(rows[s0], 0), T);
+  q.n = lower(lower(upper(rows[s1], q.r0), T) - q.r0, max_rows);
+  q.p0 = 0;
+  q.len = lower(s0, seqs - 1);
+  return q;
+}
+// The part of a row's interval [from, to) in front of `split`, or behind it, inside a table of `most` positions.
+ATTN_FN void part_of_span(int from, int to, int split, bool front, int most, int& lo, int& hi) {
+  lo = upper(from, front ? 0 : upper(split, 0));
+  hi = lower(lower(to, front ? split : to), most);
+}
+// The group that a sequence is in (n of them, in order), -1: in none.
+ATTN_FN int group_of(const int* groups, int n, int s) {
+  int a = 0, b = n;   // (the last group that does not begin behind s lies in [a, b))
+  while (b - a > 1) {
+    const int m = a + (b - a) / 2;
+    if (groups[m] <= s) a = m;
+    else b = m;
+  }
+  return n > 0 && groups[a] <= s && s < groups[a + 1] ? a : -1;
+}
 // What a plan does to a sequence: `add` tokens behind the `before` that it has, or -add taken off, in pages of 2^ps tokens, `ldt` of them at most.  Its pages
 // are then the entries [0, has) of the table, [0, had) before; `take` of them new, or those from `has` on, `give` of them, given back -- never
 // those that lie whole in the first `shared` positions.  fits: no more than max_rows tokens, no more pages than the table has.

@@ -266,6 +266,23 @@ typedef struct arcz_attn {
 int arcz_engine_attention(arcz_engine* e, arcz_kv* c, const arcz_kv_batch* b, arcz_mem* q, int ldq, int q_off, int heads, arcz_mem* out, int ldo, int o_off,
                           const arcz_attn* a);
 
+/* The same for sequences that share a prefix, whose keys are then read once for all of them: group g (of n) is the batch's sequences [groups[g],
+ * groups[g + 1]) (int32 [n + 1], not falling; a sequence may be in none), and the first len[g] positions (int32 [n]) of each of them lie in the same pages, which are looked
+ * up in the table of its first sequence; the positions behind them, and those of the rows themselves, in each one's own.  max_rows: the
+ * most rows of one group together (those past it are left as they are, like a sequence's past its max_rows); max_len: about the most positions that a group shares (0: not known).  The result is
+ * that of arcz_engine_attention, whatever the form -- windows, documents and the like go by each row's own position --, up to the rounding
+ * of sums.  groups and len are read when the launches run and held to the buffers there; out must not meet them.
+ * room: a workspace of the caller's of at least arcz_engine_attention_shared_room(...) bytes, at an address of 16, that nothing else of the call
+ * meets; what it holds between calls does not matter.  The bytes depend on the batch's seqs, T, ld_table, max_rows and max_len, those of the groups, heads, the
+ * cache's shape and whether there is a cap or slopes (0: an error). */
+typedef struct arcz_kv_shared {
+  arcz_mem *groups, *len;
+  int n, max_rows, max_len;
+} arcz_kv_shared;
+size_t arcz_engine_attention_shared_room(arcz_engine* e, arcz_kv* c, const arcz_kv_batch* b, const arcz_kv_shared* g, int heads, const arcz_attn* a);
+int arcz_engine_attention_shared(arcz_engine* e, arcz_kv* c, const arcz_kv_batch* b, const arcz_kv_shared* g, arcz_mem* q, int ldq, int q_off, int heads, arcz_mem* out, int ldo,
+                                 int o_off, const arcz_attn* a, arcz_mem* room);
+
 /* The start-up check of the tuned GEMMs of 128 tokens and of the GEMM on digits against the simple one on the reference's
  * LCG data, both against integer sums counted on the host (the pattern of xmx_check, zero/engine_setup.h:424-520): the
  * weight types that make unit-scale blocks, the three accumulate modes, K in one piece and in several.  0, or ARCZ_E_ENGINE with the first
