@@ -387,7 +387,7 @@
   // The launches of a call, by what the host knows of it, and where its workspace has what they leave.
   struct SharedShape {
     int G, form, M, M1, waves1, bm1, tiles1, n1, few, rt, pack, b2, tiles2, n2, least;
-    size_t info, ws1, ws2, bytes;
+    size_t ws1, ws2, bytes;
   };
   SharedShape shared_shape(const Kv& c, const Batch& b, const Shared& sh, int heads, const Attn& a) {
     if (heads < 1 || heads % c.heads || (int64_t)heads * c.hd > 0x7FFFFFFF) throw std::runtime_error("attention_shared: " + std::to_string(heads) + " heads over " + std::to_string(c.heads) + " of the cache");
@@ -427,8 +427,6 @@
       p.bytes += (bytes + 255) / 256 * 256;
       return at;
     };
-    place((size_t)b.T * 16);   // (spans)
-    p.info = place((size_t)b.seqs * 16);
     p.ws1 = place(pairs1 * p.tiles1 * p.n1 * p.bm1 * (c.hd + 2) * 4);
     p.ws2 = place(pairs * p.tiles2 * p.n2 * p.b2 * (c.hd + 2) * 4);
     p.bytes = std::max<size_t>(p.bytes, 256);
@@ -466,29 +464,25 @@
     int pages = c.pages, ps = c.ps, bs = c.bs, ldt = b.ld_table, T = b.T, mr = std::min(b.max_rows, b.T), kvh = c.heads, window = std::min(a.window, 1 << 30), hd = c.hd, seqs = b.seqs, n = sh.n;
     int most = ldt * c.page, mr1 = std::min(sh.max_rows, b.T), vec = rq.vec() ? 1 : 0, n1 = p.n1, n2 = p.n2, bm1 = p.bm1, b2 = p.b2, t1 = p.tiles1, t2 = p.tiles2, least = p.least;
     float scale = a.scale, cap2 = a.cap * 1.4426950408889634f;
-    {
-      cl_kernel k = variant("attn", {}, "attn_spans");
-      set_args(k, 0, b.rows, b.len, most, T, mr, window, a.prefix, a.first, sh.groups, sh.len, n, seqs, room, p.info);
-      size_t g[2] = {(size_t)std::min((mr + 255) / 256, 64) * 256, (size_t)seqs}, l[2] = {256, 1};
-      run("attention_spans", k, 2, g, l);
-    }
-    auto part = [&](const char* name, cl_mem groups, size_t sets, int rows, int waves, int tiles, int nsplit, size_t ws) {
+    auto part = [&](const char* name, int front, size_t sets, int rows, int waves, int tiles, int nsplit, size_t ws) {
       cl_kernel k = variant("attn", {{"HD", c.hd}, {"FINE", c.block < 32 ? 1 : 0}, {"FORM", p.form}, {waves == 8 ? "W8" : nullptr, 1}}, "attn_part");
-      set_args(k, 0, q, ldq, q_off, c.b[0], c.b[1], c.b[2], c.b[3], pages, ps, bs, b.rows, b.table, ldt, T, rows, heads, kvh, scale, cap2, a.slopes, groups, seqs, room, ws, nsplit, tiles, vec);
+      set_args(k, 0, q, ldq, q_off, c.b[0], c.b[1], c.b[2], c.b[3], pages, ps, bs, b.rows, b.len, b.table, ldt, T, rows, heads, kvh, scale, cap2, window, a.slopes, a.prefix, a.first,
+               sh.groups, sh.len, n, seqs, mr, front, room, ws, nsplit, tiles, vec);
       size_t g[2] = {sets * c.heads * tiles * 64 * waves, (size_t)nsplit}, l[2] = {(size_t)64 * waves, 1};
       run(name, k, 2, g, l);
     };
-    if (n1) part("attention_shared", sh.groups, (size_t)n, mr1, p.waves1, t1, n1, p.ws1);
+    if (n1) part("attention_shared", 1, (size_t)n, mr1, p.waves1, t1, n1, p.ws1);
     if (p.few) {
       cl_kernel k = variant("attn", {{"HD", c.hd}, {"RT", p.rt}, {"PACK", p.pack}, {"FINE", c.block < 4 ? 1 : 0}, {"FORM", p.form}}, "attn_part_few");
-      set_args(k, 0, q, ldq, q_off, c.b[0], c.b[1], c.b[2], c.b[3], pages, ps, bs, b.rows, b.len, b.table, ldt, T, mr, heads, kvh, scale, cap2, a.slopes, room, p.ws2, n2, least, vec);
+      set_args(k, 0, q, ldq, q_off, c.b[0], c.b[1], c.b[2], c.b[3], pages, ps, bs, b.rows, b.len, b.table, ldt, T, mr, heads, kvh, scale, cap2, window, a.slopes, a.prefix, a.first,
+               sh.groups, sh.len, n, room, p.ws2, n2, least, vec);
       size_t g[2] = {(size_t)seqs * c.heads * 256, (size_t)n2}, l[2] = {256, 1};
       run("attention_own", k, 2, g, l);
     } else {
-      part("attention_own", nullptr, (size_t)seqs, mr, 4, t2, n2, p.ws2);
+      part("attention_own", 0, (size_t)seqs, mr, 4, t2, n2, p.ws2);
     }
     cl_kernel k = variant("attn", {}, "attn_meet");
-    set_args(k, 0, room, p.info, p.ws1, n1, bm1, t1, mr1, p.ws2, n2, b2, t2, hd, b.rows, b.len, most, T, mr, heads, kvh, out, ldo, o_off);
+    set_args(k, 0, room, p.ws1, n1, bm1, t1, mr1, p.ws2, n2, b2, t2, hd, b.rows, b.len, most, T, mr, heads, kvh, sh.groups, sh.len, n, seqs, out, ldo, o_off);
     const int per = 1024 / c.hd;
     size_t g[2] = {(size_t)seqs * c.heads * 256, (size_t)((p.M + per - 1) / per)}, l[2] = {256, 1};
     run("attention_meet", k, 2, g, l);

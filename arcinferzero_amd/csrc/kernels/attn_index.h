@@ -85,6 +85,19 @@ ATTN_FN void part_of_span(int from, int to, int split, bool front, int most, int
   lo = upper(from, front ? 0 : upper(split, 0));
   hi = lower(lower(to, front ? split : to), most);
 }
+// The sequence of [s0, s1) that row t belongs to: tried first where rows of equal numbers would have it (a decode step's tokens: one look), then
+// searched for; some one of them where the rows are in no order.
+ATTN_FN int seq_of_row(const int* rows, int s0, int s1, int r0, int n, int t) {
+  const int at = s0 + (int)((long long)(t - r0) * (s1 - s0) / upper(n, 1)), guess = lower(upper(at, s0), s1 - 1);
+  if (rows[guess] <= t && t < rows[guess + 1]) return guess;
+  int a = s0, b = s1;
+  while (b - a > 1) {
+    const int m = a + (b - a) / 2;
+    if (rows[m] <= t) a = m;
+    else b = m;
+  }
+  return a;
+}
 // The group that a sequence is in (n of them, in order), -1: in none.
 ATTN_FN int group_of(const int* groups, int n, int s) {
   int a = 0, b = n;   // (the last group that does not begin behind s lies in [a, b))

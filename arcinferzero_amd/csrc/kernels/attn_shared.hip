@@ -5,49 +5,30 @@
 //   out = (o1 2^(m1 - m) + o2 2^(m2 - m)) / (l1 2^(m1 - m) + l2 2^(m2 - m)).
 // The first part takes the rows of all sequences of a group as rows of one (attn_many.inc), so the prefix is read once for all of them and
 // its products are those of matrices; the second is attention as it is, from P on.  Both leave pieces, as where keys are shared out, and one
-// launch joins them.  What a row sees of its keys is worked out once for both (attn_spans): the parts add up to what attention without
-// groups sees, whatever the form.
-#include "attn_few.inc"
+// launch joins them.  Both cut the same interval of a row's keys, so that together they see what attention without groups sees, whatever
+// the form.
 #include "attn_many.inc"
 
-// A call's workspace, the room: what these launches leave for the next ones, each from its own byte on, the rows' spans first.
-template <class T>
-__device__ inline T* in_room(char* room, size_t at) { return (T*)(room + at); }
+// A call's workspace, the room: what these launches leave for the last one, each from its own byte on.
+__device__ inline float* in_room(char* room, size_t at) { return (float*)(room + at); }
 
-// A row's interval of keys, its position and where its group's keys end.  info [seqs]: the group (-1: none), the first row of the group, where the
-// shared keys end.  grid (., seqs), 256.
-extern "C" __global__ __launch_bounds__(256) void attn_spans(const int* __restrict__ rows, const int* __restrict__ lens, int most, int T, int max_rows, int window,
-                                                             const int* __restrict__ prefix, const int* __restrict__ first, const int* __restrict__ groups,
-                                                             const int* __restrict__ shared, int n, int seqs, char* __restrict__ room, size_t info_at) {
-  int4 *const spans = (int4*)room, *const info = in_room<int4>(room, info_at);
-  const int s = blockIdx.y, g = attn::group_of(groups, n, s);
-  const Seq sq = seq_of(rows, lens, s, T, T, most);   // (all its rows: those past max_rows see nothing)
-  const int split = g < 0 ? 0 : min(max(shared[g], 0), most), pre = prefix ? prefix[s] : 0;
-  for (int i = blockIdx.x * 256 + threadIdx.x; i < sq.n; i += gridDim.x * 256) {
-    const int r = sq.r0 + i, f = first ? first[r] : 0;
-    int lo, hi;
-    sees(sq.p0 + i, sq.len, window, pre, f, lo, hi);
-    spans[r] = make_int4(lo, i < max_rows ? hi : 0, sq.p0 + i, split);
-  }
-  if (blockIdx.x == 0 && threadIdx.x == 0) info[s] = make_int4(g, g < 0 ? 0 : attn::part_at(groups, rows, g, seqs, T, T).r0, split, 0);
-}
-
-// The parts joined: ws1 has n1 pieces of the group's rows in blocks of b1, ws2 n2 of the sequence's in blocks of b2, t1 and t2 blocks each; a piece
-// is sums [b][hd], then reference and sum of weights [b][2].  Rows past the group's `most1` are left as they are.  grid (sequences x kv heads, row
-// groups of 1024 / hd), 256.
-extern "C" __global__ __launch_bounds__(256) void attn_meet(char* __restrict__ room, size_t info_at, size_t at1, int n1, int b1, int t1, int most1, size_t at2, int n2, int b2,
-                                                            int t2, int hd, const int* __restrict__ rows, const int* __restrict__ lens, int most_len, int T,
-                                                            int max_rows, int heads, int kvh, float* __restrict__ out, int ldo, int o_off) {
-  const int4* const info = in_room<int4>(room, info_at);
-  const float *const ws1 = in_room<float>(room, at1), *const ws2 = in_room<float>(room, at2);
+// The parts joined: the group's rows have n1 pieces in blocks of b1, the sequence's n2 in blocks of b2, t1 and t2 blocks each; a piece is sums
+// [b][hd], then reference and sum of weights [b][2].  Rows past the group's `most1` are left as they are.  grid (sequences x kv heads, row groups
+// of 1024 / hd), 256.
+extern "C" __global__ __launch_bounds__(256) void attn_meet(char* __restrict__ room, size_t at1, int n1, int b1, int t1, int most1, size_t at2, int n2, int b2, int t2, int hd,
+                                                            const int* __restrict__ rows, const int* __restrict__ lens, int most_len, int T, int max_rows, int heads,
+                                                            int kvh, const int* __restrict__ groups, const int* __restrict__ shared, int n, int seqs,
+                                                            float* __restrict__ out, int ldo, int o_off) {
+  const float *const ws1 = in_room(room, at1), *const ws2 = in_room(room, at2);
   const int s = blockIdx.x / kvh, h = blockIdx.x - s * kvh, G = heads / kvh, per = 1024 / hd;
   const Seq sq = seq_of(rows, lens, s, T, max_rows, most_len);
   const int r = blockIdx.y * per + threadIdx.x / (hd / 4), d = threadIdx.x % (hd / 4) * 4;
+  if (blockIdx.y * per >= sq.n * G) return;
+  const int g = attn::group_of(groups, n, s), first_row = g < 0 ? 0 : attn::part_at(groups, rows, g, seqs, T, T).r0;
   if (r >= sq.n * G || r >= t2 * b2) return;
-  const int4 at = info[s];
-  const int i = r / G, ig = sq.r0 + i - at.y;   // (its place among the group's rows)
-  if (at.x >= 0 && (ig < 0 || ig >= most1)) return;
-  const bool both = at.x >= 0 && at.z > 0;
+  const int i = r / G, ig = sq.r0 + i - first_row;   // (its place among the group's rows)
+  if (g >= 0 && (ig < 0 || ig >= most1)) return;
+  const bool both = g >= 0 && shared[g] > 0;
   const int rg = both ? ig * G + r - i * G : 0;
   float top = NOTHING, l = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -79,7 +60,7 @@ extern "C" __global__ __launch_bounds__(256) void attn_meet(char* __restrict__ r
       }
     }
   };
-  if (both) add(ws1, (size_t)(at.x * kvh + h) * t1 + rg / b1, n1, b1, rg % b1);
+  if (both) add(ws1, (size_t)(g * kvh + h) * t1 + rg / b1, n1, b1, rg % b1);
   add(ws2, (size_t)blockIdx.x * t2 + r / b2, n2, b2, r % b2);
   float* to = out + (size_t)(sq.r0 + i) * ldo + o_off + (h * G + r - i * G) * hd + d;
   const float f = l == 0.0f ? 0.0f : 1.0f / l;
@@ -87,14 +68,16 @@ extern "C" __global__ __launch_bounds__(256) void attn_meet(char* __restrict__ r
   to[0] = o.x * f; to[1] = o.y * f; to[2] = o.z * f; to[3] = o.w * f;
 }
 
+// front: the groups' part, of the rows of `max_rows` tokens of a group at most; else each sequence's own
 #define PART(NAME, HD, KT, NW, W, FINE, F)                                                                                                                      \
   extern "C" __global__ __launch_bounds__(64 * NW, W) void NAME(                                                                                                \
       const float* q, int ldq, int q_off, const int8_t* kq, const int8_t* vq, const float* ks, const float* vs, int pages, int ps, int bs, const int* rows,     \
-      const int* table, int ldt, int T, int max_rows, int heads, int kvh, float scale, float cap2, const float* slopes, const int* groups, int seqs,            \
-      char* room, size_t at, int nsplit, int tiles, int vec) {                                                                                                  \
-    many_body<HD, KT, NW, FINE, (F & 1) != 0, (F & 2) != 0, true>(q, ldq, q_off, kq, vq, ks, vs, pages, ps, bs, rows, nullptr, table, ldt, T, max_rows, heads,  \
-                                                                  kvh, nullptr, 0, 0, scale, cap2, 0, slopes, nullptr, nullptr, in_room<float>(room, at),       \
-                                                                  nsplit, tiles, vec, {groups, (const int4*)room, seqs});                                       \
+      const int* lens, const int* table, int ldt, int T, int max_rows, int heads, int kvh, float scale, float cap2, int window, const float* slopes,            \
+      const int* prefix, const int* first, const int* groups, const int* shared, int n, int seqs, int most_rows, int front, char* room, size_t at,             \
+      int nsplit, int tiles, int vec) {                                                                                                                         \
+    many_body<HD, KT, NW, FINE, (F & 1) != 0, (F & 2) != 0, true>(q, ldq, q_off, kq, vq, ks, vs, pages, ps, bs, rows, lens, table, ldt, T, max_rows, heads,     \
+                                                                  kvh, nullptr, 0, 0, scale, cap2, window, slopes, prefix, first, in_room(room, at), nsplit,    \
+                                                                  tiles, vec, {groups, shared, lens, n, seqs, most_rows, front});                               \
   }
 #define PART4(HD, KT, NW, W, FINE, S)                                     \
   PART(attn_part__HD##HD##_FINE##FINE##_FORM0##S, HD, KT, NW, W, FINE, 0) \

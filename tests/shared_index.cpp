@@ -37,6 +37,12 @@ int main() {
     for (int g = 0; g < n; ++g) {
       const attn::Seq q = attn::part_at(groups.data(), rows.data(), g, seqs, T, max_rows);
       NEED(q.r0 >= 0 && q.n >= 0 && q.r0 + q.n <= T && q.n <= max_rows && q.len >= 0 && q.len < seqs);
+      const int s1 = attn::lower(attn::upper(groups[g + 1], q.len + 1), seqs);
+      for (int i = 0; i < q.n; ++i) {
+        const int s = attn::seq_of_row(rows.data(), q.len, s1, q.r0, q.n, q.r0 + i);
+        NEED(s >= q.len && s < s1);
+        if (sound) NEED(rows[s] <= q.r0 + i && q.r0 + i < rows[s + 1]);
+      }
       if (sound && q.n) NEED(q.len == groups[g] && q.r0 == rows[groups[g]] && q.n == attn::lower(rows[groups[g + 1]] - q.r0, max_rows));
     }
     for (int s = 0; s < seqs; ++s) {
