@@ -388,6 +388,7 @@
   struct SharedShape {
     int G, form, M, M1, waves1, bm1, tiles1, n1, few, rt, pack, b2, tiles2, n2, least;
     size_t ws1, ws2, bytes;
+    bool one;
   };
   SharedShape shared_shape(const Kv& c, const Batch& b, const Shared& sh, int heads, const Attn& a) {
     if (heads < 1 || heads % c.heads || (int64_t)heads * c.hd > 0x7FFFFFFF) throw std::runtime_error("attention_shared: " + std::to_string(heads) + " heads over " + std::to_string(c.heads) + " of the cache");
@@ -401,11 +402,13 @@
     p.M1 = (int)M1;
     const size_t cus = (size_t)arcz_device_cus(), pairs = (size_t)b.seqs * c.heads, pairs1 = (size_t)sh.n * c.heads;
     const int all = b.max_len > 0 ? b.max_len : b.ld_table * c.page, shared = sh.max_len > 0 ? std::min(sh.max_len, all) : all, own = std::max(1, sh.max_len > 0 ? all - shared : all);
-    // the group's keys: as many pieces as fill the chip, of at least 256 keys
-    p.waves1 = c.hd == 128 && c.block >= 32 && M1 > 128 ? 8 : 4;
+    // The group's keys: as many pieces as fill the chip, of at least 128 keys (us, 4 to 16 sequences of a token behind 512 - 4096 keys, at least 256 /
+    // 128 / 64: 28 - 30 / 24 - 28 / 21 - 34).  Work-groups of eight waves from 512 rows on (512 rows behind 16384 keys 80 / 83 with four, 4000 behind 6000 150 /
+    // 170; 256 rows behind 1024 22 / 18, behind 8192 38 / 37).
+    p.waves1 = c.hd == 128 && c.block >= 32 && M1 >= 512 ? 8 : 4;
     p.bm1 = 32 * p.waves1;
     p.tiles1 = (int)((M1 + p.bm1 - 1) / p.bm1);
-    p.n1 = p.tiles1 && pairs1 ? (int)std::max<size_t>(1, std::min<size_t>((size_t)8 / p.waves1 * cus / (pairs1 * p.tiles1), (size_t)(shared + 255) / 256)) : 0;
+    p.n1 = p.tiles1 && pairs1 ? (int)std::max<size_t>(1, std::min<size_t>((size_t)8 / p.waves1 * cus / (pairs1 * p.tiles1), (size_t)(shared + 127) / 128)) : 0;
     // its own: as attention() does
     p.few = M <= (c.hd == 256 ? 16 : 32);
     if (p.few) {
@@ -421,6 +424,21 @@
       p.tiles2 = (int)((M + 127) / 128);
       p.n2 = (int)std::max<size_t>(1, std::min<size_t>(2 * cus / std::max<size_t>(1, pairs * p.tiles2), (size_t)(own + 255) / 256));
     }
+    // What both ways would take (us): attention as it is -- its launch, each sequence's keys of all, of which what they share comes from the caches, or
+    // its rows in whole tiles -- and three launches, the groups' rows in whole tiles, their own keys and the pieces.  Rates as measured: keys 9.5 TB/s
+    // shared (sequences of a token behind 1324 - 16984 keys 10 - 445 us), 5 of their own, products in tiles by the head's length.  (us, one launch / three:
+    // 16 sequences behind 4096 keys 24 / 28, 32 behind 2048 25 / 29, 64 behind 1024 28 / 36, 64 behind 8192 121 / 57, 128 behind 16384 445 / 115; four of 250 rows
+    // behind 6000 195 / 203, 24 of 16 heads of 256 values and up to 90 rows behind 4000 490 / 411.)
+    const double rate = c.hd == 64 ? 0.8e9 : c.hd == 128 ? 1.0e9 : 0.7e9, key = 2.0 * c.heads * c.hd, op = 8.0 * c.heads * c.hd, mean = (double)b.T / std::max(1, b.seqs) * p.G;
+    const double padded = b.seqs * std::max(128.0, mean + 64.0);   // (half of a sequence's last tile is empty)
+    const double one = 8.0 + (p.few ? b.seqs * (double)all * key / 9.5e6 : padded * all * op / rate);
+    const double three = 24.0 + (double)sh.n * p.tiles1 * p.bm1 * shared * op / rate + (p.few ? b.seqs * (double)own * key / 5.0e6 : padded * own * op / rate) +
+                         (double)b.T * heads * (p.n1 + p.n2) * (c.hd + 2) * 8.0 / 5.0e6;
+    p.one = attn_shared_ < 0 ? one <= three : attn_shared_ == 0;
+    if (p.one) {
+      p.bytes = 256;
+      return p;
+    }
     if (pairs * p.tiles2 > 0xFFFFFFFFull / 256 || pairs1 * p.tiles1 > 0xFFFFFFFFull / 512) throw std::runtime_error("attention_shared: too many rows");
     auto place = [&](size_t bytes) {
       const size_t at = p.bytes;
@@ -432,6 +450,7 @@
     p.bytes = std::max<size_t>(p.bytes, 256);
     return p;
   }
+  int attn_shared_ = -1;   // ARCZ_ATTN_SHARED
   size_t attention_shared_room(const Kv& c, const Batch& b, const Shared& sh, int heads, const Attn& a) {
     Places at;
     if (!check_batch("attention_shared", c, b, at)) return 256;
@@ -461,6 +480,7 @@
     if (at.in_cache(work) || at.in_batch(work) || overlap(work, rq.place()) || overlap(work, ro.place())) throw std::runtime_error("attention_shared: the room overlaps the cache, the batch, q or out");
     for (const Place& i : in)
       if (overlap(ro.place(), i) || overlap(work, i)) throw std::runtime_error("attention_shared: out or the room overlaps slopes, prefix, first or the groups");
+    if (p.one) return attention(c, b, q, ldq, q_off, heads, out, ldo, o_off, a);
     int pages = c.pages, ps = c.ps, bs = c.bs, ldt = b.ld_table, T = b.T, mr = std::min(b.max_rows, b.T), kvh = c.heads, window = std::min(a.window, 1 << 30), hd = c.hd, seqs = b.seqs, n = sh.n;
     int most = ldt * c.page, mr1 = std::min(sh.max_rows, b.T), vec = rq.vec() ? 1 : 0, n1 = p.n1, n2 = p.n2, bm1 = p.bm1, b2 = p.b2, t1 = p.tiles1, t2 = p.tiles2, least = p.least;
     float scale = a.scale, cap2 = a.cap * 1.4426950408889634f;

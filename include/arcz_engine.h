@@ -269,9 +269,10 @@ int arcz_engine_attention(arcz_engine* e, arcz_kv* c, const arcz_kv_batch* b, ar
 /* The same for sequences that share a prefix, whose keys are then read once for all of them: group g (of n) is the batch's sequences [groups[g],
  * groups[g + 1]) (int32 [n + 1], not falling; a sequence may be in none), and the first len[g] positions (int32 [n]) of each of them lie in the same pages, which are looked
  * up in the table of its first sequence; the positions behind them, and those of the rows themselves, in each one's own.  max_rows: the
- * most rows of one group together (those past it are left as they are, like a sequence's past its max_rows); max_len: about the most positions that a group shares (0: not known).  The result is
+ * most rows of one group together (those past it may be left as they are); max_len: about the most positions that a group shares (0: not known).  The result is
  * that of arcz_engine_attention, whatever the form -- windows, documents and the like go by each row's own position --, up to the rounding
- * of sums.  groups and len are read when the launches run and held to the buffers there; out must not meet them.
+ * of sums.  Where by the sizes that the host knows reading a prefix once would not pay (few sequences, short prefixes, many rows of each) the call is
+ * arcz_engine_attention, and each sequence's own table is used for all of its keys.  groups and len are read when the launches run and held to the buffers there; out must not meet them.
  * room: a workspace of the caller's of at least arcz_engine_attention_shared_room(...) bytes, at an address of 16, that nothing else of the call
  * meets; what it holds between calls does not matter.  The bytes depend on the batch's seqs, T, ld_table, max_rows and max_len, those of the groups, heads, the
  * cache's shape and whether there is a cap or slopes (0: an error). */

@@ -1,5 +1,7 @@
 """Attention for sequences that share prefixes in groups, on the GPU against 64 bits (attn_ref.attention, which knows no groups, with its bounds:
 the two parts of a row's keys are joined as pieces of keys are)."""
+import os
+
 import numpy as np
 import pytest
 
@@ -9,9 +11,19 @@ import attn_ref as ref
 pytestmark = pytest.mark.gpu
 
 
+def engine(way):
+    """An engine that takes the parts apart always (1), never (0), or where it pays (None)."""
+    if way is not None:
+        os.environ["ARCZ_ATTN_SHARED"] = way
+    try:
+        return az.Engine(16, 256)
+    finally:
+        os.environ.pop("ARCZ_ATTN_SHARED", None)
+
+
 @pytest.fixture(scope="module")
 def eng(rt):
-    e = az.Engine(16, 256)
+    e = engine("1")
     yield e
     e.close()
 
@@ -297,3 +309,40 @@ def test_every_kernel(eng, hd, block, form):
         k.run(eng, cap=11.0 if form & 1 else 0.0, slopes=np.linspace(0.002, 0.05, heads) if form & 2 else None)
     k = Case([(330, [(1, 3 + i % 5) for i in range(75)])], 64, block, 1, hd, 4, seed=hd)
     k.run(eng, cap=11.0 if form & 1 else 0.0, slopes=np.linspace(0.002, 0.05, 4) if form & 2 else None)
+
+
+def test_where_it_pays(rt):
+    """By the sizes alone that the caller names: a few sequences are one launch of attention as it is, many behind a long prefix the parts; the results
+    are the same."""
+    for groups, named, launches in (([(64, [(1, 5), (2, 9)])], 64, 1), ([(64, [(1, 30 + i % 7) for i in range(256)])], 9000, 3), ([(64, [(1, 30)])], 9000, 1)):
+        k = Case(groups, 32, 16, 2, 128, 8)
+        heads = 8
+        got = []
+        for way in (None, "1", "0"):
+            e = engine(way)
+            hold = []
+            kvc, batch = ref.device_cache(e, k.c, hold), k.b.device(hold)
+            batch.max_len = named + 40
+            w = heads * 128
+            q, out = az.Runtime.from_numpy(k.x), az.Runtime.alloc(k.x.nbytes)
+            gb, sb = az.Runtime.from_numpy(np.array(k.groups, np.int32)), az.Runtime.from_numpy(np.array(k.shared, np.int32))
+            sh, form = az.KvShared(gb, sb, len(k.shared), k.group_rows, named), az.Attention(0.05)
+            room = az.Runtime.alloc(e.attention_shared_room(kvc, batch, sh, heads, form))
+            hold += [q, out, gb, sb, room]
+            n = az.lib.arcz_launch_count()
+            e.attention_shared(kvc, batch, sh, q, w, 0, heads, out, w, 0, form, room)
+            n = az.lib.arcz_launch_count() - n
+            if way is None:
+                print(groups[0][0], "launches", n, flush=True)
+                first = n
+            else:
+                assert n == 3 if way == "1" else n == 1
+            got.append(out.read(np.float32).reshape(k.x.shape))
+            ref.free(hold)
+            e.close()
+        assert first == launches
+        assert np.array_equal(got[0].view(np.uint32), got[1 if first == 3 else 2].view(np.uint32))
+        only = {0, k.b.T - 1}
+        want, tol, _ = ref.attention(k.c, k.x, k.b.rows, k.b.lens, k.b.table, 0.05, only=only)
+        for y in got:
+            assert all((np.abs(y[t] - want[t]) <= tol[t]).all() for t in only)
