@@ -135,6 +135,7 @@ _sig("arcz_engine_kv_read", _i, _p, _p, _p, _p, _i, _i, _p, _i, _i)
 _sig("arcz_engine_attention", _i, _p, _p, _p, _p, _i, _i, _i, _p, _i, _i, _p)
 _sig("arcz_engine_attention_shared_room", _z, _p, _p, _p, _p, _i, _p)
 _sig("arcz_engine_attention_shared", _i, _p, _p, _p, _p, _p, _i, _i, _i, _p, _i, _i, _p, _p)
+_sig("arcz_engine_sample", _i, _p, _p, _i, _i, _i, _i, _p, _p, _p, _p)
 _sig("arcz_engine_self_check", _i)
 _sig("arcz_engine_profile", None, _p, _i)
 _sig("arcz_engine_profile_collect", _i, _p)
@@ -157,15 +158,16 @@ _quantize, _rmsnorm_quant, _swiglu_quant = lib.arcz_engine_quantize, lib.arcz_en
 _matmul, _gemv_gu, _layer_moe = lib.arcz_engine_matmul, lib.arcz_engine_gemv_gu, lib.arcz_engine_layer_moe
 _rope, _kv_write, _kv_read, _attention = lib.arcz_engine_rope, lib.arcz_engine_kv_write, lib.arcz_engine_kv_read, lib.arcz_engine_attention
 _norm_rope, _kv_plan, _attention_shared = lib.arcz_engine_norm_rope, lib.arcz_engine_kv_plan, lib.arcz_engine_attention_shared
+_sample = lib.arcz_engine_sample
 try:
     from . import _pycall
     _pycall.bind(_quantize, _rmsnorm_quant, _swiglu_quant, _matmul, _gemv_gu, _layer_moe)
     _pycall.bind_attn(_rope, _kv_write, _kv_read, _attention)
-    _pycall.bind_step(_norm_rope, _kv_plan, _attention_shared)
+    _pycall.bind_step(_norm_rope, _kv_plan, _attention_shared, _sample)
     from ._pycall import gemv_gu as _gemv_gu, layer_moe as _layer_moe, matmul as _matmul, quantize as _quantize
     from ._pycall import rmsnorm_quant as _rmsnorm_quant, swiglu_quant as _swiglu_quant
     from ._pycall import attention as _attention, kv_read as _kv_read, kv_write as _kv_write, rope as _rope
-    from ._pycall import attention_shared as _attention_shared, kv_plan as _kv_plan, norm_rope as _norm_rope
+    from ._pycall import attention_shared as _attention_shared, kv_plan as _kv_plan, norm_rope as _norm_rope, sample as _sample
 except ImportError:
     pass
 
@@ -559,6 +561,16 @@ class KvShared(C.Structure):
         self.at = C.addressof(self)
 
 
+class Sampling(C.Structure):
+    """How tokens are drawn (arcz_sampling): buffers of temperature (f32), top_k (int32), top_p and min_p (f32), a value for each row, or None."""
+    _fields_ = [(n, _p) for n in ("temperature", "top_k", "top_p", "min_p")]
+
+    def __init__(self, temperature=None, top_k=None, top_p=None, min_p=None):
+        self.held = (temperature, top_k, top_p, min_p)
+        super().__init__(*(b.h if b else None for b in self.held))
+        self.at = C.addressof(self)
+
+
 class Attention(C.Structure):
     """The form of an attention (arcz_attn): slopes f32 [heads], prefix int32 [seqs], first int32 [T], each a buffer or None."""
     _fields_ = [("scale", C.c_float), ("cap", C.c_float), ("window", _i), ("slopes", _p), ("prefix", _p), ("first", _p)]
@@ -782,6 +794,12 @@ class Engine:
     def attention_shared(self, kv, batch, shared, q, ldq, q_off, heads, out, ldo, o_off, form, room):
         """attention() for a batch whose sequences share prefixes in groups, each prefix read once; shared: a KvShared, room: a workspace."""
         r = _attention_shared(self.h, kv.h, batch.at, shared.at, q.h, ldq, q_off, heads, out.h, ldo, o_off, form.at, room.h)
+        if r:
+            _check(r, engine=True)
+
+    def sample(self, logits, ld, off, V, T, form, u, token, prob=None):
+        """A token (int32) from each of T rows of V logits, and its probability among those kept; form: a Sampling, u: f32 [T] in [0, 1)."""
+        r = _sample(self.h, logits.h, ld, off, V, T, form.at, u.h, token.h, prob.h if prob else None)
         if r:
             _check(r, engine=True)
 

@@ -334,6 +334,13 @@ int arcz_engine_attention_shared(arcz_engine* e, arcz_kv* c, const arcz_kv_batch
   });
 }
 
+int arcz_engine_sample(arcz_engine* e, arcz_mem* logits, int ld, int off, int V, int T, const arcz_sampling* f, arcz_mem* u, arcz_mem* token, arcz_mem* prob) {
+  return guarded([&] {
+    if (!f) throw std::runtime_error("sample: no parameters");
+    e->e->sample(logits, ld, off, V, T, {f->temperature, f->top_k, f->top_p, f->min_p}, u, token, prob);
+  });
+}
+
 int arcz_engine_self_check(void) {
   return guarded([&] {
     const std::string r = engine_self_check();

@@ -490,6 +490,7 @@ class Engine {
   }
 
 #include "engine_attn.h"
+#include "engine_sample.h"
 
   // ---- matmul (zero/engine.h:1080-1112): C[:, c_off : c_off+N] (+)= act * W^T for the current chunk.  acc: 0 = store,
   // 1 = accumulate into C, 2 = C = silu(C) * result (GEMM path only).  With two-pass inputs the residual's half goes

@@ -9,6 +9,7 @@
     .balign 8
     .endm
     BLOB arcz_blob_ops, "ops.hsaco"
+    BLOB arcz_blob_sample, "sample.hsaco"
     BLOB arcz_blob_decode, "decode.hsaco"
     BLOB arcz_blob_decode_q80, "decode_q80.hsaco"
     BLOB arcz_blob_decode_q40, "decode_q40.hsaco"

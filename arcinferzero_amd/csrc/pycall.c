@@ -65,10 +65,11 @@ CALL(norm_rope, "pppiipiiiiiippfpi",
      arcz_engine_norm_rope(E, v[1].p, v[2].p, v[3].i, v[4].i, v[5].p, v[6].i, v[7].i, v[8].i, v[9].i, v[10].i, v[11].i, v[12].p, v[13].p, v[14].f, v[15].p, v[16].i))
 CALL(attention_shared, "pppppiiipiipp",
      arcz_engine_attention_shared(E, v[1].p, v[2].p, v[3].p, v[4].p, v[5].i, v[6].i, v[7].i, v[8].p, v[9].i, v[10].i, v[11].p, v[12].p))
+CALL(sample, "ppiiiipppp", arcz_engine_sample(E, v[1].p, v[2].i, v[3].i, v[4].i, v[5].i, v[6].p, v[7].p, v[8].p, v[9].p))
 CALL(kv_plan, "ppp", arcz_engine_kv_plan(E, v[1].p, v[2].p))
 
 /* bind(quantize, rmsnorm_quant, swiglu_quant, matmul, gemv_gu, layer_moe), bind_attn(rope, kv_write, kv_read, attention) and
- * bind_step(norm_rope, kv_plan, attention_shared): the ctypes functions */
+ * bind_step(norm_rope, kv_plan, attention_shared, sample): the ctypes functions */
 static PyObject* bind_to(PyObject** const* to, int n, PyObject* const* args, Py_ssize_t nargs) {
   if (nargs != n) {
     PyErr_Format(PyExc_TypeError, "bind takes the %d functions", n);
@@ -92,15 +93,15 @@ static PyObject* bind_attn(PyObject* self, PyObject* const* args, Py_ssize_t nar
 }
 
 static PyObject* bind_step(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
-  PyObject** const to[3] = {&norm_rope_ctypes, &kv_plan_ctypes, &attention_shared_ctypes};
+  PyObject** const to[4] = {&norm_rope_ctypes, &kv_plan_ctypes, &attention_shared_ctypes, &sample_ctypes};
   (void)self;
-  return bind_to(to, 3, args, nargs);
+  return bind_to(to, 4, args, nargs);
 }
 
 #define METHOD(NAME) {#NAME, (PyCFunction)(void (*)(void))NAME, METH_FASTCALL, NULL}
 static PyMethodDef methods[] = {METHOD(quantize), METHOD(rmsnorm_quant), METHOD(swiglu_quant), METHOD(matmul),
                                 METHOD(gemv_gu), METHOD(layer_moe), METHOD(rope), METHOD(kv_write), METHOD(kv_read),
-                                METHOD(attention), METHOD(norm_rope), METHOD(kv_plan), METHOD(attention_shared), METHOD(bind), METHOD(bind_attn), METHOD(bind_step), {NULL, NULL, 0, NULL}};
+                                METHOD(attention), METHOD(norm_rope), METHOD(kv_plan), METHOD(attention_shared), METHOD(sample), METHOD(bind), METHOD(bind_attn), METHOD(bind_step), {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pycall", NULL, -1, methods, NULL, NULL, NULL, NULL};
 
 PyMODINIT_FUNC PyInit__pycall(void) { return PyModule_Create(&module); }

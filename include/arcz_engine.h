@@ -284,6 +284,21 @@ size_t arcz_engine_attention_shared_room(arcz_engine* e, arcz_kv* c, const arcz_
 int arcz_engine_attention_shared(arcz_engine* e, arcz_kv* c, const arcz_kv_batch* b, const arcz_kv_shared* g, arcz_mem* q, int ldq, int q_off, int heads, arcz_mem* out, int ldo,
                                  int o_off, const arcz_attn* a, arcz_mem* room);
 
+/* A token from each of T rows of V logits (1 to 2^20; f32, as a head's product leaves them), row by row on its own parameters: f32 [T] buffers, or NULL.
+ *   temperature  t (NULL: 1).  A token's weight is w = e^((x - max) / t); not above 0 (or NaN): the largest logit, of equal ones the first
+ *   top_k        int32: the k highest logits are kept, of equal ones the first (NULL, 0 and below, V and above: all)
+ *   top_p        of these the fewest highest whose weights make p of the sum of theirs, one at least (NULL, 1 and above, NaN: all)
+ *   min_p        of these the ones with w >= q, the largest always (NULL, 0 and below, NaN: all)
+ *   u            f32 [T], random numbers in [0, 1) that the caller draws (below 0 or NaN: 0; 1 and above: the last token)
+ * token [T] (int32) is the first kept one, in the order of the row, whose running sum of weights passes u times their sum; prob [T] (f32, may be
+ * NULL) its weight over that sum.  Weights and sums are held to 2^-42; a token of less than 2^-44 of the largest weight is not drawn.  A logit of -inf or NaN
+ * is no token; a row of nothing else gives -1 and 0.  Where the largest is +inf, tokens of +inf have weight 1 and no others any.  The same rows give
+ * the same tokens.  token and prob must not meet what is read, nor each other. */
+typedef struct arcz_sampling {
+  arcz_mem *temperature, *top_k, *top_p, *min_p;
+} arcz_sampling;
+int arcz_engine_sample(arcz_engine* e, arcz_mem* logits, int ld, int off, int V, int T, const arcz_sampling* f, arcz_mem* u, arcz_mem* token, arcz_mem* prob);
+
 /* The start-up check of the tuned GEMMs of 128 tokens and of the GEMM on digits against the simple one on the reference's
  * LCG data, both against integer sums counted on the host (the pattern of xmx_check, zero/engine_setup.h:424-520): the
  * weight types that make unit-scale blocks, the three accumulate modes, K in one piece and in several.  0, or ARCZ_E_ENGINE with the first
