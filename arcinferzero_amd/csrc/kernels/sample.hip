@@ -22,23 +22,23 @@
 
 namespace {
 typedef unsigned long long u64;
-constexpr int THREADS = 1024, WAVES = 16, CAP = 512, SMALL_K = 512, BINS = 3072;   // (48 octaves)
-constexpr int PER = WAVES * CAP / THREADS;                                        // tokens of the list a thread
+constexpr int THREADS = 1024, WAVES = 16, CAP = 512, SMALL_K = 512, FEW = 512, BINS = 3072;   // (48 octaves)
 constexpr uint32_t NONE = 0x007FFFFFu;                                             // the key of -inf: no token
 
 struct Lds {
-  double pow2[256];   // 2^(j / 256)
+  double pow2[16];   // 2^(43 + j / 16)
   u64 sum[BINS];
   uint32_t count[BINS];
-  uint32_t key[WAVES * CAP], at[WAVES * CAP];
+  uint32_t key[WAVES * CAP], at[WAVES * CAP];   // the list: a run of each wave's, in the row's order
+  uint32_t few_key[FEW], few_at[FEW];           // ... of few members, the runs behind one another
   u64 digit_sum[256];
   uint32_t digit[256];
-  u64 part[WAVES];
-  int number[WAVES];
+  u64 part[WAVES], kept[WAVES];
+  int number[WAVES], equal[WAVES];
   float top[WAVES];
   int where[WAVES];
-  u64 found[2];
-  int place[4];
+  u64 found[3];
+  uint32_t place[3];
 };
 
 // Logits in their order as whole numbers; -0 is 0, and what is no number is -inf.
@@ -51,8 +51,7 @@ __device__ inline float logit_of(uint32_t k) { return __uint_as_float(k & 0x8000
 struct Row {
   const float* x;   // (of V logits; the units of four begin `skew` values in front of it, where addresses are multiples of 16)
   int V, skew, units;
-  double most, scale;   // the largest logit; 256 log2(e) / t
-  bool endless;         // the largest is +inf: tokens of it alone, each of weight 1
+  double most, scale;   // the largest logit, 16 log2(e) / t; where it is +inf, above all finite ones, whose weights are then 0
 };
 __device__ inline float4 load(const Row& r, int unit) {
   const int i = 4 * unit - r.skew;
@@ -63,44 +62,56 @@ __device__ inline float4 load(const Row& r, int unit) {
   for (int j = 0; j < 4; ++j) e[j] = i + j >= 0 && i + j < r.V ? r.x[i + j] : -INFINITY;
   return v;
 }
-// The weight's logarithm in 1 / 256 of an octave, at least -15360, and what is left of it (in the same, within a half).
-__device__ inline int octaves(const Row& r, float x, double& rest) {
+// A weight's logarithm in 1 / 16 of an octave, down to 60 octaves -- of -inf and of what is no number --, its whole part and the rest of it, within a half.
+struct Octaves {
+  double y, rest;
+  int n;
+};
+__device__ inline Octaves octaves(const Row& r, float x) {
   constexpr double MAGIC = 6755399441055744.0;   // 1.5 * 2^52: its last place is 1
-  const double y = fmax(((double)x - r.most) * r.scale, -15360.0), k = y + MAGIC;
-  rest = y - (k - MAGIC);
-  return (int)(uint32_t)__double_as_longlong(k);
+  Octaves o;
+  o.y = fmin(fmax(((double)x - r.most) * r.scale, -960.0), 0.0);
+  const double k = o.y + MAGIC;
+  o.n = __double2loint(k);
+  o.rest = o.y - (k - MAGIC);
+  return o;
+}
+__device__ inline u64 weight_at(const double* pow2, const Octaves& o) {
+  // 2^(f / 16) to f^5: what is cut off is 2^-42 at most.  (Sixteen powers: no two of them lie in one bank of the LDS.)
+  constexpr double A = 0.04332169878499658, B = 0.0009383847928089871, C = 1.3550807779497455e-05, D = 1.467610032291943e-07, E = 1.271587195055813e-09;   // (ln 2 / 16)^i / i!
+  const double f = o.rest, p = fma(f, fma(f, fma(f, fma(f, fma(f, E, D), C), B), A), 1.0), t = pow2[o.n & 15];
+  const double w = fma(__hiloint2double(__double2hiint(t) + ((o.n >> 4) << 20), __double2loint(t)), p, 4503599627370496.0);   // (+ 2^52: rounded to a whole number)
+  return (u64)(uint32_t)(__double2hiint(w) & 0xFFFFF) << 32 | (uint32_t)__double2loint(w);
 }
 __device__ inline u64 weight(const Row& r, const double* pow2, float x) {
-  if (!(x > -INFINITY)) return 0;
-  if (r.endless) return x == INFINITY ? 1ull << 43 : 0;
-  double f;
-  const int n = octaves(r, x, f);
-  // 2^(f / 256) to f^3: what is cut off is 2^-42 at most
-  constexpr double A = 0.0027076061740622863, B = 3.665565596910106e-06, C = 3.308302680541371e-09;   // (ln 2 / 256)^i / i!
-  const double w = pow2[n & 255] * fma(f, fma(f, fma(f, C, B), A), 1.0);
-  return (u64)__double_as_longlong(__builtin_ldexp(w, 43 + (n >> 8)) + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;   // (+ 2^52: rounded to a whole number)
+  return weight_at(pow2, octaves(r, x));
 }
-__device__ inline int bin(const Row& r, float x) {   // (of a token: 0 for the largest)
-  if (r.endless) return x == INFINITY ? 0 : BINS - 1;
-  double f;
-  return min(-octaves(r, x, f) >> 2, BINS - 1);
+// 64 bins an octave: of a token, 0 for the largest, the last one of all that have no weight.
+__device__ inline int bin_at(const Octaves& o) { return min((int)(o.y * -4.0), BINS - 1); }
+__device__ inline int bin(const Row& r, float x) {
+  return bin_at(octaves(r, x));
 }
 
 __device__ inline int wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 __device__ inline int lane() { return threadIdx.x & 63; }
+template <int DPP, int ROWS>
+__device__ inline uint32_t moved(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, DPP, ROWS, 0xF, false); }
+template <int DPP, int ROWS>
+__device__ inline u64 moved(u64 v) { return (u64)moved<DPP, ROWS>((uint32_t)(v >> 32)) << 32 | moved<DPP, ROWS>((uint32_t)v); }
+// The sum over the lanes up to this one: in each row of sixteen, then the rows' ends.
 template <class T>
-__device__ inline T up_sum(T v) {   // (over the lanes up to this one)
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const T w = __shfl_up(v, o);
-    if (lane() >= o) v += w;
-  }
+__device__ inline T up_sum(T v) {
+  v += moved<0x111, 0xF>(v);
+  v += moved<0x112, 0xF>(v);
+  v += moved<0x114, 0xF>(v);
+  v += moved<0x118, 0xF>(v);
+  v += moved<0x142, 0xA>(v);   // (lane 15 to the next row, 47 likewise)
+  v += moved<0x143, 0xC>(v);   // (lane 31 to the second half)
   return v;
 }
 __device__ inline u64 wave_sum(u64 v) {
-#pragma unroll
-  for (int o = 32; o; o /= 2) v += __shfl_xor(v, o);
-  return v;
+  v = up_sum(v);
+  return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 // The sum over the threads in front of this one, and of all.
 __device__ inline u64 scan(Lds& s, u64 v, u64& total) {
@@ -118,9 +129,9 @@ __device__ inline u64 scan(Lds& s, u64 v, u64& total) {
   return front + up - v;
 }
 // A wave's units [a, b) in their order, 64 at a time: f(logits of this lane's unit, its first index); lanes behind the end have -inf at V.
-template <class F>
+// N: loads on their way at once.
+template <int N, class F>
 __device__ inline void walk(const Row& r, int a, int b, F f) {
-  constexpr int N = 4;   // (loads on their way at once)
   for (int u0 = a; u0 < b; u0 += 64 * N) {
     float4 v[N];
 #pragma unroll
@@ -145,53 +156,43 @@ __device__ inline Range share(Range all, int w) {
   return {a, min(a + per, all.b)};
 }
 
-// Of 256 sums, from the last one down, the one in which the running sum reaches `need`: its number in place[0], found[0] the sum in front of it.
-// (The sums reach it.)
-template <class T>
-__device__ inline void pick(Lds& s, const T* sums, T need) {
-  __syncthreads();
-  if (wave() == 0) {
-    T v[4], own = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) own += v[j] = sums[255 - 4 * lane() - j];
-    T front = up_sum(own) - own;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (front < need && front + v[j] >= need) {
-        s.place[0] = 255 - 4 * lane() - j;
-        s.found[0] = front;
-      }
-      front += v[j];
-    }
-  }
-  __syncthreads();
-}
-
-// Tokens in LDS in the vocabulary's order: each wave's run of them one behind the other, PER or fewer to a thread.
-struct List {
-  uint32_t key[PER];
-  int at[PER];
-  bool in[PER];
-  int n;
+// A cut: tokens above `key` are kept, and those of it up to index `last`.
+struct Cut {
+  uint32_t key;
+  int last;
+  __device__ bool keeps(uint32_t k, int i) const { return k > key || (k == key && i <= last); }
 };
-// The tokens of the row for which f says so; false: there are more than LDS takes.
-template <class F>
-__device__ inline bool gather(Lds& s, const Row& r, List& l, F f) {
+__device__ inline Cut higher(const Cut& a, const Cut& b) { return a.key > b.key || (a.key == b.key && a.last <= b.last) ? a : b; }
+// Tokens of a row whose keys lie in [lo, hi] and that `within` keeps; listed: in LDS.
+struct Members {
+  uint32_t lo, hi;
+  Cut within;
+  bool listed;
+  __device__ bool has(uint32_t k, int i) const { return k >= lo && k <= hi && within.keeps(k, i); }
+};
+// Over the row: its members (of a range; `within` everything) to LDS -- false: there are more than it takes --, and where `add` the weights of those that
+// `floor` keeps added up, each wave's to part[].
+__device__ inline bool pass(Lds& s, const Row& r, const Members& m, bool add, const Cut& floor) {
   const Range mine = share({0, r.units}, wave());
+  const bool any = m.lo <= m.hi;
+  const float lo = any ? logit_of(m.lo) : INFINITY, hi = any ? logit_of(m.hi) : -INFINITY, edge = logit_of(floor.key);
   int have = 0;
+  u64 sum = 0;
   __syncthreads();   // (the last list is not looked at any more)
-  walk(r, mine.a, mine.b, [&](const float4& v, int i) {
+  auto members = [&](const float4& v, int i) {
     const float* e = (const float*)&v;
+    bool some = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) some = some || (e[j] >= lo && e[j] <= hi);
+    if (!__any(some)) return;
     u64 vote[4];
-    int front = have, all = 0;
+    int front = have;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const bool yes = e[j] > -INFINITY && f(e[j], i + j);
-      vote[j] = __ballot(yes);
+      vote[j] = __ballot(e[j] >= lo && e[j] <= hi);
       front += __builtin_amdgcn_mbcnt_hi((uint32_t)(vote[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)vote[j], 0));
-      all += __popcll(vote[j]);
+      have += __popcll(vote[j]);
     }
-    if (all == 0) return;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (vote[j] >> lane() & 1) {
@@ -201,148 +202,243 @@ __device__ inline bool gather(Lds& s, const Row& r, List& l, F f) {
         }
         ++front;
       }
-    have += all;
-  });
-  if (lane() == 0) s.number[wave()] = have;
+  };
+  if (!add) {
+    walk<8>(r, mine.a, mine.b, members);
+  } else {
+    walk<4>(r, mine.a, mine.b, [&](const float4& v, int i) {
+      const float* e = (const float*)&v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // (what is not kept as -inf: of weight 0)
+        sum += weight(r, s.pow2, e[j] > edge || (e[j] == edge && i + j <= floor.last) ? e[j] : -INFINITY);
+      }
+      if (any) members(v, i);
+    });
+    sum = wave_sum(sum);
+  }
+  if (lane() == 0) {
+    s.number[wave()] = have;
+    s.part[wave()] = sum;
+  }
   __syncthreads();
   bool fits = true;
-  int starts[WAVES];
-  l.n = 0;
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    starts[w] = l.n;
-    l.n += s.number[w];
-    fits = fits && s.number[w] <= CAP;
-  }
-  if (!fits) return false;
-  const int per = (l.n + THREADS - 1) / THREADS;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int g = threadIdx.x * per + j;
-    l.in[j] = j < per && g < l.n;
-    l.key[j] = 0;
-    l.at[j] = 0;
-    if (l.in[j]) {
-      int w = 0;
-#pragma unroll
-      for (int k = 1; k < WAVES; ++k) w = starts[k] <= g ? k : w;
-      int from = 0;
-#pragma unroll
-      for (int k = 1; k < WAVES; ++k) from = k == w ? starts[k] : from;
-      l.key[j] = s.key[w * CAP + g - from];
-      l.at[j] = s.at[w * CAP + g - from];
-    }
-  }
-  return true;
+  for (int w = 0; w < WAVES; ++w) fits = fits && s.number[w] <= CAP;
+  return fits;
 }
-
-// A cut: tokens above `key` are kept, and those of it up to index `last`.
-struct Cut {
-  uint32_t key;
-  int last;
-  __device__ bool keeps(uint32_t k, int i) const { return k > key || (k == key && i <= last); }
-};
-
-// The cut behind which the count (or, by weight, the sum of weights) of the tokens that f goes over first reaches `need` -- which all of them together do.
-// each(g): g(key, index) for the tokens, in any order; nth(key, n): the index of the n-th token (from 0) of that key.  sum: of the weights that it keeps of these.
-template <bool BY_WEIGHT, class E, class N>
-__device__ inline Cut select(Lds& s, const Row& r, u64 need, E each, N nth) {
-  uint32_t prefix = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
+// g(key, index) for the members, this wave's share of them in the row's order, 64 at a time; lanes without one: key 0.
+template <class G>
+__device__ inline void each(Lds& s, const Row& r, const Members& m, G g) {
+  if (m.listed) {
+    const int n = s.number[wave()];
+    for (int p0 = 0; p0 < n; p0 += 64) {
+      const int p = min(p0 + lane(), n - 1);
+      const uint32_t k = s.key[wave() * CAP + p];
+      const int i = s.at[wave() * CAP + p];
+      g(p0 + lane() < n && m.has(k, i) ? k : 0u, i);
+    }
+    return;
+  }
+  const Range mine = share({0, r.units}, wave());
+  auto value = [&](int u0) {   // (a value a lane, of sixteen units)
+    const int u = u0 + (lane() >> 2), i = 4 * u + (lane() & 3) - r.skew;
+    return u < mine.b && i >= 0 && i < r.V ? r.x[i] : -INFINITY;
+  };
+  float x[4] = {value(mine.a), value(mine.a + 16), value(mine.a + 32), value(mine.a + 48)};   // (four of them on their way)
+  for (int u0 = mine.a; u0 < mine.b; u0 += 16) {
+    const uint32_t k = key_of(x[0]);
+    const int i = 4 * (u0 + (lane() >> 2)) + (lane() & 3) - r.skew;
+    x[0] = x[1];
+    x[1] = x[2];
+    x[2] = x[3];
+    x[3] = value(u0 + 64);
+    g(k > NONE && m.has(k, i) ? k : 0u, i);
+  }
+}
+// The cut behind which the count (by_weight: the sum of weights) of the members first reaches `need` -- which all of them together do -- going down from the
+// highest; kept: the sum of weights that it leaves of them.
+__device__ inline Cut select(Lds& s, const Row& r, const Members& m, bool by_weight, u64 need, u64& kept) {
+  const uint32_t differ = m.lo ^ m.hi;
+  int all = 0, run = 0;
+  for (int w = 0; w < WAVES; ++w) {
+    run = w == wave() ? all : run;
+    all += s.number[w];
+  }
+  if (m.listed && all <= FEW) {
+    // Few: one wave has them in its registers, and goes down the bits of their keys.
+    constexpr int N = FEW / 64;
+    for (int p = lane(); p < s.number[wave()]; p += 64) {
+      const uint32_t k = s.key[wave() * CAP + p];
+      const int i = s.at[wave() * CAP + p];
+      s.few_key[run + p] = m.has(k, i) ? k : 0;
+      s.few_at[run + p] = i;
+    }
+    __syncthreads();
+    if (wave() == 0) {
+      if (all <= 64) {
+        // how many members lie in front of this lane's, and what they weigh
+        const uint32_t key = lane() < all ? s.few_key[lane()] : 0;
+        const u64 w = key ? weight(r, s.pow2, logit_of(key)) : 0;
+        uint32_t rank = 0;
+        u64 front = 0;
+#pragma unroll 1
+        for (int p = 0; p < all; ++p) {
+          const uint32_t k = __builtin_amdgcn_readlane((int)key, p);
+          const bool before = k > key || (k == key && p < lane());
+          rank += before && k ? 1 : 0;
+          front += before ? (u64)(uint32_t)__builtin_amdgcn_readlane((int)(w >> 32), p) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)w, p) : 0;
+        }
+        if (key && (by_weight ? front < need && front + w >= need : rank == need - 1)) {
+          s.place[0] = key;
+          s.place[1] = s.few_at[lane()];
+          s.found[0] = front + w;
+        }
+      } else {
+        uint32_t key[N];
+        u64 w[N], above = 0;
+        bool in[N];
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+          const int p = 64 * c + lane();
+          key[c] = p < all ? s.few_key[p] : 0;
+          in[c] = key[c] != 0;
+          w[c] = 0;
+          if (64 * c < all) w[c] = in[c] ? weight(r, s.pow2, logit_of(key[c])) : 0;
+        }
+#pragma unroll 1
+        for (int bit = differ ? 31 - __clz((int)differ) : -1; bit >= 0; --bit) {
+          u64 sum = 0;   // (of the members that have the bit)
+          if (by_weight) {
+#pragma unroll
+            for (int c = 0; c < N; ++c)
+              if (64 * c < all) sum += in[c] && key[c] >> bit & 1 ? w[c] : 0;
+            sum = wave_sum(sum);
+          } else {
+#pragma unroll
+            for (int c = 0; c < N; ++c)
+              if (64 * c < all) sum += __popcll(__ballot(in[c] && key[c] >> bit & 1));
+          }
+          const bool up = sum >= need;   // (the cut lies among them: else they are all above it)
+          need -= up ? 0 : sum;
+#pragma unroll
+          for (int c = 0; c < N; ++c)
+            if (64 * c < all) {
+              const bool one = key[c] >> bit & 1;
+              above += in[c] && one && !up ? w[c] : 0;
+              in[c] = in[c] && one == up;
+            }
+        }
+        // What is left has one key, and one weight (not 0, where a sum had to be reached): so many of the first ones.
+        uint32_t last = 0;
+        u64 one = 0;
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+          const u64 vote = __ballot(in[c]);
+          if (vote) {
+            const int l = __ffsll((long long)vote) - 1;
+            last = __builtin_amdgcn_readlane((int)key[c], l);
+            one = (u64)(uint32_t)__builtin_amdgcn_readlane((int)(w[c] >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)w[c], l);
+          }
+        }
+        const int n = by_weight ? (int)((need + one - 1) / one) : (int)need;
+        int front = 0;
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+          const u64 vote = __ballot(in[c]);
+          const int at = front + __builtin_amdgcn_mbcnt_hi((uint32_t)(vote >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)vote, 0));
+          if (in[c] && at == n - 1) s.place[1] = s.few_at[64 * c + lane()];
+          front += __popcll(vote);
+        }
+        above = wave_sum(above) + (u64)n * one;
+        if (lane() == 0) {
+          s.place[0] = last;
+          s.found[0] = above;
+        }
+      }
+    }
+    __syncthreads();
+    kept = s.found[0];
+    return {s.place[0], (int)s.place[1]};
+  }
+  int shift = differ ? (31 - __clz((int)differ)) / 8 * 8 : 0;
+  uint32_t prefix = shift == 24 ? 0 : m.lo >> (shift + 8);
+  kept = 0;
+  for (; shift >= 0; shift -= 8) {
     __syncthreads();
     if (threadIdx.x < 256) {
       s.digit[threadIdx.x] = 0;
       s.digit_sum[threadIdx.x] = 0;
     }
     __syncthreads();
-    each([&](uint32_t k, int) {
-      if (shift < 24 && k >> (shift + 8) != prefix) return;
-      if (BY_WEIGHT) atomicAdd(&s.digit_sum[k >> shift & 255], weight(r, s.pow2, logit_of(k)));
-      else atomicAdd(&s.digit[k >> shift & 255], 1u);
+    each(s, r, m, [&](uint32_t k, int) {
+      if (k == 0 || (shift < 24 && k >> (shift + 8) != prefix)) return;
+      atomicAdd(&s.digit_sum[k >> shift & 255], weight(r, s.pow2, logit_of(k)));
+      atomicAdd(&s.digit[k >> shift & 255], 1u);
     });
-    if (BY_WEIGHT) pick<u64>(s, s.digit_sum, need);
-    else pick<uint32_t>(s, s.digit, (uint32_t)need);
-    need -= s.found[0];
-    prefix = prefix << 8 | (uint32_t)s.place[0];
     __syncthreads();
-  }
-  // (all tokens of one key have the same weight, which is not 0 where a sum had to be reached)
-  const u64 w = BY_WEIGHT ? weight(r, s.pow2, logit_of(prefix)) : 1;
-  return {prefix, nth(prefix, (int)((need + w - 1) / w) - 1)};
-}
-__device__ inline int list_nth(Lds& s, const List& l, uint32_t key, int n) {
-  int own = 0;
+    // the digit in which the running sum, from 255 down, reaches what is needed
+    if (wave() == 0) {
+      u64 v[4], w[4], own = 0, own_w = 0;
 #pragma unroll
-  for (int j = 0; j < PER; ++j) own += l.in[j] && l.key[j] == key;
-  u64 total;
-  int front = (int)scan(s, (u64)own, total);
+      for (int j = 0; j < 4; ++j) {
+        const int d = 255 - 4 * lane() - j;
+        w[j] = s.digit_sum[d];
+        v[j] = by_weight ? w[j] : s.digit[d];
+        own += v[j];
+        own_w += w[j];
+      }
+      u64 front = up_sum(own) - own, front_w = up_sum(own_w) - own_w;
 #pragma unroll
-  for (int j = 0; j < PER; ++j)
-    if (l.in[j] && l.key[j] == key) {
-      if (front == n) s.place[1] = l.at[j];
-      ++front;
+      for (int j = 0; j < 4; ++j) {
+        if (front < need && front + v[j] >= need) {
+          s.place[0] = (uint32_t)(255 - 4 * lane() - j);
+          s.found[0] = front;
+          s.found[1] = front_w;
+        }
+        front += v[j];
+        front_w += w[j];
+      }
     }
+    __syncthreads();
+    need -= s.found[0];
+    kept += s.found[1];
+    prefix = prefix << 8 | s.place[0];
+  }
+  // Tokens of one logit have one weight (not 0, where a sum had to be reached): so many of the first ones.
+  const u64 w = weight(r, s.pow2, logit_of(prefix));
+  const int n = by_weight ? (int)((need + w - 1) / w) : (int)need;
+  kept += (u64)n * w;
+  int have = 0;
+  each(s, r, m, [&](uint32_t k, int) { have += __popcll(__ballot(k == prefix)); });
+  if (lane() == 0) s.equal[wave()] = have;
   __syncthreads();
-  return s.place[1];
+  int front = 0;
+  for (int v = 0; v < wave(); ++v) front += s.equal[v];
+  if (front < n && n <= front + have)
+    each(s, r, m, [&](uint32_t k, int i) {
+      const u64 vote = __ballot(k == prefix);
+      const int mine = front + __builtin_amdgcn_mbcnt_hi((uint32_t)(vote >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)vote, 0));
+      if (k == prefix && mine == n - 1) s.place[1] = i;
+      front += __popcll(vote);
+    });
+  __syncthreads();
+  return {prefix, (int)s.place[1]};
 }
-template <bool BY_WEIGHT>
-__device__ inline Cut list_select(Lds& s, const Row& r, const List& l, u64 need) {
-  return select<BY_WEIGHT>(
-      s, r, need,
-      [&](auto g) {
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
-          if (l.in[j]) g(l.key[j], l.at[j]);
-      },
-      [&](uint32_t key, int n) { return list_nth(s, l, key, n); });
-}
-// ... over the row's tokens for which f says so
-template <bool BY_WEIGHT, class F>
-__device__ inline Cut row_select(Lds& s, const Row& r, u64 need, F f) {
-  const Range mine = share({0, r.units}, wave());
-  return select<BY_WEIGHT>(
-      s, r, need,
-      [&](auto g) {
-        walk(r, mine.a, mine.b, [&](const float4& v, int i) {
-          const float* e = (const float*)&v;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (e[j] > -INFINITY && f(e[j], i + j)) g(key_of(e[j]), i + j);
-        });
-      },
-      [&](uint32_t key, int n) {
-        auto count = [&](Range a, auto see) {
-          int have = 0;
-          walk(r, a.a, a.b, [&](const float4& v, int i) {
-            const float* e = (const float*)&v;
-            int own = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) own += key_of(e[j]) == key && f(e[j], i + j);
-            const int up = up_sum(own);
-            see(v, i, have + up - own);
-            have += __shfl(up, 63);
-          });
-          return have;
-        };
-        const int have = count(mine, [](const float4&, int, int) {});
-        __syncthreads();
-        if (lane() == 0) s.number[wave()] = have;
-        __syncthreads();
-        int front = 0;
-        for (int w = 0; w < wave(); ++w) front += s.number[w];
-        if (front <= n && n < front + have)
-          count(mine, [&](const float4& v, int i, int before) {
-            const float* e = (const float*)&v;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (key_of(e[j]) == key && f(e[j], i + j)) {
-                if (front + before == n) s.place[1] = i + j;
-                ++before;
-              }
-          });
-        __syncthreads();
-        return s.place[1];
-      });
+// The lowest key up to the largest for whose logit f holds, which it does for all above it.
+template <class F>
+__device__ inline uint32_t lowest(const Row& r, F f) {
+  uint32_t lo = NONE + 1, hi = key_of((float)r.most);
+#pragma unroll 1
+  while (lo < hi) {   // (64 keys of the range at a time)
+    const uint32_t k = lo + (uint32_t)((u64)(hi - lo) * lane() >> 6);
+    const u64 vote = __ballot(f(logit_of(k)));
+    const int first = vote ? __ffsll((long long)vote) - 1 : 64;
+    const uint32_t below = __shfl(k, max(first - 1, 0)) + 1;
+    hi = first < 64 ? __shfl(k, min(first, 63)) : hi;
+    lo = first > 0 ? below : hi;
+  }
+  return __builtin_amdgcn_readfirstlane(lo);
 }
 
 // The point that a draw looks for: below the sum, whatever u is.
@@ -374,7 +470,7 @@ extern "C" __global__ __launch_bounds__(1024) void sample(const float* __restric
   const Range mine = share({0, r.units}, wave());
   float top = -INFINITY;
   int where = 0x7FFFFFFF;
-  walk(r, mine.a, mine.b, [&](const float4& v, int i) {
+  walk<8>(r, mine.a, mine.b, [&](const float4& v, int i) {
     const float* e = (const float*)&v;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -388,7 +484,7 @@ extern "C" __global__ __launch_bounds__(1024) void sample(const float* __restric
     if (a > top || (a == top && b < where)) { top = a; where = b; }
   }
   if (lane() == 0) { s.top[wave()] = top; s.where[wave()] = where; }
-  if (threadIdx.x < 256) s.pow2[threadIdx.x] = exp2((double)threadIdx.x / 256.0);
+  if (threadIdx.x < 16) s.pow2[threadIdx.x] = exp2(43.0 + threadIdx.x / 16.0);
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) {
@@ -404,194 +500,186 @@ extern "C" __global__ __launch_bounds__(1024) void sample(const float* __restric
     if (threadIdx.x == 0) answer(where, 1.0f);
     return;
   }
-  r.most = (double)top;
-  r.endless = top == INFINITY;
-  r.scale = 369.3299304675746 / (double)t;   // 256 log2(e) / t
+  r.most = top == INFINITY ? 1e300 : (double)top;
+  r.scale = fmax(23.083120654223414 / (double)t, top == INFINITY ? 1e-200 : 0.0);   // 16 log2(e) / t
   const uint32_t most_key = key_of(top);
-  const double least = (double)fminf(fmaxf(q, 0.0f), 1.0f) * 8796093022208.0;   // (2^43; a NaN is 0)
-  auto heavy = [&](uint32_t key, u64 w) { return (double)w >= least || key == most_key; };
+  // (min_p is a cut like the others: the lowest logit whose weight is no less than q of the largest's, 2^43; a NaN is 0)
+  const u64 fewest = (u64)ceil((double)fminf(fmaxf(q, 0.0f), 1.0f) * 8796093022208.0);
+  const Cut least = {fewest ? lowest(r, [&](float x) { return weight(r, s.pow2, x) >= fewest; }) : NONE, 0x7FFFFFFF};
+
+  // ---- the cuts, one within the other: by k out of a list of few (step 0) or out of the histogram (1), by p (2)
   const bool by_p = p < 1.0f;
-  auto goal = [&](u64 sum) { return (u64)fmax(1.0, ceil((double)fmaxf(p, 0.0f) * (double)sum)); };
-  List l;
-
-  // ---- few highest: all in LDS
-  bool by_k = k > 0 && k < V;
-  if (by_k && k <= SMALL_K) {
-    // two digits of the k-th of the threads' largest: at least k tokens reach it
-    const uint32_t key = key_of(own);
-    uint32_t prefix = 0, need = (uint32_t)k;
-#pragma unroll
-    for (int shift = 24; shift >= 16; shift -= 8) {
-      __syncthreads();
-      if (threadIdx.x < 256) s.digit[threadIdx.x] = 0;
-      __syncthreads();
-      if (shift == 24 || key >> 24 == prefix) atomicAdd(&s.digit[key >> shift & 255], 1u);
-      pick<uint32_t>(s, s.digit, need);
-      need -= (uint32_t)s.found[0];
-      prefix = prefix << 8 | (uint32_t)s.place[0];
-    }
-    const uint32_t least_key = prefix << 16;
-    if (gather(s, r, l, [&](float x, int) { return key_of(x) >= least_key; })) {
-      auto keep = [&](const Cut& c) {
-#pragma unroll
-        for (int j = 0; j < PER; ++j) l.in[j] = l.in[j] && c.keeps(l.key[j], l.at[j]);
-      };
-      if (l.n > k) keep(list_select<false>(s, r, l, (u64)k));
-      u64 w[PER], mine_sum, sum;
-      auto weigh = [&] {
-        mine_sum = 0;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-          w[j] = l.in[j] ? weight(r, s.pow2, logit_of(l.key[j])) : 0;
-          mine_sum += w[j];
-        }
-      };
-      weigh();
-      scan(s, mine_sum, sum);
-      if (by_p) keep(list_select<true>(s, r, l, goal(sum)));
-#pragma unroll
-      for (int j = 0; j < PER; ++j) l.in[j] = l.in[j] && heavy(l.key[j], w[j]);
-      weigh();
-      u64 at = scan(s, mine_sum, sum);
-      const double to = target(draw, sum);
-#pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        if (w[j] && (double)at <= to && (double)(at + w[j]) > to) answer(l.at[j], (float)((double)w[j] / (double)sum));
-        at += w[j];
-      }
-      return;
-    }
-  }
-
-  // ---- the cuts out of a histogram
+  bool by_k = k > 0 && k < V, small = false, counted = false, added = false;
   Cut cut = {NONE, 0x7FFFFFFF};
-  if (by_k || by_p) {
-    __syncthreads();
-    for (int b = threadIdx.x; b < BINS; b += THREADS) {
-      s.sum[b] = 0;
-      s.count[b] = 0;
-    }
-    __syncthreads();
-    walk(r, mine.a, mine.b, [&](const float4& v, int) {
-      const float* e = (const float*)&v;
+  Members m = {1, 0, cut, true};
+  u64 front = 0, rest = 0;   // the weights in front of the members, and of those of them that the cut by k keeps
+  int bk = BINS;             // the bin of the cut by k
+  for (int step = 0; step < 3; ++step) {
+    if (step == 2 ? !by_p : !by_k || small) continue;
+    if (step == 0 && k > SMALL_K) continue;
+    u64 need = (u64)k;
+    bool look = true;   // (other members than the list has)
+    if (step == 0) {
+      // two digits of the k-th of the threads' largest logits: at least k tokens reach them
+      const uint32_t key = key_of(own);
+      uint32_t prefix = 0, left = (uint32_t)k;
+      for (int shift = 24; shift >= 16; shift -= 8) {
+        __syncthreads();
+        if (threadIdx.x < 256) s.digit[threadIdx.x] = 0;
+        __syncthreads();
+        if (shift == 24 || key >> 24 == prefix) atomicAdd(&s.digit[key >> shift & 255], 1u);
+        __syncthreads();
+        if (wave() == 0) {
+          uint32_t v[4], sum = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (e[j] > -INFINITY) {
-          const int b = bin(r, e[j]);
-          if (by_k) atomicAdd(&s.count[b], 1u);
-          if (by_p && b < BINS - 1) atomicAdd(&s.sum[b], weight(r, s.pow2, e[j]));
-        }
-    });
-    __syncthreads();
-    // the bin in which a running sum over the bins reaches `need` (found[1]: the sum in front of it, found[0] of all); BINS: none does
-    auto reach = [&](auto value, u64 need) {
-      u64 v[BINS / THREADS], mine_sum = 0, total;
+          for (int j = 0; j < 4; ++j) sum += v[j] = s.digit[255 - 4 * lane() - j];
+          uint32_t above = up_sum(sum) - sum;
 #pragma unroll
-      for (int j = 0; j < BINS / THREADS; ++j) mine_sum += v[j] = value(threadIdx.x * (BINS / THREADS) + j);
-      if (threadIdx.x == 0) s.place[2] = BINS;
-      u64 front = scan(s, mine_sum, total);
-#pragma unroll
-      for (int j = 0; j < BINS / THREADS; ++j) {
-        if (front < need && front + v[j] >= need) {
-          s.place[2] = threadIdx.x * (BINS / THREADS) + j;
-          s.found[1] = front;
-        }
-        front += v[j];
-      }
-      __syncthreads();
-      const int b = s.place[2];
-      __syncthreads();
-      return b;
-    };
-    auto sums = [&](int to) {   // of the bins in front of `to`
-      u64 v = 0, total;
-      for (int b = threadIdx.x; b < to; b += THREADS) v += s.sum[b];
-      scan(s, v, total);
-      return total;
-    };
-    int bk = BINS;
-    bool listed = false;   // the list has bin bk
-    u64 rest = 0;          // the sum of weights that the cut by k leaves of bk
-    if (by_k) {
-      bk = reach([&](int b) { return (u64)s.count[b]; }, (u64)k);
-      if (bk >= BINS - 1) {
-        by_k = false;   // (all tokens, or all that have a weight)
-        bk = BINS;
-      } else {
-        const u64 need = (u64)k - s.found[1];
-        auto there = [&](float x, int) { return bin(r, x) == bk; };
-        listed = gather(s, r, l, there);
-        cut = listed ? list_select<false>(s, r, l, need) : row_select<false>(s, r, need, there);
-        if (by_p) {
-          u64 v = 0;
-          if (listed) {
-#pragma unroll
-            for (int j = 0; j < PER; ++j)
-              if (l.in[j]) {
-                l.in[j] = cut.keeps(l.key[j], l.at[j]);
-                if (l.in[j]) v += weight(r, s.pow2, logit_of(l.key[j]));
-              }
-          } else {
-            walk(r, mine.a, mine.b, [&](const float4& x, int i) {
-              const float* e = (const float*)&x;
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (e[j] > -INFINITY && there(e[j], 0) && cut.keeps(key_of(e[j]), i + j)) v += weight(r, s.pow2, e[j]);
-            });
+          for (int j = 0; j < 4; ++j) {
+            if (above < left && above + v[j] >= left) {
+              s.place[0] = (uint32_t)(255 - 4 * lane() - j);
+              s.found[0] = above;
+            }
+            above += v[j];
           }
-          scan(s, v, rest);
         }
+        __syncthreads();
+        left -= (uint32_t)s.found[0];
+        prefix = prefix << 8 | s.place[0];
+      }
+      m.lo = max(prefix << 16, NONE + 1);
+      m.hi = most_key;
+    } else if (step == 2 && small) {
+      need = (u64)fmax(1.0, ceil((double)fmaxf(p, 0.0f) * (double)rest));
+      look = false;
+      m.within = cut;
+    } else {
+      if (!counted) {
+        counted = true;
+        __syncthreads();
+        for (int b = threadIdx.x; b < BINS; b += THREADS) {
+          s.sum[b] = 0;
+          s.count[b] = 0;
+        }
+        __syncthreads();
+        walk<4>(r, mine.a, mine.b, [&](const float4& v, int) {
+          const float* e = (const float*)&v;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const Octaves o = octaves(r, e[j]);
+            const int b = bin_at(o);
+            const u64 w = weight_at(s.pow2, o);
+            if (by_k && e[j] > -INFINITY) atomicAdd(&s.count[b], 1u);
+            if (by_p && w) atomicAdd(&s.sum[b], w);
+          }
+        });
+        __syncthreads();
+      }
+      // the bin in which the running sum reaches what is needed; by p first the sum itself, of the bins in front of bk
+      constexpr int B = BINS / THREADS;
+      u64 v[B], mine_sum = 0, total;
+#pragma unroll
+      for (int j = 0; j < B; ++j) {
+        const int b = threadIdx.x * B + j;
+        mine_sum += v[j] = step == 1 ? s.count[b] : b < bk ? s.sum[b] : 0;
+      }
+      u64 up = scan(s, mine_sum, total);
+      if (step == 2) need = (u64)fmax(1.0, ceil((double)fmaxf(p, 0.0f) * (double)(total + rest)));
+      if (threadIdx.x == 0) s.place[2] = (uint32_t)BINS;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < B; ++j) {
+        if (up < need && up + v[j] >= need) {
+          s.place[2] = threadIdx.x * B + j;
+          s.found[2] = up;
+        }
+        up += v[j];
+      }
+      __syncthreads();
+      const int b = (int)s.place[2];
+      if (step == 1 && b >= BINS - 1) {   // (all tokens, or all that have a weight)
+        by_k = false;
+        continue;
+      }
+      if (step == 1) bk = b;
+      look = b < BINS;
+      front = look ? s.found[2] : total;   // (else the cut by p lies among what the one by k leaves of its bin)
+      need -= front;
+      if (look) {
+        uint32_t edge[2];   // (where bin b begins, and the one in front of it)
+#pragma unroll 1
+        for (int j = 0; j < 2; ++j) edge[j] = lowest(r, [&](float x) { return bin(r, x) <= b - j; });
+        m.lo = edge[0];
+        m.hi = b ? edge[1] - 1 : most_key;
+        m.within = {NONE, 0x7FFFFFFF};
+      } else {
+        m.within = cut;
       }
     }
-    if (by_p) {
-      const u64 front = sums(bk), need = goal(front + rest);
-      const int bp = need <= front ? reach([&](int b) { return b < bk ? s.sum[b] : 0ull; }, need) : bk;
-      if (bp < bk) {
-        const u64 before = s.found[1];
-        auto there = [&](float x, int) { return bin(r, x) == bp; };
-        cut = gather(s, r, l, there) ? list_select<true>(s, r, l, need - before) : row_select<true>(s, r, need - before, there);
-      } else if (by_k) {   // (the cut by p lies among what the one by k leaves of its bin)
-        const Cut last = cut;
-        cut = listed ? list_select<true>(s, r, l, need - front)
-                     : row_select<true>(s, r, need - front, [&](float x, int i) { return bin(r, x) == bk && last.keeps(key_of(x), i); });
-      }
+    if (look) {
+      added = step == 2 || !by_p;   // (the last cut: what lies above its members is added up on the way)
+      m.listed = pass(s, r, m, added && step > 0, higher({m.hi, -1}, least));
+      added = added && m.listed;
+      if (step == 0 && !m.listed) continue;
     }
+    if (step == 0) {
+      small = added = true;   // (nothing lies above these members)
+      int n = 0;
+      for (int w = 0; w < WAVES; ++w) n += s.number[w];
+      need = min(need, (u64)n);
+    }
+    cut = select(s, r, m, step == 2, need, rest);
   }
 
-  // ---- what is kept, added up in the vocabulary's order; the sixteenth of the row in which the sum passes the draw's, a sixteenth of that, and the
-  // token
+  cut = higher(cut, least);
+  // ---- the sum of what is kept, of each wave's sixteenth of the row: what lies above the members and what is kept of them, or everything
+  if (!added) {
+    m = {1, 0, cut, true};
+    pass(s, r, m, true, cut);
+  }
+  u64 v = s.part[wave()];
+  if (added) {
+    u64 w = 0;
+    each(s, r, m, [&](uint32_t k, int i) {
+      if (k == 0 || !cut.keeps(k, i)) return;
+      const u64 one = weight(r, s.pow2, logit_of(k));
+      w += one;
+    });
+    v += wave_sum(w);
+  }
+  // ---- the sixteenth in which the running sum passes the draw's point, a sixteenth of that, and the token
   auto kept = [&](float x, int i) -> u64 {
     const uint32_t key = key_of(x);
-    if (key <= NONE || !cut.keeps(key, i)) return 0;
-    const u64 w = weight(r, s.pow2, x);
-    return heavy(key, w) ? w : 0;
+    return weight(r, s.pow2, cut.keeps(key, i) ? x : -INFINITY);
   };
   Range all = {0, r.units};
   u64 before = 0, sum = 0;
   double to = 0.0;
   for (int level = 0; level < 2; ++level) {
-    const Range part = share(all, wave());
-    u64 v = 0;
-    walk(r, part.a, part.b, [&](const float4& x, int i) {
-      const float* e = (const float*)&x;
+    if (level == 1) {
+      const Range part = share(all, wave());
+      v = 0;
+      walk<2>(r, part.a, part.b, [&](const float4& x, int i) {
+        const float* e = (const float*)&x;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v += kept(e[j], i + j);
-    });
-    v = wave_sum(v);
+        for (int j = 0; j < 4; ++j) v += kept(e[j], i + j);
+      });
+      v = wave_sum(v);
+    }
     __syncthreads();
-    if (lane() == 0) s.part[wave()] = v;
+    if (lane() == 0) s.kept[wave()] = v;
     __syncthreads();
     if (level == 0) {
-      for (int w = 0; w < WAVES; ++w) sum += s.part[w];
+      for (int w = 0; w < WAVES; ++w) sum += s.kept[w];
       to = target(draw, sum);
     }
     int w = 0;
-    for (; w < WAVES - 1 && !((double)(before + s.part[w]) > to); ++w) before += s.part[w];
+    for (; w < WAVES - 1 && !((double)(before + s.kept[w]) > to); ++w) before += s.kept[w];
     all = share(all, w);
   }
   if (wave() == 0) {
     bool done = false;
-    walk(r, all.a, all.b, [&](const float4& x, int i) {
+    walk<1>(r, all.a, all.b, [&](const float4& x, int i) {
       if (done) return;
       const float* e = (const float*)&x;
       u64 w[4], own_sum = 0;
