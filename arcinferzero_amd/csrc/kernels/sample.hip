@@ -59,7 +59,10 @@ __device__ inline float4 load(const Row& r, int unit) {
   float4 v;
   float* e = (float*)&v;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) e[j] = i + j >= 0 && i + j < r.V ? r.x[i + j] : -INFINITY;
+  for (int j = 0; j < 4; ++j) {
+    e[j] = r.x[min(max(i + j, 0), r.V - 1)];
+    e[j] = (i + j >= 0) & (i + j < r.V) ? e[j] : -INFINITY;
+  }
   return v;
 }
 // A weight's logarithm in 1 / 16 of an octave, down to 60 octaves -- of -inf and of what is no number --, its whole part and the rest of it, within a half.
@@ -160,7 +163,7 @@ __device__ inline Range share(Range all, int w) {
 struct Cut {
   uint32_t key;
   int last;
-  __device__ bool keeps(uint32_t k, int i) const { return k > key || (k == key && i <= last); }
+  __device__ bool keeps(uint32_t k, int i) const { return (k > key) | ((k == key) & (i <= last)); }
 };
 __device__ inline Cut higher(const Cut& a, const Cut& b) { return a.key > b.key || (a.key == b.key && a.last <= b.last) ? a : b; }
 // Tokens of a row whose keys lie in [lo, hi] and that `within` keeps; listed: in LDS.
@@ -168,7 +171,7 @@ struct Members {
   uint32_t lo, hi;
   Cut within;
   bool listed;
-  __device__ bool has(uint32_t k, int i) const { return k >= lo && k <= hi && within.keeps(k, i); }
+  __device__ bool has(uint32_t k, int i) const { return (k >= lo) & (k <= hi) & within.keeps(k, i); }
 };
 // Over the row: its members (of a range; `within` everything) to LDS -- false: there are more than it takes --, and where `add` the weights of those that
 // `floor` keeps added up, each wave's to part[].
@@ -183,13 +186,13 @@ __device__ inline bool pass(Lds& s, const Row& r, const Members& m, bool add, co
     const float* e = (const float*)&v;
     bool some = false;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) some = some || (e[j] >= lo && e[j] <= hi);
+    for (int j = 0; j < 4; ++j) some |= (e[j] >= lo) & (e[j] <= hi);
     if (!__any(some)) return;
     u64 vote[4];
     int front = have;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      vote[j] = __ballot(e[j] >= lo && e[j] <= hi);
+      vote[j] = __ballot((e[j] >= lo) & (e[j] <= hi));
       front += __builtin_amdgcn_mbcnt_hi((uint32_t)(vote[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)vote[j], 0));
       have += __popcll(vote[j]);
     }
@@ -211,7 +214,7 @@ __device__ inline bool pass(Lds& s, const Row& r, const Members& m, bool add, co
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         // (what is not kept as -inf: of weight 0)
-        sum += weight(r, s.pow2, e[j] > edge || (e[j] == edge && i + j <= floor.last) ? e[j] : -INFINITY);
+        sum += weight(r, s.pow2, (e[j] > edge) | ((e[j] == edge) & (i + j <= floor.last)) ? e[j] : -INFINITY);
       }
       if (any) members(v, i);
     });
