@@ -22,10 +22,13 @@
 
 namespace {
 typedef unsigned long long u64;
-constexpr int THREADS = 1024, WAVES = 16, CAP = 512, SMALL_K = 512, FEW = 512, BINS = 3072;   // (48 octaves)
+constexpr int THREADS = 1024, WAVES = 16, LIST = 512, SMALL_K = 512, FEW = 512, BINS = 3072;   // (48 octaves)
 constexpr uint32_t NONE = 0x007FFFFFu;                                             // the key of -inf: no token
 
-struct Lds {
+// CAP: tokens of a wave that the list takes.
+template <int CAP_>
+struct LdsOf {
+  static constexpr int CAP = CAP_;
   double pow2[16];   // 2^(43 + j / 16)
   u64 sum[BINS];
   uint32_t count[BINS];
@@ -40,6 +43,7 @@ struct Lds {
   u64 found[3];
   uint32_t place[3];
 };
+typedef LdsOf<LIST> Lds;
 
 // Logits in their order as whole numbers; -0 is 0, and what is no number is -inf.
 __device__ inline uint32_t key_of(float x) {
@@ -117,7 +121,8 @@ __device__ inline u64 wave_sum(u64 v) {
   return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 // The sum over the threads in front of this one, and of all.
-__device__ inline u64 scan(Lds& s, u64 v, u64& total) {
+template <class S>
+__device__ inline u64 scan(S& s, u64 v, u64& total) {
   const u64 up = up_sum(v);
   __syncthreads();
   if (lane() == 63) s.part[wave()] = up;
@@ -173,10 +178,12 @@ struct Members {
   bool listed;
   __device__ bool has(uint32_t k, int i) const { return (k >= lo) & (k <= hi) & within.keeps(k, i); }
 };
-// Over the row: its members (of a range; `within` everything) to LDS -- false: there are more than it takes --, and where `add` the weights of those that
+// Over units of the row: its members (of a range; `within` everything) to LDS -- false: there are more than it takes --, and where `add` the weights of those that
 // `floor` keeps added up, each wave's to part[].
-__device__ inline bool pass(Lds& s, const Row& r, const Members& m, bool add, const Cut& floor) {
-  const Range mine = share({0, r.units}, wave());
+template <class S>
+__device__ inline bool pass(S& s, const Row& r, const Range& all, const Members& m, bool add, const Cut& floor) {
+  constexpr int CAP = S::CAP;
+  const Range mine = share(all, wave());
   const bool any = m.lo <= m.hi;
   const float lo = any ? logit_of(m.lo) : INFINITY, hi = any ? logit_of(m.hi) : -INFINITY, edge = logit_of(floor.key);
   int have = 0;
@@ -237,8 +244,8 @@ __device__ inline void each(Lds& s, const Row& r, const Members& m, G g) {
     const int n = s.number[wave()];
     for (int p0 = 0; p0 < n; p0 += 64) {
       const int p = min(p0 + lane(), n - 1);
-      const uint32_t k = s.key[wave() * CAP + p];
-      const int i = s.at[wave() * CAP + p];
+      const uint32_t k = s.key[wave() * LIST + p];
+      const int i = s.at[wave() * LIST + p];
       g(p0 + lane() < n && m.has(k, i) ? k : 0u, i);
     }
     return;
@@ -272,8 +279,8 @@ __device__ inline Cut select(Lds& s, const Row& r, const Members& m, bool by_wei
     // Few: one wave has them in its registers, and goes down the bits of their keys.
     constexpr int N = FEW / 64;
     for (int p = lane(); p < s.number[wave()]; p += 64) {
-      const uint32_t k = s.key[wave() * CAP + p];
-      const int i = s.at[wave() * CAP + p];
+      const uint32_t k = s.key[wave() * LIST + p];
+      const int i = s.at[wave() * LIST + p];
       s.few_key[run + p] = m.has(k, i) ? k : 0;
       s.few_at[run + p] = i;
     }
@@ -449,179 +456,237 @@ __device__ inline double target(float u, u64 sum) {
   const double all = (double)sum, below = __longlong_as_double(__double_as_longlong(all) - 1);
   return fmin(u > 0.0f ? (double)u * all : 0.0, below);
 }
-}  // namespace
 
-// temp, top_k, top_p, min_p: of each row, or none.  grid T, 1024.
-extern "C" __global__ __launch_bounds__(1024) void sample(const float* __restrict__ logits, int ld, int off, int V, const float* __restrict__ temp,
-                                                          const int* __restrict__ top_k, const float* __restrict__ top_p, const float* __restrict__ min_p,
-                                                          const float* __restrict__ u, int* __restrict__ token, float* __restrict__ prob) {
-  __shared__ Lds s;
-  const int row = blockIdx.x;
+// What a row is drawn by.
+struct Form {
+  float t, draw, q, p;
+  int k;
+  __device__ bool by_k(int V) const { return k > 0 && k < V; }
+  __device__ bool by_p() const { return p < 1.0f; }
+  __device__ u64 goal(u64 sum) const { return (u64)fmax(1.0, ceil((double)fmaxf(p, 0.0f) * (double)sum)); }
+};
+#define SAMPLE_ARGS                                                                                                                                     \
+  const float *__restrict__ logits, int ld, int off, int V, const float *__restrict__ temp, const int *__restrict__ top_k,                              \
+      const float *__restrict__ top_p, const float *__restrict__ min_p, const float *__restrict__ u, int *__restrict__ token, float *__restrict__ prob
+__device__ inline Row row_of(const float* logits, int ld, int off, int V, int row) {
   Row r;
   r.x = logits + (size_t)row * ld + off;
   r.V = V;
   r.skew = (int)((uintptr_t)r.x >> 2 & 3);
   r.units = (V + r.skew + 3) / 4;
-  const float t = temp ? temp[row] : 1.0f, draw = u[row], q = min_p ? min_p[row] : 0.0f, p = top_p ? top_p[row] : 1.0f;
-  const int k = top_k ? top_k[row] : 0;
-  auto answer = [&](int i, float pr) {
-    token[row] = i;
-    if (prob) prob[row] = pr;
-  };
-
-  // ---- the largest logit, and where
-  const Range mine = share({0, r.units}, wave());
-  float top = -INFINITY;
-  int where = 0x7FFFFFFF;
+  r.most = r.scale = 0.0;
+  return r;
+}
+__device__ inline Form form_of(const float* temp, const int* top_k, const float* top_p, const float* min_p, const float* u, int row) {
+  return {temp ? temp[row] : 1.0f, u[row], min_p ? min_p[row] : 0.0f, top_p ? top_p[row] : 1.0f, top_k ? top_k[row] : 0};
+}
+__device__ inline void measure(Row& r, float top, float t) {
+  r.most = top == INFINITY ? 1e300 : (double)top;
+  r.scale = fmax(23.083120654223414 / (double)t, top == INFINITY ? 1e-200 : 0.0);   // 16 log2(e) / t
+}
+__device__ inline void first_of(float& top, int& where, float a, int b) {
+  if (a > top || (a == top && b < where)) { top = a; where = b; }
+}
+// The largest logit of some units and its first place, for all threads; own: this thread's.
+template <class S>
+__device__ inline void find_top(S& s, const Row& r, const Range& all, float& top, int& where, float& own) {
+  const Range mine = share(all, wave());
+  top = -INFINITY;
+  where = 0x7FFFFFFF;
   walk<8>(r, mine.a, mine.b, [&](const float4& v, int i) {
     const float* e = (const float*)&v;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (e[j] > top) { top = e[j]; where = i + j; }
   });
-  const float own = top;   // (this thread's)
+  own = top;
 #pragma unroll
-  for (int o = 32; o; o /= 2) {
-    const float a = __shfl_xor(top, o);
-    const int b = __shfl_xor(where, o);
-    if (a > top || (a == top && b < where)) { top = a; where = b; }
-  }
+  for (int o = 32; o; o /= 2) first_of(top, where, __shfl_xor(top, o), __shfl_xor(where, o));
   if (lane() == 0) { s.top[wave()] = top; s.where[wave()] = where; }
-  if (threadIdx.x < 16) s.pow2[threadIdx.x] = exp2(43.0 + threadIdx.x / 16.0);
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    const float a = s.top[w];
-    const int b = s.where[w];
-    if (a > top || (a == top && b < where)) { top = a; where = b; }
+  for (int w = 0; w < WAVES; ++w) first_of(top, where, s.top[w], s.where[w]);
+}
+template <class S>
+__device__ inline void powers(S& s) {
+  if (threadIdx.x < 16) s.pow2[threadIdx.x] = exp2(43.0 + threadIdx.x / 16.0);
+}
+// A key that at least k tokens reach, out of the threads' largest logits: two digits of the k-th of them.
+template <class S>
+__device__ inline uint32_t reached(S& s, float own, int k) {
+  const uint32_t key = key_of(own);
+  uint32_t prefix = 0, left = (uint32_t)k;
+#pragma unroll 1
+  for (int shift = 24; shift >= 16; shift -= 8) {
+    __syncthreads();
+    if (threadIdx.x < 256) s.digit[threadIdx.x] = 0;
+    __syncthreads();
+    if (shift == 24 || key >> 24 == prefix) atomicAdd(&s.digit[key >> shift & 255], 1u);
+    __syncthreads();
+    if (wave() == 0) {
+      uint32_t v[4], sum = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum += v[j] = s.digit[255 - 4 * lane() - j];
+      uint32_t above = up_sum(sum) - sum;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (above < left && above + v[j] >= left) {
+          s.place[0] = (uint32_t)(255 - 4 * lane() - j);
+          s.found[0] = above;
+        }
+        above += v[j];
+      }
+    }
+    __syncthreads();
+    left -= (uint32_t)s.found[0];
+    prefix = prefix << 8 | s.place[0];
   }
-  if (!(top > -INFINITY)) {   // (nothing can be drawn)
-    if (threadIdx.x == 0) answer(-1, 0.0f);
+  __syncthreads();
+  return max(prefix << 16, NONE + 1);
+}
+// Counts and sums of weights of some units by bins.
+template <class S>
+__device__ inline void histogram(S& s, const Row& r, const Range& all, bool by_k, bool by_p) {
+  __syncthreads();
+  for (int b = threadIdx.x; b < BINS; b += THREADS) {
+    s.sum[b] = 0;
+    s.count[b] = 0;
+  }
+  __syncthreads();
+  const Range mine = share(all, wave());
+  walk<4>(r, mine.a, mine.b, [&](const float4& v, int) {
+    const float* e = (const float*)&v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const Octaves o = octaves(r, e[j]);
+      const int b = bin_at(o);
+      const u64 w = weight_at(s.pow2, o);
+      if (by_k && e[j] > -INFINITY) atomicAdd(&s.count[b], 1u);
+      if (by_p && w) atomicAdd(&s.sum[b], w);
+    }
+  });
+  __syncthreads();
+}
+// The bin in which the running sum of counts, or of the weights of the bins in front of bk (where they and `rest` make p of their sum), reaches what is
+// needed -- BINS: none --; need: what is left of that behind `front`, the sum in front of it.
+template <class S>
+__device__ inline int reach(S& s, const Form& f, bool by_weight, int bk, u64 rest, u64& need, u64& front) {
+  constexpr int B = BINS / THREADS;
+  u64 v[B], mine_sum = 0, total;
+#pragma unroll
+  for (int j = 0; j < B; ++j) {
+    const int b = threadIdx.x * B + j;
+    mine_sum += v[j] = !by_weight ? s.count[b] : b < bk ? s.sum[b] : 0;
+  }
+  u64 up = scan(s, mine_sum, total);
+  need = by_weight ? f.goal(total + rest) : (u64)f.k;
+  if (threadIdx.x == 0) s.place[2] = (uint32_t)BINS;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < B; ++j) {
+    if (up < need && up + v[j] >= need) {
+      s.place[2] = threadIdx.x * B + j;
+      s.found[2] = up;
+    }
+    up += v[j];
+  }
+  __syncthreads();
+  const int b = (int)s.place[2];
+  front = b < BINS ? s.found[2] : total;
+  need -= min(need, front);
+  return b;
+}
+// The members of bin b.
+__device__ inline Members members_of(const Row& r, int b, uint32_t most_key) {
+  uint32_t edge[2];   // (where the bin begins, and the one in front of it)
+#pragma unroll 1
+  for (int j = 0; j < 2; ++j) edge[j] = lowest(r, [&](float x) { return bin(r, x) <= b - j; });
+  return {edge[0], b ? edge[1] - 1 : most_key, {NONE, 0x7FFFFFFF}, true};
+}
+// min_p as a cut: the lowest logit whose weight is no less than q of the largest's, 2^43.
+template <class S>
+__device__ inline Cut least_of(S& s, const Row& r, float q) {
+  const u64 fewest = (u64)ceil((double)fminf(fmaxf(q, 0.0f), 1.0f) * 8796093022208.0);   // (a NaN is 0)
+  return {fewest ? lowest(r, [&](float x) { return weight(r, s.pow2, x) >= fewest; }) : NONE, 0x7FFFFFFF};
+}
+// One wave finds the token in some units: `before` is the sum in front of them.
+template <class S>
+__device__ inline void find(S& s, const Row& r, const Range& all, const Cut& cut, u64 before, u64 sum, double to, int* token, float* prob) {
+  bool done = false;
+  walk<1>(r, all.a, all.b, [&](const float4& x, int i) {
+    if (done) return;
+    const float* e = (const float*)&x;
+    u64 w[4], own_sum = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) own_sum += w[j] = weight(r, s.pow2, cut.keeps(key_of(e[j]), i + j) ? e[j] : -INFINITY);
+    const u64 up = up_sum(own_sum);
+    u64 at = before + up - own_sum;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (w[j] && (double)at <= to && (double)(at + w[j]) > to) {
+        *token = i + j;
+        if (prob) *prob = (float)((double)w[j] / (double)sum);
+      }
+      at += w[j];
+    }
+    before += __shfl(up, 63);
+    done = (double)before > to;
+  });
+}
+// A row by one work-group.
+__device__ inline void one_row(Lds& s, Row r, const Form& f, int* token, float* prob) {
+  const Range whole = {0, r.units};
+  float top, own;
+  int where;
+  powers(s);
+  find_top(s, r, whole, top, where, own);
+  if (!(top > -INFINITY) || !(f.t > 0.0f)) {   // (nothing can be drawn; greedy)
+    if (threadIdx.x == 0) {
+      *token = top > -INFINITY ? where : -1;
+      if (prob) *prob = top > -INFINITY ? 1.0f : 0.0f;
+    }
     return;
   }
-  if (!(t > 0.0f)) {
-    if (threadIdx.x == 0) answer(where, 1.0f);
-    return;
-  }
-  r.most = top == INFINITY ? 1e300 : (double)top;
-  r.scale = fmax(23.083120654223414 / (double)t, top == INFINITY ? 1e-200 : 0.0);   // 16 log2(e) / t
+  measure(r, top, f.t);
   const uint32_t most_key = key_of(top);
-  // (min_p is a cut like the others: the lowest logit whose weight is no less than q of the largest's, 2^43; a NaN is 0)
-  const u64 fewest = (u64)ceil((double)fminf(fmaxf(q, 0.0f), 1.0f) * 8796093022208.0);
-  const Cut least = {fewest ? lowest(r, [&](float x) { return weight(r, s.pow2, x) >= fewest; }) : NONE, 0x7FFFFFFF};
+  const Cut least = least_of(s, r, f.q);
 
   // ---- the cuts, one within the other: by k out of a list of few (step 0) or out of the histogram (1), by p (2)
-  const bool by_p = p < 1.0f;
-  bool by_k = k > 0 && k < V, small = false, counted = false, added = false;
+  const bool by_p = f.by_p();
+  bool by_k = f.by_k(r.V), small = false, counted = false, added = false;
   Cut cut = {NONE, 0x7FFFFFFF};
   Members m = {1, 0, cut, true};
   u64 front = 0, rest = 0;   // the weights in front of the members, and of those of them that the cut by k keeps
   int bk = BINS;             // the bin of the cut by k
+#pragma unroll 1
   for (int step = 0; step < 3; ++step) {
     if (step == 2 ? !by_p : !by_k || small) continue;
-    if (step == 0 && k > SMALL_K) continue;
-    u64 need = (u64)k;
+    if (step == 0 && f.k > SMALL_K) continue;
+    u64 need = (u64)f.k;
     bool look = true;   // (other members than the list has)
     if (step == 0) {
-      // two digits of the k-th of the threads' largest logits: at least k tokens reach them
-      const uint32_t key = key_of(own);
-      uint32_t prefix = 0, left = (uint32_t)k;
-      for (int shift = 24; shift >= 16; shift -= 8) {
-        __syncthreads();
-        if (threadIdx.x < 256) s.digit[threadIdx.x] = 0;
-        __syncthreads();
-        if (shift == 24 || key >> 24 == prefix) atomicAdd(&s.digit[key >> shift & 255], 1u);
-        __syncthreads();
-        if (wave() == 0) {
-          uint32_t v[4], sum = 0;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) sum += v[j] = s.digit[255 - 4 * lane() - j];
-          uint32_t above = up_sum(sum) - sum;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (above < left && above + v[j] >= left) {
-              s.place[0] = (uint32_t)(255 - 4 * lane() - j);
-              s.found[0] = above;
-            }
-            above += v[j];
-          }
-        }
-        __syncthreads();
-        left -= (uint32_t)s.found[0];
-        prefix = prefix << 8 | s.place[0];
-      }
-      m.lo = max(prefix << 16, NONE + 1);
+      m.lo = reached(s, own, f.k);
       m.hi = most_key;
     } else if (step == 2 && small) {
-      need = (u64)fmax(1.0, ceil((double)fmaxf(p, 0.0f) * (double)rest));
+      need = f.goal(rest);
       look = false;
       m.within = cut;
     } else {
-      if (!counted) {
-        counted = true;
-        __syncthreads();
-        for (int b = threadIdx.x; b < BINS; b += THREADS) {
-          s.sum[b] = 0;
-          s.count[b] = 0;
-        }
-        __syncthreads();
-        walk<4>(r, mine.a, mine.b, [&](const float4& v, int) {
-          const float* e = (const float*)&v;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const Octaves o = octaves(r, e[j]);
-            const int b = bin_at(o);
-            const u64 w = weight_at(s.pow2, o);
-            if (by_k && e[j] > -INFINITY) atomicAdd(&s.count[b], 1u);
-            if (by_p && w) atomicAdd(&s.sum[b], w);
-          }
-        });
-        __syncthreads();
-      }
-      // the bin in which the running sum reaches what is needed; by p first the sum itself, of the bins in front of bk
-      constexpr int B = BINS / THREADS;
-      u64 v[B], mine_sum = 0, total;
-#pragma unroll
-      for (int j = 0; j < B; ++j) {
-        const int b = threadIdx.x * B + j;
-        mine_sum += v[j] = step == 1 ? s.count[b] : b < bk ? s.sum[b] : 0;
-      }
-      u64 up = scan(s, mine_sum, total);
-      if (step == 2) need = (u64)fmax(1.0, ceil((double)fmaxf(p, 0.0f) * (double)(total + rest)));
-      if (threadIdx.x == 0) s.place[2] = (uint32_t)BINS;
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < B; ++j) {
-        if (up < need && up + v[j] >= need) {
-          s.place[2] = threadIdx.x * B + j;
-          s.found[2] = up;
-        }
-        up += v[j];
-      }
-      __syncthreads();
-      const int b = (int)s.place[2];
+      if (!counted) histogram(s, r, whole, by_k, by_p);
+      counted = true;
+      const int b = reach(s, f, step == 2, bk, rest, need, front);
       if (step == 1 && b >= BINS - 1) {   // (all tokens, or all that have a weight)
         by_k = false;
         continue;
       }
       if (step == 1) bk = b;
       look = b < BINS;
-      front = look ? s.found[2] : total;   // (else the cut by p lies among what the one by k leaves of its bin)
-      need -= front;
-      if (look) {
-        uint32_t edge[2];   // (where bin b begins, and the one in front of it)
-#pragma unroll 1
-        for (int j = 0; j < 2; ++j) edge[j] = lowest(r, [&](float x) { return bin(r, x) <= b - j; });
-        m.lo = edge[0];
-        m.hi = b ? edge[1] - 1 : most_key;
-        m.within = {NONE, 0x7FFFFFFF};
-      } else {
-        m.within = cut;
-      }
+      if (look) m = members_of(r, b, most_key);
+      else m.within = cut;   // (the cut by p lies among what the one by k leaves of its bin)
     }
     if (look) {
       added = step == 2 || !by_p;   // (the last cut: what lies above its members is added up on the way)
-      m.listed = pass(s, r, m, added && step > 0, higher({m.hi, -1}, least));
+      m.listed = pass(s, r, whole, m, added && step > 0, higher({m.hi, -1}, least));
       added = added && m.listed;
       if (step == 0 && !m.listed) continue;
     }
@@ -638,26 +703,22 @@ extern "C" __global__ __launch_bounds__(1024) void sample(const float* __restric
   // ---- the sum of what is kept, of each wave's sixteenth of the row: what lies above the members and what is kept of them, or everything
   if (!added) {
     m = {1, 0, cut, true};
-    pass(s, r, m, true, cut);
+    pass(s, r, whole, m, true, cut);
   }
   u64 v = s.part[wave()];
   if (added) {
     u64 w = 0;
     each(s, r, m, [&](uint32_t k, int i) {
       if (k == 0 || !cut.keeps(k, i)) return;
-      const u64 one = weight(r, s.pow2, logit_of(k));
-      w += one;
+      w += weight(r, s.pow2, logit_of(k));
     });
     v += wave_sum(w);
   }
   // ---- the sixteenth in which the running sum passes the draw's point, a sixteenth of that, and the token
-  auto kept = [&](float x, int i) -> u64 {
-    const uint32_t key = key_of(x);
-    return weight(r, s.pow2, cut.keeps(key, i) ? x : -INFINITY);
-  };
-  Range all = {0, r.units};
+  Range all = whole;
   u64 before = 0, sum = 0;
   double to = 0.0;
+#pragma unroll 1
   for (int level = 0; level < 2; ++level) {
     if (level == 1) {
       const Range part = share(all, wave());
@@ -665,7 +726,7 @@ extern "C" __global__ __launch_bounds__(1024) void sample(const float* __restric
       walk<2>(r, part.a, part.b, [&](const float4& x, int i) {
         const float* e = (const float*)&x;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v += kept(e[j], i + j);
+        for (int j = 0; j < 4; ++j) v += weight(r, s.pow2, cut.keeps(key_of(e[j]), i + j) ? e[j] : -INFINITY);
       });
       v = wave_sum(v);
     }
@@ -674,29 +735,19 @@ extern "C" __global__ __launch_bounds__(1024) void sample(const float* __restric
     __syncthreads();
     if (level == 0) {
       for (int w = 0; w < WAVES; ++w) sum += s.kept[w];
-      to = target(draw, sum);
+      to = target(f.draw, sum);
     }
     int w = 0;
     for (; w < WAVES - 1 && !((double)(before + s.kept[w]) > to); ++w) before += s.kept[w];
     all = share(all, w);
   }
-  if (wave() == 0) {
-    bool done = false;
-    walk<1>(r, all.a, all.b, [&](const float4& x, int i) {
-      if (done) return;
-      const float* e = (const float*)&x;
-      u64 w[4], own_sum = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) own_sum += w[j] = kept(e[j], i + j);
-      const u64 up = up_sum(own_sum);
-      u64 at = before + up - own_sum;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (w[j] && (double)at <= to && (double)(at + w[j]) > to) answer(i + j, (float)((double)w[j] / (double)sum));
-        at += w[j];
-      }
-      before += __shfl(up, 63);
-      done = (double)before > to;
-    });
-  }
+  if (wave() == 0) find(s, r, all, cut, before, sum, to, token, prob);
+}
+}  // namespace
+
+// temp, top_k, top_p, min_p: of each row, or none.  grid T, 1024.
+extern "C" __global__ __launch_bounds__(1024) void sample(SAMPLE_ARGS) {
+  __shared__ Lds s;
+  const int row = blockIdx.x;
+  one_row(s, row_of(logits, ld, off, V, row), form_of(temp, top_k, top_p, min_p, u, row), token + row, prob ? prob + row : nullptr);
 }
