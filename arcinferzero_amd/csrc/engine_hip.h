@@ -92,6 +92,7 @@ class Engine {
     moe_fuse_off_ = getenv("ARCZ_MOE_FUSE") && atoi(getenv("ARCZ_MOE_FUSE")) == 0;
     moe_qfuse_off_ = getenv("ARCZ_MOE_QFUSE") && atoi(getenv("ARCZ_MOE_QFUSE")) == 0;
     attn_shared_ = getenv("ARCZ_ATTN_SHARED") ? atoi(getenv("ARCZ_ATTN_SHARED")) : -1;
+    sample_split_ = getenv("ARCZ_SAMPLE_SPLIT") ? atoi(getenv("ARCZ_SAMPLE_SPLIT")) : -1;
     moe_digits_ = getenv("ARCZ_MOE_DIGITS") ? atoi(getenv("ARCZ_MOE_DIGITS")) : 1;
     moe_pre_ = getenv("ARCZ_MOE_PRE") ? atoi(getenv("ARCZ_MOE_PRE")) != 0 : true;
     q4_wm_ = getenv("ARCZ_Q4_WM") ? atoi(getenv("ARCZ_Q4_WM")) : 0;

@@ -1,5 +1,13 @@
 // A token from each row of logits (kernels/sample.hip).  A part of class Engine (included in it, behind engine_attn.h).
 
+  // Sixteen work-groups a row, in four launches, for few long rows (sample.hip's Place, 108760 bytes of the attention's room, for each).  Measured, us, one
+  // work-group a row / sixteen, with a temperature, k = 50 and p, p alone, and rows of all kinds: 16 x 16384 15 39 30 29 / 19 42 37 43;
+  // 16 x 32001 20 41 46 37 / 19 43 45 42; 16 x 65536 29 45 64 55 / 19 43 44 44; 32 x 65536 29 45 65 56 / 24 48 61 57; 1 x 151936 54 43 106 55 / 19 31 35 21;
+  // 48 x 151936 58 59 125 113 / 37 58 93 70; 96 x 151936 61 61 130 123 / 60 79 158 103.  (Rows whose largest logit is all that is asked for: 13 / 14 and, 48 of
+  // them, 14 / 21; a cut by p behind one of 2000 tokens, which one work-group does behind the others' launches: 122 / 134.  A row's kind is known on the device only.)
+  int sample_split_ = -1;   // ARCZ_SAMPLE_SPLIT
+  static constexpr int SPLIT_ROWS = 96;
+  bool split_pays(int V, int T) const { return V >= 2500 * std::max(T, 16); }
   struct Sampling {
     cl_mem temperature, top_k, top_p, min_p;
   };
@@ -20,6 +28,17 @@
     for (const Place& o : out)
       for (const Place& i : in)
         if (overlap(o, i)) throw std::runtime_error("sample: token or prob overlaps what is read");
+    if (T <= SPLIT_ROWS && (sample_split_ < 0 ? split_pays(V, T) : sample_split_)) {
+      at_room();
+      for (const char* step : {"sample_top", "sample_scan", "sample_cut", "sample_draw"}) {
+        cl_kernel k = variant("ops", {}, step);
+        set_args(k, 0, logits, ld, off, V, f.temperature, f.top_k, f.top_p, f.min_p, u, token, prob, at_ws_);
+        const bool last = step[7] == 'd';
+        size_t g[2] = {last ? n * 1024 : 16 * 1024, last ? 1 : n}, l[2] = {1024, 1};
+        run(step, k, 2, g, l);
+      }
+      return;
+    }
     cl_kernel k = variant("ops", {}, "sample");
     set_args(k, 0, logits, ld, off, V, f.temperature, f.top_k, f.top_p, f.min_p, u, token, prob);
     size_t g = n * 1024, l = 1024;

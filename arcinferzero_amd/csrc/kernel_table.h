@@ -36,6 +36,10 @@ static const KernelSpec kKernelTable[] = {
     {"ops", "asc_expand", nullptr, "ppii", {nullptr}, {{nullptr, 0, false}}, 256},
     {"ops", "softcap_rows", nullptr, "piiif", {nullptr}, {{nullptr, 0, false}}, 0},
     {"ops", "sample", nullptr, "piiippppppp", {nullptr}, {{nullptr, 0, false}}, 1024},
+    {"ops", "sample_top", nullptr, "piiipppppppp", {nullptr}, {{nullptr, 0, false}}, 1024},
+    {"ops", "sample_scan", nullptr, "piiipppppppp", {nullptr}, {{nullptr, 0, false}}, 1024},
+    {"ops", "sample_cut", nullptr, "piiipppppppp", {nullptr}, {{nullptr, 0, false}}, 1024},
+    {"ops", "sample_draw", nullptr, "piiipppppppp", {nullptr}, {{nullptr, 0, false}}, 1024},
     {"ops", "fill32", nullptr, "piz", {nullptr}, {{nullptr, 0, false}}, 256},
     {"ops", "copy128", nullptr, "ppz", {nullptr}, {{nullptr, 0, false}}, 256},
     {"ops", "read_probe", nullptr, "pzp", {nullptr}, {{nullptr, 0, false}}, 256},

@@ -22,7 +22,7 @@
 
 namespace {
 typedef unsigned long long u64;
-constexpr int THREADS = 1024, WAVES = 16, LIST = 512, SMALL_K = 512, FEW = 512, BINS = 3072;   // (48 octaves)
+constexpr int THREADS = 1024, WAVES = 16, LIST = 512, SMALL_K = 512, FEW = 512, BINS = 3 * THREADS;   // (48 octaves)
 constexpr uint32_t NONE = 0x007FFFFFu;                                             // the key of -inf: no token
 
 // CAP: tokens of a wave that the list takes.
@@ -750,4 +750,228 @@ extern "C" __global__ __launch_bounds__(1024) void sample(SAMPLE_ARGS) {
   __shared__ Lds s;
   const int row = blockIdx.x;
   one_row(s, row_of(logits, ld, off, V, row), form_of(temp, top_k, top_p, min_p, u, row), token + row, prob ? prob + row : nullptr);
+}
+
+// ---- few rows: sixteen work-groups a row, in four launches -- the largest logits; what the cuts ask for of each work-group's sixteenth (the few
+// highest, a histogram, or the sums where nothing is cut); the tokens of the bin with the cut, and the sums above it; the token.
+namespace {
+constexpr int PARTS = 16, RUN = LIST;   // (tokens of a work-group that the row's list takes)
+enum Mode { ANSWERED, SMALL, BINNED, LISTED, SUMS, WHOLE };
+struct Place {   // a row's in the room (arcinferzero_amd/csrc/engine_sample.h has its size)
+  u64 sum[BINS];
+  uint32_t count[BINS];
+  u64 part[PARTS * WAVES];   // sums of weights, by sixteenths of sixteenths
+  float top[PARTS];
+  int where[PARTS];
+  float most[THREADS];       // the largest of each sixteen threads
+  int number[PARTS];         // tokens in each run of the list (-1: more than it takes)
+  uint32_t lo, hi;
+  int mode, then;
+  u64 need;
+  uint32_t key[PARTS * RUN], at[PARTS * RUN];
+};
+static_assert(sizeof(Place) == 108760, "engine_sample.h");
+typedef LdsOf<128> LdsPart;
+
+// The row's largest logit, out of its parts'; false: nothing is to be drawn by weight.
+__device__ inline bool known(Row& r, const Place& g, const Form& f, float& top, int& where) {
+  top = -INFINITY;
+  where = 0x7FFFFFFF;
+  for (int i = 0; i < PARTS; ++i) first_of(top, where, g.top[i], g.where[i]);
+  if (!(top > -INFINITY) || !(f.t > 0.0f)) return false;
+  measure(r, top, f.t);
+  return true;
+}
+// A work-group's list as its run of the row's.
+__device__ inline void publish(const LdsPart& s, Place& g, int part, bool fits) {
+  int front = 0, all = 0;
+  for (int w = 0; w < WAVES; ++w) {
+    front = w == wave() ? all : front;
+    all += s.number[w];
+  }
+  fits = fits && all <= RUN;
+  if (threadIdx.x == 0) g.number[part] = fits ? all : -1;
+  if (!fits) return;
+  for (int p = lane(); p < s.number[wave()]; p += 64) {
+    g.key[part * RUN + front + p] = s.key[wave() * LdsPart::CAP + p];
+    g.at[part * RUN + front + p] = s.at[wave() * LdsPart::CAP + p];
+  }
+}
+}  // namespace
+
+extern "C" __global__ __launch_bounds__(1024) void sample_top(SAMPLE_ARGS, char* __restrict__ room) {
+  __shared__ LdsPart s;
+  const int part = blockIdx.x, row = blockIdx.y;
+  Place& g = ((Place*)room)[row];
+  const Row r = row_of(logits, ld, off, V, row);
+  float top, own;
+  int where;
+  find_top(s, r, share({0, r.units}, part), top, where, own);
+#pragma unroll
+  for (int o = 1; o < PARTS; o *= 2) own = fmaxf(own, __shfl_xor(own, o));
+  if (threadIdx.x % PARTS == 0) g.most[part * (THREADS / PARTS) + threadIdx.x / PARTS] = own;
+  if (threadIdx.x == 0) { g.top[part] = top; g.where[part] = where; }
+  for (int b = part * (BINS / PARTS) + threadIdx.x; b < (part + 1) * (BINS / PARTS); b += THREADS) {
+    g.sum[b] = 0;
+    g.count[b] = 0;
+  }
+}
+
+extern "C" __global__ __launch_bounds__(1024) void sample_scan(SAMPLE_ARGS, char* __restrict__ room) {
+  __shared__ LdsPart s;
+  const int part = blockIdx.x, row = blockIdx.y;
+  Place& g = ((Place*)room)[row];
+  Row r = row_of(logits, ld, off, V, row);
+  const Form f = form_of(temp, top_k, top_p, min_p, u, row);
+  const Range mine = share({0, r.units}, part);
+  const bool first = part == 0 && threadIdx.x == 0, by_k = f.by_k(V), by_p = f.by_p();
+  float top;
+  int where;
+  if (!known(r, g, f, top, where)) {
+    if (first) {
+      token[row] = top > -INFINITY ? where : -1;
+      if (prob) prob[row] = top > -INFINITY ? 1.0f : 0.0f;
+      g.mode = ANSWERED;
+    }
+    return;
+  }
+  powers(s);
+  __syncthreads();
+  if (by_k && f.k <= SMALL_K) {
+    const Members m = {reached(s, g.most[threadIdx.x], f.k), key_of(top), {NONE, 0x7FFFFFFF}, true};
+    if (first) {
+      g.lo = m.lo;
+      g.hi = m.hi;
+      g.mode = SMALL;
+    }
+    publish(s, g, part, pass(s, r, mine, m, false, m.within));
+  } else if (by_k && by_p) {
+    if (first) g.mode = WHOLE;   // (the cut by p needs the one by k first: by one work-group)
+  } else if (by_k || by_p) {
+    if (first) g.mode = BINNED;
+    histogram(s, r, mine, by_k, by_p);
+    for (int b = threadIdx.x; b < BINS; b += THREADS) {   // (whole numbers: in any order)
+      if (s.sum[b]) atomicAdd(&g.sum[b], s.sum[b]);
+      if (s.count[b]) atomicAdd(&g.count[b], s.count[b]);
+    }
+  } else {
+    if (first) g.mode = SUMS;
+    const Cut least = least_of(s, r, f.q);
+    pass(s, r, mine, {1, 0, least, true}, true, least);
+    if (threadIdx.x < WAVES) g.part[part * WAVES + threadIdx.x] = s.part[threadIdx.x];
+  }
+}
+
+extern "C" __global__ __launch_bounds__(1024) void sample_cut(SAMPLE_ARGS, char* __restrict__ room) {
+  __shared__ LdsPart s;
+  const int part = blockIdx.x, row = blockIdx.y;
+  Place& g = ((Place*)room)[row];
+  if (g.mode != BINNED) return;
+  Row r = row_of(logits, ld, off, V, row);
+  const Form f = form_of(temp, top_k, top_p, min_p, u, row);
+  const bool first = part == 0 && threadIdx.x == 0, by_p = f.by_p();
+  float top;
+  int where;
+  if (!known(r, g, f, top, where)) return;
+  powers(s);
+  for (int b = threadIdx.x; b < BINS; b += THREADS) {
+    s.sum[b] = g.sum[b];
+    s.count[b] = g.count[b];
+  }
+  __syncthreads();
+  u64 need, front;
+  const int b = reach(s, f, by_p, BINS, 0, need, front);
+  const Cut least = least_of(s, r, f.q);
+  const bool all = !by_p && b >= BINS - 1;   // (all tokens are kept, or all that have a weight)
+  const Members m = all ? Members{1, 0, least, true} : members_of(r, b, key_of(top));
+  const bool fits = pass(s, r, share({0, r.units}, part), m, true, all ? least : higher({m.hi, -1}, least));
+  if (threadIdx.x < WAVES) g.part[part * WAVES + threadIdx.x] = s.part[threadIdx.x];
+  if (first) {
+    g.then = all ? SUMS : LISTED;
+    g.lo = m.lo;
+    g.hi = m.hi;
+    g.need = need;
+  }
+  if (!all) publish(s, g, part, fits);
+}
+
+extern "C" __global__ __launch_bounds__(1024) void sample_draw(SAMPLE_ARGS, char* __restrict__ room) {
+  __shared__ Lds s;
+  const int row = blockIdx.x;
+  const Place& g = ((const Place*)room)[row];
+  Row r = row_of(logits, ld, off, V, row);
+  const Form f = form_of(temp, top_k, top_p, min_p, u, row);
+  int mode = g.mode;
+  if (mode == ANSWERED) return;
+  if (mode == BINNED) mode = g.then;
+  int members = 0;
+  if (mode == SMALL || mode == LISTED) {
+    bool fits = true;
+    for (int i = 0; i < PARTS; ++i) {
+      fits = fits && (uint32_t)g.number[i] <= (uint32_t)RUN;
+      members += g.number[i];
+    }
+    if (!fits) mode = WHOLE;
+  }
+  if (mode == WHOLE) {
+    one_row(s, r, f, token + row, prob ? prob + row : nullptr);
+    return;
+  }
+  float top;
+  int where;
+  if (!known(r, g, f, top, where)) return;
+  powers(s);
+  __syncthreads();
+  const Cut least = least_of(s, r, f.q);
+  Cut cut = least;
+  for (int i = threadIdx.x; i < PARTS * WAVES; i += THREADS) s.sum[i] = mode == SMALL ? 0 : g.part[i];
+  if (mode != SUMS) {
+    const int n = g.number[wave()];
+    for (int p = lane(); p < n; p += 64) {
+      s.key[wave() * LIST + p] = g.key[wave() * RUN + p];
+      s.at[wave() * LIST + p] = g.at[wave() * RUN + p];
+    }
+    if (lane() == 0) s.number[wave()] = n;
+    __syncthreads();
+    Members m = {g.lo, g.hi, {NONE, 0x7FFFFFFF}, true};
+    u64 rest;
+    cut = select(s, r, m, mode == LISTED && f.by_p(), mode == SMALL ? (u64)min(f.k, members) : g.need, rest);
+    if (mode == SMALL && f.by_p()) {
+      m.within = cut;
+      cut = select(s, r, m, true, f.goal(rest), rest);
+    }
+    cut = higher(cut, least);
+    // the members that are kept, to the sums of their units
+    const Range c = share({0, r.units}, wave());
+    const int per = max((c.b - c.a + WAVES - 1) / WAVES, 1);
+    each(s, r, m, [&](uint32_t k, int i) {
+      if (k == 0 || !cut.keeps(k, i)) return;
+      atomicAdd(&s.sum[wave() * WAVES + min((((i + r.skew) >> 2) - c.a) / per, WAVES - 1)], weight(r, s.pow2, logit_of(k)));
+    });
+  }
+  __syncthreads();
+  if (wave()) return;
+  // ---- the units in which the running sum passes the draw's point
+  constexpr int N = PARTS * WAVES / 64;
+  u64 v[N], own = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) own += v[j] = s.sum[N * lane() + j];
+  const u64 up = up_sum(own), sum = __shfl(up, 63);
+  const double to = target(f.draw, sum);
+  u64 front = up - own, before = 0;
+  int part = -1;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if ((double)front <= to && (double)(front + v[j]) > to) {
+      part = N * lane() + j;
+      before = front;
+    }
+    front += v[j];
+  }
+  const u64 vote = __ballot(part >= 0);
+  const int l = __ffsll((long long)vote) - 1;
+  if (l < 0) return;
+  part = __builtin_amdgcn_readlane(part, l);
+  before = __shfl(before, l);
+  find(s, r, share(share({0, r.units}, part / WAVES), part % WAVES), cut, before, sum, to, token + row, prob ? prob + row : nullptr);
 }

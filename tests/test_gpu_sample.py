@@ -4,6 +4,8 @@ A token is a whole number, so it has to be equal -- unless the draw, or a cut, l
 are held to 2^-42 (and to 2^-43 of the largest), so a running sum of n of them misses by no more than n * 2^-43 of the largest and 2^-42 of itself.
 The check asks for a token that the definition gives for some u within that of the one given, and for some cut by p likewise; where the
 borders are further off (all but about one in 10^6 rows) that is one token.  prob: the same relative to the weight, and its rounding to f32, 2^-24."""
+import os
+
 import numpy as np
 import pytest
 
@@ -13,9 +15,12 @@ import attn_ref as ref
 pytestmark = pytest.mark.gpu
 
 
-@pytest.fixture(scope="module")
-def eng(rt):
+@pytest.fixture(scope="module", params=["0", "1"])
+def eng(rt, request):
+    """An engine that gives a row one work-group, or (up to 96 rows a call) sixteen."""
+    os.environ["ARCZ_SAMPLE_SPLIT"] = request.param
     e = az.Engine(16, 256)
+    del os.environ["ARCZ_SAMPLE_SPLIT"]
     yield e
     e.close()
 
@@ -237,7 +242,7 @@ def test_in_a_launch_list(eng):
         eng.sample(b[0], 20011, 0, 20011, 5, form, b[4], b[5], b[6])
     put(0)
     l = az.Runtime.record(call)
-    assert l.launches == 1
+    assert l.launches in (1, 4)
     for i in (0, 1, 2, 1):
         put(i)
         call()
@@ -247,6 +252,35 @@ def test_in_a_launch_list(eng):
         assert np.array_equal(b[5].read(np.int32, 5), want[0]) and np.array_equal(b[6].read(np.uint32, 5), want[1])
     l.free()
     ref.free(b)
+
+
+@pytest.mark.parametrize("T,V,launches", [(1, 40000, 4), (16, 40000, 4), (16, 39999, 1), (17, 42500, 4), (17, 42499, 1), (1, 2, 1)])
+def test_the_work_groups_of_a_row(T, V, launches):
+    """By the sizes; a first call of few long rows needs room, which no list being recorded can make."""
+    e = az.Engine(16, 256)
+    x = rows(T, V, seed=3)
+    b = [az.Runtime.from_numpy(x), az.Runtime.from_numpy(np.full(T, 0.37, np.float32)), az.Runtime.alloc(4 * T)]
+    f = az.Sampling(None, None, None, None)
+
+    def call():
+        e.sample(b[0], V, 0, V, T, f, b[1], b[2], None)
+    if launches > 1:
+        with pytest.raises(az.ArczError):
+            az.Runtime.record(call)
+    check(e, x, t=0.8, p=0.9, seed=5)
+    n = az.lib.arcz_launch_count()
+    call()
+    assert az.lib.arcz_launch_count() - n == launches
+    l = az.Runtime.record(call)
+    assert l.launches == launches
+    want = b[2].read(np.int32)
+    for _ in range(3):
+        b[2].fill(0)
+        l.run()
+        assert np.array_equal(b[2].read(np.int32), want)
+    l.free()
+    ref.free(b)
+    e.close()
 
 
 def test_refusals(eng):
