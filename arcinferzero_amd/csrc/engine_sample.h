@@ -1,10 +1,10 @@
 // A token from each row of logits (kernels/sample.hip).  A part of class Engine (included in it, behind engine_attn.h).
 
   // Sixteen work-groups a row, in four launches, for few long rows (sample.hip's Place, 108760 bytes of the attention's room, for each).  Measured, us, one
-  // work-group a row / sixteen, with a temperature, k = 50 and p, p alone, and rows of all kinds: 16 x 16384 15 39 30 29 / 19 42 37 43;
-  // 16 x 32001 20 41 46 37 / 19 43 45 42; 16 x 65536 29 45 64 55 / 19 43 44 44; 32 x 65536 29 45 65 56 / 24 48 61 57; 1 x 151936 54 43 106 55 / 19 31 35 21;
-  // 48 x 151936 58 59 125 113 / 37 58 93 70; 96 x 151936 61 61 130 123 / 60 79 158 103.  (Rows whose largest logit is all that is asked for: 13 / 14 and, 48 of
-  // them, 14 / 21; a cut by p behind one of 2000 tokens, which one work-group does behind the others' launches: 122 / 134.  A row's kind is known on the device only.)
+  // work-group a row / sixteen, with a temperature, k = 50 and p, p alone, and rows of all kinds: 16 x 16384 15 31 29 27 / 18 35 37 40;
+  // 16 x 32001 20 33 41 36 / 19 35 39 40; 16 x 65536 29 36 60 55 / 18 35 41 40; 32 x 65536 29 37 61 55 / 23 40 57 48; 1 x 151936 54 42 106 54 / 19 31 35 20;
+  // 48 x 151936 57 48 118 112 / 37 51 88 63; 96 x 151936 61 51 123 117 / 61 72 151 96.  (Rows whose largest logit is all that is asked for: 13 / 12 and, 48 of
+  // them, 14 / 21; a cut by p behind one of 2000 tokens, which one work-group does behind the others' launches: 122 / 132.  A row's kind is known on the device only.)
   int sample_split_ = -1;   // ARCZ_SAMPLE_SPLIT
   static constexpr int SPLIT_ROWS = 96;
   bool split_pays(int V, int T) const { return V >= 2500 * std::max(T, 16); }

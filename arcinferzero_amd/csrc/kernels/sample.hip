@@ -10,11 +10,12 @@
 // numbers and the same in any order, and two rows of the same logits give the same token.
 //
 // A work-group has a row.  The row is read once for its largest logit, and then again, out of the caches, for what the cuts ask for:
-//   k up to 512: the k-th of the threads' largest logits is one that at least k tokens reach; those that do -- few more than k -- go to LDS, and the rest
+//   k up to 960: the k-th of the threads' largest logits is one that at least k tokens reach; those that do -- few more than k -- go to LDS, and the rest
 //     happens there.
 //   else: a histogram of the row over the weight's logarithm, 64 bins an octave, counts and sums of weights; the bin in which a cut lies
 //     is found from it, its tokens go to LDS and give the cut itself.  Another pass adds up what is kept, and the token is found in a sixteenth of a
 //     sixteenth of the row.
+// Of up to 64 listed tokens one wave finds the cut, each lane the place of its own among them; of more their digits are counted, as below.
 // Where more tokens meet in a bin than LDS takes (thousands of equal logits, a very high temperature) their logits' digits are counted
 // over the whole row instead, eight bits at a time.
 #include <hip/hip_runtime.h>
@@ -22,7 +23,13 @@
 
 namespace {
 typedef unsigned long long u64;
-constexpr int THREADS = 1024, WAVES = 16, LIST = 512, SMALL_K = 512, FEW = 512, BINS = 3 * THREADS;   // (48 octaves)
+constexpr int THREADS = 1024, WAVES = 16, LIST = 512, BINS = 3 * THREADS;   // (48 octaves)
+// The highest k that is looked for among the threads' largest logits (of 1024: the nearer to them all, the more tokens reach the k-th).  Measured, us, this
+// way / by the histogram: 256 rows of 151936, k = 512 71 / 177, 960 86 / 176; with a cut by p behind it 79 / 195, 97 / 193; one row, k = 960 39 / 36, with p 48 / 132.
+constexpr int SMALL_K = 960;
+// Listed tokens that one wave orders (a lane each).  37 rows of 32001, k = 50 with p: 33 us, by digits 36; going down the bits of 512 in a
+// wave's registers took longer than the digits for any number (k = 100 31 / 26, 400 41 / 29).
+constexpr int FEW = 64;
 constexpr uint32_t NONE = 0x007FFFFFu;                                             // the key of -inf: no token
 
 // CAP: tokens of a wave that the list takes.
@@ -276,8 +283,6 @@ __device__ inline Cut select(Lds& s, const Row& r, const Members& m, bool by_wei
     all += s.number[w];
   }
   if (m.listed && all <= FEW) {
-    // Few: one wave has them in its registers, and goes down the bits of their keys.
-    constexpr int N = FEW / 64;
     for (int p = lane(); p < s.number[wave()]; p += 64) {
       const uint32_t k = s.key[wave() * LIST + p];
       const int i = s.at[wave() * LIST + p];
@@ -286,85 +291,22 @@ __device__ inline Cut select(Lds& s, const Row& r, const Members& m, bool by_wei
     }
     __syncthreads();
     if (wave() == 0) {
-      if (all <= 64) {
-        // how many members lie in front of this lane's, and what they weigh
-        const uint32_t key = lane() < all ? s.few_key[lane()] : 0;
-        const u64 w = key ? weight(r, s.pow2, logit_of(key)) : 0;
-        uint32_t rank = 0;
-        u64 front = 0;
+      // how many members lie in front of this lane's, and what they weigh
+      const uint32_t key = lane() < all ? s.few_key[lane()] : 0;
+      const u64 w = key ? weight(r, s.pow2, logit_of(key)) : 0;
+      uint32_t rank = 0;
+      u64 front = 0;
 #pragma unroll 1
-        for (int p = 0; p < all; ++p) {
-          const uint32_t k = __builtin_amdgcn_readlane((int)key, p);
-          const bool before = k > key || (k == key && p < lane());
-          rank += before && k ? 1 : 0;
-          front += before ? (u64)(uint32_t)__builtin_amdgcn_readlane((int)(w >> 32), p) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)w, p) : 0;
-        }
-        if (key && (by_weight ? front < need && front + w >= need : rank == need - 1)) {
-          s.place[0] = key;
-          s.place[1] = s.few_at[lane()];
-          s.found[0] = front + w;
-        }
-      } else {
-        uint32_t key[N];
-        u64 w[N], above = 0;
-        bool in[N];
-#pragma unroll
-        for (int c = 0; c < N; ++c) {
-          const int p = 64 * c + lane();
-          key[c] = p < all ? s.few_key[p] : 0;
-          in[c] = key[c] != 0;
-          w[c] = 0;
-          if (64 * c < all) w[c] = in[c] ? weight(r, s.pow2, logit_of(key[c])) : 0;
-        }
-#pragma unroll 1
-        for (int bit = differ ? 31 - __clz((int)differ) : -1; bit >= 0; --bit) {
-          u64 sum = 0;   // (of the members that have the bit)
-          if (by_weight) {
-#pragma unroll
-            for (int c = 0; c < N; ++c)
-              if (64 * c < all) sum += in[c] && key[c] >> bit & 1 ? w[c] : 0;
-            sum = wave_sum(sum);
-          } else {
-#pragma unroll
-            for (int c = 0; c < N; ++c)
-              if (64 * c < all) sum += __popcll(__ballot(in[c] && key[c] >> bit & 1));
-          }
-          const bool up = sum >= need;   // (the cut lies among them: else they are all above it)
-          need -= up ? 0 : sum;
-#pragma unroll
-          for (int c = 0; c < N; ++c)
-            if (64 * c < all) {
-              const bool one = key[c] >> bit & 1;
-              above += in[c] && one && !up ? w[c] : 0;
-              in[c] = in[c] && one == up;
-            }
-        }
-        // What is left has one key, and one weight (not 0, where a sum had to be reached): so many of the first ones.
-        uint32_t last = 0;
-        u64 one = 0;
-#pragma unroll
-        for (int c = 0; c < N; ++c) {
-          const u64 vote = __ballot(in[c]);
-          if (vote) {
-            const int l = __ffsll((long long)vote) - 1;
-            last = __builtin_amdgcn_readlane((int)key[c], l);
-            one = (u64)(uint32_t)__builtin_amdgcn_readlane((int)(w[c] >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)w[c], l);
-          }
-        }
-        const int n = by_weight ? (int)((need + one - 1) / one) : (int)need;
-        int front = 0;
-#pragma unroll
-        for (int c = 0; c < N; ++c) {
-          const u64 vote = __ballot(in[c]);
-          const int at = front + __builtin_amdgcn_mbcnt_hi((uint32_t)(vote >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)vote, 0));
-          if (in[c] && at == n - 1) s.place[1] = s.few_at[64 * c + lane()];
-          front += __popcll(vote);
-        }
-        above = wave_sum(above) + (u64)n * one;
-        if (lane() == 0) {
-          s.place[0] = last;
-          s.found[0] = above;
-        }
+      for (int p = 0; p < all; ++p) {
+        const uint32_t k = __builtin_amdgcn_readlane((int)key, p);
+        const bool before = k > key || (k == key && p < lane());
+        rank += before && k ? 1 : 0;
+        front += before ? (u64)(uint32_t)__builtin_amdgcn_readlane((int)(w >> 32), p) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)w, p) : 0;
+      }
+      if (key && (by_weight ? front < need && front + w >= need : rank == need - 1)) {
+        s.place[0] = key;
+        s.place[1] = s.few_at[lane()];
+        s.found[0] = front + w;
       }
     }
     __syncthreads();

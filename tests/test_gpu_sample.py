@@ -104,7 +104,7 @@ def rows(T, V, seed=0, spread=2.5):
     return x.astype(np.float32)
 
 
-CUTS = [dict(), dict(k=1), dict(k=50), dict(k=512), dict(k=513), dict(k=3000), dict(p=0.9), dict(p=0.3), dict(q=0.05), dict(k=40, p=0.95), dict(k=40, p=0.95, q=0.02), dict(k=2000, p=0.7),
+CUTS = [dict(), dict(k=1), dict(k=50), dict(k=512), dict(k=513), dict(k=960), dict(k=960, p=0.8), dict(k=961), dict(k=961, p=0.8), dict(k=3000), dict(p=0.9), dict(p=0.3), dict(q=0.05), dict(k=40, p=0.95), dict(k=40, p=0.95, q=0.02), dict(k=2000, p=0.7),
         dict(k=900, p=0.999, q=0.001), dict(p=0.97, q=0.01), dict(t=0.0), dict(t=0.2, p=0.9), dict(t=3.0, k=700), dict(t=0.7, k=20, p=0.8, q=0.1)]
 
 
