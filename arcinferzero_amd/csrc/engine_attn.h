@@ -240,12 +240,14 @@
     }
     if ((overlap(out[1], in[1]) && out[1].b != in[1].b) || (overlap(out[4], in[2]) && out[4].b != in[2].b))
       throw std::runtime_error(what + ": before and len, or state and after, overlap (in place: the same values)");
-    // Up to PLAN_ROWS rows the work-group that makes the batch writes their places too; more are a second launch.
+    // Few rows: the work-group that makes the batch writes their places too; more are a second launch.  (us, one launch / two: 256 sequences of a token
+    // 3.8 / 6.5, of four 4.4 / 6.6, of eight 5.6 / 6.3; 512 of eight 8.6 / 7.5; 64 of 32 8.3 / 6.4; one of 4096 13.4 / 6.9.)
     int seqs = b.seqs, ldt = b.ld_table, T = b.T, mr = b.max_rows, pages = p.pages, ps = log2_of(p.page);
     const bool places = (p.pos || p.slot) && T > 0 && mr > 0;
-    int with = places && std::min<int64_t>(T, (int64_t)seqs * mr) <= PLAN_ROWS ? 1 : 0;
+    int with = places && std::min<int64_t>(T, (int64_t)seqs * mr) <= (mr <= 8 ? 2048 : 1024) ? 1 : 0;
     cl_kernel k = variant("attn", {}, "kv_plan");
     set_args(k, 0, p.add, p.before, b.len, b.rows, b.table, ldt, p.ring, p.state, p.after, p.shared, p.pos, p.slot, seqs, T, mr, pages, ps, with);
+    // (us, 256 threads / 1024: 256 sequences of a token 3.8 / 5.2, 512 12.6 / 5.3)
     size_t g1 = seqs <= 256 ? 256 : 1024, l1 = g1;
     run("kv_plan", k, 1, &g1, &l1);
     if (!places || with) return;
@@ -254,7 +256,6 @@
     size_t g[2] = {(size_t)((std::min(mr, T) - 1) / 1024 + 1) * 256, n}, l[2] = {256, 1};
     run("kv_places", k2, 2, g, l);
   }
-  static constexpr int PLAN_ROWS = 8192;
   void kv_write(const Kv& c, const Batch& b, cl_mem k, int ldk, int k_off, cl_mem v, int ldv, int v_off) {
     Places at;
     if (!check_batch("kv_write", c, b, at)) return;

@@ -3,15 +3,16 @@
 //   n = x / sqrt(mean(x^2) + eps) * w  over the head's values, w the queries' weights for the first heads and the keys' for the rest;
 //   y = n turned by the row's position (rope.hip: pairs, axes, angles), what lies behind the pairs as it is.
 //
-// A lane's eight to twelve squares are added in f32, the lanes' sums, the mean and its root in 64 bits; the root's reciprocal is rounded to f32
-// and multiplied with.  Where a lane's largest value is below 2^-40 or above 2^60 (or none), whose squares f32 may not hold, the whole head is
-// done in 64 bits, so that no finite head overflows or vanishes on the way -- a head by itself, so that its bits do not hang on the heads beside
-// it.  (All squares and products in 64 bits: 42 million values took 38 us of the vector units' time, 24 heads of 256 values x 777 tokens 11.4 instead of
-// 7 us with warm rows.)
+// Squares, their sums, the mean and its root are 64-bit, so that no finite head overflows or vanishes on the way; n is rounded to f32 once.  (With f32
+// squares and the root's reciprocal in f32 the launches took the same: 777 tokens of 24 heads of 256 values 11.1 - 11.4 and 11.1 - 11.5 us, 8192 of 40 of
+// 128 63.3 and 63.3.)
 // Bound: 8 bytes of HBM a value.  A head's values stay in the registers of 8 to 64 lanes between the sum and the rotation, eight a lane (and
 // four behind the pairs), so x is read once; a work-group takes all heads of some tokens, whose sines and cosines it works out once, as it
 // brings the weights into LDS once.  Heads whose pairs are no multiple of four (of two, where neighbours) or longer ones go value by value,
 // a wave each, and read x twice.
+// Measured, 40 heads of 128 values (what rotation alone takes): 8192 tokens 63 us = 5.3 TB/s (63), 2500 23.6 (22), 777 10 (9), 256 4.8 (4.2), one 3.2 (3.0).
+// Behind the launch itself short ones wait for HBM once and for the lanes' sums; four values brought in under a lane's condition, value by value, took
+// 8192 tokens to 71 us, weights not held in LDS 777 to 12.
 #include "attn.h"
 #include "turn.h"
 
@@ -85,37 +86,19 @@ __device__ inline void norm_rope_lanes(const float* x, int ldx, int x_off, float
   // (all lanes of a head go round together: L divides 64)
   for (; u < units; u += step) {
     const int t = u / nh, h = h0 + u - t * nh;
-    auto square = [](const float4& v) { return fmaf(v.y, v.y, v.x * v.x) + fmaf(v.w, v.w, v.z * v.z); };
-    auto most = [](const float4& v) { return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))); };
-    float big = ha ? most(a) : 0.0f, some = ha ? square(a) : 0.0f;
-    if (hb) { big = fmaxf(big, most(b)); some += square(b); }
-    if (hr) { big = fmaxf(big, most(r)); some += square(r); }
-    const float g = (float)inverse_root(sum_of((double)some, L), per_value, eps);
-    auto times = [](const float4& v, float g) { return make_float4(v.x * g, v.y * g, v.z * g, v.w * g); };
-    float4 na = times(a, g), nb = times(b, g), nr = times(r, g);
-    // (a NaN is passed over by fmaxf, and makes the sum one either way)
-    const bool held = !(ha || hb || hr) || (big >= 0x1p-40f && big <= 0x1p60f);
-    const unsigned long long all = __ballot(held);
-    if (__builtin_expect(~all != 0, 0)) {
-      const unsigned long long head = (L == 64 ? ~0ull : (1ull << L) - 1) << (threadIdx.x & 63 & ~(L - 1));
-      double sum = 0.0;
-      auto square2 = [&](const float4& v) {
-        sum = fma((double)v.x, (double)v.x, sum);
-        sum = fma((double)v.y, (double)v.y, sum);
-        sum = fma((double)v.z, (double)v.z, sum);
-        sum = fma((double)v.w, (double)v.w, sum);
-      };
-      if (ha) square2(a);
-      if (hb) square2(b);
-      if (hr) square2(r);
-      const double f = inverse_root(sum_of(sum, L), per_value, eps);
-      auto times2 = [&](const float4& v) { return make_float4((float)(v.x * f), (float)(v.y * f), (float)(v.z * f), (float)(v.w * f)); };
-      if ((all & head) != head) {
-        na = times2(a);
-        nb = times2(b);
-        nr = times2(r);
-      }
-    }
+    double sum = 0.0;
+    auto square = [&](const float4& v) {
+      sum = fma((double)v.x, (double)v.x, sum);
+      sum = fma((double)v.y, (double)v.y, sum);
+      sum = fma((double)v.z, (double)v.z, sum);
+      sum = fma((double)v.w, (double)v.w, sum);
+    };
+    if (ha) square(a);
+    if (hb) square(b);
+    if (hr) square(r);
+    const double f = inverse_root(sum_of(sum, L), per_value, eps);
+    auto times = [&](const float4& v) { return make_float4((float)(v.x * f), (float)(v.y * f), (float)(v.z * f), (float)(v.w * f)); };
+    float4 na = times(a), nb = times(b), nr = times(r);
     const float* w = sw[h < nq ? 0 : 1];
     auto weigh = [&](float4& v, int c, bool has) {
       const float4 k = *(const float4*)(w + (has ? c : 0));

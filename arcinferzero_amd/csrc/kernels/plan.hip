@@ -11,6 +11,8 @@
 // Bound: latency -- one work-group for all sequences, since the sums run over them: the counts, their sums in three steps over the
 // waves, then the ring's entries and the table's, a thread each.  Places of many rows are a launch of their own (kv_places), a work-group for
 // 1024 of one sequence's, behind it.
+// Measured: 256 sequences of a token 3.8 us, 1024 5.6, 256 of eight 5.6, 64 prompts of 256 tokens 6.7 in two launches, 1024 of them 13.5; a launch that does
+// nothing takes 2.5.
 #include "attn.h"
 
 using attn::Change;
@@ -122,7 +124,8 @@ extern "C" __global__ __launch_bounds__(PLAN) void kv_plan(const int* __restrict
       rows[s] = at.rows + front.rows;
       len[s] = c.len;
     }
-    // Up to eight rows a sequence (tokens, drafts): its own thread writes their pages and places.  Else, and for pages given back, of which
+    // Up to eight rows a sequence (tokens, drafts): its own thread writes their pages and places (256 sequences of four 4.4 us, of eight 5.6; shared
+    // out 6.1, 8.6; of twelve 11.0 shared out).  Else, and for pages given back, of which
     // a sequence that ends has many, the work-group shares them out.
     const bool apart = max_rows > 8;
     if (!apart && s < seqs) {
