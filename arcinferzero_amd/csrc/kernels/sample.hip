@@ -27,8 +27,8 @@ constexpr int THREADS = 1024, WAVES = 16, LIST = 512, BINS = 3 * THREADS;   // (
 // The highest k that is looked for among the threads' largest logits (of 1024: the nearer to them all, the more tokens reach the k-th).  Measured, us, this
 // way / by the histogram: 256 rows of 151936, k = 512 71 / 177, 960 86 / 176; with a cut by p behind it 79 / 195, 97 / 193; one row, k = 960 39 / 36, with p 48 / 132.
 constexpr int SMALL_K = 960;
-// Listed tokens that one wave orders (a lane each).  37 rows of 32001, k = 50 with p: 33 us, by digits 36; going down the bits of 512 in a
-// wave's registers took longer than the digits for any number (k = 100 31 / 26, 400 41 / 29).
+// Listed tokens that one wave orders, a lane each.  37 rows of 32001, by k and p: k = 50 28 us, k = 64, whose tokens are more and go by digits, 33 (by digits,
+// as for 100, 34, and 400, 37; going down the bits of up to 512 in a wave's registers instead 41, 42 and 58).
 constexpr int FEW = 64;
 constexpr uint32_t NONE = 0x007FFFFFu;                                             // the key of -inf: no token
 
