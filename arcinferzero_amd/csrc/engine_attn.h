@@ -403,13 +403,29 @@
     p.M1 = (int)M1;
     const size_t cus = (size_t)arcz_device_cus(), pairs = (size_t)b.seqs * c.heads, pairs1 = (size_t)sh.n * c.heads;
     const int all = b.max_len > 0 ? b.max_len : b.ld_table * c.page, shared = sh.max_len > 0 ? std::min(sh.max_len, all) : all, own = std::max(1, sh.max_len > 0 ? all - shared : all);
-    // The group's keys: as many pieces as fill the chip, of at least 128 keys (us, 4 to 16 sequences of a token behind 512 - 4096 keys, at least 256 /
-    // 128 / 64: 28 - 30 / 24 - 28 / 21 - 34).  Work-groups of eight waves from 512 rows on (512 rows behind 16384 keys 80 / 83 with four, 4000 behind 6000 150 /
-    // 170; 256 rows behind 1024 22 / 18, behind 8192 38 / 37).
+    // Work-groups of eight waves from 512 rows on (us, with eight / four: 512 rows behind 16384 keys 80 / 83, 4000 behind 6000 150 / 170; 256 rows behind 1024
+    // 22 / 18, behind 8192 38 / 37).
     p.waves1 = c.hd == 128 && c.block >= 32 && M1 >= 512 ? 8 : 4;
     p.bm1 = 32 * p.waves1;
     p.tiles1 = (int)((M1 + p.bm1 - 1) / p.bm1);
-    p.n1 = p.tiles1 && pairs1 ? (int)std::max<size_t>(1, std::min<size_t>((size_t)8 / p.waves1 * cus / (pairs1 * p.tiles1), (size_t)(shared + 127) / 128)) : 0;
+    const double rate = c.hd == 64 ? 0.8e9 : c.hd == 128 ? 1.0e9 : 0.7e9, key = 2.0 * c.heads * c.hd, mean = (double)b.T / std::max(1, b.seqs) * p.G;
+    // The group's keys in pieces of at least 128 (us, 4 to 16 sequences of a token behind 512 - 4096 keys, at least 256 / 128 / 64: 28 - 30 / 24 - 28 / 21 - 34): one
+    // or the most that one to four work-groups for every compute unit make, whichever takes the least -- rounds of a piece's keys and what a work-group takes
+    // beside them (as 128 keys would), and each piece written and read.  (us, pieces 1, 2, 3 ...: 24 of 16 heads of 256 values and up to 90 rows behind 4000
+    // 370 354 333 323 335 344; eight of 32 of 128 and up to 120 rows behind 8000 366 229 179 162 215 194.)
+    double front = 0.0;
+    if (p.tiles1 && pairs1) {
+      const double sets = c.heads * std::min((double)sh.n * p.tiles1, std::ceil((double)b.T * p.G / p.bm1) + 0.5 * (sh.n - 1));
+      const int most = std::max(1, (shared + 127) / 128);
+      for (int r = 0; r <= 4; ++r) {
+        const int n = r ? std::min(most, (int)(r * cus / sets)) : 1;
+        if (n < 1) continue;
+        const double t = std::ceil(sets * n / cus) * p.bm1 * ((double)shared / n + 128.0) * 8.0 * c.hd / rate * cus + (double)b.T * heads * n * (c.hd + 2) * 8.0 / 5.0e6;
+        if (r && t >= front) continue;
+        front = t;
+        p.n1 = n;
+      }
+    }
     // its own: as attention() does
     p.few = M <= (c.hd == 256 ? 16 : 32);
     if (p.few) {
@@ -426,15 +442,19 @@
       p.n2 = (int)std::max<size_t>(1, std::min<size_t>(2 * cus / std::max<size_t>(1, pairs * p.tiles2), (size_t)(own + 255) / 256));
     }
     // What both ways would take (us): attention as it is -- its launch, each sequence's keys of all, of which what they share comes from the caches, or
-    // its rows in whole tiles -- and three launches, the groups' rows in whole tiles, their own keys and the pieces.  Rates as measured: keys 9.5 TB/s
-    // shared (sequences of a token behind 1324 - 16984 keys 10 - 445 us), 5 of their own, products in tiles by the head's length.  (us, one launch / three:
-    // 16 sequences behind 4096 keys 24 / 28, 32 behind 2048 25 / 29, 64 behind 1024 28 / 36, 64 behind 8192 121 / 57, 128 behind 16384 445 / 115; four of 250 rows
-    // behind 6000 195 / 203, 24 of 16 heads of 256 values and up to 90 rows behind 4000 490 / 411.)
-    const double rate = c.hd == 64 ? 0.8e9 : c.hd == 128 ? 1.0e9 : 0.7e9, key = 2.0 * c.heads * c.hd, op = 8.0 * c.heads * c.hd, mean = (double)b.T / std::max(1, b.seqs) * p.G;
-    const double padded = b.seqs * std::max(128.0, mean + 64.0);   // (half of a sequence's last tile is empty)
-    const double one = 8.0 + (p.few ? b.seqs * (double)all * key / 9.5e6 : padded * all * op / rate);
-    const double three = 24.0 + (double)sh.n * p.tiles1 * p.bm1 * shared * op / rate + (p.few ? b.seqs * (double)own * key / 5.0e6 : padded * own * op / rate) +
-                         (double)b.T * heads * (p.n1 + p.n2) * (c.hd + 2) * 8.0 / 5.0e6;
+    // its rows in whole tiles (a third of a round lost to their ends) -- and three launches, the groups' rows in whole tiles, their own keys and the pieces.  Rates as
+    // measured: keys 9.5 TB/s shared (sequences of a token behind 1324 - 16984 keys 10 - 445 us), 5 of their own, products in tiles by the head's
+    // length.  (us, one launch / three: 16 sequences behind 4096 keys 23 / 28, 32 behind 2048 23 / 28, 64 behind 1024 22 / 31, 64 behind 8192 124 / 51, 128 behind
+    // 16384 426 / 105; eight of up to 120 rows behind 8000 250 / 165, 24 of up to 90 behind 4000 225 / 250; of 16 heads of 256 values, 24 of up to 90
+    // behind 4000 425 / 351.  Two that the rule misses: eight of up to 200 of those heads behind 2000 187 / 147, four of 250 rows of 32 heads behind 6000 196 / 204.)
+    const double last = std::max(1.0, (mean + 64.0) / 128.0);   // (tiles of a sequence, half of the last one empty)
+    auto tiles = [&](double keys, int pieces) {   // (heads of 256 values: one work-group a compute unit, so whole rounds)
+      const double sets = b.seqs * c.heads * last * pieces / cus, rounds = c.hd == 256 ? std::ceil(sets) : std::max(1.0, sets + 0.3);
+      return rounds * cus * 128.0 * (keys / pieces + 128.0) * 8.0 * c.hd / rate;
+    };
+    const int pieces = (int)std::max<size_t>(1, std::min<size_t>(2 * cus / std::max<size_t>(1, pairs * ((M + 127) / 128)), (size_t)(all + 255) / 256));
+    const double one = 8.0 + (p.few ? b.seqs * (double)all * key / 9.5e6 : tiles(all, pieces));
+    const double three = 24.0 + front + (p.few ? b.seqs * (double)own * key / 5.0e6 : tiles(own, p.n2)) + (double)b.T * heads * p.n2 * (c.hd + 2) * 8.0 / 5.0e6;
     p.one = attn_shared_ < 0 ? one <= three : attn_shared_ == 0;
     if (p.one) {
       p.bytes = 256;
