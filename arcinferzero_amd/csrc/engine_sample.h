@@ -6,7 +6,7 @@
   // 48 x 151936 57 48 118 112 / 37 51 88 63; 96 x 151936 61 51 123 117 / 61 72 151 96.  (Rows whose largest logit is all that is asked for: 13 / 12 and, 48 of
   // them, 14 / 21; a cut by p behind one of 2000 tokens, which one work-group does behind the others' launches: 122 / 132.  A row's kind is known on the device only.)
   int sample_split_ = -1;   // ARCZ_SAMPLE_SPLIT
-  static constexpr int SPLIT_ROWS = 96;
+  static int split_rows() { return std::min(96, 2 * arcz_device_cus()); }   // (the room has 264192 bytes a compute unit)
   bool split_pays(int V, int T) const { return V >= 2500 * std::max(T, 16); }
   struct Sampling {
     cl_mem temperature, top_k, top_p, min_p;
@@ -28,7 +28,7 @@
     for (const Place& o : out)
       for (const Place& i : in)
         if (overlap(o, i)) throw std::runtime_error("sample: token or prob overlaps what is read");
-    if (T <= SPLIT_ROWS && (sample_split_ < 0 ? split_pays(V, T) : sample_split_)) {
+    if (T <= split_rows() && (sample_split_ < 0 ? split_pays(V, T) : sample_split_)) {
       at_room();
       for (const char* step : {"sample_top", "sample_scan", "sample_cut", "sample_draw"}) {
         cl_kernel k = variant("ops", {}, step);
