@@ -1,13 +1,13 @@
 // A token from each row of logits (kernels/sample.hip).  A part of class Engine (included in it, behind engine_attn.h).
 
   // Sixteen work-groups a row, in four launches, for few long rows (sample.hip's Place, 108760 bytes of the attention's room, for each).  Measured, us, one
-  // work-group a row / sixteen, with a temperature, k = 50 and p, p alone, and rows of all kinds: 16 x 16384 15 31 29 27 / 18 35 37 40;
-  // 16 x 32001 20 33 41 36 / 19 35 39 40; 16 x 65536 29 36 60 55 / 18 35 41 40; 32 x 65536 29 37 61 55 / 23 40 57 48; 1 x 151936 54 42 106 54 / 19 31 35 20;
-  // 48 x 151936 57 48 118 112 / 37 51 88 63; 96 x 151936 61 51 123 117 / 61 72 151 96.  (Rows whose largest logit is all that is asked for: 13 / 12 and, 48 of
-  // them, 14 / 21; a cut by p behind one of 2000 tokens, which one work-group does behind the others' launches: 122 / 132.  A row's kind is known on the device only.)
+  // work-group a row / sixteen, with a temperature, k = 50 and p, p alone, and rows of all kinds: 16 x 16384 15 21 28 27 / 18 30 35 36;
+  // 16 x 32001 20 23 39 36 / 19 29 36 36; 16 x 65536 29 27 59 55 / 19 29 39 37; 32 x 65536 29 28 59 55 / 23 35 54 43; 1 x 151936 54 32 106 54 / 19 27 34 21;
+  // 48 x 151936 57 36 119 109 / 37 43 88 56; 96 x 151936 61 40 122 118 / 60 65 152 90.  (Rows whose largest logit is all that is asked for: 13 / 15 and, 48 of
+  // them, 14 / 24; a cut by p behind one of 2000 tokens, which one work-group does behind the others' launches: 122 / 135.  A row's kind is known on the device only.)
   int sample_split_ = -1;   // ARCZ_SAMPLE_SPLIT
   static int split_rows() { return std::min(96, 2 * arcz_device_cus()); }   // (the room has 264192 bytes a compute unit)
-  bool split_pays(int V, int T) const { return V >= 2500 * std::max(T, 16); }
+  bool split_pays(int V, int T) const { return V >= 3000 * std::max(T, 16); }
   struct Sampling {
     cl_mem temperature, top_k, top_p, min_p;
   };

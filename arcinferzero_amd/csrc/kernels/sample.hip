@@ -15,9 +15,14 @@
 //   else: a histogram of the row over the weight's logarithm, 64 bins an octave, counts and sums of weights; the bin in which a cut lies
 //     is found from it, its tokens go to LDS and give the cut itself.  Another pass adds up what is kept, and the token is found in a sixteenth of a
 //     sixteenth of the row.
-// Of up to 64 listed tokens one wave finds the cut, each lane the place of its own among them; of more their digits are counted, as below.
+// Of up to 256 listed tokens the cut is found by the place of each among them; of more their digits are counted, as below.  Where all that is kept is listed
+// the token comes out of the list.
 // Where more tokens meet in a bin than LDS takes (thousands of equal logits, a very high temperature) their logits' digits are counted
 // over the whole row instead, eight bits at a time.
+// Bound: the 64-bit steps of the weights, some twenty instructions a token each time that they are wanted -- once for the histogram, once for the sums --, and for
+// few rows the steps themselves, of which none begins before the last one's sums have met.  A row is read from HBM once and from the caches after that.
+// Measured, 256 rows of 151936: the largest logit 27 us (5.7 TB/s), by k and p 60, drawn among all 75, by p 138; 37 rows of 32001 of all kinds 36; one row of
+// 151936 by sixteen work-groups, by k and p 26 us, by p 34.  A cut in rows that are almost flat (a temperature of 1000) takes 560.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -25,11 +30,11 @@ namespace {
 typedef unsigned long long u64;
 constexpr int THREADS = 1024, WAVES = 16, LIST = 512, BINS = 3 * THREADS;   // (48 octaves)
 // The highest k that is looked for among the threads' largest logits (of 1024: the nearer to them all, the more tokens reach the k-th).  Measured, us, this
-// way / by the histogram: 256 rows of 151936, k = 512 71 / 177, 960 86 / 176; with a cut by p behind it 79 / 195, 97 / 193; one row, k = 960 39 / 36, with p 48 / 132.
+// way / by the histogram: 256 rows of 151936, k = 512 65 / 175, 960 80 / 173; with a cut by p behind it 73 / 190, 91 / 189; one row, k = 960 37 / 35, with p 46 / 134.
 constexpr int SMALL_K = 960;
-// Listed tokens that one wave orders, a lane each.  37 rows of 32001, by k and p: k = 50 28 us, k = 64, whose tokens are more and go by digits, 33 (by digits,
-// as for 100, 34, and 400, 37; going down the bits of up to 512 in a wave's registers instead 41, 42 and 58).
-constexpr int FEW = 64;
+// Listed tokens of which each is compared with all others.  37 rows of 32001, by k and p: k = 50 21 us (by digits 36), k = 200, 220 tokens, 32, k = 256, which go by
+// digits, 33.  (Going down the bits of up to 512 in one wave's registers: 42 for 100, 58 for 400.)
+constexpr int FEW = 256;
 constexpr uint32_t NONE = 0x007FFFFFu;                                             // the key of -inf: no token
 
 // CAP: tokens of a wave that the list takes.
@@ -41,6 +46,7 @@ struct LdsOf {
   uint32_t count[BINS];
   uint32_t key[WAVES * CAP], at[WAVES * CAP];   // the list: a run of each wave's, in the row's order
   uint32_t few_key[FEW], few_at[FEW];           // ... of few members, the runs behind one another
+  u64 few_weight[FEW];
   u64 digit_sum[256];
   uint32_t digit[256];
   u64 part[WAVES], kept[WAVES];
@@ -283,29 +289,44 @@ __device__ inline Cut select(Lds& s, const Row& r, const Members& m, bool by_wei
     all += s.number[w];
   }
   if (m.listed && all <= FEW) {
+    if (threadIdx.x < FEW) {
+      s.digit[threadIdx.x] = 0;
+      s.digit_sum[threadIdx.x] = 0;
+    }
     for (int p = lane(); p < s.number[wave()]; p += 64) {
       const uint32_t k = s.key[wave() * LIST + p];
       const int i = s.at[wave() * LIST + p];
-      s.few_key[run + p] = m.has(k, i) ? k : 0;
+      const bool has = m.has(k, i);
+      s.few_key[run + p] = has ? k : 0;
+      s.few_weight[run + p] = has ? weight(r, s.pow2, logit_of(k)) : 0;
       s.few_at[run + p] = i;
     }
     __syncthreads();
-    if (wave() == 0) {
-      // how many members lie in front of this lane's, and what they weigh
-      const uint32_t key = lane() < all ? s.few_key[lane()] : 0;
-      const u64 w = key ? weight(r, s.pow2, logit_of(key)) : 0;
+    // how many members lie in front of each, and what they weigh: four waves for 64 of them, each against a fourth of all
+    constexpr int EACH = WAVES * 64 / FEW;
+    const int mine = wave() / EACH * 64 + lane();
+    if (wave() / EACH * 64 < all) {
+      const uint32_t key = mine < all ? s.few_key[mine] : 0;
       uint32_t rank = 0;
       u64 front = 0;
-#pragma unroll 1
-      for (int p = 0; p < all; ++p) {
-        const uint32_t k = __builtin_amdgcn_readlane((int)key, p);
-        const bool before = k > key || (k == key && p < lane());
-        rank += before && k ? 1 : 0;
-        front += before ? (u64)(uint32_t)__builtin_amdgcn_readlane((int)(w >> 32), p) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)w, p) : 0;
+      for (int p = wave() % EACH; p < all; p += EACH) {
+        const uint32_t k = s.few_key[p];
+        const bool before = (k > key) | ((k == key) & (p < mine));
+        rank += before ? 1 : 0;
+        front += before ? s.few_weight[p] : 0;
       }
+      if (key && rank) {
+        atomicAdd(&s.digit[mine], rank);
+        atomicAdd(&s.digit_sum[mine], front);
+      }
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < all) {   // (FEW at most)
+      const uint32_t key = s.few_key[threadIdx.x], rank = s.digit[threadIdx.x];
+      const u64 w = s.few_weight[threadIdx.x], front = s.digit_sum[threadIdx.x];
       if (key && (by_weight ? front < need && front + w >= need : rank == need - 1)) {
         s.place[0] = key;
-        s.place[1] = s.few_at[lane()];
+        s.place[1] = s.few_at[threadIdx.x];
         s.found[0] = front + w;
       }
     }
@@ -555,7 +576,7 @@ __device__ inline Cut least_of(S& s, const Row& r, float q) {
 template <class S>
 __device__ inline void find(S& s, const Row& r, const Range& all, const Cut& cut, u64 before, u64 sum, double to, int* token, float* prob) {
   bool done = false;
-  walk<1>(r, all.a, all.b, [&](const float4& x, int i) {
+  walk<4>(r, all.a, all.b, [&](const float4& x, int i) {
     if (done) return;
     const float* e = (const float*)&x;
     u64 w[4], own_sum = 0;
@@ -575,8 +596,40 @@ __device__ inline void find(S& s, const Row& r, const Range& all, const Cut& cut
     done = (double)before > to;
   });
 }
+// The token where all that is kept is listed.
+__device__ inline void from_list(Lds& s, const Row& r, const Cut& cut, float draw, int* token, float* prob) {
+  const int n = s.number[wave()];
+  auto entry = [&](int p, int& i) {   // (its weight)
+    if (p >= n) return (u64)0;
+    const uint32_t k = s.key[wave() * LIST + p];
+    i = s.at[wave() * LIST + p];
+    return cut.keeps(k, i) ? weight(r, s.pow2, logit_of(k)) : 0;
+  };
+  u64 own = 0;
+  int i = 0;
+  for (int p = lane(); p < n; p += 64) own += entry(p, i);
+  own = wave_sum(own);
+  __syncthreads();
+  if (lane() == 0) s.kept[wave()] = own;
+  __syncthreads();
+  u64 sum = 0, at = 0;
+  for (int w = 0; w < WAVES; ++w) {
+    at += w < wave() ? s.kept[w] : 0;
+    sum += s.kept[w];
+  }
+  const double to = target(draw, sum);
+  if ((double)at > to || !((double)(at + own) > to)) return;
+  for (int p0 = 0; p0 < n; p0 += 64) {
+    const u64 w = entry(p0 + lane(), i), up = up_sum(w), front = at + up - w;
+    if (w && (double)front <= to && (double)(front + w) > to) {
+      *token = i;
+      if (prob) *prob = (float)((double)w / (double)sum);
+    }
+    at += __shfl(up, 63);
+  }
+}
 // A row by one work-group.
-__device__ inline void one_row(Lds& s, Row r, const Form& f, int* token, float* prob) {
+__device__ __forceinline__ void one_row(Lds& s, Row r, const Form& f, int* token, float* prob) {
   const Range whole = {0, r.units};
   float top, own;
   int where;
@@ -642,6 +695,10 @@ __device__ inline void one_row(Lds& s, Row r, const Form& f, int* token, float* 
   }
 
   cut = higher(cut, least);
+  if (small) {
+    from_list(s, r, cut, f.draw, token, prob);
+    return;
+  }
   // ---- the sum of what is kept, of each wave's sixteenth of the row: what lies above the members and what is kept of them, or everything
   if (!added) {
     m = {1, 0, cut, true};
@@ -719,7 +776,10 @@ typedef LdsOf<128> LdsPart;
 __device__ inline bool known(Row& r, const Place& g, const Form& f, float& top, int& where) {
   top = -INFINITY;
   where = 0x7FFFFFFF;
-  for (int i = 0; i < PARTS; ++i) first_of(top, where, g.top[i], g.where[i]);
+  const float t = g.top[lane() % PARTS];
+  const int w = g.where[lane() % PARTS];
+  for (int i = 0; i < PARTS; ++i)
+    first_of(top, where, __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(t), i)), __builtin_amdgcn_readlane(w, i));
   if (!(top > -INFINITY) || !(f.t > 0.0f)) return false;
   measure(r, top, f.t);
   return true;
@@ -767,6 +827,7 @@ extern "C" __global__ __launch_bounds__(1024) void sample_scan(SAMPLE_ARGS, char
   const Form f = form_of(temp, top_k, top_p, min_p, u, row);
   const Range mine = share({0, r.units}, part);
   const bool first = part == 0 && threadIdx.x == 0, by_k = f.by_k(V), by_p = f.by_p();
+  const float most = g.most[threadIdx.x];
   float top;
   int where;
   if (!known(r, g, f, top, where)) {
@@ -780,7 +841,7 @@ extern "C" __global__ __launch_bounds__(1024) void sample_scan(SAMPLE_ARGS, char
   powers(s);
   __syncthreads();
   if (by_k && f.k <= SMALL_K) {
-    const Members m = {reached(s, g.most[threadIdx.x], f.k), key_of(top), {NONE, 0x7FFFFFFF}, true};
+    const Members m = {reached(s, most, f.k), key_of(top), {NONE, 0x7FFFFFFF}, true};
     if (first) {
       g.lo = m.lo;
       g.hi = m.hi;
@@ -843,46 +904,52 @@ extern "C" __global__ __launch_bounds__(1024) void sample_draw(SAMPLE_ARGS, char
   const Place& g = ((const Place*)room)[row];
   Row r = row_of(logits, ld, off, V, row);
   const Form f = form_of(temp, top_k, top_p, min_p, u, row);
-  int mode = g.mode;
-  if (mode == ANSWERED) return;
-  if (mode == BINNED) mode = g.then;
-  int members = 0;
+  // (all on its way at once)
+  const int told = g.mode, then = g.then, number = g.number[lane() % PARTS];
+  const uint32_t lo = g.lo, hi = g.hi, key = g.key[wave() * RUN + lane()], at = g.at[wave() * RUN + lane()];
+  const u64 need = g.need, sums = threadIdx.x < PARTS * WAVES ? g.part[threadIdx.x] : 0;
+  float top;
+  int where;
+  const bool drawn = known(r, g, f, top, where);
+  if (told == ANSWERED) return;
+  int mode = told == BINNED ? then : told, members = 0;
   if (mode == SMALL || mode == LISTED) {
-    bool fits = true;
-    for (int i = 0; i < PARTS; ++i) {
-      fits = fits && (uint32_t)g.number[i] <= (uint32_t)RUN;
-      members += g.number[i];
-    }
-    if (!fits) mode = WHOLE;
+    for (int i = 0; i < PARTS; ++i) members += __builtin_amdgcn_readlane(number, i);
+    if (__any((uint32_t)number > (uint32_t)RUN)) mode = WHOLE;
   }
   if (mode == WHOLE) {
     one_row(s, r, f, token + row, prob ? prob + row : nullptr);
     return;
   }
-  float top;
-  int where;
-  if (!known(r, g, f, top, where)) return;
+  if (!drawn) return;
   powers(s);
-  __syncthreads();
-  const Cut least = least_of(s, r, f.q);
-  Cut cut = least;
-  for (int i = threadIdx.x; i < PARTS * WAVES; i += THREADS) s.sum[i] = mode == SMALL ? 0 : g.part[i];
+  if (threadIdx.x < PARTS * WAVES) s.sum[threadIdx.x] = sums;
   if (mode != SUMS) {
-    const int n = g.number[wave()];
-    for (int p = lane(); p < n; p += 64) {
+    const int n = __builtin_amdgcn_readlane(number, wave());
+    s.key[wave() * LIST + lane()] = key;
+    s.at[wave() * LIST + lane()] = at;
+    for (int p = 64 + lane(); p < n; p += 64) {
       s.key[wave() * LIST + p] = g.key[wave() * RUN + p];
       s.at[wave() * LIST + p] = g.at[wave() * RUN + p];
     }
     if (lane() == 0) s.number[wave()] = n;
-    __syncthreads();
-    Members m = {g.lo, g.hi, {NONE, 0x7FFFFFFF}, true};
+  }
+  __syncthreads();
+  const Cut least = least_of(s, r, f.q);
+  Cut cut = least;
+  if (mode != SUMS) {
+    Members m = {lo, hi, {NONE, 0x7FFFFFFF}, true};
     u64 rest;
-    cut = select(s, r, m, mode == LISTED && f.by_p(), mode == SMALL ? (u64)min(f.k, members) : g.need, rest);
+    cut = select(s, r, m, mode == LISTED && f.by_p(), mode == SMALL ? (u64)min(f.k, members) : need, rest);
     if (mode == SMALL && f.by_p()) {
       m.within = cut;
       cut = select(s, r, m, true, f.goal(rest), rest);
     }
     cut = higher(cut, least);
+    if (mode == SMALL) {
+      from_list(s, r, cut, f.draw, token + row, prob ? prob + row : nullptr);
+      return;
+    }
     // the members that are kept, to the sums of their units
     const Range c = share({0, r.units}, wave());
     const int per = max((c.b - c.a + WAVES - 1) / WAVES, 1);

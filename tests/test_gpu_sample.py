@@ -254,7 +254,7 @@ def test_in_a_launch_list(eng):
     ref.free(b)
 
 
-@pytest.mark.parametrize("T,V,launches", [(1, 40000, 4), (16, 40000, 4), (16, 39999, 1), (17, 42500, 4), (17, 42499, 1), (1, 2, 1)])
+@pytest.mark.parametrize("T,V,launches", [(1, 48000, 4), (16, 48000, 4), (16, 47999, 1), (17, 51000, 4), (17, 50999, 1), (1, 2, 1)])
 def test_the_work_groups_of_a_row(T, V, launches):
     """By the sizes; a first call of few long rows needs room, which no list being recorded can make."""
     e = az.Engine(16, 256)
