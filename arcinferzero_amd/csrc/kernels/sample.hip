@@ -21,7 +21,7 @@
 // over the whole row instead, eight bits at a time.
 // Bound: the 64-bit steps of the weights, some twenty instructions a token each time that they are wanted -- once for the histogram, once for the sums --, and for
 // few rows the steps themselves, of which none begins before the last one's sums have met.  A row is read from HBM once and from the caches after that.
-// Measured, 256 rows of 151936: the largest logit 27 us (5.7 TB/s), by k and p 60, drawn among all 75, by p 138; 37 rows of 32001 of all kinds 36; one row of
+// Measured, 256 rows of 151936: the largest logit 27 us (5.7 TB/s), by k and p 60, drawn among all 74, by min_p 60, by p 139; 37 rows of 32001 of all kinds 36; one row of
 // 151936 by sixteen work-groups, by k and p 26 us, by p 34.  A cut in rows that are almost flat (a temperature of 1000) takes 560.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -30,11 +30,15 @@ namespace {
 typedef unsigned long long u64;
 constexpr int THREADS = 1024, WAVES = 16, LIST = 512, BINS = 3 * THREADS;   // (48 octaves)
 // The highest k that is looked for among the threads' largest logits (of 1024: the nearer to them all, the more tokens reach the k-th).  Measured, us, this
-// way / by the histogram: 256 rows of 151936, k = 512 65 / 175, 960 80 / 173; with a cut by p behind it 73 / 190, 91 / 189; one row, k = 960 37 / 35, with p 46 / 134.
+// way / by the histogram: 256 rows of 151936, k = 512 65 / 175, 960 80 / 173; with a cut by p behind it 73 / 190, 91 / 189; one row, k = 960 37 / 35, with p 46 / 116.
 constexpr int SMALL_K = 960;
 // Listed tokens of which each is compared with all others.  37 rows of 32001, by k and p: k = 50 21 us (by digits 36), k = 200, 220 tokens, 32, k = 256, which go by
 // digits, 33.  (Going down the bits of up to 512 in one wave's registers: 42 for 100, 58 for 400.)
 constexpr int FEW = 256;
+// Kept logits of 256 that are put together before their weights are worked out.  Measured, us, all where they lie / put together: 256 rows of 151936 cut by
+// min_p 75 / 60, one row of 32001 by p 36 / 33, one of 151936 by k = 2000 and p 135 / 116; rows of which half is kept 138 / 139 (of which all is: where they lie,
+// 74; with the votes 80).
+constexpr int SPARSE = 128;
 constexpr uint32_t NONE = 0x007FFFFFu;                                             // the key of -inf: no token
 
 // CAP: tokens of a wave that the list takes.
@@ -47,6 +51,7 @@ struct LdsOf {
   uint32_t key[WAVES * CAP], at[WAVES * CAP];   // the list: a run of each wave's, in the row's order
   uint32_t few_key[FEW], few_at[FEW];           // ... of few members, the runs behind one another
   u64 few_weight[FEW];
+  float held[WAVES * (64 + SPARSE)];            // logits that are kept, a wave's on their way to their weights
   u64 digit_sum[256];
   uint32_t digit[256];
   u64 part[WAVES], kept[WAVES];
@@ -192,7 +197,7 @@ struct Members {
   __device__ bool has(uint32_t k, int i) const { return (k >= lo) & (k <= hi) & within.keeps(k, i); }
 };
 // Over units of the row: its members (of a range; `within` everything) to LDS -- false: there are more than it takes --, and where `add` the weights of those that
-// `floor` keeps added up, each wave's to part[].
+// `floor` keeps added up, each wave's to part[] (where it keeps everything there are no members).
 template <class S>
 __device__ inline bool pass(S& s, const Row& r, const Range& all, const Members& m, bool add, const Cut& floor) {
   constexpr int CAP = S::CAP;
@@ -229,15 +234,44 @@ __device__ inline bool pass(S& s, const Row& r, const Range& all, const Members&
   if (!add) {
     walk<8>(r, mine.a, mine.b, members);
   } else {
+    // Where few are kept of 256 they are put together first, so that a wave works out the weights of 64 of them at a time.
+    float* const held = s.held + wave() * (64 + SPARSE);
+    const bool every = floor.key <= NONE;
+    int pending = 0;
     walk<4>(r, mine.a, mine.b, [&](const float4& v, int i) {
       const float* e = (const float*)&v;
+      bool keep[4];
+      u64 vote[4];
+      int n = 0;
+      if (every) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum += weight(r, s.pow2, e[j]);
+        return;
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        // (what is not kept as -inf: of weight 0)
-        sum += weight(r, s.pow2, (e[j] > edge) | ((e[j] == edge) & (i + j <= floor.last)) ? e[j] : -INFINITY);
+        keep[j] = (e[j] > edge) | ((e[j] == edge) & (i + j <= floor.last));
+        vote[j] = __ballot(keep[j]);
+        n += __popcll(vote[j]);
+      }
+      if (n > SPARSE) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum += weight(r, s.pow2, keep[j] ? e[j] : -INFINITY);   // (of weight 0)
+      } else if (n) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int at = pending + __builtin_amdgcn_mbcnt_hi((uint32_t)(vote[j] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)vote[j], 0));
+          if (keep[j]) held[at] = e[j];
+          pending += __popcll(vote[j]);
+        }
+        while (pending >= 64) {
+          pending -= 64;
+          sum += weight(r, s.pow2, held[pending + lane()]);
+        }
       }
       if (any) members(v, i);
     });
+    if (pending) sum += weight(r, s.pow2, lane() < pending ? held[lane()] : -INFINITY);
     sum = wave_sum(sum);
   }
   if (lane() == 0) {
