@@ -50,6 +50,26 @@ __device__ inline int find(const int (&sums)[PLAN], int i) {
   return at;
 }
 
+// Of `total` things, so many of each sequence, one a thread, four of a thread's on their way at once: put(sequence, thing, get(sequence, thing)).
+template <class G, class P>
+__device__ inline void deal(const int (&sums)[PLAN], int total, G get, P put) {
+  const int local = blockDim.x;
+  for (int i0 = threadIdx.x; i0 < total; i0 += 4 * local) {
+    int at[4] = {0, 0, 0, 0}, i[4], v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) i[k] = min(i0 + k * local, total - 1);
+    for (int step = local / 2; step; step /= 2)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (sums[at[k] + step] <= i[k]) at[k] += step;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = get(at[k], i[k]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i0 + k * local < total) put(at[k], i[k], v[k]);
+  }
+}
+
 // state, after: the ring's first place, how many pages it holds, what was missing (0: nothing; pages; -1: rows or table), the rows of the plan.
 // before may be len, state may be after.  grid 1, local 256 (no more sequences than that) or 1024.  with_rows: pos and slot too.
 extern "C" __global__ __launch_bounds__(PLAN) void kv_plan(const int* __restrict__ add, const int* before, int* len, int* __restrict__ rows, int* __restrict__ table,
@@ -146,16 +166,12 @@ extern "C" __global__ __launch_bounds__(PLAN) void kv_plan(const int* __restrict
       s_has[threadIdx.x] = c.has;
       s_before[threadIdx.x] = c.before;
       __syncthreads();
-      for (int i = threadIdx.x; i < total.give; i += local) {
-        const int j = find(s_give, i);
-        ring[attn::ring_at(tail, at.give + i, pages)] = table[(size_t)(s0 + j) * ldt + s_has[j] + (i - s_give[j])];
-      }
+      deal(s_give, total.give, [&](int j, int i) { return table[(size_t)(s0 + j) * ldt + s_has[j] + (i - s_give[j])]; },
+           [&](int, int i, int page) { ring[attn::ring_at(tail, at.give + i, pages)] = page; });
     }
     if (apart) {
-      for (int i = threadIdx.x; i < total.take; i += local) {
-        const int j = find(s_take, i);
-        table[(size_t)(s0 + j) * ldt + s_had[j] + (i - s_take[j])] = ring[attn::ring_at(head, at.take + i, pages)];
-      }
+      deal(s_take, total.take, [&](int, int i) { return ring[attn::ring_at(head, at.take + i, pages)]; },
+           [&](int j, int i, int page) { table[(size_t)(s0 + j) * ldt + s_had[j] + (i - s_take[j])] = page; });
       if (with_rows)
         for (int i = threadIdx.x; i < total.rows; i += local) {
           const int j = find(s_rows, i), p = s_before[j] + (i - s_rows[j]), e = p >> ps;
