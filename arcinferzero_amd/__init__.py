@@ -1,5 +1,6 @@
 """MI355X-native GGUF block-quantized matmul (prefill GEMM, decode GEMV, MoE grouped GEMM) and the
-attention block beside it (rotary positions, an 8-bit cache, attention over it) behind a C ABI.
+attention block beside it (rotary positions with and without norms, an 8-bit cache and plans for its pages, attention over it,
+also behind shared prefixes) and tokens drawn from logits, behind a C ABI.
 
 The compute path is the in-tree shared library ``libarcz_hip.so`` (hand-written HIP for gfx950 plus the C++ host
 dispatch); this package is a thin ctypes binding over ``include/arcz_hip.h`` and ``include/arcz_engine.h`` with numpy

@@ -11,7 +11,8 @@
 // Bound: latency -- one work-group for all sequences, since the sums run over them: the counts, their sums in three steps over the
 // waves, then the ring's entries and the table's, a thread each.  Places of many rows are a launch of their own (kv_places), a work-group for
 // 1024 of one sequence's, behind it.
-// Measured: 256 sequences of a token 3.8 us, 1024 5.6, 256 of eight 5.6, 64 prompts of 256 tokens 6.7 in two launches, 1024 of them 13.5; a launch that does
+// Measured: 256 sequences of a token 3.8 us, 1024 5.6, 256 of eight 5.6, 64 prompts of 256 tokens 6.7 in two launches, 1024 of up to 500 12.1 (13.6 with one page of a thread's looked up
+// at a time); a launch that does
 // nothing takes 2.5.
 #include "attn.h"
 
@@ -53,11 +54,12 @@ __device__ inline int find(const int (&sums)[PLAN], int i) {
 // Of `total` things, so many of each sequence, one a thread, four of a thread's on their way at once: put(sequence, thing, get(sequence, thing)).
 template <class G, class P>
 __device__ inline void deal(const int (&sums)[PLAN], int total, G get, P put) {
-  const int local = blockDim.x;
-  for (int i0 = threadIdx.x; i0 < total; i0 += 4 * local) {
+  const unsigned local = blockDim.x, all = total;   // (no sum here passes 32 bits: total is below 2^31)
+  unsigned i0 = 0;
+  for (; all > i0 + local; i0 += 4 * local) {
     int at[4] = {0, 0, 0, 0}, i[4], v[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) i[k] = min(i0 + k * local, total - 1);
+    for (int k = 0; k < 4; ++k) i[k] = (int)min(i0 + k * local + threadIdx.x, all - 1);
     for (int step = local / 2; step; step /= 2)
 #pragma unroll
       for (int k = 0; k < 4; ++k)
@@ -66,7 +68,11 @@ __device__ inline void deal(const int (&sums)[PLAN], int total, G get, P put) {
     for (int k = 0; k < 4; ++k) v[k] = get(at[k], i[k]);
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (i0 + k * local < total) put(at[k], i[k], v[k]);
+      if (i0 + k * local + threadIdx.x < all) put(at[k], i[k], v[k]);
+  }
+  if (i0 + threadIdx.x < all) {
+    const int i = (int)(i0 + threadIdx.x), at = find(sums, i);
+    put(at, i, get(at, i));
   }
 }
 
