@@ -320,3 +320,73 @@ def test_refusals(eng):
     eng.sample(x, 128, 0, 128, 0, none, u, tok, pr)
     assert az.lib.arcz_launch_count() == n
     ref.free([x, small, u, tok, pr, short, view])
+
+
+@pytest.fixture
+def two():
+    e = []
+    for split in ("0", "1"):
+        os.environ["ARCZ_SAMPLE_SPLIT"] = split
+        e.append(az.Engine(16, 256))
+        del os.environ["ARCZ_SAMPLE_SPLIT"]
+    yield e
+    for x in e:
+        x.close()
+
+
+@pytest.mark.parametrize("V,off,ld", [(60001, 0, 60001), (151936, 3, 151940), (2049, 1, 2051), (63, 0, 64), (1, 0, 1)])
+def test_one_work_group_and_sixteen_give_the_same_bits(rt, two, V, off, ld):
+    """Sums of whole numbers: which work-group adds them does not matter."""
+    T, rng = 24, np.random.default_rng(V)
+    x = np.zeros((T, ld), np.float32)
+    x[:, off:off + V] = rows(T, V, seed=2)
+    x[5, off:off + V] = 1.25                                     # (all equal)
+    x[6, off:off + V] = np.round(x[6, off:off + V])              # (many equal)
+    x[7, off:off + V] = -np.inf
+    x[8, off + V // 2] = np.inf
+    given = [np.array(rng.choice(a, T), d) for a, d in (([0.0, 0.3, 1.0, 1.7, 40.0], np.float32), ([0, 1, 50, 300, 960, 961, 5000], np.int32), ([1.0, 0.95, 0.5, 0.01], np.float32),
+                                                        ([0.0, 0.001, 0.2], np.float32))]
+    hold = [az.Runtime.from_numpy(a) for a in (x, rng.random(T).astype(np.float32), *given)]
+    got = []
+    for e in two:
+        out = [az.Runtime.from_numpy(np.full(T, -9, np.int32)) for _ in range(2)]
+        e.sample(hold[0], ld, off, V, T, az.Sampling(*hold[2:]), hold[1], *out)
+        got.append([o.read(np.int32) for o in out])
+        ref.free(out)
+    assert np.array_equal(got[0], got[1])
+    ref.free(hold)
+
+
+def test_lists_that_share_the_engines_room(rt):
+    """Keys shared out and rows in sixteen parts go through one room: recorded lists of both, replayed in turn with eager calls between them."""
+    eng, V, hold = az.Engine(16, 256), 50000, []
+    c = ref.Cache(40, 128, 64, 2, 128, seed=4)
+    kv = ref.device_cache(eng, c, hold)
+    rng = np.random.default_rng(6)
+    dev = {n: az.Runtime.from_numpy(a) for n, a in dict(rows=np.arange(3, dtype=np.int32), len=np.array([4900, 120], np.int32), table=rng.permutation(80).astype(np.int32) % 40,
+                                                       q=rng.standard_normal((2, 8 * 128)).astype(np.float32), out=np.zeros((2, 8 * 128), np.float32), x=rows(3, V, seed=8),
+                                                       u=np.array([0.1, 0.5, 0.9], np.float32), p=np.array([0.9, 1.0, 0.4], np.float32), token=np.zeros(3, np.int32)).items()}
+    batch, form, how = az.KvBatch(dev["rows"], dev["len"], dev["table"], 2, 40, 2, 1, 4900), az.Attention(0.1), az.Sampling(top_p=dev["p"])
+
+    def attend():
+        eng.attention(kv, batch, dev["q"], 8 * 128, 0, 8, dev["out"], 8 * 128, 0, form)
+
+    def draw():
+        eng.sample(dev["x"], V, 0, V, 3, how, dev["u"], dev["token"])
+    calls, outs = (attend, draw), ("out", "token")
+    for f in calls:
+        f()
+    want = [dev[n].read(np.uint32) for n in outs]
+    lists = [az.Runtime.record(f) for f in calls]
+    assert lists[1].launches == 4
+    for i in range(3):
+        for j in ((0, 1), (1, 0), (1, 1))[i]:
+            dev[outs[j]].fill(0)
+            dev[outs[1 - j]].fill(0)
+            lists[j].run()
+            calls[1 - j]()
+            assert all(np.array_equal(dev[n].read(np.uint32), w) for n, w in zip(outs, want))
+    for l in lists:
+        l.free()
+    ref.free(hold + list(dev.values()))
+    eng.close()
