@@ -416,7 +416,8 @@
     double front = 0.0;
     if (p.tiles1 && pairs1) {
       const double sets = c.heads * std::min((double)sh.n * p.tiles1, std::ceil((double)b.T * p.G / p.bm1) + 0.5 * (sh.n - 1));
-      const int most = std::max(1, (shared + 127) / 128);
+      // (max_rows may say more than the groups have: the room is for what it says)
+      const int most = (int)std::max<size_t>(1, std::min<size_t>((size_t)(shared + 127) / 128, 8 * cus / (pairs1 * p.tiles1)));
       for (int r = 0; r <= 4; ++r) {
         const int n = r ? std::min(most, (int)(r * cus / sets)) : 1;
         if (n < 1) continue;
