@@ -440,7 +440,7 @@ def _plain_sample(s):
     V = s.case["V"]
     top = s.x.amax(-1, keepdim=True)
     greedy = s.x.argmax(-1)
-    w = ((s.x.double() - top.double()) / s.temp.double().clamp_min(1e-30)[:, None]).exp()
+    w = ((s.x - top).double() / s.temp.double().clamp_min(1e-30)[:, None]).exp()
     order = torch.sort(s.x, dim=-1, descending=True, stable=True).indices
     sorted_w = w.gather(1, order)
     rank = torch.arange(V, device="cuda")
