@@ -129,6 +129,18 @@ ATTN_FN Change change_of(int before, int add, int shared, int ps, int ldt, int m
   c.give = upper(c.had - c.has, 0);
   return c;
 }
+// ... and the change that a plan takes: no row in one of the whole pages of the first `shared` positions, which are others' too -- what is written there
+// would be theirs as well, and a page that is taken for it would be given back by nobody, since those entries stay.
+ATTN_FN Change planned(int before, int add, int shared, int ps, int ldt, int max_rows) {
+  Change c = change_of(before, add, shared, ps, ldt, max_rows);
+  if (add > 0 && c.before < lower(upper(shared, 0), ldt << ps) >> ps << ps) {
+    c.fits = false;
+    c.rows = c.take = 0;
+    c.len = c.before;
+    c.has = c.had;
+  }
+  return c;
+}
 // The i-th place behind `from` in a ring of n (from below n, i at most n).
 ATTN_FN unsigned ring_at(unsigned from, unsigned i, unsigned n) {
   const unsigned k = from + i;   // (below 2^32: n is below 2^31)

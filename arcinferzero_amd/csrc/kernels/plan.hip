@@ -5,8 +5,8 @@
 //   of free pages, in the order of the sequences; those that a shorter sequence leaves go to the ring's end;  row i of a sequence has the
 //   position before + i and the place page * (tokens a page) + position % (tokens a page).
 // What is taken lies in front of what is given back, so a page that one sequence loses is not another's in the same plan, and no
-// work depends on the order in which it is done.  All or nothing: where the pages, the table or the rows do not suffice nothing is
-// changed and no sequence has rows.
+// work depends on the order in which it is done.  All or nothing: where the pages, the table or the rows do not suffice, or a row would lie in
+// a page that other sequences share, nothing is changed and no sequence has rows.
 //
 // Bound: latency -- one work-group for all sequences, since the sums run over them: the counts, their sums in three steps over the
 // waves, then the ring's entries and the table's, a thread each.  Places of many rows are a launch of their own (kv_places), a work-group for
@@ -86,7 +86,7 @@ extern "C" __global__ __launch_bounds__(PLAN) void kv_plan(const int* __restrict
   __shared__ int s_rows[PLAN], s_take[PLAN], s_give[PLAN], s_had[PLAN], s_has[PLAN], s_before[PLAN];
   __shared__ unsigned long long sums[3];
   const int local = blockDim.x, mask = (1 << ps) - 1;
-  auto change = [&](int s) { return attn::change_of(before[s], add[s], shared ? shared[s] : 0, ps, ldt, max_rows); };
+  auto change = [&](int s) { return attn::planned(before[s], add[s], shared ? shared[s] : 0, ps, ldt, max_rows); };
   auto place = [&](int pg, int p) { return (unsigned)pg < (unsigned)pages ? (pg << ps) + (p & mask) : -1; };
   Change c = {0, 0, 0, 0, 0, 0, 0, true};   // (of this thread's first sequence)
   if ((int)threadIdx.x < seqs) c = change(threadIdx.x);

@@ -224,12 +224,14 @@ typedef struct arcz_kv_batch {
  *                  sequence by sequence; pages that a shorter sequence leaves go behind its end, to be taken by later plans
  *   state [4]      in: the ring's first place and its count.  after [4], which may be state itself, out: both behind the plan; what was missing;
  *                  the rows of the plan
- *   shared [seqs]  (NULL: 0) the positions of a sequence's prefix whose whole pages are also others': they are not given back
+ *   shared [seqs]  (NULL: 0) the positions of a sequence's prefix whose whole pages are also others': these stay in its table, are not given back
+ *                  and get no rows.  A sequence that is shorter than them (taken back that far, or ended) gets tokens again once its length
+ *                  has been set to theirs, or above; one that is to fill such pages itself has shared 0 until they are full
  *   pos [T]        (NULL: not wanted) the position of each row, as arcz_engine_rope takes them
  *   slot [T]       (NULL: not wanted) page * (tokens a page) + position % (tokens a page), -1 where the table has no page of the cache
- * `page` is the cache's tokens a page, `pages` its pages.  rows [seqs + 1] = the running sum of max(add, 0), len = max(0, before + add), row i
+ * `page` is the cache's tokens a page, `pages` its pages.  rows [seqs + 1] = the running sum of max(add, 0), len = max(0, before + add) (before held to 0 ... what the table holds), row i
  * of a sequence has position before + i.  All or nothing: where pages are missing (after[2] = how many), or an add is above max_rows, the rows
- * above T, a length above what the table holds or the state none of such a ring (after[2] = -1), the lengths, the ring and the table stay as
+ * above T, a length above what the table holds, a row in a page that is shared or the state none of such a ring (after[2] = -1), the lengths, the ring and the table stay as
  * they are, rows is all 0 -- the pass's other calls then have nothing to do -- and pos and slot are left alone; else after[2] = 0.  Entries behind a sequence's pages are left as
  * they are, and so are pos and slot behind the last row.  What is written must not meet what is read, nor each other, but for the two
  * that may be brought on in place.  Pages of a table entry that is none of the cache are given back as they are found. */
