@@ -387,7 +387,7 @@
   };
   // The launches of a call, by what the host knows of it, and where its workspace has what they leave.
   struct SharedShape {
-    int G, form, M, M1, waves1, bm1, tiles1, n1, few, rt, pack, b2, tiles2, n2, least;
+    int G, form, M, M1, waves1, bm1, tiles1, n1, few, rt, pack, tiles2, n2, least;
     size_t ws1, ws2, bytes;
     bool one;
   };
@@ -416,7 +416,7 @@
     double front = 0.0;
     if (p.tiles1 && pairs1) {
       const double sets = c.heads * std::min((double)sh.n * p.tiles1, std::ceil((double)b.T * p.G / p.bm1) + 0.5 * (sh.n - 1));
-      // (max_rows may say more than the groups have: the room is for what it says)
+      // (max_rows may say more than the groups have: the grid is for what it says)
       const int most = (int)std::max<size_t>(1, std::min<size_t>((size_t)(shared + 127) / 128, 8 * cus / (pairs1 * p.tiles1)));
       for (int r = 0; r <= 4; ++r) {
         const int n = r ? std::min(most, (int)(r * cus / sets)) : 1;
@@ -432,13 +432,11 @@
     if (p.few) {
       p.rt = M > 16 ? 2 : 1;
       p.pack = M <= 8 ? 1 : 0;
-      p.b2 = p.pack ? 8 : 16 * p.rt;
       p.tiles2 = 1;
       const size_t want = (2 * cus + pairs - 1) / std::max<size_t>(1, pairs);
       p.least = (int)std::max<size_t>(8, ((size_t)(own + 31) / 32 + want - 1) / std::max<size_t>(1, want));
       p.n2 = (int)(((int64_t)own + (int64_t)32 * p.least - 1) / ((int64_t)32 * p.least));
     } else {
-      p.b2 = 128;
       p.tiles2 = (int)((M + 127) / 128);
       p.n2 = (int)std::max<size_t>(1, std::min<size_t>(2 * cus / std::max<size_t>(1, pairs * p.tiles2), (size_t)(own + 255) / 256));
     }
@@ -461,14 +459,16 @@
       p.bytes = 256;
       return p;
     }
-    if (pairs * p.tiles2 > 0xFFFFFFFFull / 256 || pairs1 * p.tiles1 > 0xFFFFFFFFull / 512) throw std::runtime_error("attention_shared: too many rows");
+    // (the last launch has a thread for each four values)
+    const size_t each = (size_t)b.T * heads;   // (rows of a piece)
+    if (pairs * p.tiles2 > 0xFFFFFFFFull / 256 || pairs1 * p.tiles1 > 0xFFFFFFFFull / 512 || each > 0x7FFFFFFF || each * c.hd / 4 > 0xFFFFFF00ull) throw std::runtime_error("attention_shared: too many rows");
     auto place = [&](size_t bytes) {
       const size_t at = p.bytes;
       p.bytes += (bytes + 255) / 256 * 256;
       return at;
     };
-    p.ws1 = place(pairs1 * p.tiles1 * p.n1 * p.bm1 * (c.hd + 2) * 4);
-    p.ws2 = place(pairs * p.tiles2 * p.n2 * p.b2 * (c.hd + 2) * 4);
+    p.ws1 = place(each * p.n1 * (c.hd + 2) * 4);
+    p.ws2 = place(each * p.n2 * (c.hd + 2) * 4);
     p.bytes = std::max<size_t>(p.bytes, 256);
     return p;
   }
@@ -504,7 +504,7 @@
       if (overlap(ro.place(), i) || overlap(work, i)) throw std::runtime_error("attention_shared: out or the room overlaps slopes, prefix, first or the groups");
     if (p.one) return attention(c, b, q, ldq, q_off, heads, out, ldo, o_off, a);
     int pages = c.pages, ps = c.ps, bs = c.bs, ldt = b.ld_table, T = b.T, mr = std::min(b.max_rows, b.T), kvh = c.heads, window = std::min(a.window, 1 << 30), hd = c.hd, seqs = b.seqs, n = sh.n;
-    int most = ldt * c.page, mr1 = std::min(sh.max_rows, b.T), vec = rq.vec() ? 1 : 0, n1 = p.n1, n2 = p.n2, bm1 = p.bm1, b2 = p.b2, t1 = p.tiles1, t2 = p.tiles2, least = p.least;
+    int mr1 = std::min(sh.max_rows, b.T), vec = rq.vec() ? 1 : 0, n1 = p.n1, n2 = p.n2, t1 = p.tiles1, t2 = p.tiles2, least = p.least;
     float scale = a.scale, cap2 = a.cap * 1.4426950408889634f;
     auto part = [&](const char* name, int front, size_t sets, int rows, int waves, int tiles, int nsplit, size_t ws) {
       cl_kernel k = variant("attn", {{"HD", c.hd}, {"FINE", c.block < 32 ? 1 : 0}, {"FORM", p.form}, {waves == 8 ? "W8" : nullptr, 1}}, "attn_part");
@@ -524,10 +524,10 @@
       part("attention_own", 0, (size_t)seqs, mr, 4, t2, n2, p.ws2);
     }
     cl_kernel k = variant("attn", {}, "attn_meet");
-    set_args(k, 0, room, p.ws1, n1, bm1, t1, mr1, p.ws2, n2, b2, t2, hd, b.rows, b.len, most, T, mr, heads, kvh, sh.groups, sh.len, n, seqs, out, ldo, o_off);
-    const int per = 1024 / c.hd;
-    size_t g[2] = {(size_t)seqs * c.heads * 256, (size_t)((p.M + per - 1) / per)}, l[2] = {256, 1};
-    run("attention_meet", k, 2, g, l);
+    set_args(k, 0, room, p.ws1, n1, p.ws2, n2, hd, b.rows, T, mr, heads, sh.groups, sh.len, n, seqs, mr1, out, ldo, o_off);
+    const size_t per = 1024 / c.hd;
+    size_t g = ((size_t)T * heads + per - 1) / per * 256, l = 256;
+    run("attention_meet", k, 1, &g, &l);
   }
   void join(const Kv& c, const Batch& b, cl_mem w, int nsplit, int rows, int blocks, int mr, int heads, cl_mem out, int ldo, int o_off) {
     int hd = c.hd, most_len = b.ld_table * c.page, T = b.T, kvh = c.heads, per = 1024 / c.hd;

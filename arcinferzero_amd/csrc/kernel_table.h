@@ -142,7 +142,7 @@ static const KernelSpec kKernelTable[] = {
     {"attn", "attn_part", "W8", "piippppiiipppiiiiiffipppppiiiipziii", {"HD", "FINE", "FORM", "W8", nullptr}, {{nullptr, 0, false}}, 512},
     {"attn", "attn_part", nullptr, "piippppiiipppiiiiiffipppppiiiipziii", {"HD", "FINE", "FORM", nullptr}, {{nullptr, 0, false}}, 256},
     {"attn", "attn_part_few", nullptr, "piippppiiipppiiiiiffipppppipziii", {"HD", "RT", "PACK", "FINE", "FORM", nullptr}, {{nullptr, 0, false}}, 256},
-    {"attn", "attn_meet", nullptr, "pziiiiziiiippiiiiippiipii", {nullptr}, {{nullptr, 0, false}}, 256},
+    {"attn", "attn_meet", nullptr, "pziziipiiippiiipii", {nullptr}, {{nullptr, 0, false}}, 256},
     {"attn", "attn_join", nullptr, "piiiippiiiiipii", {nullptr}, {{nullptr, 0, false}}, 256},
     {"moe", "moe_combine", nullptr, "pppppi", {nullptr}, {{"NU", 0, true}, {nullptr, 0, false}}, 256},
 };

@@ -19,38 +19,52 @@
 // A call's workspace, the room: what these launches leave for the last one, each from its own byte on.
 __device__ inline float* in_room(char* room, size_t at) { return (float*)(room + at); }
 
-// The parts joined: the group's rows have n1 pieces in blocks of b1, the sequence's n2 in blocks of b2, t1 and t2 blocks each; a piece is sums
-// [b][hd], then reference and sum of weights [b][2].  Rows past the group's `most1` are left as they are.  grid (sequences x kv heads, row groups
-// of 1024 / hd), 256.
-extern "C" __global__ __launch_bounds__(256) void attn_meet(char* __restrict__ room, size_t at1, int n1, int b1, int t1, int most1, size_t at2, int n2, int b2, int t2, int hd,
-                                                            const int* __restrict__ rows, const int* __restrict__ lens, int most_len, int T, int max_rows, int heads,
-                                                            int kvh, const int* __restrict__ groups, const int* __restrict__ shared, int n, int seqs,
-                                                            float* __restrict__ out, int ldo, int o_off) {
-  const float *const ws1 = in_room(room, at1), *const ws2 = in_room(room, at2);
-  const int s = blockIdx.x / kvh, h = blockIdx.x - s * kvh, G = heads / kvh, per = 1024 / hd;
-  const Seq sq = seq_of(rows, lens, s, T, max_rows, most_len);
-  const int r = blockIdx.y * per + threadIdx.x / (hd / 4), d = threadIdx.x % (hd / 4) * 4;
-  if (blockIdx.y * per >= sq.n * G) return;
-  const int g = attn::group_of(groups, n, s), first_row = g < 0 ? 0 : attn::part_at(groups, rows, g, seqs, T, T).r0;
-  if (r >= sq.n * G || r >= t2 * b2) return;
-  const int i = r / G, ig = sq.r0 + i - first_row;   // (its place among the group's rows)
-  if (g >= 0 && (ig < 0 || ig >= most1)) return;
+// The sequence that a row belongs to, the row being the same in all lanes, each of which looks at one of 64 boundaries at a time; some one of them where
+// the rows are in no order.
+__device__ inline int seq_of_one_row(const int* __restrict__ rows, int seqs, int t) {
+  int a = 0, n = seqs;   // (one of [a, a + n))
+  while (n > 1) {
+    const int step = (n + 63) / 64, b = a + step * ((int)(threadIdx.x & 63) + 1), end = a + n;
+    a += step * __popcll(__ballot(b < end && rows[min(b, seqs)] <= t));
+    n = min(step, end - a);
+  }
+  return a;
+}
+
+// The parts joined: a row and head has n1 pieces of its group's keys and n2 of its own, in the batch's order of rows: sums [piece][T][heads][hd], then
+// reference and sum of weights [piece][T][heads][2].  (So the room, and this launch, are as large as the batch, however unlike its sequences are:
+// one of 2048 tokens beside 255 of a token, 64 heads of 128 values, 0.15 GB; blocks of the longest one's rows for each would be 8.8.)  Rows
+// past the group's `most1`, past max_rows of a sequence, or of none, are left as they are.  grid (T x heads / (1024 / hd)), 256.
+extern "C" __global__ __launch_bounds__(256) void attn_meet(char* __restrict__ room, size_t at1, int n1, size_t at2, int n2, int hd, const int* __restrict__ rows, int T,
+                                                            int max_rows, int heads, const int* __restrict__ groups, const int* __restrict__ shared, int n, int seqs,
+                                                            int most1, float* __restrict__ out, int ldo, int o_off) {
+  const unsigned at = blockIdx.x * (1024u / hd) + threadIdx.x / (hd / 4), t = at / heads, hq = at - t * heads;   // (the host holds T * heads below 2^31)
+  const int d = threadIdx.x % (hd / 4) * 4;
+  const int t0 = min(__builtin_amdgcn_readfirstlane(t), T - 1), s0 = seq_of_one_row(rows, seqs, t0);
+  if (t >= (unsigned)T) return;
+  const int s = (int)t == t0 ? s0 : attn::seq_of_row(rows, s0, seqs, t0, T - t0, t);   // (few heads: a wave has values of several rows)
+  const Seq sq = attn::part_at(nullptr, rows, s, seqs, T, max_rows);
+  if ((int)t < sq.r0 || (int)t - sq.r0 >= sq.n) return;
+  const int g = attn::group_of(groups, n, s);
+  if (g >= 0) {
+    const int ig = (int)t - attn::part_at(groups, rows, g, seqs, T, T).r0;   // (its place among the group's rows)
+    if (ig < 0 || ig >= most1) return;
+  }
   const bool both = g >= 0 && shared[g] > 0;
-  const int rg = both ? ig * G + r - i * G : 0;
+  const size_t all = (size_t)T * heads;
   float top = NOTHING, l = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  auto add = [&](const float* ws, size_t block, int n, int b, int row) {
-    const size_t piece = (size_t)b * (hd + 2);
-    const float* p = ws + block * n * piece;
+  auto add = [&](const float* ws, int n) {
+    const float* const ml_of = ws + n * all * hd;
     constexpr int N = 8;   // (pieces on the way at once; past the last: the last again, of no weight)
     for (int z = 0; z < n; z += N) {
       float4 v[N];
       float2 ml[N];
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        const float* q = p + min(z + k, n - 1) * piece;
-        v[k] = *(const float4*)(q + (size_t)row * hd + d);
-        ml[k] = *(const float2*)(q + (size_t)b * hd + 2 * row);
+        const size_t q = min(z + k, n - 1) * all + at;
+        v[k] = *(const float4*)(ws + q * hd + d);
+        ml[k] = *(const float2*)(ml_of + 2 * q);
       }
       float t = top;
 #pragma unroll
@@ -67,9 +81,9 @@ extern "C" __global__ __launch_bounds__(256) void attn_meet(char* __restrict__ r
       }
     }
   };
-  if (both) add(ws1, (size_t)(g * kvh + h) * t1 + rg / b1, n1, b1, rg % b1);
-  add(ws2, (size_t)blockIdx.x * t2 + r / b2, n2, b2, r % b2);
-  float* to = out + (size_t)(sq.r0 + i) * ldo + o_off + (h * G + r - i * G) * hd + d;
+  if (both) add(in_room(room, at1), n1);
+  add(in_room(room, at2), n2);
+  float* to = out + (size_t)t * ldo + o_off + (size_t)hq * hd + d;
   const float f = l == 0.0f ? 0.0f : 1.0f / l;
   if (l == 0.0f) o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   to[0] = o.x * f; to[1] = o.y * f; to[2] = o.z * f; to[3] = o.w * f;
