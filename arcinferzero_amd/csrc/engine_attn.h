@@ -316,6 +316,39 @@
     }
     at_counts_ = m;
   }
+  // How attention() takes a batch, by what the host knows of it: rows in tiles of 32 to a wave (few: all of a sequence's in one), its keys in nsplit pieces.
+  struct Pieces {
+    bool few;
+    int waves, tiles, least, nsplit;
+  };
+  static Pieces pieces_of(const Kv& c, const Batch& b, int heads, const Attn& a) {
+    Pieces p = {};
+    const int most = std::min(b.max_rows, b.T), window = std::min(a.window, 1 << 30);
+    const int64_t M = (int64_t)most * (heads / c.heads);
+    const size_t pairs = (size_t)b.seqs * c.heads;
+    const int keys = std::max(1, std::min(b.max_len > 0 ? b.max_len : b.ld_table * c.page, window ? (int)std::min<int64_t>((int64_t)most + window, 0x7FFFF000) : 0x7FFFF000));
+    p.few = M <= (c.hd == 256 ? 16 : 32);
+    if (p.few) {
+      // Pieces of one length for all sequences, so that long ones are more work-groups, not longer ones: two work-groups a
+      // compute unit if every sequence has the most keys, of at least 256 keys each.
+      const size_t want = ((size_t)2 * arcz_device_cus() + pairs - 1) / pairs;
+      p.least = (int)std::max<size_t>(8, ((size_t)(keys + 31) / 32 + want - 1) / want);
+      p.nsplit = (int)(((int64_t)keys + (int64_t)32 * p.least - 1) / ((int64_t)32 * p.least));
+      return p;
+    }
+    // Heads of 128 values, blocks of 32 tokens and more: work-groups of eight waves and 256 rows, one a compute unit, where rows are many
+    // and see thousands of keys; else of four and 128 rows, two of them, which fill the chip sooner and read and write rows while the
+    // other computes.  (us, 32 heads over 8, eight waves / four: 1024 rows over 9000 keys 266 / 287, 4096 over 4096 257 / 279, 512 over
+    // 8192 139 / 145, 2048 over 16000 854 / 905, 8192 over 9000 1103 / 1158; 512 over 3000 71.2 / 70.8, 3000 over 3000 163 / 154, 2048 over
+    // 2048 107 / 99, 512 over 512 43 / 34, ragged documents 74.5 / 62.3.  Two that the rule misses: 1024 over 1024 54 / 55.5, 100 over 4000
+    // 44.7 / 46.2.)
+    const int seen = std::max(0, (b.max_len > 0 ? b.max_len : b.ld_table * c.page) - most / 2);
+    p.waves = c.hd == 128 && c.block >= 32 && M >= 1024 && !a.first && (window ? std::min(window, seen) : seen) >= 2000 ? 8 : 4;
+    p.tiles = (int)((M + 32 * p.waves - 1) / (32 * p.waves));
+    // rows that fill less than the chip: their keys shared out, at least 256 to a piece
+    p.nsplit = (int)std::max<size_t>(1, std::min<size_t>((size_t)8 / p.waves * arcz_device_cus() / (pairs * p.tiles), (size_t)(keys + 255) / 256));
+    return p;
+  }
   void attention(const Kv& c, const Batch& b, cl_mem q, int ldq, int q_off, int heads, cl_mem out, int ldo, int o_off, const Attn& a) {
     Places at;
     if (!check_batch("attention", c, b, at)) return;
@@ -335,19 +368,16 @@
     const int64_t M = (int64_t)most * G;
     if (M > 0x7FFFFF00) throw std::runtime_error("attention: too many rows");
     const size_t pairs = (size_t)b.seqs * c.heads;
-    int pages = c.pages, ps = c.ps, bs = c.bs, ldt = b.ld_table, T = b.T, mr = most, kvh = c.heads, window = std::min(a.window, 1 << 30), nsplit = 1;
+    int pages = c.pages, ps = c.ps, bs = c.bs, ldt = b.ld_table, T = b.T, mr = most, kvh = c.heads, window = std::min(a.window, 1 << 30);
     float scale = a.scale, cap2 = a.cap * 1.4426950408889634f;
     const int form = (a.cap > 0.0f ? 1 : 0) | (a.slopes ? 2 : 0);
-    const int keys = std::max(1, std::min(b.max_len > 0 ? b.max_len : ldt * c.page, window ? (int)std::min<int64_t>((int64_t)most + window, 0x7FFFF000) : 0x7FFFF000));
+    const Pieces p = pieces_of(c, b, heads, a);
+    int nsplit = p.nsplit;
     int vec = rq.vec() ? 1 : 0;
     if (ro.vec()) vec |= 2;
-    if (M <= (c.hd == 256 ? 16 : 32)) {
+    if (p.few) {
       const int rt = M > 16 ? 2 : 1, pack = M <= 8 ? 1 : 0;
-      // Pieces of one length for all sequences, so that long ones are more work-groups, not longer ones: two work-groups a
-      // compute unit if every sequence has the most keys, of at least 256 keys each.
-      const size_t want = ((size_t)2 * arcz_device_cus() + pairs - 1) / pairs;
-      int least = (int)std::max<size_t>(8, ((size_t)(keys + 31) / 32 + want - 1) / want);
-      nsplit = (int)(((int64_t)keys + (int64_t)32 * least - 1) / ((int64_t)32 * least));
+      int least = p.least;
       if (nsplit > 1) at_room();
       cl_mem w = nsplit > 1 ? at_ws_ : nullptr, counts = nsplit > 1 ? at_counts_ : nullptr;
       if (pairs > 0xFFFFFFFFull / 256) throw std::runtime_error("attention: too many sequences");
@@ -359,18 +389,9 @@
       run("attention", k, 2, g, l);
       return;
     }
-    // Heads of 128 values, blocks of 32 tokens and more: work-groups of eight waves and 256 rows, one a compute unit, where rows are many
-    // and see thousands of keys; else of four and 128 rows, two of them, which fill the chip sooner and read and write rows while the
-    // other computes.  (us, 32 heads over 8, eight waves / four: 1024 rows over 9000 keys 266 / 287, 4096 over 4096 257 / 279, 512 over
-    // 8192 139 / 145, 2048 over 16000 854 / 905, 8192 over 9000 1103 / 1158; 512 over 3000 71.2 / 70.8, 3000 over 3000 163 / 154, 2048 over
-    // 2048 107 / 99, 512 over 512 43 / 34, ragged documents 74.5 / 62.3.  Two that the rule misses: 1024 over 1024 54 / 55.5, 100 over 4000
-    // 44.7 / 46.2.)
-    const int seen = std::max(0, (b.max_len > 0 ? b.max_len : ldt * c.page) - most / 2);
-    const int waves = c.hd == 128 && c.block >= 32 && M >= 1024 && !a.first && (window ? std::min(window, seen) : seen) >= 2000 ? 8 : 4, bm = 32 * waves;
-    int tiles = (int)((M + bm - 1) / bm);
+    const int waves = p.waves, bm = 32 * waves;
+    int tiles = p.tiles;
     if (pairs * tiles > 0xFFFFFFFFull / (64 * waves)) throw std::runtime_error("attention: too many rows");
-    // rows that fill less than the chip: their keys shared out, at least 256 to a piece
-    nsplit = (int)std::max<size_t>(1, std::min<size_t>((size_t)8 / waves * arcz_device_cus() / (pairs * tiles), (size_t)(keys + 255) / 256));
     if (nsplit > 1) at_room();
     cl_mem w = nsplit > 1 ? at_ws_ : nullptr;
     cl_kernel k = variant("attn", {{"HD", c.hd}, {"FINE", c.block < 32 ? 1 : 0}, {"FORM", form}, {waves == 8 ? "W8" : nullptr, 1}}, "attn_many");
@@ -476,7 +497,9 @@
   size_t attention_shared_room(const Kv& c, const Batch& b, const Shared& sh, int heads, const Attn& a) {
     Places at;
     if (!check_batch("attention_shared", c, b, at)) return 256;
-    return shared_shape(c, b, sh, heads, a).bytes;
+    const SharedShape p = shared_shape(c, b, sh, heads, a);
+    if (p.one && pieces_of(c, b, heads, a).nsplit > 1) at_room();   // (so that no call does)
+    return p.bytes;
   }
   void attention_shared(const Kv& c, const Batch& b, const Shared& sh, cl_mem q, int ldq, int q_off, int heads, cl_mem out, int ldo, int o_off, const Attn& a, cl_mem room) {
     Places at;

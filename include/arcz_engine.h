@@ -277,7 +277,9 @@ int arcz_engine_attention(arcz_engine* e, arcz_kv* c, const arcz_kv_batch* b, ar
  * arcz_engine_attention, and each sequence's own table is used for all of its keys.  groups and len are read when the launches run and held to the buffers there; out must not meet them.
  * room: a workspace of the caller's of at least arcz_engine_attention_shared_room(...) bytes, at an address of 16, that nothing else of the call
  * meets; what it holds between calls does not matter.  The bytes depend on the batch's seqs, T, ld_table, max_rows and max_len, those of the groups, heads, the
- * cache's shape and whether there is a cap or slopes (0: an error). */
+ * cache's shape and whether there is a cap or slopes (0: an error).  Asking for them also makes what the engine itself needs for such a call, where that is
+ * arcz_engine_attention with keys shared out: its room for their pieces (68 MB on 256 compute units, once an engine; an error while a list is
+ * recorded).  So no call of a batch that was asked for allocates, and its first one may be a recorded one. */
 typedef struct arcz_kv_shared {
   arcz_mem *groups, *len;
   int n, max_rows, max_len;
