@@ -19,10 +19,11 @@
 constexpr int CS = 512;   // sines and cosines of a work-group's tokens
 constexpr int WS = 768;   // a head's weights (64 lanes, twelve values each)
 
-// 1 / sqrt(sum / hd + eps), to 2^-40 (the instruction's 2^-24 and one step); a head of zeros without eps stays zeros
+// 1 / sqrt(sum / hd + eps), to 2^-40 (the instruction's 2^-24 and one step); a head of zeros without eps stays zeros, and the finite values of
+// one with an infinity are 0
 __device__ inline double inverse_root(double sum, double per, float eps) {
   const double v = fma(sum, per, (double)eps), y = __builtin_amdgcn_rsq(v);
-  return v == 0.0 ? 0.0 : y * fma(-0.5 * v * y, y, 1.5);
+  return v == 0.0 || v == __builtin_inf() ? 0.0 : y * fma(-0.5 * v * y, y, 1.5);
 }
 __device__ inline float normed(float x, double f, float w) { return (float)((double)x * f) * w; }
 __device__ inline void sines(float2* cs, const int* __restrict__ pos, int ld_pos, const uint64_t* __restrict__ tab, int pairs, int axes, float mscale, int t0, int nt) {

@@ -187,7 +187,8 @@ int arcz_engine_rope(arcz_engine* e, arcz_rope* r, arcz_mem* x, int ldx, int x_o
 /* Norms of queries and keys, a head at a time, with the rotation in the same pass: the first `heads` heads of x are queries, kv_heads of keys
  * lie behind them (either may be 0).  A head's values n = x / sqrt(mean(x^2) + eps) * w -- wq for queries, wk for keys, f32 [hd], NULL: no
  * weight -- are then turned as arcz_engine_rope turns them; what lies behind the pairs is n as it is.  eps is finite and not below 0 (a head of
- * zeros gives zeros).  No finite head overflows or vanishes on the way.  x, y, pos as there; y must not meet wq, wk or pos. */
+ * zeros gives zeros).  No finite head overflows or vanishes on the way; in one with an infinity that value is NaN (and with it the other of its
+ * pair) and the finite ones are 0.  x, y, pos as there; y must not meet wq, wk or pos. */
 int arcz_engine_norm_rope(arcz_engine* e, arcz_rope* r, arcz_mem* x, int ldx, int x_off, arcz_mem* y, int ldy, int y_off, int T, int heads, int kv_heads, int hd, arcz_mem* wq,
                           arcz_mem* wk, float eps, arcz_mem* pos, int ld_pos);
 
