@@ -3,7 +3,8 @@
 //   n = x / sqrt(mean(x^2) + eps) * w  over the head's values, w the queries' weights for the first heads and the keys' for the rest;
 //   y = n turned by the row's position (rope.hip: pairs, axes, angles), what lies behind the pairs as it is.
 //
-// Squares, their sums, the mean and its root are 64-bit, so that no finite head overflows or vanishes on the way; n is rounded to f32 once.  (With f32
+// Squares, their sums, the mean and its root are 64-bit, so that no finite head overflows or vanishes on the way; n is rounded to f32 twice, behind the root and
+// behind the weight.  (With f32
 // squares and the root's reciprocal in f32 the launches took the same: 777 tokens of 24 heads of 256 values 11.1 - 11.4 and 11.1 - 11.5 us, 8192 of 40 of
 // 128 63.3 and 63.3.)
 // Bound: 8 bytes of HBM a value.  A head's values stay in the registers of 8 to 64 lanes between the sum and the rotation, eight a lane (and
