@@ -189,6 +189,11 @@ struct Cut {
   __device__ bool keeps(uint32_t k, int i) const { return (k > key) | ((k == key) & (i <= last)); }
 };
 __device__ inline Cut higher(const Cut& a, const Cut& b) { return a.key > b.key || (a.key == b.key && a.last <= b.last) ? a : b; }
+// What lanes of a wave have written to LDS is there for its other lanes behind this, and what they have read may be written over.
+__device__ inline void met() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
 // Tokens of a row whose keys lie in [lo, hi] and that `within` keeps; listed: in LDS.
 struct Members {
   uint32_t lo, hi;
@@ -264,10 +269,12 @@ __device__ inline bool pass(S& s, const Row& r, const Range& all, const Members&
           if (keep[j]) held[at] = e[j];
           pending += __popcll(vote[j]);
         }
+        met();
         while (pending >= 64) {
           pending -= 64;
           sum += weight(r, s.pow2, held[pending + lane()]);
         }
+        met();
       }
       if (any) members(v, i);
     });
