@@ -38,3 +38,23 @@ def test_the_first_call_is_recorded(rt, way, rows, hd, heads):
     l.free()
     ref.free(hold)
     e.close()
+
+
+def test_room_that_cannot_be_made_while_recording(rt):
+    """Asked for while a list is recorded, by an engine that has none yet: an error, and none behind it."""
+    e = engine("0")
+    k = Case([(900, [(1, 400), (1, 700)])], 32, 16, 2, 128, 8)
+    hold = []
+    kv, batch = ref.device_cache(e, k.c, hold), k.b.device(hold)
+    gb, sb = az.Runtime.from_numpy(np.array(k.groups, np.int32)), az.Runtime.from_numpy(np.array(k.shared, np.int32))
+    sh, form = az.KvShared(gb, sb, 1, 2, 900), az.Attention(0.07)
+    hold += [gb, sb]
+
+    def ask():
+        return e.attention_shared_room(kv, batch, sh, 8, form)
+    with pytest.raises(az.ArczError):
+        az.Runtime.record(ask)
+    n = ask()
+    assert n > 0 and ask() == n
+    ref.free(hold)
+    e.close()
