@@ -4,7 +4,8 @@
   // work-group a row / sixteen, with a temperature, k = 50 and p, p alone, and rows of all kinds: 16 x 16384 15 21 28 27 / 18 30 35 36;
   // 16 x 32001 20 23 39 36 / 19 29 36 36; 16 x 65536 29 27 59 55 / 19 29 39 37; 32 x 65536 29 28 59 55 / 23 35 54 43; 1 x 151936 54 32 106 54 / 19 27 34 21;
   // 48 x 151936 57 36 119 109 / 37 43 88 56; 96 x 151936 61 40 122 118 / 60 65 152 90.  (Rows whose largest logit is all that is asked for: 13 / 15 and, 48 of
-  // them, 14 / 24; a cut by p behind one of 2000 tokens, which one work-group does behind the others' launches: 104 / 116.  A row's kind is known on the device only.)
+  // them, 14 / 24; a cut by p behind one of 2000 tokens, which one work-group does behind the others' launches: 104 / 116.  What a row asks for is
+  // known on the device only; which buffers a call does not give is known here, and the rule does not go by it.)
   int sample_split_ = -1;   // ARCZ_SAMPLE_SPLIT
   static int split_rows() { return std::min(96, 2 * arcz_device_cus()); }   // (the room has 264192 bytes a compute unit)
   bool split_pays(int V, int T) const { return V >= 3000 * std::max(T, 16); }

@@ -66,7 +66,7 @@ ATTN_FN int tile_at(int from, int to, int tile, int i) {
 // behind it; most_len is at most 2^31 - 4096).
 ATTN_FN int entry_of(int p, int ps, int ldt) { return lower(p >> ps, ldt - 1); }
 // Sequences behind a shared prefix.  Group g has sequences [groups[g], groups[g + 1]), whose rows are one behind the other; without groups g is a
-// sequence.  Its rows, held to the buffers; len: its first sequence (0 where it has no rows).
+// sequence.  Its rows, held to the buffers; len: its first sequence (held to those there are, whether it has rows or not).
 ATTN_FN Seq part_at(const int* groups, const int* rows, int g, int seqs, int T, int max_rows) {
   int s0 = g, s1 = g + 1;
   if (groups) {

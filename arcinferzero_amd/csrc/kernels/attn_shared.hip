@@ -9,11 +9,13 @@
 // the form.
 //
 // Bound: the prefix's products on the matrix pipe (rows and weights in two halves, so twice the operations), the sequences' own keys by latency, the pieces by
-// the caches.  Measured, 128 tokens of 32 heads over 8 of 128 values behind 16384 shared keys and up to 600 of their own: 80 + 23 + 9.6 us (attention that reads the
+// the caches.  Measured, 128 tokens of 32 heads over 8 of 128 values behind 16384 shared keys and up to 600 of their own: 80 + 24 + 10 us (attention that reads the
 // prefix once a sequence 426); the first of them makes 69 G operations, 860 TFLOP/s, in one round of 256 work-groups of 1024 keys each, the matrix pipe busy 47 % of
-// the cycles (62 % where a work-group has ten times the keys).  24 questions of up to 90 tokens behind three documents of 4000, 16 heads over 8 of 256 values, a cap: 313 + 59 + 31 us (425): one work-group a compute
+// the cycles (62 % where a work-group has ten times the keys).  24 questions of up to 90 tokens behind three documents of 4000, 16 heads over 8 of 256 values, a cap: 312 + 58 + 30 us (425): one work-group a compute
 // unit, 2.5 rounds of the pieces' tiles, tiles of which the last is half empty, and 128 values of each lane's registers for the sums alone.
 // The pieces: a row's are read once, eight at a time.
+// Those 128 tokens with a window of 2048 keys 64 us, with a bias by distance 127, capped 131 (116 on the same card with neither).
+// Registers that do not fit: 32 bytes of scratch a lane in eight waves with a bias, 12 in heads of 256 with a scale for each few keys and a cap.
 #include "attn_many.inc"
 
 // A call's workspace, the room: what these launches leave for the last one, each from its own byte on.

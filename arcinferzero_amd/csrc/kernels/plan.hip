@@ -11,7 +11,7 @@
 // Bound: latency -- one work-group for all sequences, since the sums run over them: the counts, their sums in three steps over the
 // waves, then the ring's entries and the table's, a thread each.  Places of many rows are a launch of their own (kv_places), a work-group for
 // 1024 of one sequence's, behind it.
-// Measured: 256 sequences of a token 3.8 us, 1024 5.6, 256 of eight 5.6, 64 prompts of 256 tokens 6.7 in two launches, 1024 of up to 500 12.1 (13.6 with one page of a thread's looked up
+// Measured: 256 sequences of a token 3.8 us, 1024 5.6, 256 of eight 5.6, 64 prompts of 256 tokens 6.7 in two launches, 1024 of up to 500 12.0 (13.6 with one page of a thread's looked up
 // at a time); a launch that does
 // nothing takes 2.5.
 #include "attn.h"

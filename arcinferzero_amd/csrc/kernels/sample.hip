@@ -22,7 +22,7 @@
 // Bound: the 64-bit steps of the weights, some twenty instructions a token each time that they are wanted -- once for the histogram, once for the sums --, and for
 // few rows the steps themselves, of which none begins before the last one's sums have met.  A row is read from HBM once and from the caches after that.
 // Measured, 256 rows of 151936: the largest logit 27 us (5.7 TB/s), by k and p 60, drawn among all 74, by min_p 60, by p 139; 37 rows of 32001 of all kinds 36; one row of
-// 151936 by sixteen work-groups, by k and p 26 us, by p 34.  A cut in rows that are almost flat (a temperature of 1000) takes 560.
+// 151936 by sixteen work-groups, by k and p 26 us, by p 34; 16 bytes of scratch a lane in sample and sample_draw.  A cut in rows that are almost flat (a temperature of 1000) takes 560.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

@@ -299,7 +299,7 @@ int arcz_engine_attention_shared(arcz_engine* e, arcz_kv* c, const arcz_kv_batch
  * NULL) its weight over that sum.  Weights and sums are held to 2^-42; a token of less than 2^-44 of the largest weight is not drawn.  A logit of -inf or NaN
  * is no token; a row of nothing else gives -1 and 0.  Where the largest is +inf, tokens of +inf have weight 1 and no others any.  The same rows give
  * the same tokens.  token and prob must not meet what is read, nor each other.  Nothing here waits or allocates, but for an engine's first call of few rows of
- * 48000 logits and more, which makes room (like the first attention that shares keys out: not while a list is recorded). */
+ * 48000 logits and more, which makes room (the same, 68 MB on 256 compute units, that the first attention that shares keys out makes: not while a list is recorded). */
 typedef struct arcz_sampling {
   arcz_mem *temperature, *top_k, *top_p, *min_p;
 } arcz_sampling;
