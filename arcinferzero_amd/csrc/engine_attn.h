@@ -408,7 +408,7 @@
   };
   // The launches of a call, by what the host knows of it, and where its workspace has what they leave.
   struct SharedShape {
-    int G, form, M, M1, waves1, bm1, tiles1, n1, few, rt, pack, tiles2, n2, least;
+    int G, form, M, M1, waves1, bm1, tiles1, n1, few, rt, pack, tiles2, n2, least, places, per;
     size_t ws1, ws2, bytes;
     bool one;
   };
@@ -480,8 +480,12 @@
       p.bytes = 256;
       return p;
     }
-    // (the last launch has a thread for each four values)
-    const size_t each = (size_t)b.T * heads;   // (rows of a piece)
+    // A piece has a place for each row of the buffers or, where that is less (buffers for more rows than the batch may have), for each of the most
+    // rows of every sequence.  (The last launch has a thread for each four values of it.)
+    const int mr = std::min(b.max_rows, b.T);
+    p.per = (int64_t)b.seqs * mr <= b.T ? mr : 0;
+    p.places = p.per ? b.seqs * mr : b.T;
+    const size_t each = (size_t)p.places * heads;
     if (pairs * p.tiles2 > 0xFFFFFFFFull / 256 || pairs1 * p.tiles1 > 0xFFFFFFFFull / 512 || each > 0x7FFFFFFF || each * c.hd / 4 > 0xFFFFFF00ull) throw std::runtime_error("attention_shared: too many rows");
     auto place = [&](size_t bytes) {
       const size_t at = p.bytes;
@@ -527,12 +531,12 @@
       if (overlap(ro.place(), i) || overlap(work, i)) throw std::runtime_error("attention_shared: out or the room overlaps slopes, prefix, first or the groups");
     if (p.one) return attention(c, b, q, ldq, q_off, heads, out, ldo, o_off, a);
     int pages = c.pages, ps = c.ps, bs = c.bs, ldt = b.ld_table, T = b.T, mr = std::min(b.max_rows, b.T), kvh = c.heads, window = std::min(a.window, 1 << 30), hd = c.hd, seqs = b.seqs, n = sh.n;
-    int mr1 = std::min(sh.max_rows, b.T), vec = rq.vec() ? 1 : 0, n1 = p.n1, n2 = p.n2, t1 = p.tiles1, t2 = p.tiles2, least = p.least;
+    int mr1 = std::min(sh.max_rows, b.T), vec = rq.vec() ? 1 : 0, n1 = p.n1, n2 = p.n2, t1 = p.tiles1, t2 = p.tiles2, least = p.least, places = p.places, per = p.per;
     float scale = a.scale, cap2 = a.cap * 1.4426950408889634f;
     auto part = [&](const char* name, int front, size_t sets, int rows, int waves, int tiles, int nsplit, size_t ws) {
       cl_kernel k = variant("attn", {{"HD", c.hd}, {"FINE", c.block < 32 ? 1 : 0}, {"FORM", p.form}, {waves == 8 ? "W8" : nullptr, 1}}, "attn_part");
       set_args(k, 0, q, ldq, q_off, c.b[0], c.b[1], c.b[2], c.b[3], pages, ps, bs, b.rows, b.len, b.table, ldt, T, rows, heads, kvh, scale, cap2, window, a.slopes, a.prefix, a.first,
-               sh.groups, sh.len, n, seqs, mr, front, room, ws, nsplit, tiles, vec);
+               sh.groups, sh.len, n, seqs, mr, front, places, per, room, ws, nsplit, tiles, vec);
       size_t g[2] = {sets * c.heads * tiles * 64 * waves, (size_t)nsplit}, l[2] = {(size_t)64 * waves, 1};
       run(name, k, 2, g, l);
     };
@@ -540,16 +544,16 @@
     if (p.few) {
       cl_kernel k = variant("attn", {{"HD", c.hd}, {"RT", p.rt}, {"PACK", p.pack}, {"FINE", c.block < 4 ? 1 : 0}, {"FORM", p.form}}, "attn_part_few");
       set_args(k, 0, q, ldq, q_off, c.b[0], c.b[1], c.b[2], c.b[3], pages, ps, bs, b.rows, b.len, b.table, ldt, T, mr, heads, kvh, scale, cap2, window, a.slopes, a.prefix, a.first,
-               sh.groups, sh.len, n, room, p.ws2, n2, least, vec);
+               sh.groups, sh.len, n, places, per, room, p.ws2, n2, least, vec);
       size_t g[2] = {(size_t)seqs * c.heads * 256, (size_t)n2}, l[2] = {256, 1};
       run("attention_own", k, 2, g, l);
     } else {
       part("attention_own", 0, (size_t)seqs, mr, 4, t2, n2, p.ws2);
     }
     cl_kernel k = variant("attn", {}, "attn_meet");
-    set_args(k, 0, room, p.ws1, n1, p.ws2, n2, hd, b.rows, T, mr, heads, sh.groups, sh.len, n, seqs, mr1, out, ldo, o_off);
-    const size_t per = 1024 / c.hd;
-    size_t g = ((size_t)T * heads + per - 1) / per * 256, l = 256;
+    set_args(k, 0, room, p.ws1, n1, p.ws2, n2, hd, b.rows, T, mr, heads, sh.groups, sh.len, n, seqs, mr1, places, per, out, ldo, o_off);
+    const size_t each = 1024 / c.hd;
+    size_t g = ((size_t)places * heads + each - 1) / each * 256, l = 256;
     run("attention_meet", k, 1, &g, &l);
   }
   void join(const Kv& c, const Batch& b, cl_mem w, int nsplit, int rows, int blocks, int mr, int heads, cl_mem out, int ldo, int o_off) {

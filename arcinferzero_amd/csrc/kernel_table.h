@@ -139,10 +139,10 @@ static const KernelSpec kKernelTable[] = {
     {"attn", "attn_few", nullptr, "piippppiiipppiiiiipiiffipppppiii", {"HD", "RT", "PACK", "FINE", "FORM", nullptr}, {{nullptr, 0, false}}, 256},
     {"attn", "attn_many", "W8", "piippppiiipppiiiiipiiffippppiii", {"HD", "FINE", "FORM", "W8", nullptr}, {{nullptr, 0, false}}, 512},
     {"attn", "attn_many", nullptr, "piippppiiipppiiiiipiiffippppiii", {"HD", "FINE", "FORM", nullptr}, {{nullptr, 0, false}}, 256},
-    {"attn", "attn_part", "W8", "piippppiiipppiiiiiffipppppiiiipziii", {"HD", "FINE", "FORM", "W8", nullptr}, {{nullptr, 0, false}}, 512},
-    {"attn", "attn_part", nullptr, "piippppiiipppiiiiiffipppppiiiipziii", {"HD", "FINE", "FORM", nullptr}, {{nullptr, 0, false}}, 256},
-    {"attn", "attn_part_few", nullptr, "piippppiiipppiiiiiffipppppipziii", {"HD", "RT", "PACK", "FINE", "FORM", nullptr}, {{nullptr, 0, false}}, 256},
-    {"attn", "attn_meet", nullptr, "pziziipiiippiiipii", {nullptr}, {{nullptr, 0, false}}, 256},
+    {"attn", "attn_part", "W8", "piippppiiipppiiiiiffipppppiiiiiipziii", {"HD", "FINE", "FORM", "W8", nullptr}, {{nullptr, 0, false}}, 512},
+    {"attn", "attn_part", nullptr, "piippppiiipppiiiiiffipppppiiiiiipziii", {"HD", "FINE", "FORM", nullptr}, {{nullptr, 0, false}}, 256},
+    {"attn", "attn_part_few", nullptr, "piippppiiipppiiiiiffipppppiiipziii", {"HD", "RT", "PACK", "FINE", "FORM", nullptr}, {{nullptr, 0, false}}, 256},
+    {"attn", "attn_meet", nullptr, "pziziipiiippiiiiipii", {nullptr}, {{nullptr, 0, false}}, 256},
     {"attn", "attn_join", nullptr, "piiiippiiiiipii", {nullptr}, {{nullptr, 0, false}}, 256},
     {"moe", "moe_combine", nullptr, "pppppi", {nullptr}, {{"NU", 0, true}, {nullptr, 0, false}}, 256},
 };

@@ -98,6 +98,8 @@ ATTN_FN int seq_of_row(const int* rows, int s0, int s1, int r0, int n, int t) {
   }
   return a;
 }
+// Where a row's pieces are among those of a batch: row t, the i-th of sequence s -- `per` places for each sequence, or (0) one for each row of the buffers.
+ATTN_FN int place_of(int per, int s, int i, int t) { return per ? s * per + i : t; }
 // The group that a sequence is in (n of them, in order), -1: in none.
 ATTN_FN int group_of(const int* groups, int n, int s) {
   int a = 0, b = n;   // (the last group that does not begin behind s lies in [a, b))

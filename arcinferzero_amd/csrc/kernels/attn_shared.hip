@@ -33,27 +33,34 @@ __device__ inline int seq_of_one_row(const int* __restrict__ rows, int seqs, int
   return a;
 }
 
-// The parts joined: a row and head has n1 pieces of its group's keys and n2 of its own, in the batch's order of rows: sums [piece][T][heads][hd], then
-// reference and sum of weights [piece][T][heads][2].  (So the room, and this launch, are as large as the batch, however unlike its sequences are:
-// one of 2048 tokens beside 255 of a token, 64 heads of 128 values, 0.15 GB; blocks of the longest one's rows for each would be 8.8.)  Rows
-// past the group's `most1`, past max_rows of a sequence, or of none, are left as they are.  grid (T x heads / (1024 / hd)), 256.
+// The parts joined: a row and head has n1 pieces of its group's keys and n2 of its own: sums [piece][places][heads][hd], then reference and sum of weights
+// [piece][places][heads][2], a place for each row of the buffers or, where that is less, for each of the most rows of every sequence.  (So the room, and this
+// launch, are no larger than the batch may be, however unlike its sequences are: one of 2048 tokens beside 255 of a token, 64 heads of 128 values, 0.15 GB; blocks of the
+// longest one's rows for each would be 8.8.)  Rows past the group's `most1`, past max_rows of a sequence, or of none, are left as they are.
+// grid (places x heads / (1024 / hd)), 256.
 extern "C" __global__ __launch_bounds__(256) void attn_meet(char* __restrict__ room, size_t at1, int n1, size_t at2, int n2, int hd, const int* __restrict__ rows, int T,
                                                             int max_rows, int heads, const int* __restrict__ groups, const int* __restrict__ shared, int n, int seqs,
-                                                            int most1, float* __restrict__ out, int ldo, int o_off) {
-  const unsigned at = blockIdx.x * (1024u / hd) + threadIdx.x / (hd / 4), t = at / heads, hq = at - t * heads;   // (the host holds T * heads below 2^31)
+                                                            int most1, int places, int per, float* __restrict__ out, int ldo, int o_off) {
+  const unsigned at = blockIdx.x * (1024u / hd) + threadIdx.x / (hd / 4), u = at / heads, hq = at - u * heads;   // (the host holds places * heads below 2^31)
   const int d = threadIdx.x % (hd / 4) * 4;
-  const int t0 = min(__builtin_amdgcn_readfirstlane(t), T - 1), s0 = seq_of_one_row(rows, seqs, t0);
-  if (t >= (unsigned)T) return;
-  const int s = (int)t == t0 ? s0 : attn::seq_of_row(rows, s0, seqs, t0, T - t0, t);   // (few heads: a wave has values of several rows)
+  int s = 0, t = (int)u;
+  if (per) {
+    s = min(u / per, (unsigned)(seqs - 1));
+  } else {
+    const int t0 = min(__builtin_amdgcn_readfirstlane(t), T - 1), s0 = seq_of_one_row(rows, seqs, t0);
+    s = t <= t0 ? s0 : attn::seq_of_row(rows, s0, seqs, t0, T - t0, t);   // (few heads: a wave has values of several rows)
+  }
+  if (u >= (unsigned)places) return;
   const Seq sq = attn::part_at(nullptr, rows, s, seqs, T, max_rows);
-  if ((int)t < sq.r0 || (int)t - sq.r0 >= sq.n) return;
+  if (per) t = sq.r0 + ((int)u - s * per);
+  if (t < sq.r0 || t - sq.r0 >= sq.n) return;
   const int g = attn::group_of(groups, n, s);
   if (g >= 0) {
-    const int ig = (int)t - attn::part_at(groups, rows, g, seqs, T, T).r0;   // (its place among the group's rows)
+    const int ig = t - attn::part_at(groups, rows, g, seqs, T, T).r0;   // (its place among the group's rows)
     if (ig < 0 || ig >= most1) return;
   }
   const bool both = g >= 0 && shared[g] > 0;
-  const size_t all = (size_t)T * heads;
+  const size_t all = (size_t)places * heads;
   float top = NOTHING, l = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   auto add = [&](const float* ws, int n) {
@@ -96,11 +103,11 @@ extern "C" __global__ __launch_bounds__(256) void attn_meet(char* __restrict__ r
   extern "C" __global__ __launch_bounds__(64 * NW, W) void NAME(                                                                                                \
       const float* q, int ldq, int q_off, const int8_t* kq, const int8_t* vq, const float* ks, const float* vs, int pages, int ps, int bs, const int* rows,     \
       const int* lens, const int* table, int ldt, int T, int max_rows, int heads, int kvh, float scale, float cap2, int window, const float* slopes,            \
-      const int* prefix, const int* first, const int* groups, const int* shared, int n, int seqs, int most_rows, int front, char* room, size_t at,             \
-      int nsplit, int tiles, int vec) {                                                                                                                         \
+      const int* prefix, const int* first, const int* groups, const int* shared, int n, int seqs, int most_rows, int front, int places, int per, char* room,   \
+      size_t at, int nsplit, int tiles, int vec) {                                                                                                              \
     many_body<HD, KT, NW, FINE, (F & 1) != 0, (F & 2) != 0, true>(q, ldq, q_off, kq, vq, ks, vs, pages, ps, bs, rows, lens, table, ldt, T, max_rows, heads,     \
                                                                   kvh, nullptr, 0, 0, scale, cap2, window, slopes, prefix, first, in_room(room, at), nsplit,    \
-                                                                  tiles, vec, {groups, shared, lens, n, seqs, most_rows, front});                               \
+                                                                  tiles, vec, {groups, shared, lens, n, seqs, most_rows, front, places, per});                  \
   }
 #define PART4(HD, KT, NW, W, FINE, S)                                     \
   PART(attn_part__HD##HD##_FINE##FINE##_FORM0##S, HD, KT, NW, W, FINE, 0) \

@@ -45,6 +45,20 @@ int main() {
       const bool takes = t >= q.r0 && t - q.r0 < q.n;
       if (sound) NEED(takes ? of[t] == s : of[t] == -1);
     }
+    // the places of their pieces: one for each row, inside what there is of them, and found again from the sequence and its row
+    const int most = max_rows < T ? max_rows : T, per = (long long)seqs * most <= T ? most : 0, places = per ? seqs * per : T;
+    std::vector<char> used(places, 0);
+    for (int s = 0; s < seqs; ++s) {
+      const attn::Seq q = attn::part_at(nullptr, rows.data(), s, seqs, T, most);
+      for (int i = 0; i < q.n; ++i) {
+        const int u = attn::place_of(per, s, i, q.r0 + i);
+        NEED(u >= 0 && u < places);
+        if (sound) NEED(!used[u]);
+        used[u] = 1;
+        if (per) NEED(u / per == s && u % per == i);
+        else NEED(u == q.r0 + i);
+      }
+    }
   }
   printf("%ld rows of batches\n", checks);
   return 0;

@@ -41,6 +41,23 @@ def test_a_loose_most_of_rows(eng):
             assert m <= max(2 * n, 12 * piece), (m, n, piece)
 
 
+def test_buffers_of_more_rows_than_the_batch_may_have(eng):
+    """A recorded step's buffers are made for its largest batch: what the sequences can have, seqs * max_rows, is less."""
+    n, _ = room(eng, 128, 128, 1, 128)
+    m, _ = room(eng, 128, 8192, 1, 128)
+    assert m <= n
+
+
+@pytest.mark.parametrize("hd,kv,heads", [(64, 2, 8), (128, 1, 4), (256, 1, 3)])
+@pytest.mark.parametrize("max_rows", [None, 1, 3])
+def test_loose_buffers(eng, hd, kv, heads, max_rows):
+    """Places by sequences: rows left out of some, sequences of none, a group and sequences of no group."""
+    k = Case([(130, [(1, 9), (3, 40), (0, 7), (2, 2), (1, 200)]), (50, [(1, 1), (3, 77)])], 32, 16, kv, hd, heads, T=90, max_rows=max_rows)
+    k.run(eng, again=2)
+    k.groups, k.shared = [1, 4], [130]
+    k.run(eng)
+
+
 @pytest.mark.parametrize("hd,kv,heads", [(64, 2, 8), (128, 1, 4), (256, 1, 3)])
 def test_unlike_sequences(eng, hd, kv, heads):
     """A chunk of 300 rows between tokens, in a group and in none; rows behind the last sequence; a loose max_rows."""
