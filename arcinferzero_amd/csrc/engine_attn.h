@@ -422,6 +422,7 @@
     if (M > 0x7FFFFF00 || M1 > 0x7FFFFF00) throw std::runtime_error("attention_shared: too many rows");
     p.M = (int)M;
     p.M1 = (int)M1;
+    const double rows = (double)std::min<int64_t>(b.T, (int64_t)b.seqs * std::min(b.max_rows, b.T));   // (that the batch may have: its buffers may be for more)
     const size_t cus = (size_t)arcz_device_cus(), pairs = (size_t)b.seqs * c.heads, pairs1 = (size_t)sh.n * c.heads;
     const int all = b.max_len > 0 ? b.max_len : b.ld_table * c.page, shared = sh.max_len > 0 ? std::min(sh.max_len, all) : all, own = std::max(1, sh.max_len > 0 ? all - shared : all);
     // Work-groups of eight waves from 512 rows on (us, with eight / four: 512 rows behind 16384 keys 80 / 83, 4000 behind 6000 150 / 170; 256 rows behind 1024
@@ -429,20 +430,20 @@
     p.waves1 = c.hd == 128 && c.block >= 32 && M1 >= 512 ? 8 : 4;
     p.bm1 = 32 * p.waves1;
     p.tiles1 = (int)((M1 + p.bm1 - 1) / p.bm1);
-    const double rate = c.hd == 64 ? 0.8e9 : c.hd == 128 ? 1.0e9 : 0.7e9, key = 2.0 * c.heads * c.hd, mean = (double)b.T / std::max(1, b.seqs) * p.G;
+    const double rate = c.hd == 64 ? 0.8e9 : c.hd == 128 ? 1.0e9 : 0.7e9, key = 2.0 * c.heads * c.hd, mean = rows / std::max(1, b.seqs) * p.G;
     // The group's keys in pieces of at least 128 (us, 4 to 16 sequences of a token behind 512 - 4096 keys, at least 256 / 128 / 64: 28 - 30 / 24 - 28 / 21 - 34): one
     // or the most that one to four work-groups for every compute unit make, whichever takes the least -- rounds of a piece's keys and what a work-group takes
     // beside them (as 128 keys would), and each piece written and read.  (us, pieces 1, 2, 3 ...: 24 of 16 heads of 256 values and up to 90 rows behind 4000
     // 370 354 333 323 335 344; eight of 32 of 128 and up to 120 rows behind 8000 366 229 179 162 215 194.)
     double front = 0.0;
     if (p.tiles1 && pairs1) {
-      const double sets = c.heads * std::min((double)sh.n * p.tiles1, std::ceil((double)b.T * p.G / p.bm1) + 0.5 * (sh.n - 1));
+      const double sets = c.heads * std::min((double)sh.n * p.tiles1, std::ceil(rows * p.G / p.bm1) + 0.5 * (sh.n - 1));
       // (max_rows may say more than the groups have: the grid is for what it says)
       const int most = (int)std::max<size_t>(1, std::min<size_t>((size_t)(shared + 127) / 128, 8 * cus / (pairs1 * p.tiles1)));
       for (int r = 0; r <= 4; ++r) {
         const int n = r ? std::min(most, (int)(r * cus / sets)) : 1;
         if (n < 1) continue;
-        const double t = std::ceil(sets * n / cus) * p.bm1 * ((double)shared / n + 128.0) * 8.0 * c.hd / rate * cus + (double)b.T * heads * n * (c.hd + 2) * 8.0 / 5.0e6;
+        const double t = std::ceil(sets * n / cus) * p.bm1 * ((double)shared / n + 128.0) * 8.0 * c.hd / rate * cus + rows * heads * n * (c.hd + 2) * 8.0 / 5.0e6;
         if (r && t >= front) continue;
         front = t;
         p.n1 = n;
@@ -474,7 +475,7 @@
     };
     const int pieces = (int)std::max<size_t>(1, std::min<size_t>(2 * cus / std::max<size_t>(1, pairs * ((M + 127) / 128)), (size_t)(all + 255) / 256));
     const double one = 8.0 + (p.few ? b.seqs * (double)all * key / 9.5e6 : tiles(all, pieces));
-    const double three = 24.0 + front + (p.few ? b.seqs * (double)own * key / 5.0e6 : tiles(own, p.n2)) + (double)b.T * heads * p.n2 * (c.hd + 2) * 8.0 / 5.0e6;
+    const double three = 24.0 + front + (p.few ? b.seqs * (double)own * key / 5.0e6 : tiles(own, p.n2)) + rows * heads * p.n2 * (c.hd + 2) * 8.0 / 5.0e6;
     p.one = attn_shared_ < 0 ? one <= three : attn_shared_ == 0;
     if (p.one) {
       p.bytes = 256;

@@ -90,3 +90,27 @@ def test_many_rows_and_heads(eng):
     want, tol, _ = ref.attention(k.c, k.x, k.b.rows, k.b.lens, k.b.table, 0.11)
     assert (np.abs(y[:n] - want) <= tol).all() and (y[n:] == 7.25).all()
     ref.free(hold)
+
+
+def test_loose_buffers_pay_as_tight_ones_do(rt):
+    """256 sequences of a token behind a long prefix are three launches, also in buffers of 8192 rows; the values are the same."""
+    e, got = engine(None), []
+    for T in (256, 8192):
+        k = Case([(64, [(1, 30 + i % 7) for i in range(256)])], 32, 16, 2, 128, 8, T=T)
+        hold, w = [], 8 * 128
+        k.x[256:] = 0
+        kv, batch = ref.device_cache(e, k.c, hold), k.b.device(hold)
+        batch.max_len = 9040
+        q, out = az.Runtime.from_numpy(k.x), az.Runtime.alloc(k.x.nbytes)
+        gb, sb = az.Runtime.from_numpy(np.array(k.groups, np.int32)), az.Runtime.from_numpy(np.array(k.shared, np.int32))
+        sh, form = az.KvShared(gb, sb, 1, 256, 9000), az.Attention(0.05)
+        rm = az.Runtime.alloc(e.attention_shared_room(kv, batch, sh, 8, form))
+        hold += [q, out, gb, sb, rm]
+        q.write(np.random.default_rng(1).standard_normal((256, w)).astype(np.float32))
+        n = az.lib.arcz_launch_count()
+        e.attention_shared(kv, batch, sh, q, w, 0, 8, out, w, 0, form, rm)
+        assert az.lib.arcz_launch_count() == n + 3
+        got.append(out.read(np.uint32, 256 * w))
+        ref.free(hold)
+    assert np.array_equal(*got)
+    e.close()
