@@ -15,7 +15,7 @@
 // unit, 2.5 rounds of the pieces' tiles, tiles of which the last is half empty, and 128 values of each lane's registers for the sums alone.
 // The pieces: a row's are read once, eight at a time.
 // Those 128 tokens with a window of 2048 keys 64 us, with a bias by distance 127, capped 131 (116 on the same card with neither).
-// Registers that do not fit: 32 bytes of scratch a lane in eight waves with a bias, 12 in heads of 256 with a scale for each few keys and a cap.
+// Registers that do not fit: 36 bytes of scratch a lane in eight waves with a bias, 12 in heads of 256 with a scale for each few keys and a cap.
 #include "attn_many.inc"
 
 // A call's workspace, the room: what these launches leave for the last one, each from its own byte on.
