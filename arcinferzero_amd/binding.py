@@ -761,7 +761,8 @@ class Engine:
         return KvCache(self, h, pages, page, block, heads, hd)
 
     def kv_plan(self, batch, plan):
-        """The batch's rows, lengths and new pages (and its rows' positions and places) out of how many tokens each sequence gets."""
+        """The batch's rows, lengths and new pages (and its rows' positions and places) out of how many tokens each sequence gets.  A plan that does
+        not fit, or would put rows in pages that others share, changes nothing (after[2] says so)."""
         r = _kv_plan(self.h, batch.at, plan.at)
         if r:
             _check(r, engine=True)
@@ -785,7 +786,8 @@ class Engine:
             _check(r, engine=True)
 
     def attention_shared_room(self, kv, batch, shared, heads, form):
-        """The bytes of workspace that attention_shared takes for such a call."""
+        """The bytes of workspace that attention_shared takes for such a call; what the engine itself needs for it is made here (not while a list is
+        recorded), so that no such call allocates."""
         n = lib.arcz_engine_attention_shared_room(self.h, kv.h, batch.at, shared.at, heads, form.at)
         if not n:
             raise ArczError(-100, lib.arcz_engine_error().decode())
