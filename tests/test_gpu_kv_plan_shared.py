@@ -16,7 +16,7 @@ def eng(rt):
 
 
 def refused(p, eng, add):
-    """The plan changes nothing: held to the walk over adds that take more than the batch has room for."""
+    """The plan changes nothing, and says so."""
     was = [a.copy() for a in (p.len, p.table, p.ring, p.state)]
     rows, lens, table, ring, after, pos, slot = p_run(p, eng, add)
     assert not rows.any() and np.array_equal(lens, was[0]) and np.array_equal(table, was[1]) and np.array_equal(ring, was[2])
